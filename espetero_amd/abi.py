@@ -9,11 +9,12 @@ import os
 
 import numpy as np
 
-ESP_F16, ESP_BF16 = 0, 1
+ESP_F16, ESP_BF16, ESP_F32 = 0, 1, 2
 ESP_EWORKSPACE = 4
 ESP_LAYOUT_REFERENCE, ESP_LAYOUT_NATIVE = 0, 1
 ESP_ABI_VERSION = 3
-ESP_PASS_FUSED, ESP_PASS_ROWS_IN_POOL = 1, 2
+ESP_PASS_FUSED, ESP_PASS_ROWS_IN_POOL, ESP_PASS_DIFF = 1, 2, 4
+ESP_LOWRANK_SLICES = 4
 ESP_STATIC_SCRATCH_BYTES = 32 << 20
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -59,11 +60,29 @@ class GateParams(C.Structure):
                 ("q_ld", C.c_int32), ("x_ld", C.c_int32)]
 
 
+class DiffParams(C.Structure):
+    _fields_ = [("weight", C.c_void_p), ("norm_w", C.c_void_p), ("eps", C.c_float), ("factor", C.c_float)]
+
+
+class LowRankParams(C.Structure):
+    _fields_ = [("D", C.c_int32), ("rank", C.c_int32), ("n_slices", C.c_int32), ("dtype", C.c_int32), ("x_ld", C.c_int32),
+                ("y_ld", C.c_int32), ("n_adapters", C.c_int32), ("rows_per_tile", C.c_int32),
+                ("y_off", C.c_int32 * ESP_LOWRANK_SLICES), ("width", C.c_int32 * ESP_LOWRANK_SLICES)]
+
+
+class LogitsParams(C.Structure):
+    _fields_ = [("vocab", C.c_int32), ("dtype", C.c_int32), ("in_ld", C.c_int32), ("out_ld", C.c_int32), ("n_slots", C.c_int32),
+                ("n_masks", C.c_int32), ("n_bias", C.c_int32), ("pad", C.c_int32)]
+
+
 TREE_DT = np.dtype([("base", "<i4"), ("P", "<i4"), ("table", "<i4"), ("M", "<i4")])
 TILE_DT = np.dtype([("tree", "<i4"), ("r0", "<i4"), ("k0", "<i4"), ("k1", "<i4"),
                     ("part", "<i4"), ("last", "<i4"), ("b0", "<i4"), ("pad", "<i4")])
 COMBINE_DT = np.dtype([("r0", "<i4"), ("rows", "<i4"), ("part0", "<i4"), ("nparts", "<i4")])
 KVSAVE_DT = np.dtype([("src_row", "<i4"), ("block", "<i4"), ("pos", "<i4"), ("pad", "<i4")])
+LOWRANK_TILE_DT = np.dtype([("adapter", "<i4"), ("first", "<i4"), ("count", "<i4"), ("pad", "<i4")])
+LOGITS_ROW_DT = np.dtype([("slot", "<i4"), ("mask", "<i4"), ("bias0", "<i4"), ("n_bias", "<i4"), ("repetition", "<f4"),
+                          ("frequency", "<f4"), ("presence", "<f4"), ("pad", "<i4")])
 
 assert C.sizeof(Tree) == TREE_DT.itemsize == 16
 assert C.sizeof(Tile) == TILE_DT.itemsize == 32
@@ -72,6 +91,10 @@ assert C.sizeof(KVSave) == KVSAVE_DT.itemsize == 16
 assert C.sizeof(AttnParams) == 80
 assert C.sizeof(PrepParams) == 72
 assert C.sizeof(GateParams) == 24
+assert C.sizeof(DiffParams) == 24
+assert C.sizeof(LowRankParams) == 64
+assert C.sizeof(LogitsParams) == 32
+assert LOWRANK_TILE_DT.itemsize == 16 and LOGITS_ROW_DT.itemsize == 32
 
 # name -> (restype, argtypes); every symbol the header declares.
 _P = C.POINTER(AttnParams)
@@ -102,6 +125,19 @@ ATTN_SYMBOLS = {
     "esp_head_gate": (C.c_int, (C.POINTER(GateParams), _V, _V, _V, _V, C.c_int32, _V) + _ERR),
     "esp_attn_decode_fused": (C.c_int, (C.POINTER(PrepParams), _P, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, C.c_int32, _V, C.c_int32,
                                         _V, C.c_int32, C.c_int32, C.c_int32, _V, C.c_size_t, _V) + _ERR),
+    "esp_attn_diff_rows": (C.c_int32, (_P, C.c_int32)),
+    "esp_attn_diff_hint": (C.c_int, (_P, C.c_int, C.POINTER(C.c_int32), C.POINTER(C.c_int32)) + _ERR),
+    "esp_attn_diff_workspace_bytes": (C.c_size_t, (_P, C.c_int32)),
+    "esp_attn_diff": (C.c_int, (_P, C.POINTER(DiffParams), _V, _V, _V, _V, _V, C.c_int32, _V, C.c_int32, _V, C.c_int32, C.c_int32, C.c_int32,
+                                _V, C.c_size_t, _V) + _ERR),
+    "esp_lowrank_rows": (C.c_int32, (C.POINTER(LowRankParams), C.c_int32)),
+    "esp_lowrank_workspace_bytes": (C.c_size_t, (C.POINTER(LowRankParams), C.c_int32, C.c_int32)),
+    "esp_lowrank_add": (C.c_int, (C.POINTER(LowRankParams), _V, _V, _V, _V, _V, _V, C.c_int32, _V, C.c_int32, _V, C.c_size_t, _V) + _ERR),
+    "esp_logits_workspace_bytes": (C.c_size_t, (C.POINTER(LogitsParams), C.c_int32)),
+    "esp_logits_process": (C.c_int, (C.POINTER(LogitsParams), _V, _V, _V, _V, C.c_int32, _V, _V, _V, _V, _V, C.c_int32, _V, C.c_size_t, _V) + _ERR),
+    "esp_logits_validate": (C.c_int, (C.POINTER(LogitsParams), _V, C.c_int32, _V) + _ERR),
+    "esp_history_record": (C.c_int, (C.POINTER(LogitsParams), _V, _V, _V, _V, C.c_int32, C.c_int32, _V) + _ERR),
+    "esp_history_clear": (C.c_int, (C.POINTER(LogitsParams), _V, _V, _V, C.c_int32, _V) + _ERR),
     "esp_attn_prep": (C.c_int, (C.POINTER(PrepParams), _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, C.c_int32, _V) + _ERR),
 }
 

@@ -1,5 +1,7 @@
 // The C ABI (include/espetero_attn.h): argument checks, workspace carving and
 // kernel selection. Nothing here allocates device memory or synchronises.
+#include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -7,6 +9,9 @@
 #include <vector>
 
 #include "common.hpp"
+#include "diff_math.hpp"
+#include "logits_shape.hpp"
+#include "lowrank_shape.hpp"
 
 namespace esp {
 hipError_t launch_stream(int dt, int HD, int NC, const KArgs& a, const PrepArgs* pa, int n_tiles, hipStream_t st);
@@ -31,6 +36,14 @@ hipError_t stream_init_attributes();
 hipError_t tiled_init_attributes();
 hipError_t tiled256_init_attributes();
 hipError_t tiled512_init_attributes();
+hipError_t launch_diff_stream(int dt, const DiffArgs& a, int n_tiles, hipStream_t st);
+hipError_t launch_diff_merge(int dt, const DiffArgs& a, const esp_combine* jobs, int n_jobs, hipStream_t st);
+hipError_t diff_init_attributes();
+hipError_t launch_lowrank(int dt, const LowRankArgs& a, int n_tiles, hipStream_t st);
+hipError_t launch_logits(int dt, const LogitsArgs& a, int n_rows, hipStream_t st);
+hipError_t launch_history_record(const esp_logits_params* p, uint32_t* seen, int32_t* counts, const int32_t* tokens, const int32_t* slots, int n,
+                                 int given, hipStream_t st);
+hipError_t launch_history_clear(const esp_logits_params* p, uint32_t* seen, int32_t* counts, const int32_t* slots, int n, hipStream_t st);
 }  // namespace esp
 
 // Library-owned device memory, one copy per GPU, held until the process ends: what
@@ -77,6 +90,16 @@ int check_params(const esp_attn_params* p, char* err, size_t errlen) {
 // streaming kernel's column tiles (1, 2) or -1 for the tiled kernel.
 int family(const esp_attn_params* p) {
   return esp::kernel_family(p->head_dim, p->rows_per_tile, p->H / p->Hkv);
+}
+
+// What differential attention asks of a layer's parameters beyond check_params.
+int check_diff(const esp_attn_params* p, char* err, size_t errlen) {
+  if (int rc = check_params(p, err, errlen)) return rc;
+  if (p->head_dim != esp::kDiffHD) return fail(err, errlen, ESP_EUNSUPPORTED, "head_dim %d: differential attention serves %d", p->head_dim, esp::kDiffHD);
+  if (p->H % 2 || p->Hkv % 2) return fail(err, errlen, ESP_EINVAL, "H=%d Hkv=%d: heads work in pairs", p->H, p->Hkv);
+  if (p->gate || p->bidi) return fail(err, errlen, ESP_EUNSUPPORTED, "differential attention takes neither a gate nor bidirectional rows");
+  if (!(p->scale > 0.0f)) return fail(err, errlen, ESP_EINVAL, "scale must be positive");
+  return ESP_OK;
 }
 
 using esp::Carve;
@@ -143,6 +166,7 @@ int device_state(DeviceState** out, char* err, size_t errlen) {
     if ((e = esp::tiled256_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (tiled kernels, head dim 256)", e);
     if ((e = esp::tiled512_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (tiled kernels, head dim 512)", e);
     if ((e = esp::gate_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (head gate)", e);
+    if ((e = esp::diff_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (differential attention)", e);
     d.scratch = static_cast<unsigned char*>(ps);
     d.ready = true;
   }
@@ -383,7 +407,19 @@ int esp_attn_validate_for(const esp_attn_params* p, int32_t mode, const esp_tile
   if (int rc = esp_attn_validate(p, tiles, n_tiles, trees, n_trees, jobs, n_jobs, n_parts, n_rows, blocks, n_block_entries, pool_blocks,
                                  err, errlen))
     return rc;
-  if (mode & ~(ESP_PASS_FUSED | ESP_PASS_ROWS_IN_POOL)) return fail(err, errlen, ESP_EINVAL, "mode %d", mode);
+  if (mode & ~(ESP_PASS_FUSED | ESP_PASS_ROWS_IN_POOL | ESP_PASS_DIFF)) return fail(err, errlen, ESP_EINVAL, "mode %d", mode);
+  if (mode & ESP_PASS_DIFF) {
+    if (mode != ESP_PASS_DIFF) return fail(err, errlen, ESP_EINVAL, "mode %d: a pass of differential attention has no other form", mode);
+    if (int rc = check_diff(p, err, errlen)) return rc;
+    if (!esp::diff_family(p->rows_per_tile, p->H / p->Hkv))
+      return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_attn_diff_rows)", p->rows_per_tile);
+    for (int i = 0; i < n_tiles; ++i) {
+      const esp_tile& t = tiles[i];
+      const int32_t P = trees[t.tree].P, k1 = std::min(t.k1, P);
+      if (t.last && k1 > t.k0 && (k1 != P || t.b0 != 0))
+        return fail(err, errlen, ESP_EINVAL, "tile %d: cached keys [%d, %d) and rows from %d on of a tree with %d cached keys do not meet", i, t.k0, k1, t.b0, P);
+    }
+  }
   if (mode & ESP_PASS_FUSED) {
     if (p->head_dim == 512 || p->rows_per_tile > 4 || family(p) <= 0)
       return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d at head_dim %d: the fused decode takes trees of 1 to 4 rows on the streaming kernel, head dim 128 or 256",
@@ -399,13 +435,13 @@ int esp_attn_validate_for(const esp_attn_params* p, int32_t mode, const esp_tile
         return fail(err, errlen, ESP_EINVAL, "tile %d: first row %d is not its tree's first row %d (a fused pass has one tile group per tree)", i,
                     tiles[i].r0, trees[tiles[i].tree].base);
   }
-  if (mode & ESP_PASS_ROWS_IN_POOL) {
+  if (mode & (ESP_PASS_ROWS_IN_POOL | ESP_PASS_DIFF)) {
     // Row j of a tree is read at position P + j of the tree's own block list (or ring).
     const int64_t bt = p->bt;
     for (int i = 0; i < n_trees; ++i) {
       const esp_tree& t = trees[i];
       if (t.M == 0) continue;
-      if (family(p) < 0 && (t.P - t.base) % 16)
+      if ((mode & ESP_PASS_ROWS_IN_POOL) && family(p) < 0 && (t.P - t.base) % 16)
         return fail(err, errlen, ESP_EINVAL, "tree %d: P %d - base %d is no multiple of 16: the tiled kernel reads a pass's rows from the pool in "
                     "16-token sub-blocks (pass Kb / Vb for this pass)", i, t.P, t.base);
       if (p->ring) {
@@ -631,6 +667,263 @@ int esp_attn_decode_fused(const esp_prep_params* pp, const esp_attn_params* p, c
                         reinterpret_cast<const int4*>(row_table), static_cast<uint16_t*>(kv_pool), *pp};
   return forward_impl(p, nullptr, nullptr, nullptr, kv_pool, blocks, desc, pos, O, tiles, n_tiles, trees, n_trees, jobs, n_jobs, n_parts,
                       n_rows, workspace, workspace_bytes, false, &a, stream, err, errlen);
+}
+
+// ---- differential attention ------------------------------------------------------
+int32_t esp_attn_diff_rows(const esp_attn_params* p, int32_t rows) {
+  if (check_diff(p, nullptr, 0) != ESP_OK || rows <= 0) return 0;
+  return esp::diff_rows(rows, p->H / p->Hkv);
+}
+
+int esp_attn_diff_hint(const esp_attn_params* p, int device, int32_t* workgroups, int32_t* groups_per_tile, char* err, size_t errlen) {
+  if (int rc = check_diff(p, err, errlen)) return rc;
+  const int fam = esp::diff_family(p->rows_per_tile, p->H / p->Hkv);
+  if (!workgroups || !groups_per_tile) return fail(err, errlen, ESP_EINVAL, "NULL output");
+  if (!fam) return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_attn_diff_rows)", p->rows_per_tile);
+  int cus = 0;
+  const hipError_t e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
+  if (e != hipSuccess) return hip_fail(err, errlen, "hipDeviceGetAttribute", e);
+  *workgroups = cus * esp::diff_workgroups_per_cu(fam);
+  *groups_per_tile = p->Hkv / 2;
+  return ESP_OK;
+}
+
+size_t esp_attn_diff_workspace_bytes(const esp_attn_params* p, int32_t n_parts) {
+  if (!p || p->Hkv <= 0 || p->H <= 0 || p->rows_per_tile <= 0) return 0;
+  return esp::carve_diff(p->H, p->rows_per_tile, n_parts).total;
+}
+
+int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void* Q, const void* kv_pool, const int32_t* blocks, void* O,
+                  const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees, int32_t n_trees, const esp_combine* jobs, int32_t n_jobs,
+                  int32_t n_parts, int32_t n_rows, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  if (int rc = check_diff(p, err, errlen)) return rc;
+  if (!d || !d->weight) return fail(err, errlen, ESP_EINVAL, "the pairs' weights must not be NULL");
+  if (d->norm_w && !(d->eps >= 0.0f)) return fail(err, errlen, ESP_EINVAL, "eps must not be negative");
+  if (n_tiles < 0 || n_trees < 0 || n_jobs < 0 || n_parts < 0 || n_rows < 0) return fail(err, errlen, ESP_EINVAL, "negative count");
+  if (n_tiles == 0) return ESP_OK;
+  if (!Q || !O || !tiles || !trees || !kv_pool) return fail(err, errlen, ESP_EINVAL, "Q, O, tiles, trees, kv_pool must not be NULL");
+  if (n_trees == 0 || n_rows == 0) return fail(err, errlen, ESP_EINVAL, "%d tiles without trees or rows", n_tiles);
+  if (!p->ring && !blocks) return fail(err, errlen, ESP_EINVAL, "blocks is NULL on a layer without rings");
+  if (n_jobs > 0 && !jobs) return fail(err, errlen, ESP_EINVAL, "jobs is NULL");
+  if ((n_jobs > 0) != (n_parts > 0)) return fail(err, errlen, ESP_EINVAL, "%d merge jobs with %d partial records", n_jobs, n_parts);
+  const int fam = esp::diff_family(p->rows_per_tile, p->H / p->Hkv);
+  if (!fam) return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_attn_diff_rows)", p->rows_per_tile);
+  if (n_tiles > 65535 || n_jobs > 65535) return fail(err, errlen, ESP_EUNSUPPORTED, "%d tiles, %d jobs in one pass: at most 65535", n_tiles, n_jobs);
+  const esp::DiffCarve c = esp::carve_diff(p->H, p->rows_per_tile, n_parts);
+  if (n_parts > 0 && (!workspace || workspace_bytes < c.total))
+    return fail(err, errlen, ESP_EWORKSPACE, "workspace %zu bytes, %zu needed", workspace ? workspace_bytes : size_t(0), c.total);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(err, errlen, ESP_EINVAL, "workspace must be 16-byte aligned");
+  DeviceState* dev = nullptr;
+  if (int rc = device_state(&dev, err, errlen)) return rc;
+  esp::DiffArgs a{};
+  a.Q = static_cast<const uint16_t*>(Q);
+  a.pool = static_cast<const uint16_t*>(kv_pool);
+  a.blocks = blocks;
+  a.O = static_cast<uint16_t*>(O);
+  a.tiles = tiles;
+  a.trees = trees;
+  a.parts_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + c.parts_o);
+  a.parts_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + c.parts_ml);
+  a.weight = d->weight;
+  a.norm_w = d->norm_w;
+  a.H = p->H;
+  a.Hkv = p->Hkv;
+  a.G = p->H / p->Hkv;
+  a.q_ld = p->q_ld;
+  a.bt = p->bt;
+  a.window = p->window;
+  a.ring = p->ring;
+  a.R = p->rows_per_tile;
+  a.cols = a.R * a.G;
+  a.scale_log2 = p->scale * esp::kLog2e;
+  a.eps = d->eps;
+  a.factor = d->factor;
+  a.kv_base = p->kv_base;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e = esp::launch_diff_stream(p->dtype, a, n_tiles, st);
+  if (e != hipSuccess) return hip_fail(err, errlen, "attn_diff launch", e);
+  if (n_jobs > 0) {
+    e = esp::launch_diff_merge(p->dtype, a, jobs, n_jobs, st);
+    if (e != hipSuccess) return hip_fail(err, errlen, "attn_diff_merge launch", e);
+  }
+  return ESP_OK;
+}
+
+// ---- low-rank adapters -------------------------------------------------------------
+static int check_lowrank(const esp_lowrank_params* p, char* err, size_t errlen) {
+  if (!p) return fail(err, errlen, ESP_EINVAL, "params is NULL");
+  if (p->dtype != ESP_F16 && p->dtype != ESP_BF16) return fail(err, errlen, ESP_EINVAL, "dtype %d", p->dtype);
+  if (p->D <= 0 || p->D % 8) return fail(err, errlen, ESP_EINVAL, "D %d: a positive multiple of 8", p->D);
+  if (p->rank <= 0 || p->rank % 8 || p->rank > esp::kLowRankMost)
+    return fail(err, errlen, ESP_EINVAL, "rank %d: a positive multiple of 8, at most %d", p->rank, esp::kLowRankMost);
+  if (p->n_slices < 1 || p->n_slices > ESP_LOWRANK_SLICES) return fail(err, errlen, ESP_EINVAL, "n_slices %d (1 to %d)", p->n_slices, int(ESP_LOWRANK_SLICES));
+  if (p->n_adapters <= 0) return fail(err, errlen, ESP_EINVAL, "n_adapters %d", p->n_adapters);
+  if (p->x_ld < p->D || p->x_ld % 8) return fail(err, errlen, ESP_EINVAL, "x_ld %d", p->x_ld);
+  int64_t blocks = 0, out = 0;
+  for (int s = 0; s < p->n_slices; ++s) {
+    if (p->width[s] <= 0 || p->y_off[s] < 0 || int64_t(p->y_off[s]) + p->width[s] > p->y_ld)
+      return fail(err, errlen, ESP_EINVAL, "slice %d: columns [%d, %d + %d) of a row of %d", s, p->y_off[s], p->y_off[s], p->width[s], p->y_ld);
+    for (int q = 0; q < s; ++q)
+      if (p->y_off[s] < p->y_off[q] + p->width[q] && p->y_off[q] < p->y_off[s] + p->width[s])
+        return fail(err, errlen, ESP_EINVAL, "slices %d and %d overlap", q, s);
+    blocks += (p->width[s] + 255) / 256;
+    out += p->width[s];
+  }
+  if (blocks > 65535 || out > INT32_MAX) return fail(err, errlen, ESP_EUNSUPPORTED, "%lld columns in the slices", (long long)out);
+  return ESP_OK;
+}
+
+int32_t esp_lowrank_rows(const esp_lowrank_params* p, int32_t n_rows) {
+  if (check_lowrank(p, nullptr, 0) != ESP_OK || n_rows <= 0) return 0;
+  return esp::lowrank_rows(n_rows);
+}
+
+size_t esp_lowrank_workspace_bytes(const esp_lowrank_params* p, int32_t n_tiles, int32_t n_slots) {
+  if (check_lowrank(p, nullptr, 0) != ESP_OK || n_tiles <= 0 || n_slots <= 0) return 0;
+  return esp::lowrank_workspace(*p, n_tiles, n_slots);
+}
+
+int esp_lowrank_add(const esp_lowrank_params* p, const void* X, const void* A, const void* B, const float* scale, float* Y, const int32_t* order,
+                    int32_t n_slots, const esp_lowrank_tile* tiles, int32_t n_tiles, void* workspace, size_t workspace_bytes, void* stream,
+                    char* err, size_t errlen) {
+  if (int rc = check_lowrank(p, err, errlen)) return rc;
+  if (n_slots < 0 || n_tiles < 0) return fail(err, errlen, ESP_EINVAL, "negative count");
+  if (p->rows_per_tile != 16) return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_lowrank_rows)", p->rows_per_tile);
+  if (n_tiles == 0) return ESP_OK;
+  if (n_slots == 0) return fail(err, errlen, ESP_EINVAL, "%d tiles without rows", n_tiles);
+  if (!X || !A || !B || !scale || !Y || !order || !tiles) return fail(err, errlen, ESP_EINVAL, "X, A, B, scale, Y, order, tiles must not be NULL");
+  if ((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(workspace)) % 16)
+    return fail(err, errlen, ESP_EINVAL, "X, A, B and the workspace must be 16-byte aligned");
+  const size_t need = esp::lowrank_workspace(*p, n_tiles, n_slots);
+  if (!workspace || workspace_bytes < need) return fail(err, errlen, ESP_EWORKSPACE, "workspace %zu bytes, %zu needed", workspace ? workspace_bytes : size_t(0), need);
+  esp::LowRankArgs a{};
+  a.X = static_cast<const uint16_t*>(X);
+  a.A = static_cast<const uint16_t*>(A);
+  a.B = static_cast<const uint16_t*>(B);
+  a.scale = scale;
+  a.Y = Y;
+  a.order = order;
+  a.tiles = tiles;
+  a.low = static_cast<float*>(workspace);
+  a.D = p->D;
+  a.rank = p->rank;
+  a.n_slices = p->n_slices;
+  a.n_low = p->n_slices * p->rank;
+  a.x_ld = p->x_ld;
+  a.y_ld = p->y_ld;
+  a.n_slots = n_slots;
+  a.splits = esp::lowrank_splits(p->D, n_tiles);
+  a.chunk = esp::lowrank_chunk(p->D, a.splits);
+  for (int s = 0; s < p->n_slices; ++s) {
+    a.y_off[s] = p->y_off[s];
+    a.width[s] = p->width[s];
+    a.n_out += p->width[s];
+  }
+  const hipError_t e = esp::launch_lowrank(p->dtype, a, n_tiles, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? ESP_OK : hip_fail(err, errlen, "lowrank launch", e);
+}
+
+// ---- logits ------------------------------------------------------------------------
+static int check_logits(const esp_logits_params* p, char* err, size_t errlen) {
+  if (!p) return fail(err, errlen, ESP_EINVAL, "params is NULL");
+  if (p->dtype != ESP_F16 && p->dtype != ESP_BF16 && p->dtype != ESP_F32) return fail(err, errlen, ESP_EINVAL, "dtype %d", p->dtype);
+  if (p->vocab <= 0 || p->vocab > INT32_MAX - 65536) return fail(err, errlen, ESP_EINVAL, "vocab %d", p->vocab);
+  if (p->n_slots < 0 || p->n_masks < 0 || p->n_bias < 0) return fail(err, errlen, ESP_EINVAL, "negative count");
+  return ESP_OK;
+}
+
+size_t esp_logits_workspace_bytes(const esp_logits_params* p, int32_t n_rows) {
+  if (check_logits(p, nullptr, 0) != ESP_OK || n_rows <= 0) return 0;
+  return esp::logits_workspace(p->vocab, n_rows);
+}
+
+int esp_logits_process(const esp_logits_params* p, const void* logits, float* out, int32_t* tokens, const esp_logits_row* rows, int32_t n_rows,
+                       const int32_t* bias_tokens, const float* bias_values, const uint32_t* masks, uint32_t* seen, int32_t* counts,
+                       int32_t record, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  if (int rc = check_logits(p, err, errlen)) return rc;
+  if (n_rows < 0 || n_rows > 65535) return fail(err, errlen, ESP_EINVAL, "%d rows (at most 65535)", n_rows);
+  if (n_rows == 0) return ESP_OK;
+  if (!logits || !rows || (!out && !tokens)) return fail(err, errlen, ESP_EINVAL, "logits, rows and one of out and tokens must not be NULL");
+  if (p->in_ld < p->vocab) return fail(err, errlen, ESP_EINVAL, "in_ld %d of a vocabulary of %d", p->in_ld, p->vocab);
+  if (out && p->out_ld < p->vocab) return fail(err, errlen, ESP_EINVAL, "out_ld %d of a vocabulary of %d", p->out_ld, p->vocab);
+  if (out == logits && (p->dtype != ESP_F32 || p->in_ld != p->out_ld)) return fail(err, errlen, ESP_EINVAL, "out may be the logits only where both are fp32 rows of one stride");
+  if (record != 0 && record != 1) return fail(err, errlen, ESP_EINVAL, "record %d (0 or 1)", record);
+  if (record && (!tokens || !p->n_slots)) return fail(err, errlen, ESP_EINVAL, "record without tokens or without slots");
+  if (p->n_slots && (!seen || !counts)) return fail(err, errlen, ESP_EINVAL, "%d slots without histories", p->n_slots);
+  if (p->n_masks && !masks) return fail(err, errlen, ESP_EINVAL, "masks is NULL");
+  if (p->n_bias && (!bias_tokens || !bias_values)) return fail(err, errlen, ESP_EINVAL, "bias_tokens or bias_values is NULL");
+  const size_t need = esp::logits_workspace(p->vocab, n_rows);
+  if (!workspace || workspace_bytes < need) return fail(err, errlen, ESP_EWORKSPACE, "workspace %zu bytes, %zu needed", workspace ? workspace_bytes : size_t(0), need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 4) return fail(err, errlen, ESP_EINVAL, "workspace must be 4-byte aligned");
+  esp::LogitsArgs a{};
+  a.logits = logits;
+  a.out = out;
+  a.tokens = tokens;
+  a.rows = rows;
+  a.bias_tokens = bias_tokens;
+  a.bias_values = bias_values;
+  a.masks = masks;
+  a.seen = seen;
+  a.counts = counts;
+  a.part_v = static_cast<float*>(workspace);
+  a.part_t = static_cast<int32_t*>(workspace) + size_t(esp::logits_chunks(p->vocab)) * size_t(n_rows);
+  a.vocab = p->vocab;
+  a.words = esp::logits_words(p->vocab);
+  a.in_ld = p->in_ld;
+  a.out_ld = p->out_ld;
+  a.n_slots = p->n_slots;
+  a.n_masks = p->n_masks;
+  a.n_bias = p->n_bias;
+  a.record = record;
+  const hipError_t e = esp::launch_logits(p->dtype, a, n_rows, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? ESP_OK : hip_fail(err, errlen, "logits launch", e);
+}
+
+int esp_logits_validate(const esp_logits_params* p, const esp_logits_row* rows, int32_t n_rows, const int32_t* bias_tokens, char* err,
+                        size_t errlen) {
+  if (int rc = check_logits(p, err, errlen)) return rc;
+  if (n_rows < 0 || (n_rows && !rows) || (p->n_bias && !bias_tokens)) return fail(err, errlen, ESP_EINVAL, "rows or bias_tokens is NULL");
+  for (int i = 0; i < n_rows; ++i) {
+    const esp_logits_row& r = rows[i];
+    if (r.slot < -1 || r.slot >= p->n_slots) return fail(err, errlen, ESP_EINVAL, "row %d: slot %d of %d", i, r.slot, p->n_slots);
+    if (r.mask < -1 || r.mask >= p->n_masks) return fail(err, errlen, ESP_EINVAL, "row %d: mask %d of %d", i, r.mask, p->n_masks);
+    if (!(r.repetition > 0.0f) || !std::isfinite(r.repetition) || !std::isfinite(r.frequency) || !std::isfinite(r.presence))
+      return fail(err, errlen, ESP_EINVAL, "row %d: penalties %g, %g, %g", i, r.repetition, r.frequency, r.presence);
+    if (r.n_bias < 0 || (r.n_bias && (r.bias0 < 0 || int64_t(r.bias0) + r.n_bias > p->n_bias)))
+      return fail(err, errlen, ESP_EINVAL, "row %d: bias entries [%d, %d + %d) of %d", i, r.bias0, r.bias0, r.n_bias, p->n_bias);
+    for (int32_t e = 0; e < r.n_bias; ++e) {
+      const int32_t t = bias_tokens[r.bias0 + e];
+      if (t < 0 || t >= p->vocab || (e && t <= bias_tokens[r.bias0 + e - 1]))
+        return fail(err, errlen, ESP_EINVAL, "row %d: token %d at bias entry %d: in [0, %d), ascending, none twice", i, t, e, p->vocab);
+    }
+  }
+  return ESP_OK;
+}
+
+static int check_history(const esp_logits_params* p, const uint32_t* seen, const int32_t* counts, const int32_t* slots, int32_t n, char* err, size_t errlen) {
+  if (int rc = check_logits(p, err, errlen)) return rc;
+  if (n < 0) return fail(err, errlen, ESP_EINVAL, "negative count");
+  if (n && (!seen || !counts || !slots)) return fail(err, errlen, ESP_EINVAL, "seen, counts and slots must not be NULL");
+  return ESP_OK;
+}
+
+int esp_history_record(const esp_logits_params* p, uint32_t* seen, int32_t* counts, const int32_t* tokens, const int32_t* slots, int32_t n,
+                       int32_t given, void* stream, char* err, size_t errlen) {
+  if (int rc = check_history(p, seen, counts, slots, n, err, errlen)) return rc;
+  if (given != 0 && given != 1) return fail(err, errlen, ESP_EINVAL, "given %d (0 or 1)", given);
+  if (n == 0) return ESP_OK;
+  if (!tokens) return fail(err, errlen, ESP_EINVAL, "tokens is NULL");
+  const hipError_t e = esp::launch_history_record(p, seen, counts, tokens, slots, n, given, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? ESP_OK : hip_fail(err, errlen, "history_record launch", e);
+}
+
+int esp_history_clear(const esp_logits_params* p, uint32_t* seen, int32_t* counts, const int32_t* slots, int32_t n, void* stream, char* err,
+                      size_t errlen) {
+  if (int rc = check_history(p, seen, counts, slots, n, err, errlen)) return rc;
+  if (n > 65535) return fail(err, errlen, ESP_EINVAL, "%d slots (at most 65535)", n);
+  if (n == 0) return ESP_OK;
+  const hipError_t e = esp::launch_history_clear(p, seen, counts, slots, n, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? ESP_OK : hip_fail(err, errlen, "history_clear launch", e);
 }
 
 }  // extern "C"

@@ -1,6 +1,6 @@
 // CPython entry points of the calls a decode loop makes per layer and step (include/espetero_attn.h), arguments in the
 // header's order without the error buffer: records as instances of their own ctypes classes (abi.AttnParams, PrepParams,
-// GateParams), device memory as torch tensors or None, the stream as an integer. Anything else is refused before the library
+// GateParams, DiffParams, LowRankParams, LogitsParams), device memory as torch tensors or None, the stream as an integer. Anything else is refused before the library
 // is called: it would read another record's bytes, or a number, as an address. A failing call raises abi.EspError.
 //
 // Why native: a decode step of one short sequence is 8 us of GPU work behind two launches, and the ctypes form of the
@@ -22,7 +22,7 @@ namespace {
 PyObject* g_data_ptr;  // interned "data_ptr"
 PyObject* g_error;     // abi.EspError
 // abi's classes of the parameter records
-PyTypeObject *g_attn_params, *g_prep_params, *g_gate_params;
+PyTypeObject *g_attn_params, *g_prep_params, *g_gate_params, *g_diff_params, *g_lowrank_params, *g_logits_params;
 
 // A structure's bytes, held until the call has returned.
 struct Record {
@@ -50,12 +50,16 @@ PyTypeObject* record_class() {
   if constexpr (std::is_same_v<T, const esp_attn_params*>) return g_attn_params;
   else if constexpr (std::is_same_v<T, const esp_prep_params*>) return g_prep_params;
   else if constexpr (std::is_same_v<T, const esp_gate_params*>) return g_gate_params;
+  else if constexpr (std::is_same_v<T, const esp_diff_params*>) return g_diff_params;
+  else if constexpr (std::is_same_v<T, const esp_lowrank_params*>) return g_lowrank_params;
+  else if constexpr (std::is_same_v<T, const esp_logits_params*>) return g_logits_params;
   else return nullptr;
 }
 
 template <typename T>
 constexpr bool is_params = std::is_same_v<T, const esp_attn_params*> || std::is_same_v<T, const esp_prep_params*> ||
-                           std::is_same_v<T, const esp_gate_params*>;
+                           std::is_same_v<T, const esp_gate_params*> || std::is_same_v<T, const esp_diff_params*> ||
+                           std::is_same_v<T, const esp_lowrank_params*> || std::is_same_v<T, const esp_logits_params*>;
 
 // stream: the call's last argument, a hipStream_t as an integer.
 template <bool stream, typename T>
@@ -127,7 +131,9 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define ESP_CALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<esp_##name>)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {ESP_CALL(attn_forward),   ESP_CALL(attn_forward_static), ESP_CALL(attn_decode_fused), ESP_CALL(attn_prep),
                            ESP_CALL(attn_combine),   ESP_CALL(head_gate),           ESP_CALL(kv_save),           ESP_CALL(kv_copy_blocks),
-                           ESP_CALL(kv_export_blocks), ESP_CALL(kv_import_blocks),  ESP_CALL(chain_advance),     {nullptr, nullptr, 0, nullptr}};
+                           ESP_CALL(kv_export_blocks), ESP_CALL(kv_import_blocks),  ESP_CALL(chain_advance),
+                           ESP_CALL(attn_diff),      ESP_CALL(lowrank_add),         ESP_CALL(logits_process),    ESP_CALL(history_record),
+                           ESP_CALL(history_clear),  {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
@@ -139,10 +145,13 @@ PyMODINIT_FUNC PyInit__calls() {
   g_attn_params = reinterpret_cast<PyTypeObject*>(PyObject_GetAttrString(abi, "AttnParams"));
   g_prep_params = reinterpret_cast<PyTypeObject*>(PyObject_GetAttrString(abi, "PrepParams"));
   g_gate_params = reinterpret_cast<PyTypeObject*>(PyObject_GetAttrString(abi, "GateParams"));
+  g_diff_params = reinterpret_cast<PyTypeObject*>(PyObject_GetAttrString(abi, "DiffParams"));
+  g_lowrank_params = reinterpret_cast<PyTypeObject*>(PyObject_GetAttrString(abi, "LowRankParams"));
+  g_logits_params = reinterpret_cast<PyTypeObject*>(PyObject_GetAttrString(abi, "LogitsParams"));
   PyObject* version = PyObject_GetAttrString(abi, "ESP_ABI_VERSION");
   Py_DECREF(abi);
   g_data_ptr = PyUnicode_InternFromString("data_ptr");
-  if (!g_error || !g_attn_params || !g_prep_params || !g_gate_params || !version || !g_data_ptr) {
+  if (!g_error || !g_attn_params || !g_prep_params || !g_gate_params || !g_diff_params || !g_lowrank_params || !g_logits_params || !version || !g_data_ptr) {
     Py_XDECREF(version);
     return nullptr;
   }

@@ -52,4 +52,23 @@ constexpr Carve carve_workspace(int H, int Hkv, int head_dim, int rows_per_tile,
   return c;
 }
 
+// Differential attention, G query pairs per KV pair: 1, the streaming kernel, which takes up to 16 packed rows; 0, no kernel.
+constexpr int diff_family(int rows_per_tile, int G) { return rows_per_tile > 0 && G > 0 && rows_per_tile * G <= 16 ? 1 : 0; }
+// Rows per tile for trees of at most `rows` rows; 0: no kernel.
+constexpr int diff_rows(int rows, int G) { return G > 16 ? 0 : rows * G <= 16 ? rows : 16 / G; }
+constexpr int diff_workgroups_per_cu(int) { return 1; }
+
+// Its partial records: both maps of every packed row.
+struct DiffCarve {
+  size_t parts_o, parts_ml, total;
+};
+constexpr DiffCarve carve_diff(int H, int rows_per_tile, int64_t n_parts) {
+  const size_t recs = size_t(n_parts > 0 ? n_parts : 0) * size_t(H) * size_t(rows_per_tile);
+  DiffCarve c{};
+  c.parts_o = 0;
+  c.parts_ml = (recs * 256 * sizeof(float) + 255) & ~size_t(255);
+  c.total = c.parts_ml + recs * 2 * sizeof(float);
+  return c;
+}
+
 }  // namespace esp

@@ -9,7 +9,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from . import abi
+from . import abi, host
 
 try:
     from . import _calls  # the per-step calls, csrc/calls.cpp
@@ -77,17 +77,18 @@ def forward_static(params, Q, Kb, Vb, pool, blocks, desc, pos, O, tiles, n_tiles
                                _stream(stream))
 
 
-def validate(params, tiles, trees, jobs, n_parts, n_rows, blocks, pool_blocks, fused=False, rows_in_pool=False):
+def validate(params, tiles, trees, jobs, n_parts, n_rows, blocks, pool_blocks, fused=False, rows_in_pool=False, diff=False):
     """Host-side bounds check of a pass's records (numpy arrays) before they are uploaded. Raises EspError.
     fused: the pass goes to esp_attn_decode_fused (also: one tile group per tree, trees of at most rows_per_tile rows).
-    rows_in_pool: the pass runs without Kb / Vb (also: block lists that reach P + M, P - base a multiple of 16 on the tiled kernel)."""
+    rows_in_pool: the pass runs without Kb / Vb (also: block lists that reach P + M, P - base a multiple of 16 on the tiled kernel).
+    diff: the pass goes to esp_attn_diff (also: block lists that reach P + M)."""
     tiles = np.ascontiguousarray(tiles, dtype=abi.TILE_DT)
     trees = np.ascontiguousarray(trees, dtype=abi.TREE_DT)
     jobs = np.ascontiguousarray(jobs, dtype=abi.COMBINE_DT)
     blocks = None if blocks is None else np.ascontiguousarray(blocks, dtype=np.int32)
     hp = lambda a: None if a is None or a.size == 0 else a.ctypes.data  # noqa: E731
     err = C.create_string_buffer(_ERRLEN)
-    mode = (abi.ESP_PASS_FUSED if fused else 0) | (abi.ESP_PASS_ROWS_IN_POOL if rows_in_pool else 0)
+    mode = (abi.ESP_PASS_FUSED if fused else 0) | (abi.ESP_PASS_ROWS_IN_POOL if rows_in_pool else 0) | (abi.ESP_PASS_DIFF if diff else 0)
     rc = abi.attn_lib().esp_attn_validate_for(C.byref(params), mode, hp(tiles), len(tiles), hp(trees), len(trees), hp(jobs), len(jobs),
                                               n_parts, n_rows, hp(blocks), 0 if blocks is None else len(blocks), pool_blocks, err, _ERRLEN)
     abi.check(rc, err)
@@ -194,3 +195,121 @@ class DevicePass:
     def merge(self, O, stream=None):
         if self.n_jobs:
             combine(self.params, O, self.jobs, self.n_jobs, self.n_parts, self.n_rows, self.workspace, stream)
+
+
+def diff_params(weight, norm_w, eps, factor):
+    """weight fp32 [H / 2], norm_w fp32 [2 * head_dim] or None: device tensors, kept alive by the record."""
+    d = abi.DiffParams(_ptr(weight), _ptr(norm_w), eps, factor)
+    d._keep = (weight, norm_w)
+    return d
+
+
+def attn_diff_rows(params, rows):
+    """rows_per_tile to plan a pass of differential attention with whose trees have at most `rows` rows."""
+    r = abi.attn_lib().esp_attn_diff_rows(C.byref(params), rows)
+    if r <= 0:
+        raise abi.EspError("parameters or rows that esp_attn_diff does not serve")
+    return r
+
+
+def attn_diff_hint(params, device=0):
+    """(workgroups resident at once, workgroups per tile) of the differential attention kernel serving `params`."""
+    err = C.create_string_buffer(_ERRLEN)
+    n, g = C.c_int32(0), C.c_int32(0)
+    abi.check(abi.attn_lib().esp_attn_diff_hint(C.byref(params), device, C.byref(n), C.byref(g), err, _ERRLEN), err)
+    return n.value, g.value
+
+
+class DiffPass:
+    """One planned pass of differential attention resident on the device (the rows of the pass are in the pool when it runs)."""
+
+    def __init__(self, params, diff, trees, tiles, jobs, n_parts, n_rows, blocks, device="cuda", pool_blocks=None):
+        """pool_blocks: blocks in the pool; when given, the records are checked on the host before the upload."""
+        if pool_blocks is not None:
+            validate(params, tiles, trees, jobs, n_parts, n_rows, blocks, pool_blocks, diff=True)
+        self.params, self.diff = params, diff
+        self.n_trees, self.n_tiles, self.n_jobs = len(trees), len(tiles), len(jobs)
+        self.n_parts, self.n_rows = n_parts, n_rows
+        self.trees = to_dev(np.ascontiguousarray(trees, dtype=abi.TREE_DT), device)
+        self.tiles = to_dev(np.ascontiguousarray(tiles, dtype=abi.TILE_DT), device)
+        self.jobs = to_dev(np.ascontiguousarray(jobs, dtype=abi.COMBINE_DT), device) if len(jobs) else None
+        self.blocks = to_dev(np.ascontiguousarray(blocks, dtype=np.int32), device) if blocks is not None else None
+        nbytes = abi.attn_lib().esp_attn_diff_workspace_bytes(C.byref(params), n_parts)
+        self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+    def run(self, Q, pool, O, stream=None):
+        ws = self.workspace
+        _calls.attn_diff(self.params, self.diff, Q, pool, self.blocks, O, self.tiles, self.n_tiles, self.trees, self.n_trees, self.jobs, self.n_jobs,
+                         self.n_parts, self.n_rows, ws, ws.nbytes, _stream(stream))
+
+
+def lowrank_params(D, rank, slices, dtype, x_ld, y_ld, n_adapters):
+    """slices: (first column, columns) of each part of the projection that the adapters add to."""
+    if not 1 <= len(slices) <= abi.ESP_LOWRANK_SLICES:
+        raise abi.EspError(f"{len(slices)} slices (1 to {abi.ESP_LOWRANK_SLICES})")
+    p = abi.LowRankParams(D, rank, len(slices), dtype, x_ld, y_ld, n_adapters, 0)
+    for i, (off, width) in enumerate(slices):
+        p.y_off[i], p.width[i] = off, width
+    return p
+
+
+class LowRankPass:
+    """Which rows of a pass take which adapter, planned and resident on the device."""
+
+    def __init__(self, params, adapter, device="cuda"):
+        """adapter: int32 per row, -1 for a row without one. Sets params.rows_per_tile."""
+        lib = abi.attn_lib()
+        n_rows = len(adapter)
+        params.rows_per_tile = lib.esp_lowrank_rows(C.byref(params), max(n_rows, 1))
+        if params.rows_per_tile <= 0:
+            raise abi.EspError("parameters that esp_lowrank_add does not serve")
+        self.params = params
+        order, tiles = host.plan_lowrank(params, adapter)
+        self.n_slots, self.n_tiles = len(order), len(tiles)
+        self.order = to_dev(order, device) if self.n_slots else None
+        self.tiles = to_dev(tiles, device) if self.n_tiles else None
+        nbytes = lib.esp_lowrank_workspace_bytes(C.byref(params), self.n_tiles, self.n_slots)
+        self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+    def run(self, X, A, B, scale, Y, stream=None):
+        """Y += the adapters' products, in place."""
+        ws = self.workspace
+        _calls.lowrank_add(self.params, X, A, B, scale, Y, self.order, self.n_slots, self.tiles, self.n_tiles, ws, ws.nbytes, _stream(stream))
+
+
+def logits_params(vocab, dtype, n_slots, n_masks=0, n_bias=0, in_ld=None, out_ld=None):
+    return abi.LogitsParams(vocab, dtype, in_ld or vocab, out_ld or vocab, n_slots, n_masks, n_bias, 0)
+
+
+class LogitsPass:
+    """The records of the rows of a decode batch, resident on the device."""
+
+    def __init__(self, params, rows, bias_tokens=None, device="cuda"):
+        """rows: LOGITS_ROW_DT. bias_tokens: the host's copy of the bias entries' tokens; when given, records and entries are checked
+        before the upload."""
+        rows = np.ascontiguousarray(rows, dtype=abi.LOGITS_ROW_DT)
+        lib = abi.attn_lib()
+        if bias_tokens is not None:
+            bias_tokens = np.ascontiguousarray(bias_tokens, dtype=np.int32)
+            if len(bias_tokens) < params.n_bias:
+                raise abi.EspError(f"{len(bias_tokens)} bias entries, {params.n_bias} named")
+            err = C.create_string_buffer(_ERRLEN)
+            abi.check(lib.esp_logits_validate(C.byref(params), rows.ctypes.data, len(rows), bias_tokens.ctypes.data, err, _ERRLEN), err)
+        self.params, self.n_rows = params, len(rows)
+        self.rows = to_dev(rows, device) if len(rows) else None
+        nbytes = lib.esp_logits_workspace_bytes(C.byref(params), self.n_rows)
+        self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+    def run(self, logits, out, tokens, bias_tokens, bias_values, masks, seen, counts, record=False, stream=None):
+        """Device tensors; out or tokens may be None, and so may what no row names. record: the tokens join their slots' histories."""
+        ws = self.workspace
+        _calls.logits_process(self.params, logits, out, tokens, self.rows, self.n_rows, bias_tokens, bias_values, masks, seen, counts, int(record), ws,
+                              ws.nbytes, _stream(stream))
+
+
+def history_record(params, seen, counts, tokens, slots, n, given, stream=None):
+    _calls.history_record(params, seen, counts, tokens, slots, n, int(given), _stream(stream))
+
+
+def history_clear(params, seen, counts, slots, n, stream=None):
+    _calls.history_clear(params, seen, counts, slots, n, _stream(stream))

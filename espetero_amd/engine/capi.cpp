@@ -98,6 +98,28 @@ int esp_plan_tiles_for(const esp_attn_params* p, const esp_tree* trees, int32_t 
   }
 }
 
+int esp_plan_lowrank(const esp_lowrank_params* p, const int32_t* adapter, int32_t n_rows, int32_t* order, int32_t* n_slots, esp_lowrank_tile* tiles,
+                     int32_t tiles_cap, int32_t* n_tiles, char* err, size_t errlen) {
+  if (!p || !n_slots || !n_tiles || (n_rows > 0 && (!adapter || !order))) return put_err(err, errlen, ESP_EINVAL, "NULL argument");
+  if (n_rows < 0 || tiles_cap < 0 || p->rows_per_tile <= 0 || p->n_adapters <= 0) return put_err(err, errlen, ESP_EINVAL, "counts / rows_per_tile / n_adapters");
+  try {
+    LowRankPlan plan;
+    if (const int bad = plan_lowrank(plan, adapter, n_rows, p->n_adapters, p->rows_per_tile); bad >= 0) {
+      char msg[96];
+      snprintf(msg, sizeof msg, "row %d: adapter %d of %d", bad, adapter[bad], p->n_adapters);
+      return put_err(err, errlen, ESP_EINVAL, msg);
+    }
+    *n_slots = int32_t(plan.order.size());
+    *n_tiles = int32_t(plan.tiles.size());
+    if (*n_tiles > tiles_cap || (!tiles && *n_tiles > 0)) return put_err(err, errlen, ESP_EWORKSPACE, "tiles capacity too small");
+    if (!plan.order.empty()) memcpy(order, plan.order.data(), plan.order.size() * sizeof(int32_t));
+    if (!plan.tiles.empty()) memcpy(tiles, plan.tiles.data(), plan.tiles.size() * sizeof(esp_lowrank_tile));
+    return ESP_OK;
+  } catch (const std::exception& e) {
+    return put_err(err, errlen, ESP_EINVAL, e.what());
+  }
+}
+
 esp_engine* esp_engine_create(int32_t n_blocks, int32_t bt, int32_t n_slots, int32_t max_ctx) {
   try {
     return new esp_engine(n_blocks, bt, n_slots, max_ctx);

@@ -641,4 +641,29 @@ inline void plan_tiles(AttnPlan& A, int groups, int window, const int32_t* pos, 
   }
 }
 
+// Rows grouped by their adapter, in tiles of at most rows_per_tile: which tiles esp_lowrank_add runs.
+struct LowRankPlan {
+  std::vector<int32_t> order;  // row numbers, slot by slot
+  std::vector<esp_lowrank_tile> tiles;
+};
+
+// The first row whose adapter does not exist, or -1: planned.
+inline int plan_lowrank(LowRankPlan& plan, const int32_t* adapter, int n_rows, int n_adapters, int rows_per_tile) {
+  plan.order.clear();
+  plan.tiles.clear();
+  std::vector<int> first(size_t(n_adapters) + 1, 0);
+  for (int r = 0; r < n_rows; ++r) {
+    if (adapter[r] < -1 || adapter[r] >= n_adapters) return r;
+    if (adapter[r] >= 0) ++first[size_t(adapter[r]) + 1];
+  }
+  for (int a = 0; a < n_adapters; ++a) first[size_t(a) + 1] += first[size_t(a)];
+  plan.order.resize(size_t(first[size_t(n_adapters)]));
+  for (int a = 0; a < n_adapters; ++a)
+    for (int at = first[size_t(a)]; at < first[size_t(a) + 1]; at += rows_per_tile)
+      plan.tiles.push_back({a, at, std::min(rows_per_tile, first[size_t(a) + 1] - at), 0});
+  for (int r = 0; r < n_rows; ++r)
+    if (adapter[r] >= 0) plan.order[size_t(first[size_t(adapter[r])]++)] = r;
+  return -1;
+}
+
 }  // namespace espetero::engine

@@ -32,6 +32,7 @@ ENGINE_SYMBOLS = {
     "esp_plan_options_mi355x": (None, (_PO, _I, _I)),
     "esp_plan_tiles": (C.c_int, (_V, _I, _I, _I, _V, _PO, _V, _I, _IP, _V, _I, _IP, _IP) + _ERR),
     "esp_plan_tiles_for": (C.c_int, (_AP, _V, _I, _I, _I, _V, _PO, _V, _I, _IP, _V, _I, _IP, _IP) + _ERR),
+    "esp_plan_lowrank": (C.c_int, (C.POINTER(abi.LowRankParams), _V, _I, _V, _IP, _V, _I, _IP) + _ERR),
     "esp_engine_create": (_V, (_I, _I, _I, _I)),
     "esp_engine_destroy": (None, (_V,)),
     "esp_engine_slot_alloc": (C.c_int, (_V,)),
@@ -127,6 +128,18 @@ def plan_tiles(trees, groups, window, pos, options):
         n_tiles, n_jobs = max(n_tiles, nt.value), max(n_jobs, nj.value)
     abi.check(rc, err)
     return tiles[:nt.value].copy(), jobs[:nj.value].copy(), npart.value
+
+
+def plan_lowrank(params, adapter):
+    """adapter: int32 per row, -1 for none. Returns (order int32, tiles LOWRANK_TILE_DT) of the rows that have one."""
+    adapter = np.ascontiguousarray(adapter, dtype=np.int32)
+    n = len(adapter)
+    order, tiles = np.empty(max(n, 1), np.int32), np.empty(max(n, 1), abi.LOWRANK_TILE_DT)
+    slots, nt = C.c_int32(0), C.c_int32(0)
+    err = C.create_string_buffer(256)
+    abi.check(engine_lib().esp_plan_lowrank(C.byref(params), adapter.ctypes.data, n, order.ctypes.data, C.byref(slots), tiles.ctypes.data, len(tiles),
+                                            C.byref(nt), err, 256), err)
+    return order[:slots.value].copy(), tiles[:nt.value].copy()
 
 
 def slot_file_save(path, length, next_pos, n_layers, blocks_kv):

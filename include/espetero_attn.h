@@ -205,9 +205,11 @@ int esp_attn_validate(const esp_attn_params* p, const esp_tile* tiles, int32_t n
  *                          starting at its tree's first row, i.e. one tile group per tree;
  *   ESP_PASS_ROWS_IN_POOL  the pass goes to esp_attn_forward without Kb / Vb: row j of every tree is read at position
  *                          P + j of the tree's own block list, which must reach that far; on the tiled kernel P - base
- *                          is a multiple of 16; on ring layers a tree's rows must not overwrite keys its first rows see.
+ *                          is a multiple of 16; on ring layers a tree's rows must not overwrite keys its first rows see;
+ *   ESP_PASS_DIFF          the pass goes to esp_attn_diff: rows in the pool as above (any P - base), a tile that has both
+ *                          cached keys and rows of the pass has the former up to P and the latter from row 0 on.
  * Same arguments as esp_attn_validate otherwise. Host pointers; touches no device. */
-enum { ESP_PASS_FUSED = 1, ESP_PASS_ROWS_IN_POOL = 2 };
+enum { ESP_PASS_FUSED = 1, ESP_PASS_ROWS_IN_POOL = 2, ESP_PASS_DIFF = 4 };
 int esp_attn_validate_for(const esp_attn_params* p, int32_t mode, const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees,
                           int32_t n_trees, const esp_combine* jobs, int32_t n_jobs, int32_t n_parts, int32_t n_rows, const int32_t* blocks,
                           int32_t n_block_entries, int32_t pool_blocks, char* err, size_t errlen);
@@ -371,6 +373,127 @@ typedef struct esp_gate_params {
 
 int esp_head_gate(const esp_gate_params* p, void* O, const void* X, const void* Wg, float* dots, int32_t n_rows,
                   void* stream, char* err, size_t errlen);
+
+/* ---- differential attention over the paged pool ------------------------------------
+ * No counterpart in the reference. Heads work in pairs: query heads 2 i and 2 i + 1 over KV heads 2 j and 2 j + 1,
+ * j = i / (H / Hkv). Head 2 i scores the keys of KV head 2 j, head 2 i + 1 those of 2 j + 1; both softmax maps weigh
+ * the same values of 2 * head_dim dims, the two KV heads' V side by side; the second map's output is taken off the
+ * first's with a learned weight per pair, the pair's 2 * head_dim outputs are normalised (RMS, norm_w, eps) and
+ * multiplied by factor:
+ *   O[row, i] = factor * norm( softmax(scale q1 K1^T) V - weight[i] * softmax(scale q2 K2^T) V )
+ * Pool, records, planner and append are those of esp_attn_forward without Kb / Vb: the pass's rows are in the pool
+ * (esp_attn_prep with a row_table, or esp_kv_save), row j of a tree at position P + j of its own block list or ring.
+ * Rows are plain causal: row j sees the keys 0 .. P + j, of them the last `window` where window > 0. Softmax, difference
+ * and norm are held in fp32; the probabilities are rounded to the storage type before P.V, O once at the end. */
+typedef struct esp_diff_params {
+  const float* weight; /* [H / 2] fp32, device memory */
+  const float* norm_w; /* [2 * head_dim] fp32, device memory; NULL: no norm (eps is then not read) */
+  float eps;
+  float factor;
+} esp_diff_params;
+
+/* The rows_per_tile to plan a pass with whose trees have at most `rows` rows, or 0 for parameters that
+ * esp_attn_diff refuses. Host-only arithmetic. */
+int32_t esp_attn_diff_rows(const esp_attn_params* p, int32_t rows);
+/* As esp_attn_plan_hint, of the kernel that serves p->rows_per_tile. */
+int esp_attn_diff_hint(const esp_attn_params* p, int device, int32_t* workgroups, int32_t* groups_per_tile, char* err, size_t errlen);
+/* Bytes of workspace for a plan of n_parts partial records. Host-only arithmetic. */
+size_t esp_attn_diff_workspace_bytes(const esp_attn_params* p, int32_t n_parts);
+/* Of p: head_dim 128, H and Hkv even, no gate, no bidi; kv_ld is not read. Q and O [n_rows][q_ld], O's pair i at column
+ * 2 * head_dim * i; rows outside the tiles are left as they are. Tiles, trees and jobs as planned by esp_plan_tiles;
+ * what the records have to promise is what esp_attn_validate_for(ESP_PASS_DIFF) checks. Tiles with k1 = INT32_MAX end at
+ * the tree's cached length as it is when the kernel runs (decode chains). */
+int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void* Q, const void* kv_pool, const int32_t* blocks, void* O,
+                  const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees, int32_t n_trees, const esp_combine* jobs, int32_t n_jobs,
+                  int32_t n_parts, int32_t n_rows, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen);
+
+/* ---- low-rank adapters of many requests beside a shared projection -----------------
+ * No counterpart in the reference. Every row adds its own adapter's product to the fp32 projection that esp_attn_prep
+ * reads, in place:
+ *   Y[row, y_off[s] + c] += scale[a] * sum_k B[a][c of slice s][k] * (A[a][s * rank + k] . X[row])
+ * for the slices s of the fused projection (queries, keys, values, ...; columns outside the slices are not touched).
+ * Rows without an adapter are in no tile and stay as they are. An adapter of a smaller rank is stored with zeros in the
+ * rows of A and columns of B that it lacks. The sums and the intermediate are held in fp32. */
+enum { ESP_LOWRANK_SLICES = 4 };
+typedef struct esp_lowrank_params {
+  int32_t D;             /* width of X, a multiple of 8 */
+  int32_t rank;          /* rows of A per slice: a multiple of 8, at most 128 */
+  int32_t n_slices;      /* 1 .. 4 */
+  int32_t dtype;         /* ESP_F16 | ESP_BF16: X, A and B */
+  int32_t x_ld;          /* X row stride, elements, a multiple of 8 */
+  int32_t y_ld;          /* Y row stride, floats */
+  int32_t n_adapters;
+  int32_t rows_per_tile; /* what the tiles were planned with: esp_lowrank_rows */
+  int32_t y_off[4];      /* first column of a slice in Y */
+  int32_t width[4];      /* columns of a slice; slices do not overlap */
+} esp_lowrank_params;
+
+/* Rows of one adapter: slots [first, first + count) of `order`, which holds row numbers. */
+typedef struct esp_lowrank_tile {
+  int32_t adapter, first, count, pad;
+} esp_lowrank_tile;
+
+/* The rows_per_tile to plan a pass of n_rows rows with, or 0 for parameters that esp_lowrank_add refuses. */
+int32_t esp_lowrank_rows(const esp_lowrank_params* p, int32_t n_rows);
+size_t esp_lowrank_workspace_bytes(const esp_lowrank_params* p, int32_t n_tiles, int32_t n_slots);
+/* X [rows][x_ld]; A [n_adapters][n_slices * rank][D]; B [n_adapters][sum of the widths][rank]; scale [n_adapters] fp32;
+ * Y [rows][y_ld] fp32. order [n_slots], tiles: device copies of what esp_plan_lowrank (include/espetero_engine.h) made,
+ * whose tiles name each row at most once. X, A, B and the workspace 16-byte aligned. */
+int esp_lowrank_add(const esp_lowrank_params* p, const void* X, const void* A, const void* B, const float* scale, float* Y, const int32_t* order,
+                    int32_t n_slots, const esp_lowrank_tile* tiles, int32_t n_tiles, void* workspace, size_t workspace_bytes, void* stream,
+                    char* err, size_t errlen);
+
+/* ---- the logits at the end of a decode step ----------------------------------------
+ * No counterpart in the reference's kernels (it samples on the host; its chains take the argmax on the GPU,
+ * src/model/model.mm:779-850). Per row, in this order, each operation rounded to fp32 by itself:
+ *   a token that the row's slot has seen, in its prompt or among those given out:  x > 0 ? x / repetition : x * repetition
+ *   one that was given out n > 0 times:                                           x - frequency * n - presence
+ *   one of the row's bias entries:                                                x + value
+ *   one that the row's mask does not allow:                                       -infinity
+ * out receives the logits, tokens the best token of each row: the largest logit, the lowest token among equal ones, never
+ * one whose logit is NaN or -infinity; -1 where nothing is left. With record != 0 that token then joins the history of the
+ * row's slot as one given out. Results do not depend on the order in which rows run. */
+enum { ESP_F32 = 2 };
+typedef struct esp_logits_params {
+  int32_t vocab;
+  int32_t dtype;   /* ESP_F16 | ESP_BF16 | ESP_F32: the logits as they come */
+  int32_t in_ld;   /* their row stride, elements */
+  int32_t out_ld;  /* row stride of out, floats */
+  int32_t n_slots; /* slots of the histories */
+  int32_t n_masks; /* rows of masks */
+  int32_t n_bias;  /* entries of bias_tokens / bias_values */
+  int32_t pad;
+} esp_logits_params;
+
+typedef struct esp_logits_row {
+  int32_t slot;   /* of the histories; -1: a row without one */
+  int32_t mask;   /* row of masks; -1: every token is allowed */
+  int32_t bias0;  /* first of the row's bias entries */
+  int32_t n_bias; /* how many: tokens in ascending order, none twice */
+  float repetition, frequency, presence; /* 1, 0, 0: none */
+  int32_t pad;
+} esp_logits_row;
+
+size_t esp_logits_workspace_bytes(const esp_logits_params* p, int32_t n_rows);
+/* logits [n_rows][in_ld]; out [n_rows][out_ld] fp32 or NULL (it may be the logits themselves where those are fp32 and
+ * out_ld == in_ld); tokens [n_rows] or NULL (then record is 0). rows: n_rows records. masks [n_masks][ceil(vocab / 32)]:
+ * bit t % 32 of word t / 32 set where token t is allowed. Histories: seen [n_slots][2][ceil(vocab / 32)], bits of the
+ * tokens of the prompt and of those given out; counts [n_slots][vocab], how often each was given out. Arrays that no row
+ * names may be NULL. All device memory. Slots, masks and entries outside their arrays count as none. */
+int esp_logits_process(const esp_logits_params* p, const void* logits, float* out, int32_t* tokens, const esp_logits_row* rows, int32_t n_rows,
+                       const int32_t* bias_tokens, const float* bias_values, const uint32_t* masks, uint32_t* seen, int32_t* counts,
+                       int32_t record, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen);
+/* Host-side check of the records and bias entries before they are uploaded (host pointers): slots, masks and entries
+ * inside their arrays, finite penalties, repetition > 0, every row's tokens in [0, vocab), ascending, none twice. */
+int esp_logits_validate(const esp_logits_params* p, const esp_logits_row* rows, int32_t n_rows, const int32_t* bias_tokens, char* err,
+                        size_t errlen);
+/* tokens[i] joins the history of slots[i]: of its prompt (given = 0) or of the tokens given out (given = 1). Entries may repeat;
+ * ones outside the vocabulary or the slots are skipped. */
+int esp_history_record(const esp_logits_params* p, uint32_t* seen, int32_t* counts, const int32_t* tokens, const int32_t* slots, int32_t n,
+                       int32_t given, void* stream, char* err, size_t errlen);
+/* Empties the histories of n slots. */
+int esp_history_clear(const esp_logits_params* p, uint32_t* seen, int32_t* counts, const int32_t* slots, int32_t n, void* stream, char* err,
+                      size_t errlen);
 
 #ifdef __cplusplus
 }

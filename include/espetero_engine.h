@@ -66,6 +66,13 @@ int esp_plan_tiles_for(const esp_attn_params* p, const esp_tree* trees, int32_t 
                        const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                        int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen);
 
+/* The tiles of a pass of esp_lowrank_add: the rows that have an adapter, grouped by it (adapters ascending, rows ascending within
+ * one), in tiles of p->rows_per_tile rows and fewer at an adapter's end. adapter[n_rows]: each row's, -1 for none; ESP_EINVAL for one
+ * that p->n_adapters does not hold. order (room for n_rows) and tiles (capacity given) out; on ESP_EWORKSPACE the counts are still
+ * written. */
+int esp_plan_lowrank(const esp_lowrank_params* p, const int32_t* adapter, int32_t n_rows, int32_t* order, int32_t* n_slots, esp_lowrank_tile* tiles,
+                     int32_t tiles_cap, int32_t* n_tiles, char* err, size_t errlen);
+
 /* ---- KV engine: pool + slots + pass builder ---- */
 typedef struct esp_engine esp_engine;
 
