@@ -37,8 +37,10 @@ hipError_t tiled_init_attributes();
 hipError_t tiled256_init_attributes();
 hipError_t tiled512_init_attributes();
 hipError_t launch_diff_stream(int dt, const DiffArgs& a, int n_tiles, hipStream_t st);
+hipError_t launch_diff_tiled(int dt, const DiffArgs& a, int n_tiles, hipStream_t st);
 hipError_t launch_diff_merge(int dt, const DiffArgs& a, const esp_combine* jobs, int n_jobs, hipStream_t st);
 hipError_t diff_init_attributes();
+hipError_t diff_tiled_init_attributes();
 hipError_t launch_lowrank(int dt, const LowRankArgs& a, int n_tiles, hipStream_t st);
 hipError_t launch_logits(int dt, const LogitsArgs& a, int n_rows, hipStream_t st);
 hipError_t launch_history_record(const esp_logits_params* p, uint32_t* seen, int32_t* counts, const int32_t* tokens, const int32_t* slots, int n,
@@ -167,6 +169,7 @@ int device_state(DeviceState** out, char* err, size_t errlen) {
     if ((e = esp::tiled512_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (tiled kernels, head dim 512)", e);
     if ((e = esp::gate_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (head gate)", e);
     if ((e = esp::diff_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (differential attention)", e);
+    if ((e = esp::diff_tiled_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (tiled differential attention)", e);
     d.scratch = static_cast<unsigned char*>(ps);
     d.ready = true;
   }
@@ -740,7 +743,7 @@ int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void
   a.factor = d->factor;
   a.kv_base = p->kv_base;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipError_t e = esp::launch_diff_stream(p->dtype, a, n_tiles, st);
+  hipError_t e = fam > 0 ? esp::launch_diff_stream(p->dtype, a, n_tiles, st) : esp::launch_diff_tiled(p->dtype, a, n_tiles, st);
   if (e != hipSuccess) return hip_fail(err, errlen, "attn_diff launch", e);
   if (n_jobs > 0) {
     e = esp::launch_diff_merge(p->dtype, a, jobs, n_jobs, st);

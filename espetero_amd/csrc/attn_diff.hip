@@ -82,9 +82,8 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
 
   const int lane_k = c16 * HD + 8 * q4, lane_v = c16 * kVtDim + 4 * q4;
   const size_t head = size_t(2 * a.bt * HD);  // elements of one (block, KV head)
-  auto unit_base = [&](int u) { return a.pool + diff_head_base(a, diff_block(a, table, u << 4), 2 * j); };
   auto load = [&](int u, DiffUnit& U) {
-    const uint16_t* hb = unit_base(u);
+    const uint16_t* hb = a.pool + diff_head_base(a, diff_block(a, table, u << 4), 2 * j);
     const int t0 = (u << 4) % a.bt;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -159,8 +158,8 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
       U.v[mt].y &= in[2] | in[3];
       bad |= not_finite2<DT>(U.v[mt].x) | not_finite2<DT>(U.v[mt].y);
     }
-    // Nor may the infinite V of a key that one row sees reach a row that does not: such elements leave the product and are added to
-    // the rows that see them one by one.
+    // Nor may the infinite V of a key that one row sees reach a row that does not: such elements leave the product, and a product of
+    // marks in their places says which rows see them.
     const bool rare = rg.rows > 1 && __any(bad != 0);
     if (rare) {
 #pragma unroll
@@ -183,27 +182,24 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
         s[c][e] = vis ? s[c][e] * a.scale_log2 : -INFINITY;
       }
     softmax_pv(U, s, p);
-    if (rare) {
+    if (__builtin_expect(rare, 0)) {
+      DiffUnit W;
+      load(u, W);
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
+      for (int mt = 0; mt < MT; ++mt) {
+        const uint32_t lo = W.v[mt].x & (in[0] | in[1]), hi = W.v[mt].y & (in[2] | in[3]);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) mfma_settle(acc[c][mt]);
-      const uint16_t* hb = unit_base(u);
-      for (int t = 0; t < 16; ++t) {
-        const int key = (u << 4) + t;
-        if (key < rg.lo || key >= rg.hi) continue;
+        for (int neg = 0; neg < 2; ++neg)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const float pe = (t & 3) == 0 ? p[c][0] : (t & 3) == 1 ? p[c][1] : (t & 3) == 2 ? p[c][2] : p[c][3];
-          const float pt = __shfl(pe, 16 * (t >> 2) + c16);
+          for (int c = 0; c < NC; ++c) {
+            const u32x2 pb = {pack2<DT>(p[c][0], p[c][1]), pack2<DT>(p[c][2], p[c][3])};
+            f32x4 seen = mfma16x16<DT>(u32x2{not_finite_marks<DT>(lo, neg != 0), not_finite_marks<DT>(hi, neg != 0)}, pb, f32x4{0, 0, 0, 0});
+            mfma_settle(seen);
+            mfma_settle(acc[c][mt]);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t w = hb[(mt >> 3) * head + vt_elem(a.bt, HD, key % a.bt, 16 * (mt & 7) + 4 * q4 + e)];
-              if ((not_finite2<DT>(w) & 0xffffu) && pt > 0.0f) acc[c][mt][e] += pt * unpack_lo<DT>(w);
-            }
-        }
+            for (int e = 0; e < 4; ++e)
+              if (seen[e] > 0.0f) acc[c][mt][e] += neg ? -INFINITY : INFINITY;
+          }
       }
     }
   };

@@ -84,4 +84,13 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
   return ((w & e) == e ? 0xffffu : 0u) | ((w >> 16 & e) == e ? 0xffff0000u : 0u);
 }
 
+// 1.0 in the storage type where an element is an infinity of the given sign or NaN, else 0. A product of such marks with the weights is
+// finite whatever they are, and positive where a row sees such a value.
+template <int DT>
+__device__ __forceinline__ uint32_t not_finite_marks(uint32_t w, bool negative) {
+  constexpr uint32_t e = DT == ESP_F16 ? 0x7c00u : 0x7f80u, one = DT == ESP_F16 ? 0x3c00u : 0x3f80u;
+  auto mark = [&](uint32_t x) { return (x & e) == e && ((x & 0x7fffu) != e || (x >> 15 != 0) == negative) ? one : 0u; };
+  return mark(w & 0xffffu) | mark(w >> 16) << 16;
+}
+
 }  // namespace esp

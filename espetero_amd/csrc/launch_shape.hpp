@@ -52,10 +52,14 @@ constexpr Carve carve_workspace(int H, int Hkv, int head_dim, int rows_per_tile,
   return c;
 }
 
-// Differential attention, G query pairs per KV pair: 1, the streaming kernel, which takes up to 16 packed rows; 0, no kernel.
-constexpr int diff_family(int rows_per_tile, int G) { return rows_per_tile > 0 && G > 0 && rows_per_tile * G <= 16 ? 1 : 0; }
+// Differential attention, G query pairs per KV pair: 1, the streaming kernel, which takes up to 16 packed rows; -1, the tiled one, up to
+// 128; 0, no kernel.
+constexpr int diff_family(int rows_per_tile, int G) {
+  if (rows_per_tile <= 0 || G <= 0 || rows_per_tile > 128 / G) return 0;
+  return rows_per_tile * G <= 16 ? 1 : -1;
+}
 // Rows per tile for trees of at most `rows` rows; 0: no kernel.
-constexpr int diff_rows(int rows, int G) { return G > 16 ? 0 : rows * G <= 16 ? rows : 16 / G; }
+constexpr int diff_rows(int rows, int G) { return rows < 128 / G ? rows : 128 / G; }
 constexpr int diff_workgroups_per_cu(int) { return 1; }
 
 // Its partial records: both maps of every packed row.

@@ -52,7 +52,7 @@ def check(case, bits, rows=None):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("heads", [(4, 2), (8, 4), (16, 4), (10, 2), (16, 2), (32, 2)])
+@pytest.mark.parametrize("heads", [(4, 2), (8, 4), (16, 4), (10, 2), (16, 2), (32, 2), (64, 2), (256, 2)])
 @pytest.mark.parametrize("bt,seqs", [(16, [(0, 1), (1, 1), (15, 1), (16, 1), (130, 1), (700, 1)]), (64, [(63, 1), (64, 1), (250, 1)])])
 def test_single_tokens(heads, dtype, bt, seqs):
     c = DiffCase(*heads, dtype, bt, seqs, seed=heads[0])
@@ -70,7 +70,8 @@ def test_drafts(heads, rows, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("heads,seqs", [((4, 2), [(0, 300)]), ((8, 2), [(50, 133), (0, 17), (7, 64)]), ((8, 4), [(129, 130)])])
+@pytest.mark.parametrize("heads,seqs", [((4, 2), [(0, 300)]), ((8, 2), [(50, 133), (0, 17), (7, 64)]), ((8, 4), [(129, 130)]),
+                                        ((4, 4), [(0, 129), (31, 127)]), ((10, 2), [(13, 60)]), ((64, 2), [(40, 9), (0, 3)])])
 def test_prompts_and_chunks(heads, seqs, dtype):
     c = DiffCase(*heads, dtype, 16, seqs, seed=3)
     check(c, Run(c)())

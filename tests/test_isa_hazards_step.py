@@ -7,7 +7,7 @@ import pytest
 import isa_hazards
 from test_isa_hazards import HIPCC, _assembly
 
-SOURCES = ["attn_diff.hip", "lowrank.hip"]
+SOURCES = ["attn_diff.hip", "attn_diff_tiled.hip", "lowrank.hip"]
 
 
 @pytest.fixture(scope="module")
