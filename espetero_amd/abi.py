@@ -148,11 +148,13 @@ class EspError(RuntimeError):
 
 class PlanGroups(int):
     """Workgroups per tile, as plan_hint reports them: a plain count, which also knows the layer it was asked for, so that the
-    planner needs no argument of its own for that. A count worked out otherwise is planned for any layer."""
+    planner needs no argument of its own for that. A count worked out otherwise is planned for any layer. diff: as
+    attn_diff_hint reports them."""
 
-    def __new__(cls, value, params=None):
+    def __new__(cls, value, params=None, diff=False):
         g = super().__new__(cls, value)
-        g.layer = None if params is None else (params.H, params.Hkv, params.head_dim)
+        layer = None if params is None else (params.H, params.Hkv, params.head_dim)
+        g.layer, g.diff = (None, layer) if diff else (layer, None)
         return g
 
 

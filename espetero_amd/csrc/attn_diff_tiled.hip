@@ -21,14 +21,23 @@ namespace esp {
 
 namespace {
 constexpr int kRing = 4, kStage = 32 * 1024;  // stages; bytes of one
-constexpr size_t kDiffTiledLds = size_t(kRing) * kStage + 64;  // and 16 ints behind the ring
+constexpr int kOffBad = kRing * kStage, kOffMarks = kOffBad + 64;     // 16 ints behind the ring; then a word per lane and 32 dims
+constexpr size_t kDiffTiledLds = kOffMarks + 8 * (kDiffVD / 32) * 256;
 constexpr float kSlack = 8.0f;  // a row's reference moves when a score exceeds it by more (log2 units): P stays below 2^8
+
+// The maximum over the two lanes that hold a row. (Of the builtin for this instruction the compiler keeps one result only; the two
+// wait states are what it puts between a vector instruction and the exchange of its result.)
+__device__ __forceinline__ float max_halves(float x) {
+  float y = x;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  return fmaxf(x, y);
+}
 }  // namespace
 
 template <int DT>
 __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs a) {
   constexpr int HD = kDiffHD, VD = kDiffVD, NT = VD / 32, KS = HD / 16;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
   const uint32_t lds_base = uint32_t(uintptr_t(lds));
   const int j = blockIdx.x;  // KV pair
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -40,13 +49,22 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   const int cols_live = rg.rows * a.G;
 
   // ---- this lane's packed row
-  const int col = col0 + l32;
-  const bool ok = col < cols_live;
-  const int m = ok ? col / a.G : 0, hg = ok ? col - m * a.G : 0;
-  const int qpos = tree.P + rg.rr0 + m;
+  struct Place {
+    bool ok;
+    int m, hg;  // row in the tile, query pair of the KV pair; row 0's first where there is none
+  };
+  auto place = [&](int l) {
+    const int col = col0 + (l & 31);
+    const bool ok = col < cols_live;
+    const int m = ok ? col / a.G : 0;
+    return Place{ok, m, ok ? col - m * a.G : 0};
+  };
   u32x4 qf[KS];
+  int qpos;
   {
-    const uint16_t* qp = a.Q + size_t(tile.r0 + m) * a.q_ld + size_t(2 * (j * a.G + hg) + map) * HD + 8 * hb;
+    const Place pl = place(lane);
+    qpos = tree.P + rg.rr0 + pl.m;
+    const uint16_t* qp = a.Q + size_t(tile.r0 + pl.m) * a.q_ld + size_t(2 * (j * a.G + pl.hg) + map) * HD + 8 * hb;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + 16 * ks);
   }
@@ -74,25 +92,37 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   // ---- staging: wavefront w loads sub-block w % 2 of K1, K2, V1 or V2 (w / 2) of every stage
   const int kind = wave >> 1, last_sub = rg.hi > rg.lo ? (rg.hi - 1) & ~15 : s0;
   const size_t head = size_t(2 * a.bt * HD);
-  uint32_t voff[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 4 * i + (lane >> 4);
-    voff[i] = kind < 2 ? uint32_t((lane >> 4) * 256 + (((lane & 15) ^ swap23(r)) << 4)) : uint32_t((2 * l32 + hb) << 4);
-  }
+  // Where the first of a run's four loads finds this lane's 16 bytes. K: four rows a load, the chunks of row r of the sub-block turned by
+  // pi(r), so those of the other loads differ by pi(4 i); V^T: alike in all of them.
+  const uint32_t from = kind < 2 ? uint32_t((lane >> 4) * 256 + (((lane & 15) ^ swap23(lane >> 4)) << 4)) : uint32_t((2 * l32 + hb) << 4);
+  const uint32_t turn1 = kind < 2 ? swap23(4) << 4 : 0, turn2 = kind < 2 ? swap23(8) << 4 : 0;
   const uint32_t dst = lds_base + wave * 4096;
-  auto stage = [&](int h) {
-    const int key = min(s0 + 32 * h + 16 * (wave & 1), last_sub);  // past the range: its last sub-block again
-    const int t0 = key % a.bt;
-    const uint16_t* hb_ = a.pool + diff_head_base(a, diff_block(a, table, key), 2 * j) + (kind & 1) * head;
-    const uint16_t* src = kind < 2 ? hb_ + t0 * HD : hb_ + vt_elem(a.bt, HD, t0, 0);
-    load_to_lds16_x4(src, voff[0], voff[1], voff[2], voff[3], dst + uint32_t(h % kRing) * kStage);
+  // Where this wavefront's next sub-block lies; a stage further is 32 tokens further, past the range the last sub-block again.
+  int next_key = min(s0 + 16 * (wave & 1), last_sub), next_at = next_key / a.bt, next_t0 = next_key - next_at * a.bt;
+  if (a.ring) next_at %= a.ring;
+  using const_i32 = const int32_t __attribute__((address_space(4)));
+  const const_i32* const list = (const const_i32*)a.blocks;
+  auto block_id = [&] { return a.ring ? table + next_at : list[table + next_at]; };
+  const char* const plane = reinterpret_cast<const char*>(a.pool + size_t(a.kv_base) + size_t(2 * j + (kind & 1)) * head + (kind < 2 ? 0 : size_t(a.bt) * HD));
+  const uint64_t block_bytes = uint64_t(a.Hkv) * head * 2;
+  auto stage = [&](int h, int id) __attribute__((always_inline)) {
+    // (t0 is a multiple of 16: a V^T sub-block starts as far behind its plane as the K row of its first token does)
+    load_to_lds16_x4(plane + uint64_t(uint32_t(id)) * block_bytes + uint32_t(next_t0 * (HD * 2)), from, from ^ turn1, from ^ turn2, from ^ turn1 ^ turn2,
+                     dst + uint32_t(h & (kRing - 1)) * kStage);
+    if (next_key + 32 <= last_sub) {
+      next_key += 32;
+      next_t0 += 32;
+      while (next_t0 >= a.bt) {
+        next_t0 -= a.bt;
+        if (++next_at == a.ring) next_at = 0;  // (0 on a layer without rings, which it never is again)
+      }
+    }
   };
   // Runs in a stage: K of head 0 sub-block 0, 1, K of head 1, V^T of head 0, V^T of head 1; 4 KB each.
   using lds_u32x4 = const __attribute__((address_space(3))) u32x4;
   auto lds_read = [&](uint32_t at) { return *reinterpret_cast<lds_u32x4*>(at); };
   const int prow = swap23(l32);  // the lane with S^T row l32 reads this key of the stage
-  const uint32_t k_at = lds_base + map * 8192 + prow * 256;
+  const uint32_t k_at = lds_base + map * 8192 + prow * 256 + ((hb ^ (l32 & 15)) << 4);  // its chunk 2 ks + hb: this ^ (ks << 5)
   const uint32_t v_at = lds_base + 16384 + lane * 16;
 
   f32x16 acc[NT];
@@ -101,50 +131,55 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   for (int nt = 0; nt < NT; ++nt) acc[nt] = f32x16{};
   u32x4 P[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
 
-  auto scores = [&](int h) {
-    const uint32_t at = k_at + uint32_t(h % kRing) * kStage;
-    f32x16 s{};
-    u32x4 k[KS];
+  f32x16 s{};
+  // Matrix work of a turn: P . V of stage h - 1 and the scores of stage h, a score product in front of every two of P . V so that neither
+  // waits for its own last result; operands are read a group of three ahead.
+  auto products = [&](int h) __attribute__((always_inline)) {
+    u32x4 v[2][2], k[2];
+    const uint32_t ka = k_at + uint32_t(h & (kRing - 1)) * kStage;
+    uint32_t va = v_at + uint32_t((h - 1) & (kRing - 1)) * kStage;
+    asm("" : "+v"(va));  // one register, the operands' places as immediates: left alone the compiler keeps eight
+    auto fetch = [&](int g) {
+      k[g & 1] = lds_read(ka ^ uint32_t(g << 5));
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) k[ks] = lds_read(at + (((2 * ks + hb) ^ (l32 & 15)) << 4));
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = mfma32x16<DT>(k[ks], qf[ks], s);
-    return s;
-  };
-  auto pv = [&](int h) {
-    const uint32_t at = v_at + uint32_t(h % kRing) * kStage;
-    u32x4 v[2][4];
-    auto fetch = [&](int g) {  // of 4 groups: sub-block g / 2, dims 128 (g % 2) ..
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[g & 1][i] = lds_read(at + (g & 1) * 8192 + (g >> 1) * 4096 + i * 1024);
+      for (int i = 0; i < 2; ++i) v[g & 1][i] = lds_read(va + ((2 * g + i) >> 2 & 1) * 8192 + ((2 * g + i) >> 3) * 4096 + ((2 * g + i) & 3) * 1024);
     };
+    s = f32x16{};
     fetch(0);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      if (g < 3) fetch(g + 1);
+    for (int g = 0; g < 8; ++g) {
+      if (g < 7) fetch(g + 1);
+      s = mfma32x16<DT>(k[g & 1], qf[g], s);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[4 * (g & 1) + i] = mfma32x16<DT>(v[g & 1][i], P[g >> 1], acc[4 * (g & 1) + i]);
+      for (int i = 0; i < 2; ++i) acc[(2 * g + i) & 7] = mfma32x16<DT>(v[g & 1][i], P[g >> 2], acc[(2 * g + i) & 7]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   // Lane l holds of S^T, at index 8 sb + i, key 16 sb + 8 hb + i of the stage.
-  auto key_of = [&](int h, int sb, int i) { return s0 + 32 * h + 16 * sb + 8 * hb + i; };
   auto in_range = [&](int k0) {  // the bits of two keys' values
     return (k0 >= rg.lo && k0 < rg.hi ? 0xffffu : 0u) | (k0 + 1 >= rg.lo && k0 + 1 < rg.hi ? 0xffff0000u : 0u);
   };
   // Values of a stage with keys that some row does not see, by the wavefront that has staged them: those outside the range may be
   // memory never written, and infinite values of keys that only other rows see must not meet a zero weight. Both become zeros; where
-  // there were any of the latter, `bad` says so and marks() adds them to the rows that see them.
-  int* const bad = reinterpret_cast<int*>(lds + kRing * kStage);  // [stage of the ring][staging wavefront of the four]
-  auto mend = [&](int h) {
+  // there were any of the latter, `bad` says so and marks() keeps which of this lane's outputs they reach: bit e of a word for index e
+  // of 32 dims, bit 16 + e for negative ones. They are added at the end (a branch of the loop that touched the accumulators would cost
+  // registers in every turn).
+  int* const bad = reinterpret_cast<int*>(lds + kOffBad);  // [stage of the ring][staging wavefront of the four]
+  // (What such rare code works out from the lane's number is worked out there: kept in registers through the loop it would cost spills.)
+  auto here = [](int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  auto mend = [&](int h) __attribute__((always_inline)) {
     uint32_t found = 0;
-    char* const mine = lds + (h % kRing) * kStage + wave * 4096 + lane * 16;
+    const int ln = here(lane), key0 = s0 + 32 * h + 16 * (wave & 1) + 8 * (ln >> 5);
+    char* const mine = lds + (uint32_t(h) & (kRing - 1)) * kStage + wave * 4096 + ln * 16;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32x4 v = *reinterpret_cast<const u32x4*>(mine + i * 1024);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[e] &= in_range(key_of(h, wave & 1, 2 * e));
+        v[e] &= in_range(key0 + 2 * e);
         const uint32_t nf = not_finite2<DT>(v[e]);
         found |= nf;
         v[e] &= ~nf;
@@ -152,131 +187,170 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
       *reinterpret_cast<u32x4*>(mine + i * 1024) = v;
     }
     const bool any = __any(found != 0);
-    if (lane == 0) bad[4 * (h % kRing) + (wave & 3)] = any;
+    if (ln == 0) bad[4 * (uint32_t(h) & (kRing - 1)) + (wave & 3)] = any;
   };
+  bool marked = false;
   auto marks = [&](int h) {
-    const uint16_t* src[2];
+    const int ln = here(lane);
+#pragma unroll 1
+    for (int w = 0; w < NT; ++w) {
+      uint32_t* const word = reinterpret_cast<uint32_t*>(lds + kOffMarks) + (wave * NT + w) * 64 + ln;
+      uint32_t found = marked ? *word : 0u;
+#pragma unroll 1
+      for (int t = 0; t < 32; ++t) {
+        const int key = s0 + 32 * h + t;
+        if (key < rg.lo || key >= rg.hi) continue;
+        // The row's weight of the key: element t % 8 of P[t / 16], in the lane half (t / 8) % 2.
+        uint32_t p2 = 0;
 #pragma unroll
-    for (int sb = 0; sb < 2; ++sb) {
-      const int key = min(s0 + 32 * h + 16 * sb, last_sub);
-      src[sb] = a.pool + diff_head_base(a, diff_block(a, table, key), 2 * j) + vt_elem(a.bt, HD, key % a.bt, l32) + 8 * hb;
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int neg = 0; neg < 2; ++neg) {
-        f32x16 seen{};
-#pragma unroll
-        for (int sb = 0; sb < 2; ++sb) {
-          u32x4 v = *reinterpret_cast<const u32x4*>(src[sb] + (nt >> 2) * head + 32 * (nt & 3) * kVtDim);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = not_finite_marks<DT>(v[e] & in_range(key_of(h, sb, 2 * e)), neg != 0);
-          seen = mfma32x16<DT>(v, P[sb], seen);
+        for (int i = 0; i < 8; ++i) p2 = i == 4 * (t >> 4) + ((t >> 1) & 3) ? P[i >> 2][i & 3] : p2;
+        const float p = __shfl((t & 1) ? unpack_hi<DT>(p2) : unpack_lo<DT>(p2), 32 * ((t >> 3) & 1) + (ln & 31));
+        const uint16_t* v = a.pool + diff_head_base(a, diff_block(a, table, key), 2 * j + (w >> 2)) +
+                            vt_elem(a.bt, HD, key % a.bt, 32 * (w & 3) + 4 * (ln >> 5));
+#pragma unroll 1
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t x = v[(8 * (e >> 2) + (e & 3)) * kVtDim];
+          if (!(p > 0.0f)) continue;
+          found |= (not_finite_marks<DT>(x, false) & 0xffffu ? 1u << e : 0u) | (not_finite_marks<DT>(x, true) & 0xffffu ? 0x10000u << e : 0u);
         }
-        mfma_settle(seen);
-        mfma_settle(acc[nt]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (seen[e] > 0.0f) acc[nt][e] += neg ? -INFINITY : INFINITY;
-        __builtin_amdgcn_sched_barrier(0);
       }
+      *word = found;
+    }
+    marked = true;
   };
 
-  if (n_st > 0) stage(0);
-  if (n_st > 1) stage(1);
-  if (n_st > 2) stage(2);
-  // One turn more than stages: turn h has S of stage h and P . V of stage h - 1.
-  for (int h = 0; h <= n_st; ++h) {
-    // Stage h is in LDS for everybody, and everybody is done with stage h - 2, whose place stage h + 2 takes.
-    const int behind = min(n_st, h + 2) - (h + 1);  // stages requested behind stage h, 4 loads each
-    if (behind >= 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (wave >= 4 && h < n_st && (h < w0 || h >= w1)) {
-      mend(h);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
+  for (int h = 0; h < min(n_st, 3); ++h) stage(h, block_id());
+  // Q is waited for here, not at its first use in the loop: that wait would be on the counter of the stages on their way.
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
+  auto meet = [&] {
+    asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (h >= 1 && h + 2 < n_st) stage(h + 2);
-    const bool do_s = h >= v0 && h < v1, do_pv = h - 1 >= v0 && h - 1 < v1;
-    const bool s_full = h >= f0 && h < f1, pv_full = h - 1 >= w0 && h - 1 < w1;
-    f32x16 s{};
-    float c = 1.0f;
-    bool move = false;
-    if (do_s) {
-      s = scores(h);
-      mfma_settle(s);
-      if (!s_full) {
+  };
+  auto wait_behind = [&](int n) {  // all but the last n stages requested have landed for this wavefront, 4 loads each
+    if (n >= 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    else if (n == 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
+  auto softmax = [&]() __attribute__((always_inline)) {
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+    mx = max_halves(mx) * a.scale_log2;
+    const bool up = mx > m_ref + kSlack;  // from -inf on: the first key that the row sees
+    if (__builtin_expect(__any(up), 0)) {
+      const float c = up ? fast_exp2(m_ref - mx) : 1.0f;
+      const bool first = m_ref == -INFINITY;
+      m_ref = up ? mx : m_ref;
+      l_run *= c;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mfma_settle(acc[nt]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[nt][e] = first ? 0.0f : acc[nt][e] * c;
+      }
+    }
+    const float off = m_ref == -INFINITY ? 0.0f : m_ref;
+    float lx = 0.0f;
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = 8 * sb + 2 * e;
+        P[sb][e] = pack2<DT>(fast_exp2(s[at] * a.scale_log2 - off), fast_exp2(s[at + 1] * a.scale_log2 - off));
+        (sb ? lx : l_run) = sum2<DT>(P[sb][e], sb ? lx : l_run);  // of the weights as the product takes them
+      }
+    l_run += lx;
+  };
+  // A turn of the two groups of wavefronts: the early one (0 .. 3, which stage K) and the late one (4 .. 7, which stage V), half a turn
+  // behind it. A barrier in front of each half; while one group has its matrix work the other has its softmax. On a SIMD there is one
+  // wavefront of each.
+  auto within = [](int h, int lo, int hi) { return uint32_t(h - lo) < uint32_t(hi - lo); };  // (lo <= hi)
+  const bool late = wave >= 4;
+  if (late) meet();
+  for (int h = 0; h <= n_st; ++h) {
+    const bool do_pv = within(h - 1, v0, v1);
+    if (!late) wait_behind(n_st - 1 - h);           // K of stage h: up to two stages requested behind it
+    meet();
+    // On a wavefront's first stage P is zero and the V of "the stage before" whatever lies there, infinities and NaN among it: what that
+    // makes of the accumulators goes when a row's reference is first set. On its last turn the scores are not used.
+    if (do_pv || within(h, v0, v1)) products(h);
+    if (late) {
+      wait_behind(n_st - 1 - h);                    // V of stage h
+      if (h < n_st && !within(h, w0, w1)) {
+        mend(h);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+    }
+    meet();
+    const int id = block_id();
+    if (do_pv && !within(h - 1, w0, w1)) {
+      const int* b = bad + 4 * ((h - 1) & (kRing - 1));
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(b[0] | b[1] | b[2] | b[3]), 0)) marks(h - 1);
+    }
+    if (within(h, v0, v1)) {
+      if (!within(h, f0, f1)) {
+        mfma_settle(s);
+        const int key0 = s0 + 32 * h + 8 * (here(lane) >> 5);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int key = key_of(h, e >> 3, e & 7);
+          const int key = key0 + 16 * (e >> 3) + (e & 7);
           bool vis = key >= rg.lo && key < rg.hi && key <= qpos;
           if (a.window > 0) vis = vis && qpos - key < a.window;
           s[e] = vis ? s[e] : -INFINITY;
         }
       }
-      float mx = s[0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.scale_log2;
-      const bool up = mx > m_ref + kSlack;  // from -inf on: the first key that the row sees
-      c = up ? fast_exp2(m_ref - mx) : 1.0f;
-      m_ref = up ? mx : m_ref;
-      move = __any(up);
+      softmax();
     }
-    if (do_pv) {
-      pv(h - 1);
-      if (!pv_full) {
-        const int* b = bad + 4 * ((h - 1) % kRing);
-        if (__builtin_expect(__builtin_amdgcn_readfirstlane(b[0] | b[1] | b[2] | b[3]), 0)) marks(h - 1);
-      }
-    }
-    if (do_s) {
-      if (__builtin_expect(move, 0)) {
-        l_run *= c;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mfma_settle(acc[nt]);
-          acc[nt] *= c;
-        }
-      }
-      const float off = m_ref == -INFINITY ? 0.0f : m_ref;
-      float p[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        p[e] = fast_exp2(s[e] * a.scale_log2 - off);
-        l_run += p[e];
-      }
-#pragma unroll
-      for (int sb = 0; sb < 2; ++sb)
-        P[sb] = u32x4{pack2<DT>(p[8 * sb], p[8 * sb + 1]), pack2<DT>(p[8 * sb + 2], p[8 * sb + 3]), pack2<DT>(p[8 * sb + 4], p[8 * sb + 5]),
-                      pack2<DT>(p[8 * sb + 6], p[8 * sb + 7])};
-    }
+    if (h + 3 < n_st) stage(h + 3, id);
   }
+  if (!late) meet();
 
   // ---- the row's end
+  const int ln = here(lane), half = ln >> 5;
+  const Place pl = place(ln);
   float l = l_run + __shfl_xor(l_run, 32);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) mfma_settle(acc[nt]);
+  const bool none = l == 0.0f;  // a row that has seen nothing
+  if (__any(none)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[nt][e] = none ? 0.0f : acc[nt][e];
+  }
+  if (__builtin_expect(marked, 0)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const uint32_t word = reinterpret_cast<const uint32_t*>(lds + kOffMarks)[(wave * NT + nt) * 64 + ln];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        acc[nt][e] += word >> e & 1 ? INFINITY : 0.0f;
+        acc[nt][e] -= word >> (16 + e) & 1 ? INFINITY : 0.0f;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
   if (tile.part >= 0) {  // a partial record: dims 32 nt + 8 i + 4 hb .. + 3 of this lane's packed row
-    if (!ok) return;
-    const size_t rec = ((size_t(tile.part) * (a.Hkv / 2) + j) * 2 + map) * a.cols + col;
+    if (!pl.ok) return;
+    const size_t rec = ((size_t(tile.part) * (a.Hkv / 2) + j) * 2 + map) * a.cols + col0 + (ln & 31);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(a.parts_o + rec * VD + 32 * nt + 8 * i + 4 * hb) = f32x4{acc[nt][4 * i], acc[nt][4 * i + 1], acc[nt][4 * i + 2], acc[nt][4 * i + 3]};
-    if (hb == 0) {
+        *reinterpret_cast<f32x4*>(a.parts_o + rec * VD + 32 * nt + 8 * i + 4 * half) = f32x4{acc[nt][4 * i], acc[nt][4 * i + 1], acc[nt][4 * i + 2], acc[nt][4 * i + 3]};
+    if (half == 0) {
       a.parts_ml[rec * 2] = m_ref;
       a.parts_ml[rec * 2 + 1] = l;
     }
     return;
   }
   __syncthreads();  // the ring is free
-  f32x4* const sh = reinterpret_cast<f32x4*>(lds + (wave >> 1) * 32768) + lane;  // [32 groups of 4 dims][64 lanes]
-  const int pair = j * a.G + hg;
+  f32x4* const sh = reinterpret_cast<f32x4*>(lds + (wave >> 1) * 32768) + ln;  // [32 groups of 4 dims][64 lanes]
+  const int pair = j * a.G + pl.hg;
   if (map == 1) {
-    const float i2 = (l > 0.0f ? 1.0f / l : 0.0f) * a.weight[pair];
+    const float i2 = diff_inverse(l) * a.weight[pair];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -285,7 +359,7 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   }
   __syncthreads();
   if (map == 1) return;
-  const float i1 = l > 0.0f ? 1.0f / l : 0.0f;
+  const float i1 = diff_inverse(l);
   float ss = 0.0f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -298,21 +372,26 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
         acc[nt][4 * i + e] = o;
         ss += o * o;
       }
+      if (i == 3) __builtin_amdgcn_sched_barrier(0);  // four reads at a time: all 32 do not fit the registers
     }
   ss += __shfl_xor(ss, 32);
-  if (!ok) return;
+  if (!pl.ok) return;
   const float f = a.norm_w ? a.factor * rsqrtf(ss * (1.0f / VD) + a.eps) : a.factor;
-  uint16_t* const to = a.O + size_t(tile.r0 + m) * a.q_ld + size_t(pair) * VD;
+  uint16_t* const to = a.O + size_t(tile.r0 + pl.m) * a.q_ld + size_t(pair) * VD;
+  auto put = [&](auto weight_of) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = 32 * nt + 8 * i + 4 * hb;
-      f32x4 w = {f, f, f, f};
-      if (a.norm_w) w *= *reinterpret_cast<const f32x4*>(a.norm_w + d);
-      *reinterpret_cast<u32x2*>(to + d) = u32x2{pack2<DT>(acc[nt][4 * i] * w[0], acc[nt][4 * i + 1] * w[1]),
-                                                pack2<DT>(acc[nt][4 * i + 2] * w[2], acc[nt][4 * i + 3] * w[3])};
-    }
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * nt + 8 * i + 4 * half;
+        const f32x4 w = weight_of(d);
+        *reinterpret_cast<u32x2*>(to + d) = u32x2{pack2<DT>(acc[nt][4 * i] * w[0], acc[nt][4 * i + 1] * w[1]),
+                                                  pack2<DT>(acc[nt][4 * i + 2] * w[2], acc[nt][4 * i + 3] * w[3])};
+        if (i == 3 && (nt & 1)) __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  if (a.norm_w) put([&](int d) { return *reinterpret_cast<const f32x4*>(a.norm_w + d) * f; });
+  else put([&](int) { return f32x4{f, f, f, f}; });
 }
 
 hipError_t diff_tiled_init_attributes() {

@@ -59,11 +59,14 @@ __device__ __forceinline__ DiffRange diff_range(const esp_tile& t, const esp_tre
   return d;
 }
 
+// 0 for a row that has seen no key; NaN stays NaN.
+__device__ __forceinline__ float diff_inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
 // A wavefront's 256 dims of one (row, pair), 4 per lane: o1 and o2 unnormalised with sums l1 and l2. The difference of the two maps'
 // outputs, its norm over the pair's dims and the factor in fp32, then the one rounding to the storage type.
 template <int DT>
 __device__ __forceinline__ void diff_finish(const DiffArgs& a, int row, int pair, int lane, f32x4 o1, float l1, f32x4 o2, float l2) {
-  const float i1 = l1 > 0.0f ? 1.0f / l1 : 0.0f, i2 = (l2 > 0.0f ? 1.0f / l2 : 0.0f) * a.weight[pair];
+  const float i1 = diff_inverse(l1), i2 = diff_inverse(l2) * a.weight[pair];
   f32x4 o = o1 * i1 - o2 * i2;
   float f = a.factor;
   if (a.norm_w) {

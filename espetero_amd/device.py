@@ -217,7 +217,7 @@ def attn_diff_hint(params, device=0):
     err = C.create_string_buffer(_ERRLEN)
     n, g = C.c_int32(0), C.c_int32(0)
     abi.check(abi.attn_lib().esp_attn_diff_hint(C.byref(params), device, C.byref(n), C.byref(g), err, _ERRLEN), err)
-    return n.value, g.value
+    return n.value, abi.PlanGroups(g.value, params, diff=True)
 
 
 class DiffPass:

@@ -65,6 +65,11 @@ void esp_plan_options_mi355x(esp_plan_options* o, int32_t rows, int32_t workgrou
   to_c(PlanOptions::mi355x(rows, workgroups), o);
 }
 
+void esp_plan_options_diff(esp_plan_options* o, const esp_attn_params* p) {
+  if (!o || !p || p->H <= 0 || p->Hkv <= 0 || o->groups_target <= 0) return;
+  if (esp::diff_family(o->rows_per_tile, p->H / p->Hkv) < 0) to_c(to_cpp(*o).for_diff_tiled(), o);
+}
+
 int esp_plan_tiles(const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
                    const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                    int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen) {

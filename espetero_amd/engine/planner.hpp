@@ -76,6 +76,20 @@ struct PlanOptions {
     }
     return o;
   }
+  // These options where the tiled differential attention kernel runs the pass: what mi355x() takes for a streaming pass by its rows is
+  // planned by the hand-out of workgroups to slots like any tiled pass. Set fields stay.
+  PlanOptions for_diff_tiled() const {
+    const PlanOptions had = mi355x(1, groups_target), tiled = mi355x(64, groups_target);
+    PlanOptions o = *this;
+    if (!o.balanced || o.item_steps) return o;
+    auto turn = [](int& field, int from, int to) { field = field == from ? to : field; };
+    turn(o.granule, had.granule, tiled.granule);
+    turn(o.min_chunk, had.min_chunk, tiled.min_chunk);
+    turn(o.min_span, had.min_span, tiled.min_span);
+    turn(o.item_steps, had.item_steps, tiled.item_steps);
+    turn(o.part_steps, had.part_steps, tiled.part_steps);
+    return o;
+  }
 };
 
 struct AttnPlan {

@@ -30,6 +30,7 @@ _IP = C.POINTER(C.c_int32)
 ENGINE_SYMBOLS = {
     "esp_plan_options_reference": (None, (_PO,)),
     "esp_plan_options_mi355x": (None, (_PO, _I, _I)),
+    "esp_plan_options_diff": (None, (_PO, _AP)),
     "esp_plan_tiles": (C.c_int, (_V, _I, _I, _I, _V, _PO, _V, _I, _IP, _V, _I, _IP, _IP) + _ERR),
     "esp_plan_tiles_for": (C.c_int, (_AP, _V, _I, _I, _I, _V, _PO, _V, _I, _IP, _V, _I, _IP, _IP) + _ERR),
     "esp_plan_lowrank": (C.c_int, (C.POINTER(abi.LowRankParams), _V, _I, _V, _IP, _V, _I, _IP) + _ERR),
@@ -100,8 +101,8 @@ def options_mi355x(rows, workgroups):
 
 
 def plan_tiles(trees, groups, window, pos, options):
-    """trees: TREE_DT array. groups: plan_hint's, which plans for that layer, or a number, which plans for any.
-    Returns (tiles TILE_DT, jobs COMBINE_DT, n_parts)."""
+    """trees: TREE_DT array. groups: plan_hint's, which plans for that layer (attn_diff_hint's: for differential attention on it), or a
+    number, which plans for any. Returns (tiles TILE_DT, jobs COMBINE_DT, n_parts)."""
     lib = engine_lib()
     trees = np.ascontiguousarray(trees, dtype=abi.TREE_DT)
     pos_a = None if pos is None else np.ascontiguousarray(pos, dtype=np.int32)
@@ -110,6 +111,11 @@ def plan_tiles(trees, groups, window, pos, options):
     if layer is not None:
         p = abi.AttnParams()
         p.H, p.Hkv, p.head_dim = layer
+    if getattr(groups, "diff", None) is not None:
+        q = abi.AttnParams()
+        q.H, q.Hkv, q.head_dim = groups.diff
+        options = PlanOptions.from_buffer_copy(options)
+        lib.esp_plan_options_diff(C.byref(options), C.byref(q))
     err = C.create_string_buffer(256)
     nt, nj, npart = C.c_int32(0), C.c_int32(0), C.c_int32(0)
     # Room for one tile per row group and three resident rounds of parts (of a chip as large as any) serves nearly every plan in one

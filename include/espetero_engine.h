@@ -52,6 +52,11 @@ void esp_plan_options_reference(esp_plan_options* o);
 /* Tuned for 256 CUs: rows query rows per tile, workgroups what esp_attn_plan_hint reports for the kernel. */
 void esp_plan_options_mi355x(esp_plan_options* o, int32_t rows, int32_t workgroups);
 
+/* For a pass of esp_attn_diff with the parameters `p`: where its tiled kernel serves them, options for the streaming kernel become
+ * those of the tiled one (its tiles may have few rows, by which esp_plan_options_mi355x tells the two apart). Fields that do not hold
+ * what that function gave them stay as they are. */
+void esp_plan_options_diff(esp_plan_options* o, const esp_attn_params* p);
+
 /* Plan a pass. trees[n_trees] in; tiles / jobs out (capacities given; on
  * ESP_EWORKSPACE the needed counts are still written). groups: workgroups per
  * tile (KV heads). window > 0 needs pos (4 ints per row). */

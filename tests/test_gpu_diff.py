@@ -141,6 +141,18 @@ def test_an_infinite_value_reaches_the_rows_that_see_it():
     assert not np.isfinite(got[3:, col]).any()
 
 
+@pytest.mark.parametrize("seqs,workgroups", [([(40, 1)], None), ([(40, 4)], None), ([(300, 3)], 4096), ([(10, 90)], None), ([(700, 40)], 2048)])
+def test_a_key_of_nan_shows_in_every_row_that_sees_it(seqs, workgroups):
+    """The first key, alone in its part's first unit for no row: every row and every pair whose map it is in."""
+    c = DiffCase(8, 4, BF16, 16, seqs, seed=15)
+    r = Run(c, workgroups=workgroups, cut_batch=workgroups is not None)
+    pool = c.pool.copy().reshape(c.n_blocks, c.Hkv, 2, c.bt * HD)
+    pool[c.block_list[int(c.trees["table"][0])], 1, 0, 5] = 0x7FC0     # K of KV head 1, key 0: the second map of the first KV pair
+    r.pool = dev(pool.reshape(-1))
+    got = ob.to_f32(r()[:, :8 * HD], BF16).reshape(c.n_rows, 4, 2 * HD)
+    assert np.isnan(got[:, :2]).all() and np.isfinite(got[:, 2:]).all()
+
+
 def test_a_second_pass_and_another_stream_give_the_same_bits():
     c = DiffCase(16, 4, BF16, 16, [(900, 1), (300, 1), (77, 1)], seed=9)
     r = Run(c, workgroups=4096)
