@@ -133,25 +133,26 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
 
   f32x16 s{};
   // Matrix work of a turn: P . V of stage h - 1 and the scores of stage h, a score product in front of every two of P . V so that neither
-  // waits for its own last result; operands are read a group of three ahead.
+  // waits for its own last result; operands are read two groups of three ahead.
   auto products = [&](int h) __attribute__((always_inline)) {
-    u32x4 v[2][2], k[2];
+    u32x4 v[3][2], k[3];
     const uint32_t ka = k_at + uint32_t(h & (kRing - 1)) * kStage;
     uint32_t va = v_at + uint32_t((h - 1) & (kRing - 1)) * kStage;
     asm("" : "+v"(va));  // one register, the operands' places as immediates: left alone the compiler keeps eight
     auto fetch = [&](int g) {
-      k[g & 1] = lds_read(ka ^ uint32_t(g << 5));
+      k[g % 3] = lds_read(ka ^ uint32_t(g << 5));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) v[g & 1][i] = lds_read(va + ((2 * g + i) >> 2 & 1) * 8192 + ((2 * g + i) >> 3) * 4096 + ((2 * g + i) & 3) * 1024);
+      for (int i = 0; i < 2; ++i) v[g % 3][i] = lds_read(va + ((2 * g + i) >> 2 & 1) * 8192 + ((2 * g + i) >> 3) * 4096 + ((2 * g + i) & 3) * 1024);
     };
     s = f32x16{};
     fetch(0);
+    fetch(1);
 #pragma unroll
     for (int g = 0; g < 8; ++g) {
-      if (g < 7) fetch(g + 1);
-      s = mfma32x16<DT>(k[g & 1], qf[g], s);
+      if (g < 6) fetch(g + 2);
+      s = mfma32x16<DT>(k[g % 3], qf[g], s);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) acc[(2 * g + i) & 7] = mfma32x16<DT>(v[g & 1][i], P[g >> 2], acc[(2 * g + i) & 7]);
+      for (int i = 0; i < 2; ++i) acc[(2 * g + i) & 7] = mfma32x16<DT>(v[g % 3][i], P[g >> 2], acc[(2 * g + i) & 7]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -263,27 +264,34 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
       }
     l_run += lx;
   };
-  // A turn of the two groups of wavefronts: the early one (0 .. 3, which stage K) and the late one (4 .. 7, which stage V), half a turn
-  // behind it. A barrier in front of each half; while one group has its matrix work the other has its softmax. On a SIMD there is one
-  // wavefront of each.
+  // The two groups of wavefronts, one wavefront of each on a SIMD: the early one (0 .. 3, which stage K) and the late one (4 .. 7, which
+  // stage V). One barrier a turn: the early group passes it in front of its matrix work, the late one in front of its softmax, so that
+  // while one has its matrix work the other has its softmax. Behind barrier h, K of stage h and V of stage h - 1 have landed for
+  // everybody, and nobody reads K of stage h - 1 (whose place the early group's next request takes) or V of stage h - 2 (the late's) any more.
   auto within = [](int h, int lo, int hi) { return uint32_t(h - lo) < uint32_t(hi - lo); };  // (lo <= hi)
   const bool late = wave >= 4;
   if (late) meet();
   for (int h = 0; h <= n_st; ++h) {
-    const bool do_pv = within(h - 1, v0, v1);
-    if (!late) wait_behind(n_st - 1 - h);           // K of stage h: up to two stages requested behind it
-    meet();
+    if (!late) {
+      wait_behind(n_st - 1 - h);  // K of stage h: up to two stages requested behind it
+      meet();
+    }
     // On a wavefront's first stage P is zero and the V of "the stage before" whatever lies there, infinities and NaN among it: what that
     // makes of the accumulators goes when a row's reference is first set. On its last turn the scores are not used.
-    if (do_pv || within(h, v0, v1)) products(h);
+    const bool do_pv = within(h - 1, v0, v1);
+    if (do_pv || within(h, v0, v1)) {
+      __builtin_amdgcn_s_setprio(1);
+      products(h);
+      __builtin_amdgcn_s_setprio(0);
+    }
     if (late) {
-      wait_behind(n_st - 1 - h);                    // V of stage h
+      wait_behind(n_st - 1 - h);  // V of stage h
       if (h < n_st && !within(h, w0, w1)) {
         mend(h);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
+      meet();
     }
-    meet();
     const int id = block_id();
     if (do_pv && !within(h - 1, w0, w1)) {
       const int* b = bad + 4 * ((h - 1) & (kRing - 1));
