@@ -105,10 +105,15 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   auto block_id = [&] { return a.ring ? table + next_at : list[table + next_at]; };
   const char* const plane = reinterpret_cast<const char*>(a.pool + size_t(a.kv_base) + size_t(2 * j + (kind & 1)) * head + (kind < 2 ? 0 : size_t(a.bt) * HD));
   const uint64_t block_bytes = uint64_t(a.Hkv) * head * 2;
-  auto stage = [&](int h, int id) __attribute__((always_inline)) {
+  const char* next_from = nullptr;  // the run of the stage to be requested next
+  auto locate = [&](int id) {
     // (t0 is a multiple of 16: a V^T sub-block starts as far behind its plane as the K row of its first token does)
-    load_to_lds16_x4(plane + uint64_t(uint32_t(id)) * block_bytes + uint32_t(next_t0 * (HD * 2)), from, from ^ turn1, from ^ turn2, from ^ turn1 ^ turn2,
-                     dst + uint32_t(h & (kRing - 1)) * kStage);
+    next_from = plane + uint64_t(uint32_t(id)) * block_bytes + uint32_t(next_t0 * (HD * 2));
+  };
+  auto request = [&](int h) __attribute__((always_inline)) {
+    load_to_lds16_x4(next_from, from, from ^ turn1, from ^ turn2, from ^ turn1 ^ turn2, dst + uint32_t(h & (kRing - 1)) * kStage);
+  };
+  auto advance = [&] {
     if (next_key + 32 <= last_sub) {
       next_key += 32;
       next_t0 += 32;
@@ -132,9 +137,9 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   u32x4 P[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
 
   f32x16 s{};
-  // Matrix work of a turn: P . V of stage h - 1 and the scores of stage h, a score product in front of every two of P . V so that neither
+  // Matrix work of a turn, and the request of stage `next` (-1: none) between it: P . V of stage h - 1 and the scores of stage h, a score product in front of every two of P . V so that neither
   // waits for its own last result; operands are read two groups of three ahead.
-  auto products = [&](int h) __attribute__((always_inline)) {
+  auto products = [&](int h, int next) __attribute__((always_inline)) {
     u32x4 v[3][2], k[3];
     const uint32_t ka = k_at + uint32_t(h & (kRing - 1)) * kStage;
     uint32_t va = v_at + uint32_t((h - 1) & (kRing - 1)) * kStage;
@@ -153,6 +158,8 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
       s = mfma32x16<DT>(k[g % 3], qf[g], s);
 #pragma unroll
       for (int i = 0; i < 2; ++i) acc[(2 * g + i) & 7] = mfma32x16<DT>(v[g % 3][i], P[g >> 2], acc[(2 * g + i) & 7]);
+      if (g == 3 && next >= 0) request(next);
+      if (g == 5 && next >= 0) advance();
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -220,7 +227,14 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
     marked = true;
   };
 
-  for (int h = 0; h < min(n_st, 3); ++h) stage(h, block_id());
+  const bool late = wave >= 4;
+  const int ahead = late ? 2 : 3;  // how many stages ahead of its matrix work a wavefront requests
+  locate(block_id());
+  for (int h = 0; h < min(n_st, ahead); ++h) {
+    request(h);
+    advance();
+    locate(block_id());
+  }
   // Q is waited for here, not at its first use in the loop: that wait would be on the counter of the stages on their way.
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
@@ -267,9 +281,8 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   // The two groups of wavefronts, one wavefront of each on a SIMD: the early one (0 .. 3, which stage K) and the late one (4 .. 7, which
   // stage V). One barrier a turn: the early group passes it in front of its matrix work, the late one in front of its softmax, so that
   // while one has its matrix work the other has its softmax. Behind barrier h, K of stage h and V of stage h - 1 have landed for
-  // everybody, and nobody reads K of stage h - 1 (whose place the early group's next request takes) or V of stage h - 2 (the late's) any more.
+  // everybody, and nobody reads K of stage h - 1 (whose place the early group's next request takes) or V of stage h - 2 (the late one's) any more.
   auto within = [](int h, int lo, int hi) { return uint32_t(h - lo) < uint32_t(hi - lo); };  // (lo <= hi)
-  const bool late = wave >= 4;
   if (late) meet();
   for (int h = 0; h <= n_st; ++h) {
     if (!late) {
@@ -279,10 +292,14 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
     // On a wavefront's first stage P is zero and the V of "the stage before" whatever lies there, infinities and NaN among it: what that
     // makes of the accumulators goes when a row's reference is first set. On its last turn the scores are not used.
     const bool do_pv = within(h - 1, v0, v1);
+    const int next = h + ahead < n_st ? h + ahead : -1;
     if (do_pv || within(h, v0, v1)) {
       __builtin_amdgcn_s_setprio(1);
-      products(h);
+      products(h, next);
       __builtin_amdgcn_s_setprio(0);
+    } else if (next >= 0) {
+      request(next);
+      advance();
     }
     if (late) {
       wait_behind(n_st - 1 - h);  // V of stage h
@@ -300,18 +317,15 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
     if (within(h, v0, v1)) {
       if (!within(h, f0, f1)) {
         mfma_settle(s);
-        const int key0 = s0 + 32 * h + 8 * (here(lane) >> 5);
+        // The row sees the keys [from, from + n); index e of this lane's half is key 16 (e / 8) + e % 8 behind the first.
+        const int from = a.window > 0 ? max(rg.lo, qpos - a.window + 1) : rg.lo, n = max(0, min(rg.hi, qpos + 1) - from);
+        const int at = s0 + 32 * h + 8 * (here(lane) >> 5) - from;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = key0 + 16 * (e >> 3) + (e & 7);
-          bool vis = key >= rg.lo && key < rg.hi && key <= qpos;
-          if (a.window > 0) vis = vis && qpos - key < a.window;
-          s[e] = vis ? s[e] : -INFINITY;
-        }
+        for (int e = 0; e < 16; ++e) s[e] = uint32_t(at + 16 * (e >> 3) + (e & 7)) < uint32_t(n) ? s[e] : -INFINITY;
       }
       softmax();
     }
-    if (h + 3 < n_st) stage(h + 3, id);
+    locate(id);
   }
   if (!late) meet();
 
