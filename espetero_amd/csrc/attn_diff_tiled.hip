@@ -50,14 +50,13 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
 
   // ---- this lane's packed row
   struct Place {
-    bool ok;
     int m, hg;  // row in the tile, query pair of the KV pair; row 0's first where there is none
   };
   auto place = [&](int l) {
     const int col = col0 + (l & 31);
     const bool ok = col < cols_live;
     const int m = ok ? col / a.G : 0;
-    return Place{ok, m, ok ? col - m * a.G : 0};
+    return Place{m, ok ? col - m * a.G : 0};
   };
   u32x4 qf[KS];
   int qpos;
@@ -98,7 +97,7 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   const uint32_t turn1 = kind < 2 ? swap23(4) << 4 : 0, turn2 = kind < 2 ? swap23(8) << 4 : 0;
   const uint32_t dst = lds_base + wave * 4096;
   // Where this wavefront's next sub-block lies; a stage further is 32 tokens further, past the range the last sub-block again.
-  int next_key = min(s0 + 16 * (wave & 1), last_sub), next_at = next_key / a.bt, next_t0 = next_key - next_at * a.bt;
+  int next_key = n_st > 0 ? min(s0 + 16 * (wave & 1), last_sub) : 0, next_at = next_key / a.bt, next_t0 = next_key - next_at * a.bt;
   if (a.ring) next_at %= a.ring;
   using const_i32 = const int32_t __attribute__((address_space(4)));
   const const_i32* const list = (const const_i32*)a.blocks;
@@ -329,19 +328,13 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   }
   if (!late) meet();
 
-  // ---- the row's end
-  const int ln = here(lane), half = ln >> 5;
-  const Place pl = place(ln);
+  // ---- the rows' end. 32 packed rows of 256 fp32 numbers pass through 32 KB of the ring, the two wavefronts of the rows' maps on each
+  // side: written by a lane for its row (4 dims at a time: g = 0 .. 31, its half's of dims 8 g .. 8 g + 7), read a row by 32 lanes, 8 dims
+  // each, so that rows leave in whole lines. Lane by lane from the accumulators they left 8 bytes at a time: 8 us of a workgroup's time.
+  const int ln = here(lane), half = ln >> 5, l5 = ln & 31;
   float l = l_run + __shfl_xor(l_run, 32);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) mfma_settle(acc[nt]);
-  const bool none = l == 0.0f;  // a row that has seen nothing
-  if (__any(none)) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[nt][e] = none ? 0.0f : acc[nt][e];
-  }
   if (__builtin_expect(marked, 0)) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -354,66 +347,91 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  if (tile.part >= 0) {  // a partial record: dims 32 nt + 8 i + 4 hb .. + 3 of this lane's packed row
-    if (!pl.ok) return;
-    const size_t rec = ((size_t(tile.part) * (a.Hkv / 2) + j) * 2 + map) * a.cols + col0 + (ln & 31);
+  const bool none = l == 0.0f;  // a row that has seen nothing
+  if (__any(none)) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(a.parts_o + rec * VD + 32 * nt + 8 * i + 4 * half) = f32x4{acc[nt][4 * i], acc[nt][4 * i + 1], acc[nt][4 * i + 2], acc[nt][4 * i + 3]};
-    if (half == 0) {
-      a.parts_ml[rec * 2] = m_ref;
-      a.parts_ml[rec * 2 + 1] = l;
+      for (int e = 0; e < 16; ++e) acc[nt][e] = none ? 0.0f : acc[nt][e];
+  }
+  // 4 dims of a row: at 1 KB * g + 512 * half + 16 * (row ^ g), turned by g: no bank conflicts on either side. The lane's own are at
+  // mine() ^ 16 g + 1 KB * g, its part asked for anew by each pass over them: 32 addresses kept for the next pass would be spilled.
+  char* const rows = lds + (wave >> 1) * 32768;
+  auto mine = [&] {
+    const int x = here(lane);
+    return 512 * (x >> 5) + 16 * (x & 31);
+  };
+  auto own = [&](int at, int g) { return reinterpret_cast<f32x4*>(rows + (at ^ (16 * g)) + 1024 * g); };
+  auto put = [&](float f) __attribute__((always_inline)) {
+    const int at = mine();
+#pragma unroll
+    for (int g = 0; g < 32; ++g)
+      *own(at, g) = f32x4{acc[g >> 2][4 * (g & 3)] * f, acc[g >> 2][4 * (g & 3) + 1] * f, acc[g >> 2][4 * (g & 3) + 2] * f, acc[g >> 2][4 * (g & 3) + 3] * f};
+  };
+  // The wavefront's half of the rows, two at a time: take(packed row, its dims 8 l5 .. + 3, + 4 .. + 7).
+  auto leave = [&](auto take) {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const int row = 16 * map + 2 * i + half;
+      const char* const at = rows + 1024 * l5 + 16 * (row ^ l5);
+      if (col0 + row < cols_live) take(col0 + row, *reinterpret_cast<const f32x4*>(at), *reinterpret_cast<const f32x4*>(at + 512));
+    }
+  };
+  __syncthreads();  // the ring is free
+  if (tile.part >= 0) {  // partial records
+    float* const to = a.parts_o + (size_t(tile.part) * (a.Hkv / 2) + j) * 2 * a.cols * VD + 8 * l5;
+#pragma unroll 1
+    for (int e = 0; e < 2; ++e) {
+      if (map == e) put(1.0f);
+      __syncthreads();
+      leave([&](int col, f32x4 x, f32x4 y) {
+        f32x4* const rec = reinterpret_cast<f32x4*>(to + (size_t(e) * a.cols + col) * VD);
+        rec[0] = x;
+        rec[1] = y;
+      });
+      __syncthreads();
+    }
+    if (half == 0 && col0 + l5 < cols_live) {
+      float* const ml = a.parts_ml + (((size_t(tile.part) * (a.Hkv / 2) + j) * 2 + map) * a.cols + col0 + l5) * 2;
+      ml[0] = m_ref;
+      ml[1] = l;
     }
     return;
   }
-  __syncthreads();  // the ring is free
-  f32x4* const sh = reinterpret_cast<f32x4*>(lds + (wave >> 1) * 32768) + ln;  // [32 groups of 4 dims][64 lanes]
-  const int pair = j * a.G + pl.hg;
-  if (map == 1) {
-    const float i2 = diff_inverse(l) * a.weight[pair];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sh[64 * (4 * nt + i)] = f32x4{acc[nt][4 * i] * i2, acc[nt][4 * i + 1] * i2, acc[nt][4 * i + 2] * i2, acc[nt][4 * i + 3] * i2};
+  if (map == 1) put(diff_inverse(l) * a.weight[j * a.G + place(ln).hg]);
+  f32x4 w[2] = {{1, 1, 1, 1}, {1, 1, 1, 1}};
+  if (a.norm_w) {
+    w[0] = *reinterpret_cast<const f32x4*>(a.norm_w + 8 * l5);
+    w[1] = *reinterpret_cast<const f32x4*>(a.norm_w + 8 * l5 + 4);
   }
   __syncthreads();
-  if (map == 1) return;
-  const float i1 = diff_inverse(l);
-  float ss = 0.0f;
+  if (map == 0) {
+    const float f1 = diff_inverse(l);
+    float ss = 0.0f;
+    const int at = mine();
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 o2 = sh[64 * (4 * nt + i)];
+    for (int g = 0; g < 32; ++g) {
+      const f32x4 o2 = *own(at, g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float o = acc[nt][4 * i + e] * i1 - o2[e];
-        acc[nt][4 * i + e] = o;
+        const float o = acc[g >> 2][4 * (g & 3) + e] * f1 - o2[e];
+        acc[g >> 2][4 * (g & 3) + e] = o;
         ss += o * o;
       }
-      if (i == 3) __builtin_amdgcn_sched_barrier(0);  // four reads at a time: all 32 do not fit the registers
+      if ((g & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // four reads at a time: all 32 do not fit the registers
     }
-  ss += __shfl_xor(ss, 32);
-  if (!pl.ok) return;
-  const float f = a.norm_w ? a.factor * rsqrtf(ss * (1.0f / VD) + a.eps) : a.factor;
-  uint16_t* const to = a.O + size_t(tile.r0 + pl.m) * a.q_ld + size_t(pair) * VD;
-  auto put = [&](auto weight_of) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = 32 * nt + 8 * i + 4 * half;
-        const f32x4 w = weight_of(d);
-        *reinterpret_cast<u32x2*>(to + d) = u32x2{pack2<DT>(acc[nt][4 * i] * w[0], acc[nt][4 * i + 1] * w[1]),
-                                                  pack2<DT>(acc[nt][4 * i + 2] * w[2], acc[nt][4 * i + 3] * w[3])};
-        if (i == 3 && (nt & 1)) __builtin_amdgcn_sched_barrier(0);
-      }
-  };
-  if (a.norm_w) put([&](int d) { return *reinterpret_cast<const f32x4*>(a.norm_w + d) * f; });
-  else put([&](int) { return f32x4{f, f, f, f}; });
+    ss += __shfl_xor(ss, 32);
+    put(a.norm_w ? a.factor * rsqrtf(ss * (1.0f / VD) + a.eps) : a.factor);
+  }
+  __syncthreads();
+  leave([&](int col, f32x4 x, f32x4 y) {
+    x *= w[0];
+    y *= w[1];
+    const int m = col / a.G;
+    using out16 = uint32_t __attribute__((ext_vector_type(4), aligned(8)));  // a row of O starts at any multiple of 8 bytes
+    *reinterpret_cast<out16*>(a.O + size_t(tile.r0 + m) * a.q_ld + size_t(j * a.G + col - m * a.G) * VD + 8 * l5) =
+        out16{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]), pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+  });
 }
 
 hipError_t diff_tiled_init_attributes() {
