@@ -399,34 +399,32 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
     return;
   }
   if (map == 1) put(diff_inverse(l) * a.weight[j * a.G + place(ln).hg]);
-  f32x4 w[2] = {{1, 1, 1, 1}, {1, 1, 1, 1}};
-  if (a.norm_w) {
-    w[0] = *reinterpret_cast<const f32x4*>(a.norm_w + 8 * l5);
-    w[1] = *reinterpret_cast<const f32x4*>(a.norm_w + 8 * l5 + 4);
-  }
   __syncthreads();
+  float* const factors = reinterpret_cast<float*>(lds + kOffMarks) + col0;  // the norm's of every packed row
   if (map == 0) {
     const float f1 = diff_inverse(l);
     float ss = 0.0f;
     const int at = mine();
 #pragma unroll
     for (int g = 0; g < 32; ++g) {
-      const f32x4 o2 = *own(at, g);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float o = acc[g >> 2][4 * (g & 3) + e] * f1 - o2[e];
-        acc[g >> 2][4 * (g & 3) + e] = o;
-        ss += o * o;
-      }
-      if ((g & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // four reads at a time: all 32 do not fit the registers
+      f32x4* const x = own(at, g);
+      f32x4 o = f32x4{acc[g >> 2][4 * (g & 3)], acc[g >> 2][4 * (g & 3) + 1], acc[g >> 2][4 * (g & 3) + 2], acc[g >> 2][4 * (g & 3) + 3]} * f1 - *x;
+      *x = o;
+      ss += o[0] * o[0] + o[1] * o[1] + o[2] * o[2] + o[3] * o[3];
     }
     ss += __shfl_xor(ss, 32);
-    put(a.norm_w ? a.factor * rsqrtf(ss * (1.0f / VD) + a.eps) : a.factor);
+    if (half == 0) factors[l5] = a.norm_w ? a.factor * rsqrtf(ss * (1.0f / VD) + a.eps) : a.factor;
+  }
+  f32x4 w[2] = {{1, 1, 1, 1}, {1, 1, 1, 1}};
+  if (a.norm_w) {
+    w[0] = *reinterpret_cast<const f32x4*>(a.norm_w + 8 * l5);
+    w[1] = *reinterpret_cast<const f32x4*>(a.norm_w + 8 * l5 + 4);
   }
   __syncthreads();
   leave([&](int col, f32x4 x, f32x4 y) {
-    x *= w[0];
-    y *= w[1];
+    const float f = factors[col - col0];
+    x *= w[0] * f;
+    y *= w[1] * f;
     const int m = col / a.G;
     using out16 = uint32_t __attribute__((ext_vector_type(4), aligned(8)));  // a row of O starts at any multiple of 8 bytes
     *reinterpret_cast<out16*>(a.O + size_t(tile.r0 + m) * a.q_ld + size_t(j * a.G + col - m * a.G) * VD + 8 * l5) =
