@@ -38,7 +38,7 @@ hipError_t tiled256_init_attributes();
 hipError_t tiled512_init_attributes();
 hipError_t launch_diff_stream(int dt, const DiffArgs& a, int n_tiles, hipStream_t st);
 hipError_t launch_diff_tiled(int dt, const DiffArgs& a, int n_tiles, hipStream_t st);
-hipError_t launch_diff_merge(int dt, const DiffArgs& a, const esp_combine* jobs, int n_jobs, hipStream_t st);
+hipError_t launch_diff_merge(int dt, const DiffArgs& a, const esp_combine* jobs, int n_jobs, int n_parts, hipStream_t st);
 hipError_t diff_init_attributes();
 hipError_t diff_tiled_init_attributes();
 hipError_t launch_lowrank(int dt, const LowRankArgs& a, int n_tiles, hipStream_t st);
@@ -746,7 +746,7 @@ int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void
   hipError_t e = fam > 0 ? esp::launch_diff_stream(p->dtype, a, n_tiles, st) : esp::launch_diff_tiled(p->dtype, a, n_tiles, st);
   if (e != hipSuccess) return hip_fail(err, errlen, "attn_diff launch", e);
   if (n_jobs > 0) {
-    e = esp::launch_diff_merge(p->dtype, a, jobs, n_jobs, st);
+    e = esp::launch_diff_merge(p->dtype, a, jobs, n_jobs, n_parts, st);
     if (e != hipSuccess) return hip_fail(err, errlen, "attn_diff_merge launch", e);
   }
   return ESP_OK;

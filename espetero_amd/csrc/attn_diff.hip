@@ -296,69 +296,79 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
   }
 }
 
-// Merge of the partial records of a split tile, then the difference, the norm and the one rounding. One workgroup is one (job, row,
-// query pair); its 4 wavefronts take the records round robin and meet in LDS.
-template <int DT>
+// Merge of the partial records of a split tile, then the difference, the norm and the one rounding. Bound by the records' bytes, 2 KB
+// of fp32 each, and for few rows by the latency of their loads. W wavefronts share one (job, row, query pair), taking its records round
+// robin and meeting in LDS: 4 where groups have many records, else one, which keeps the records of four outputs in flight per workgroup
+// (126 parts of 128 packed rows, two a group: 27.1 us with four wavefronts an output, 15.6 with one).
+template <int DT, int W>
 __global__ __launch_bounds__(256) void attn_diff_merge_kernel(const DiffArgs a, const esp_combine* jobs) {
   constexpr int VD = kDiffVD;
-  __shared__ __attribute__((aligned(16))) float o_sh[4][2][VD];
-  __shared__ float ml_sh[4][2][2];
+  __shared__ __attribute__((aligned(16))) float o_sh[W > 1 ? W : 1][2][W > 1 ? VD : 4];
+  __shared__ float ml_sh[W > 1 ? W : 1][2][2];
   const esp_combine job = jobs[blockIdx.y];
-  const int pairs = a.H / 2, r = blockIdx.x / pairs, pair = blockIdx.x - r * pairs;
-  if (r >= job.rows) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int pairs = a.H / 2, out = W > 1 ? int(blockIdx.x) : int(blockIdx.x) * 4 + wave;
+  const int r = out / pairs, pair = out - r * pairs;
+  if (r >= job.rows) return;  // (for W > 1 the whole workgroup)
   const int j = pair / a.G, col = r * a.G + pair - j * a.G;
   const size_t step = size_t(a.Hkv) * a.cols;  // records from one part to the next (Hkv / 2 pairs x 2 maps)
+  float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.0f, 0.0f};
+  f32x4 o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  const size_t rec0 = (size_t(job.part0) * (a.Hkv / 2) + j) * 2 * a.cols + col;
+  for (int s = W > 1 ? wave : 0; s < job.nparts; s += 4 * W) {
+    float mN[2][4], lN[2][4];
+    f32x4 oN[2][4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const size_t rec0 = (size_t(job.part0) * (a.Hkv / 2) + j) * 2 * a.cols + size_t(h) * a.cols + col;
-    float M = -INFINITY, L = 0.0f;
-    f32x4 o = {0, 0, 0, 0};
-    for (int s = wave; s < job.nparts; s += 16) {
-      float mN[4], lN[4];
-      f32x4 oN[4];
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // all loads before the first use; slots past the last record weigh nothing
-        const bool in = s + 4 * i < job.nparts;
-        const size_t rec = rec0 + size_t(in ? s + 4 * i : s) * step;
-        mN[i] = in ? a.parts_ml[rec * 2] : -INFINITY;
-        lN[i] = a.parts_ml[rec * 2 + 1];
-        oN[i] = *reinterpret_cast<const f32x4*>(a.parts_o + rec * VD + 4 * lane);
+        const bool in = s + W * i < job.nparts;
+        const size_t rec = rec0 + size_t(h) * a.cols + size_t(in ? s + W * i : s) * step;
+        mN[h][i] = in ? a.parts_ml[rec * 2] : -INFINITY;
+        lN[h][i] = a.parts_ml[rec * 2 + 1];
+        oN[h][i] = *reinterpret_cast<const f32x4*>(a.parts_o + rec * VD + 4 * lane);
       }
-      float Mn = M;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) Mn = fmaxf(Mn, mN[i]);
-      const float c = M == -INFINITY ? 0.0f : fast_exp2(M - Mn);
-      L *= c;
-      o *= c;
-      M = Mn;
+    for (int h = 0; h < 2; ++h) {
+      float Mn = M[h];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) Mn = fmaxf(Mn, mN[h][i]);
+      const float c = M[h] == -INFINITY ? 0.0f : fast_exp2(M[h] - Mn);
+      L[h] *= c;
+      o[h] *= c;
+      M[h] = Mn;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float w = mN[i] == -INFINITY ? 0.0f : fast_exp2(mN[i] - M);
-        L += w * lN[i];
-        o += oN[i] * w;
+        const float w = mN[h][i] == -INFINITY ? 0.0f : fast_exp2(mN[h][i] - Mn);
+        L[h] += w * lN[h][i];
+        o[h] += oN[h][i] * w;
       }
     }
-    *reinterpret_cast<f32x4*>(&o_sh[wave][h][4 * lane]) = o;
-    if (lane == 0) {
-      ml_sh[wave][h][0] = M;
-      ml_sh[wave][h][1] = L;
-    }
   }
-  __syncthreads();
-  if (wave != 0) return;
-  f32x4 o[2];
-  float L[2];
+  if constexpr (W > 1) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float M = fmaxf(fmaxf(ml_sh[0][h][0], ml_sh[1][h][0]), fmaxf(ml_sh[2][h][0], ml_sh[3][h][0]));
-    o[h] = f32x4{0, 0, 0, 0};
-    L[h] = 0.0f;
+    for (int h = 0; h < 2; ++h) {
+      *reinterpret_cast<f32x4*>(&o_sh[wave][h][4 * lane]) = o[h];
+      if (lane == 0) {
+        ml_sh[wave][h][0] = M[h];
+        ml_sh[wave][h][1] = L[h];
+      }
+    }
+    __syncthreads();
+    if (wave != 0) return;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = ml_sh[w][h][0] == -INFINITY ? 0.0f : fast_exp2(ml_sh[w][h][0] - M);
-      L[h] += f * ml_sh[w][h][1];
-      o[h] += *reinterpret_cast<const f32x4*>(&o_sh[w][h][4 * lane]) * f;
+    for (int h = 0; h < 2; ++h) {
+      float Mn = ml_sh[0][h][0];
+#pragma unroll
+      for (int w = 1; w < W; ++w) Mn = fmaxf(Mn, ml_sh[w][h][0]);
+      o[h] = f32x4{0, 0, 0, 0};
+      L[h] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float f = ml_sh[w][h][0] == -INFINITY ? 0.0f : fast_exp2(ml_sh[w][h][0] - Mn);
+        L[h] += f * ml_sh[w][h][1];
+        o[h] += *reinterpret_cast<const f32x4*>(&o_sh[w][h][4 * lane]) * f;
+      }
     }
   }
   diff_finish<DT>(a, job.r0 + r, pair, lane, o[0], L[0], o[1], L[1]);
@@ -391,10 +401,15 @@ hipError_t launch_diff_stream(int dt, const DiffArgs& a, int n_tiles, hipStream_
 }
 
 // n_jobs <= 65535: the caller has checked.
-hipError_t launch_diff_merge(int dt, const DiffArgs& a, const esp_combine* jobs, int n_jobs, hipStream_t st) {
-  const dim3 grid(unsigned(a.R * (a.H / 2)), unsigned(n_jobs));
-  if (dt == ESP_F16) hipLaunchKernelGGL(attn_diff_merge_kernel<ESP_F16>, grid, dim3(256), 0, st, a, jobs);
-  else hipLaunchKernelGGL(attn_diff_merge_kernel<ESP_BF16>, grid, dim3(256), 0, st, a, jobs);
+hipError_t launch_diff_merge(int dt, const DiffArgs& a, const esp_combine* jobs, int n_jobs, int n_parts, hipStream_t st) {
+  const unsigned outs = unsigned(a.R * (a.H / 2)), jobs_n = unsigned(n_jobs);
+  if (n_parts > 4 * n_jobs && size_t(outs) * n_jobs < 2048) {
+    if (dt == ESP_F16) hipLaunchKernelGGL((attn_diff_merge_kernel<ESP_F16, 4>), dim3(outs, jobs_n), dim3(256), 0, st, a, jobs);
+    else hipLaunchKernelGGL((attn_diff_merge_kernel<ESP_BF16, 4>), dim3(outs, jobs_n), dim3(256), 0, st, a, jobs);
+  } else {
+    if (dt == ESP_F16) hipLaunchKernelGGL((attn_diff_merge_kernel<ESP_F16, 1>), dim3((outs + 3) / 4, jobs_n), dim3(256), 0, st, a, jobs);
+    else hipLaunchKernelGGL((attn_diff_merge_kernel<ESP_BF16, 1>), dim3((outs + 3) / 4, jobs_n), dim3(256), 0, st, a, jobs);
+  }
   return hipGetLastError();
 }
 

@@ -54,6 +54,8 @@ struct PlanOptions {
   // 80 -> 72 us, head dim 128: 42.5 -> 36.4 us) and the step with the merge of the partial records behind it does not
   // (79.5 -> 82.9 us, 42.0 -> 43.3 us).
   bool cut_batch = false;
+  // Tiled kernels: tiles in the order of their longest part whatever their tree, longest last.
+  bool by_length = false;
 
   static PlanOptions reference() { return PlanOptions{}; }
   // rows: query rows per tile (decode 1..8 -> 8-row budget is irrelevant; prefill 64/128).
@@ -81,11 +83,12 @@ struct PlanOptions {
   PlanOptions for_diff_tiled() const {
     const PlanOptions had = mi355x(1, groups_target), tiled = mi355x(64, groups_target);
     PlanOptions o = *this;
-    if (!o.balanced || o.item_steps) return o;
+    if (!o.balanced) return o;
+    o.by_length = true;
     auto turn = [](int& field, int from, int to) { field = field == from ? to : field; };
     turn(o.granule, had.granule, tiled.granule);
-    turn(o.min_chunk, had.min_chunk, tiled.min_chunk);
-    turn(o.min_span, had.min_span, tiled.min_span);
+    turn(o.min_chunk, had.min_chunk, 128);  // (100 rows over 1000 keys, 32 / 8 heads: 51 us at 512 and 1024, 35 so; fresh prompts alike)
+    turn(o.min_span, had.min_span, 256);
     turn(o.item_steps, had.item_steps, tiled.item_steps);
     turn(o.part_steps, had.part_steps, tiled.part_steps);
     return o;
@@ -398,6 +401,11 @@ inline void plan_tiles(AttnPlan& A, int groups, int window, const int32_t* pos, 
     std::vector<int> longest(A.trees.size(), 0);
     auto order_records = [&](const std::vector<int>& ns_v) {
       for (int i = 0; i < n_tiles; ++i) emit[size_t(i)] = i;
+      if (o.by_length) {
+        auto part = [&](int i) { return (rts[size_t(i)].span + rts[size_t(i)].batch) / ns_v[size_t(i)]; };
+        std::stable_sort(emit.begin(), emit.end(), [&](int x, int y) { return part(x) < part(y); });
+        return;
+      }
       if (!by_tree) return;
       std::fill(longest.begin(), longest.end(), 0);
       for (int i = 0; i < n_tiles; ++i) {

@@ -30,9 +30,9 @@ _IP = C.POINTER(C.c_int32)
 ENGINE_SYMBOLS = {
     "esp_plan_options_reference": (None, (_PO,)),
     "esp_plan_options_mi355x": (None, (_PO, _I, _I)),
-    "esp_plan_options_diff": (None, (_PO, _AP)),
     "esp_plan_tiles": (C.c_int, (_V, _I, _I, _I, _V, _PO, _V, _I, _IP, _V, _I, _IP, _IP) + _ERR),
     "esp_plan_tiles_for": (C.c_int, (_AP, _V, _I, _I, _I, _V, _PO, _V, _I, _IP, _V, _I, _IP, _IP) + _ERR),
+    "esp_plan_tiles_diff": (C.c_int, (_AP, _V, _I, _I, _I, _V, _PO, _V, _I, _IP, _V, _I, _IP, _IP) + _ERR),
     "esp_plan_lowrank": (C.c_int, (C.POINTER(abi.LowRankParams), _V, _I, _V, _IP, _V, _I, _IP) + _ERR),
     "esp_engine_create": (_V, (_I, _I, _I, _I)),
     "esp_engine_destroy": (None, (_V,)),
@@ -106,16 +106,13 @@ def plan_tiles(trees, groups, window, pos, options):
     lib = engine_lib()
     trees = np.ascontiguousarray(trees, dtype=abi.TREE_DT)
     pos_a = None if pos is None else np.ascontiguousarray(pos, dtype=np.int32)
-    layer = getattr(groups, "layer", None)
+    diff = getattr(groups, "diff", None)
+    layer = diff or getattr(groups, "layer", None)
+    plan = lib.esp_plan_tiles_diff if diff else lib.esp_plan_tiles_for
     p = None
     if layer is not None:
         p = abi.AttnParams()
         p.H, p.Hkv, p.head_dim = layer
-    if getattr(groups, "diff", None) is not None:
-        q = abi.AttnParams()
-        q.H, q.Hkv, q.head_dim = groups.diff
-        options = PlanOptions.from_buffer_copy(options)
-        lib.esp_plan_options_diff(C.byref(options), C.byref(q))
     err = C.create_string_buffer(256)
     nt, nj, npart = C.c_int32(0), C.c_int32(0), C.c_int32(0)
     # Room for one tile per row group and three resident rounds of parts (of a chip as large as any) serves nearly every plan in one
@@ -126,9 +123,8 @@ def plan_tiles(trees, groups, window, pos, options):
     while True:
         tiles = np.empty(n_tiles, abi.TILE_DT)
         jobs = np.empty(n_jobs, abi.COMBINE_DT)
-        rc = lib.esp_plan_tiles_for(p, trees.ctypes.data, len(trees), groups, window, None if pos_a is None else pos_a.ctypes.data,
-                                    C.byref(options), tiles.ctypes.data, n_tiles, C.byref(nt), jobs.ctypes.data, n_jobs, C.byref(nj),
-                                    C.byref(npart), err, 256)
+        rc = plan(p, trees.ctypes.data, len(trees), groups, window, None if pos_a is None else pos_a.ctypes.data, C.byref(options), tiles.ctypes.data,
+                  n_tiles, C.byref(nt), jobs.ctypes.data, n_jobs, C.byref(nj), C.byref(npart), err, 256)
         if rc != abi.ESP_EWORKSPACE or (nt.value <= n_tiles and nj.value <= n_jobs):
             break
         n_tiles, n_jobs = max(n_tiles, nt.value), max(n_jobs, nj.value)

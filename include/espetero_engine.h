@@ -52,11 +52,6 @@ void esp_plan_options_reference(esp_plan_options* o);
 /* Tuned for 256 CUs: rows query rows per tile, workgroups what esp_attn_plan_hint reports for the kernel. */
 void esp_plan_options_mi355x(esp_plan_options* o, int32_t rows, int32_t workgroups);
 
-/* For a pass of esp_attn_diff with the parameters `p`: where its tiled kernel serves them, options for the streaming kernel become
- * those of the tiled one (its tiles may have few rows, by which esp_plan_options_mi355x tells the two apart). Fields that do not hold
- * what that function gave them stay as they are. */
-void esp_plan_options_diff(esp_plan_options* o, const esp_attn_params* p);
-
 /* Plan a pass. trees[n_trees] in; tiles / jobs out (capacities given; on
  * ESP_EWORKSPACE the needed counts are still written). groups: workgroups per
  * tile (KV heads). window > 0 needs pos (4 ints per row). */
@@ -70,6 +65,14 @@ int esp_plan_tiles(const esp_tree* trees, int32_t n_trees, int32_t groups, int32
 int esp_plan_tiles_for(const esp_attn_params* p, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
                        const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                        int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen);
+
+/* The same for a pass of esp_attn_diff (p: its parameters; groups: what esp_attn_diff_hint reports). Options as from
+ * esp_plan_options_mi355x: where the tiled kernel serves p, those of a streaming pass (its tiles may have few rows, by which that
+ * function tells the two apart) become its own, and its tiles come longest last, which is the order the kernel starts them in,
+ * reversed. Fields that do not hold what that function gave them stay as they are. */
+int esp_plan_tiles_diff(const esp_attn_params* p, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
+                        const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
+                        int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen);
 
 /* The tiles of a pass of esp_lowrank_add: the rows that have an adapter, grouped by it (adapters ascending, rows ascending within
  * one), in tiles of p->rows_per_tile rows and fewer at an adapter's end. adapter[n_rows]: each row's, -1 for none; ESP_EINVAL for one
