@@ -7,10 +7,8 @@
 //
 // Streaming kernel: decode and short trees. Bound by HBM: every visible key's 1 KB per KV pair (K1, K2 and V, 16 bits) is read
 // once for both maps and all G query pairs. One workgroup is one tile and one KV pair; up to 8 packed rows (row in tile * G + query
-// pair) of both maps share the 16 columns of a matrix tile: columns 0 .. 7 are the first map's, 8 .. 15 the second's. The Q operand
-// of K1 holds zeros in the second half of the columns and that of K2 in the first, so that
-//   S^T[16 keys][16 columns] = K1 . Q1'^T + K2 . Q2'^T
-// is both maps' scores in one accumulator, one softmax serves them, and P . V is one product for both. A wavefront takes 16-key
+// pair) of both maps share the 16 columns of a matrix tile: columns 0 .. 7 are the first map's, 8 .. 15 the second's. Of the products
+// with K1 and with K2 a lane keeps its own map's, one softmax serves both, and so does one product P . V. A wavefront takes 16-key
 // units round robin straight from HBM (64 registers of operands: 16 KB per wavefront and set) with the next unit's loads in flight.
 #include "diff_math.hpp"
 
@@ -39,8 +37,8 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
   const DiffRange rg = diff_range(tile, tree, a.R, a.window);
   const int cols_live = rg.rows * a.G;
 
-  // ---- this lane's packed rows: Q operands (zero for the other map's keys) and positions
-  u32x4 qf[NC][2][4];
+  // ---- this lane's packed rows: Q operands and positions
+  u32x4 qf[NC][4];
   int qpos[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -50,11 +48,7 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
     qpos[c] = tree.P + rg.rr0 + m;
     const uint16_t* qp = a.Q + size_t(tile.r0 + m) * a.q_ld + size_t(2 * (j * a.G + hg) + map) * HD + 8 * q4;
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const u32x4 q = ok ? *reinterpret_cast<const u32x4*>(qp + 32 * kk) : u32x4{0, 0, 0, 0};
-      qf[c][0][kk] = map == 0 ? q : u32x4{0, 0, 0, 0};
-      qf[c][1][kk] = map == 1 ? q : u32x4{0, 0, 0, 0};
-    }
+    for (int kk = 0; kk < 4; ++kk) qf[c][kk] = ok ? *reinterpret_cast<const u32x4*>(qp + 32 * kk) : u32x4{0, 0, 0, 0};
   }
 
   // ---- 16-key units; interior ones are seen whole by every row of the tile
@@ -80,29 +74,37 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
     for (int mt = 0; mt < MT; ++mt) acc[c][mt] = f32x4{0, 0, 0, 0};
   }
 
-  const int lane_k = c16 * HD + 8 * q4, lane_v = c16 * kVtDim + 4 * q4;
-  const size_t head = size_t(2 * a.bt * HD);  // elements of one (block, KV head)
+  // Where a unit's operands lie: one address for the block's KV pair, everything else are offsets from it.
+  const uint32_t lane_k = uint32_t(c16 * HD + 8 * q4) * 2, lane_v = uint32_t(c16 * kVtDim + 4 * q4) * 2;
+  const uint32_t head = uint32_t(2 * a.bt * HD) * 2, to_v = uint32_t(a.bt * HD) * 2;  // bytes of one (block, KV head); from its K to its V^T
+  const uint64_t block_bytes = uint64_t(a.Hkv) * head;
+  const char* const pool = reinterpret_cast<const char*>(a.pool + a.kv_base) + uint64_t(2 * j) * head;
+  auto block_of = [&](int u) {  // (a sub-block of V^T starts as far behind the first as its first token's K row does)
+    const int key = u << 4, bi = key / a.bt;
+    return pool + uint64_t(uint32_t(diff_block(a, table, bi))) * block_bytes + uint32_t(key - bi * a.bt) * (HD * 2);
+  };
   auto load = [&](int u, DiffUnit& U) {
-    const uint16_t* hb = a.pool + diff_head_base(a, diff_block(a, table, u << 4), 2 * j);
-    const int t0 = (u << 4) % a.bt;
+    const char* const base = block_of(u);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint16_t* kp = hb + h * head + t0 * HD + lane_k;
-      const uint16_t* vp = hb + h * head + vt_elem(a.bt, HD, t0, 0) + lane_v;
+      const char* const kp = base + h * head;
+      const char* const vp = kp + to_v;
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) U.k[h][kk] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + 32 * kk));
+      for (int kk = 0; kk < 4; ++kk) U.k[h][kk] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + lane_k + 64 * kk));
 #pragma unroll
-      for (int mt = 0; mt < 8; ++mt) U.v[8 * h + mt] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(vp + 16 * kVtDim * mt));
+      for (int mt = 0; mt < 8; ++mt) U.v[8 * h + mt] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(vp + lane_v + 32 * kVtDim * mt));
     }
   };
   auto scores = [&](const DiffUnit& U, f32x4 (&s)[NC]) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      s[c] = f32x4{0, 0, 0, 0};
+      f32x4 of[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) s[c] = mfma16x32<DT>(U.k[h][kk], qf[c][h][kk], s[c]);
+        for (int h = 0; h < 2; ++h) of[h] = mfma16x32<DT>(U.k[h][kk], qf[c][kk], of[h]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[c][e] = map ? of[1][e] : of[0][e];
     }
   };
   // Online softmax over scores x (log2 units, -inf where masked), then O^T += V^T . P^T; P in the storage type, which is what the
@@ -176,18 +178,17 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int key = jv + e;
-        bool vis = key >= rg.lo && key < rg.hi && key <= qpos[c];
-        if (a.window > 0) vis = vis && qpos[c] - key < a.window;
-        s[c][e] = vis ? s[c][e] * a.scale_log2 : -INFINITY;
+        // The row sees the keys [from, from + n).
+        const int from = a.window > 0 ? max(rg.lo, qpos[c] - a.window + 1) : rg.lo, n = max(0, min(rg.hi, qpos[c] + 1) - from);
+        s[c][e] = uint32_t(jv + e - from) < uint32_t(n) ? s[c][e] * a.scale_log2 : -INFINITY;
       }
     softmax_pv(U, s, p);
     if (__builtin_expect(rare, 0)) {
-      DiffUnit W;
-      load(u, W);
+      const char* const vp = block_of(u) + to_v + lane_v;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const uint32_t lo = W.v[mt].x & (in[0] | in[1]), hi = W.v[mt].y & (in[2] | in[3]);
+        const u32x2 v = *reinterpret_cast<const u32x2*>(vp + (mt >> 3) * head + 32 * kVtDim * (mt & 7));
+        const uint32_t lo = v.x & (in[0] | in[1]), hi = v.y & (in[2] | in[3]);
 #pragma unroll
         for (int neg = 0; neg < 2; ++neg)
 #pragma unroll
@@ -200,6 +201,7 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
             for (int e = 0; e < 4; ++e)
               if (seen[e] > 0.0f) acc[c][mt][e] += neg ? -INFINITY : INFINITY;
           }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   };

@@ -212,7 +212,7 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
 #pragma unroll
         for (int i = 0; i < 8; ++i) p2 = i == 4 * (t >> 4) + ((t >> 1) & 3) ? P[i >> 2][i & 3] : p2;
         const float p = __shfl((t & 1) ? unpack_hi<DT>(p2) : unpack_lo<DT>(p2), 32 * ((t >> 3) & 1) + (ln & 31));
-        const uint16_t* v = a.pool + diff_head_base(a, diff_block(a, table, key), 2 * j + (w >> 2)) +
+        const uint16_t* v = a.pool + diff_head_base(a, diff_block(a, table, key / a.bt), 2 * j + (w >> 2)) +
                             vt_elem(a.bt, HD, key % a.bt, 32 * (w & 3) + 4 * (ln >> 5));
 #pragma unroll 1
         for (int e = 0; e < 16; ++e) {

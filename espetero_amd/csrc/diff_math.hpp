@@ -30,9 +30,9 @@ struct DiffArgs {
 __device__ __forceinline__ size_t diff_head_base(const DiffArgs& a, int b, int kvh) {
   return size_t(a.kv_base) + (size_t(b) * size_t(a.Hkv) + size_t(kvh)) * size_t(2 * a.bt * kDiffHD);
 }
-__device__ __forceinline__ int diff_block(const DiffArgs& a, int table, int key) {
+// The pool's block behind a tree's block number bi: from its list, or in its slot's ring.
+__device__ __forceinline__ int diff_block(const DiffArgs& a, int table, int bi) {
   using const_i32 = const int32_t __attribute__((address_space(4)));  // read only: scalar loads
-  const int bi = key / a.bt;
   return a.ring ? table + bi % a.ring : ((const_i32*)a.blocks)[table + bi];
 }
 
