@@ -831,7 +831,8 @@ static int check_logits(const esp_logits_params* p, char* err, size_t errlen) {
   if (!p) return fail(err, errlen, ESP_EINVAL, "params is NULL");
   if (p->dtype != ESP_F16 && p->dtype != ESP_BF16 && p->dtype != ESP_F32) return fail(err, errlen, ESP_EINVAL, "dtype %d", p->dtype);
   if (p->vocab <= 0 || p->vocab > INT32_MAX - 65536) return fail(err, errlen, ESP_EINVAL, "vocab %d", p->vocab);
-  if (p->n_slots < 0 || p->n_masks < 0 || p->n_bias < 0) return fail(err, errlen, ESP_EINVAL, "negative count");
+  if (p->n_slots < 0 || p->n_masks < 0 || p->n_bias < 0 || p->n_bias > INT32_MAX - 65536)
+    return fail(err, errlen, ESP_EINVAL, "%d slots, %d masks, %d bias entries", p->n_slots, p->n_masks, p->n_bias);
   return ESP_OK;
 }
 

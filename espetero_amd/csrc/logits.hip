@@ -29,6 +29,17 @@ __device__ __forceinline__ float logit_at(const void* L, size_t i) {
   if constexpr (DT == ESP_F32) return static_cast<const float*>(L)[i];
   else return unpack_lo<DT>(static_cast<const uint16_t*>(L)[i]);
 }
+// 16 bytes at any address, and the logit e of them.
+__device__ __forceinline__ u32x4 load16(const char* p) {
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+template <int DT>
+__device__ __forceinline__ float logit_of(u32x4 v, int e) {
+  if constexpr (DT == ESP_F32) return __uint_as_float(v[e]);
+  else return e & 1 ? unpack_hi<DT>(v[e >> 1]) : unpack_lo<DT>(v[e >> 1]);
+}
 
 }  // namespace
 
@@ -45,62 +56,208 @@ __device__ __forceinline__ float penalised(float x, bool known, bool given, int 
   return x;
 }
 
-template <int DT, bool OUT>
-__global__ __launch_bounds__(256) void logits_kernel(const LogitsArgs a) {
-  __shared__ float bias[kLogitsChunk];
-  __shared__ Best best_sh[4];
-  const int row = blockIdx.y, c0 = blockIdx.x * kLogitsChunk;
-  const esp_logits_row r = a.rows[row];
-  const bool hist = r.slot >= 0 && r.slot < a.n_slots;
-  const uint8_t* prompt = hist ? reinterpret_cast<const uint8_t*>(a.seen + size_t(r.slot) * 2 * a.words) : nullptr;
-  const uint8_t* given = hist ? prompt + size_t(a.words) * 4 : nullptr;
-  const int32_t* counts = hist ? a.counts + size_t(r.slot) * a.vocab : nullptr;
-  const uint8_t* mask = r.mask >= 0 && r.mask < a.n_masks ? reinterpret_cast<const uint8_t*>(a.masks + size_t(r.mask) * a.words) : nullptr;
-  // The row's bias entries that fall into this chunk.
-  const int e0 = max(r.bias0, 0), e1 = r.n_bias > 0 ? int(min(int64_t(a.n_bias), int64_t(r.bias0) + r.n_bias)) : e0;
-  bool any = false;
-  if (e1 > e0) {  // the same for the whole workgroup
-    for (int i = threadIdx.x; i < kLogitsChunk; i += 256) bias[i] = 0.0f;
-    __syncthreads();
-    for (int e = e0 + int(threadIdx.x); e < e1; e += 256) {
-      const int t = a.bias_tokens[e] - c0;
-      if (t >= 0 && t < kLogitsChunk) {
-        bias[t] = a.bias_values[e];
-        any = true;
-      }
-    }
-    any = __syncthreads_or(any);
-  }
-  Best best{-INFINITY, INT32_MAX};
-  for (int i = threadIdx.x * 8; i < kLogitsChunk; i += 256 * 8) {
-    const int t0 = c0 + i, n = min(8, a.vocab - t0);
-    if (n <= 0) break;
-    const uint32_t pb = hist ? prompt[t0 / 8] : 0u, gb = hist ? given[t0 / 8] : 0u, mb = mask ? mask[t0 / 8] : 255u;
-    for (int e = 0; e < n; ++e) {
-      const int t = t0 + e;
-      float x = logit_at<DT>(a.logits, size_t(row) * a.in_ld + t);
-      const bool gv = gb >> e & 1, kn = gv || (pb >> e & 1);
-      x = penalised(x, kn, gv, gv ? counts[t] : 0, r.repetition, r.frequency, r.presence);
-      if (any && e1 > e0) x = x + bias[i + e];
-      if (!(mb >> e & 1)) x = -INFINITY;
-      if constexpr (OUT) a.out[size_t(row) * a.out_ld + t] = x;
-      if (x > best.v) best = Best{x, t};
-    }
-  }
-  best = wave_best(best);
-  if ((threadIdx.x & 63) == 0) best_sh[threadIdx.x >> 6] = best;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    best = better(better(best_sh[0], best_sh[1]), better(best_sh[2], best_sh[3]));
-    a.part_v[size_t(row) * gridDim.x + blockIdx.x] = best.v;
-    a.part_t[size_t(row) * gridDim.x + blockIdx.x] = best.t;
-  }
-}
-
 __device__ __forceinline__ void record_token(uint32_t* seen, int32_t* counts, int vocab, int words, int n_slots, int slot, int t, bool given) {
   if (slot < 0 || slot >= n_slots || t < 0 || t >= vocab) return;
   atomicOr(seen + (size_t(slot) * 2 + (given ? 1 : 0)) * words + t / 32, 1u << (t & 31));
   if (given) atomicAdd(counts + size_t(slot) * vocab + t, 1);
+}
+
+// A workgroup of W threads takes 32 W tokens of a row at a time: a chunk of its own (SOLO = false), or all of the row's, one after
+// the other, and then the row's token too (SOLO).
+template <int DT, bool OUT, int W, bool SOLO>
+__global__ __launch_bounds__(W) void logits_kernel(const LogitsArgs a) {
+  constexpr int CH = 32 * W, VT = DT == ESP_F32 ? 4 : 8, U = 32 / VT;  // tokens of a chunk, of a load, loads of a thread
+  __shared__ uint16_t list[CH];                                          // the chunk's tokens that only the penalties touch
+  __shared__ uint32_t skip_sh[W + 1], allowed_sh[W + 1], known_sh[W], given_sh[W], biased_sh[W];
+  __shared__ float best_sh[W / 64];
+  __shared__ int n_list, token_sh;
+  const int row = blockIdx.y, tid = threadIdx.x;
+  const char* const in = static_cast<const char*>(a.logits) + size_t(row) * a.in_ld * (16 / VT);
+  float* const out = OUT ? a.out + size_t(row) * a.out_ld : nullptr;
+  // A chunk's logits are on their way while the words of bits are looked at, the first ones before the row's record. A load that
+  // would reach over the chunk's n tokens is moved back to end there, and those behind it do the same again: nothing comes of
+  // seeing a token twice, and no load waits for a branch.
+  u32x4 x[U];
+  auto at = [&](int u, int n) { return max(0, min((u * W + tid) * VT, n - VT)); };
+  auto load_at = [&](int c0, int n, int at) {
+    if (n >= VT) return load16(in + size_t(c0) * (16 / VT) + uint32_t(at * (16 / VT)));
+    u32x4 few;  // the vocabulary's last few
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (DT == ESP_F32) {
+        few[e] = e < n ? reinterpret_cast<const uint32_t*>(in)[c0 + e] : 0u;
+      } else {
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(in) + c0 + 2 * e;
+        few[e] = (2 * e < n ? p[0] : 0u) | (2 * e + 1 < n ? uint32_t(p[1]) << 16 : 0u);
+      }
+    }
+    return few;
+  };
+  auto load = [&](int c0) {
+    const int n = min(CH, a.vocab - c0);
+    if (n >= VT) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = load_at(c0, VT, at(u, n));
+    } else {
+      x[0] = load_at(c0, n, 0);
+#pragma unroll
+      for (int u = 1; u < U; ++u) x[u] = x[0];
+    }
+  };
+  int c0 = SOLO ? 0 : int(blockIdx.x) * CH;
+  load(c0);
+  __builtin_amdgcn_sched_barrier(0);
+  const esp_logits_row r = a.rows[row];
+  const bool hist = r.slot >= 0 && r.slot < a.n_slots;
+  const uint32_t* prompt = a.seen + (hist ? size_t(r.slot) * 2 * a.words : 0);
+  const int32_t* counts = a.counts + (hist ? size_t(r.slot) * a.vocab : 0);
+  const bool masked = r.mask >= 0 && r.mask < a.n_masks;
+  const uint32_t* mask = a.masks + (masked ? size_t(r.mask) * a.words : 0);
+  // The row's bias entries that there are.
+  const int64_t e0 = max(r.bias0, 0), e1 = min(int64_t(a.n_bias), int64_t(r.bias0) + r.n_bias);
+  const int n_bias = r.n_bias > 0 && e1 > e0 ? int(e1 - e0) : 0;
+  const int32_t* bias_tokens = a.bias_tokens + (n_bias ? e0 : 0);
+  const float* bias_values = a.bias_values + (n_bias ? e0 : 0);
+  Best best{-INFINITY, INT32_MAX};
+  for (;;) {
+    const int n = min(CH, a.vocab - c0);  // the chunk's tokens
+    auto bits_at = [&](const uint32_t* sh, int i) { return uint32_t((uint64_t(sh[(i >> 5) + 1]) << 32 | sh[i >> 5]) >> (i & 31)); };
+    const int w = c0 / 32 + tid, left = n - 32 * tid;
+    const uint32_t real = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u;
+    uint32_t known = 0, given = 0, allowed = real;
+    uint32_t first = ~0u;  // the thread's first bias entry
+    if (real) {
+      uint32_t ok = ~0u;
+      if (hist) known = prompt[w], given = prompt[a.words + w];
+      if (masked) ok = mask[w];
+      known |= given;
+      allowed &= ok;
+    }
+    if (tid < n_bias) first = uint32_t(bias_tokens[tid]) - uint32_t(c0);
+    biased_sh[tid] = 0;
+    if (tid == 0) n_list = 0, token_sh = INT32_MAX, skip_sh[W] = allowed_sh[W] = 0;
+    __syncthreads();
+    if (n_bias) {  // the same for the whole workgroup
+      for (int e = tid; e < n_bias; e += W) {
+        const uint32_t t = e == tid ? first : uint32_t(bias_tokens[e]) - uint32_t(c0);
+        if (t < uint32_t(n)) atomicOr(&biased_sh[t >> 5], 1u << (t & 31));
+      }
+      __syncthreads();
+    }
+    {
+      const uint32_t biased = biased_sh[tid];
+      uint32_t mine = known & allowed & ~biased;
+      allowed_sh[tid] = allowed;
+      known_sh[tid] = known;
+      given_sh[tid] = given;
+      skip_sh[tid] = known | biased | ~allowed;
+      // Where in the list the thread's tokens go: behind those of the lanes below, and those behind the other wavefronts' as they come.
+      const int lane = tid & 63, have = __popc(mine);
+      int upto = have;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int below = __shfl_up(upto, d);
+        if (lane >= d) upto += below;
+      }
+      int to = 0;
+      if (lane == 63) to = atomicAdd(&n_list, upto);
+      for (to = __shfl(to, 63) + upto - have; mine; mine &= mine - 1) list[to++] = uint16_t(32 * tid + __ffs(mine) - 1);
+    }
+    __syncthreads();
+    // The tokens that nothing but the mask touches.
+    float most = -INFINITY;
+    int where = 0;  // of the largest, and the load it came with
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t skip = bits_at(skip_sh, at(u, n));
+      float top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < VT; ++e) top = fmaxf(top, skip >> e & 1 ? -INFINITY : logit_of<DT>(x[u], e));
+      where = top > most ? u : where;
+      most = fmaxf(most, top);
+      if constexpr (OUT) {
+        const uint32_t ok = bits_at(allowed_sh, at(u, n));
+        float y[VT];
+#pragma unroll
+        for (int e = 0; e < VT; ++e) y[e] = ok >> e & 1 ? logit_of<DT>(x[u], e) : -INFINITY;
+        if (n >= VT) {
+          if ((u * W + tid) * VT < n) __builtin_memcpy(out + c0 + uint32_t(at(u, n)), y, sizeof y);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VT; ++e)
+            if (e < n) out[c0 + e] = y[e];
+        }
+      }
+    }
+    if constexpr (OUT) __syncthreads();  // what follows writes over some of these
+    // The others, spread over the lanes whichever tokens they are, a few of a lane's on their way at once; past the list's end the
+    // last again.
+    constexpr int B = SOLO ? 2 : 4;
+    Best other{-INFINITY, INT32_MAX};
+    auto given_times = [&](int i) { return (counts + c0)[given_sh[i >> 5] >> (i & 31) & 1 ? uint32_t(i) : 0u]; };
+    auto penalty = [&](float v, int i, bool known, int times) {
+      return penalised(v, known, given_sh[i >> 5] >> (i & 31) & 1, times, r.repetition, r.frequency, r.presence);
+    };
+    auto done = [&](int i, float y) {
+      if constexpr (OUT) (out + c0)[uint32_t(i)] = y;
+      other = better(other, Best{y, c0 + i});
+    };
+    const int listed = n_list;
+    for (int k = tid; k < listed; k += B * W) {
+      int i[B], times[B];
+      float v[B];
+#pragma unroll
+      for (int j = 0; j < B; ++j) i[j] = list[min(k + j * W, listed - 1)];
+#pragma unroll
+      for (int j = 0; j < B; ++j) v[j] = logit_at<DT>(in + size_t(c0) * (16 / VT), uint32_t(i[j])), times[j] = given_times(i[j]);
+#pragma unroll
+      for (int j = 0; j < B; ++j) done(i[j], penalty(v[j], i[j], true, times[j]));
+    }
+    for (int k = tid; k < n_bias; k += W) {
+      const uint32_t t = k == tid ? first : uint32_t(bias_tokens[k]) - uint32_t(c0);
+      if (t >= uint32_t(n) || !(allowed_sh[t >> 5] >> (t & 31) & 1)) continue;
+      const int i = int(t);
+      const float v = logit_at<DT>(in + size_t(c0) * (16 / VT), t);
+      done(i, penalty(v, i, known_sh[i >> 5] >> (i & 31) & 1, hist ? given_times(i) : 0) + bias_values[k]);
+    }
+    if (a.tokens) {  // the same for every workgroup
+      float v = fmaxf(most, other.v);
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+      if ((tid & 63) == 0) best_sh[tid >> 6] = v;
+      __syncthreads();
+      v = best_sh[0];
+#pragma unroll
+      for (int i = 1; i < W / 64; ++i) v = fmaxf(v, best_sh[i]);
+      // Only lanes that hold the chunk's best logit look for its token, in the load that it came with.
+      if (v > -INFINITY) {
+        int t = other.v == v ? other.t : INT32_MAX;
+        if (most == v) {
+          const int i = at(where, n);
+          const u32x4 again = load_at(c0, n, i);
+          const uint32_t skip = bits_at(skip_sh, i);
+#pragma unroll
+          for (int e = VT - 1; e >= 0; --e) t = (int(~skip >> e & 1) & int(logit_of<DT>(again, e) == v)) ? min(t, c0 + i + e) : t;
+        }
+        if (t != INT32_MAX) atomicMin(&token_sh, t);
+      }
+      __syncthreads();
+      if (v > best.v) best = Best{v, token_sh};
+    }
+    c0 += CH;
+    if (!SOLO || c0 >= a.vocab) break;
+    load(c0);
+    __syncthreads();
+  }
+  if (tid != 0 || !a.tokens) return;
+  if constexpr (SOLO) {
+    const int t = best.t == INT32_MAX ? -1 : best.t;
+    a.tokens[row] = t;
+    if (a.record) record_token(a.seen, a.counts, a.vocab, a.words, a.n_slots, r.slot, t, true);
+  } else {
+    a.part_v[size_t(row) * gridDim.x + blockIdx.x] = best.v;
+    a.part_t[size_t(row) * gridDim.x + blockIdx.x] = best.t;
+  }
 }
 
 // One wavefront per row: the best of the chunks' best.
@@ -130,21 +287,27 @@ __global__ __launch_bounds__(256) void history_clear_kernel(uint32_t* seen, int3
   }
 }
 
-hipError_t launch_logits(int dt, const LogitsArgs& a, int n_rows, hipStream_t st) {
-  const int chunks = logits_chunks(a.vocab);
-  const dim3 grid{unsigned(chunks), unsigned(n_rows)}, block{256};
-  if (a.out) {
-    if (dt == ESP_F32) hipLaunchKernelGGL((logits_kernel<ESP_F32, true>), grid, block, 0, st, a);
-    else if (dt == ESP_F16) hipLaunchKernelGGL((logits_kernel<ESP_F16, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((logits_kernel<ESP_BF16, true>), grid, block, 0, st, a);
+template <int DT>
+static void run_logits(const LogitsArgs& a, int n_rows, bool solo, hipStream_t st) {
+  if (solo) {
+    const dim3 grid{1, unsigned(n_rows)}, block{kLogitsSolo};
+    if (a.out) hipLaunchKernelGGL((logits_kernel<DT, true, kLogitsSolo, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((logits_kernel<DT, false, kLogitsSolo, true>), grid, block, 0, st, a);
   } else {
-    if (dt == ESP_F32) hipLaunchKernelGGL((logits_kernel<ESP_F32, false>), grid, block, 0, st, a);
-    else if (dt == ESP_F16) hipLaunchKernelGGL((logits_kernel<ESP_F16, false>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((logits_kernel<ESP_BF16, false>), grid, block, 0, st, a);
+    const dim3 grid{unsigned(logits_chunks(a.vocab)), unsigned(n_rows)}, block{kLogitsChunk / 32};
+    if (a.out) hipLaunchKernelGGL((logits_kernel<DT, true, kLogitsChunk / 32, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((logits_kernel<DT, false, kLogitsChunk / 32, false>), grid, block, 0, st, a);
   }
+}
+
+hipError_t launch_logits(int dt, const LogitsArgs& a, int n_rows, hipStream_t st) {
+  const bool solo = logits_solo(a.vocab, n_rows, a.record != 0);
+  if (dt == ESP_F32) run_logits<ESP_F32>(a, n_rows, solo, st);
+  else if (dt == ESP_F16) run_logits<ESP_F16>(a, n_rows, solo, st);
+  else run_logits<ESP_BF16>(a, n_rows, solo, st);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !a.tokens) return e;
-  hipLaunchKernelGGL(logits_pick_kernel, dim3(unsigned(n_rows)), dim3(64), 0, st, a, chunks);
+  if (e != hipSuccess || !a.tokens || solo) return e;
+  hipLaunchKernelGGL(logits_pick_kernel, dim3(unsigned(n_rows)), dim3(64), 0, st, a, logits_chunks(a.vocab));
   return hipGetLastError();
 }
 

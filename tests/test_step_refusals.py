@@ -179,7 +179,7 @@ def logits_params(**kw):
     return p
 
 
-@pytest.mark.parametrize("p", [dict(dtype=3), dict(vocab=0), dict(vocab=2**31 - 1), dict(n_slots=-1), dict(n_masks=-1), dict(n_bias=-1), dict(in_ld=99),
+@pytest.mark.parametrize("p", [dict(dtype=3), dict(vocab=0), dict(vocab=2**31 - 1), dict(n_slots=-1), dict(n_masks=-1), dict(n_bias=-1), dict(n_bias=2**31 - 1), dict(in_ld=99),
                                dict(out_ld=99)])
 def test_logits_refuses_parameters(p):
     assert call("esp_logits_process", *logits_args(logits_params(**p)))[0] == 1
