@@ -41,7 +41,7 @@ hipError_t launch_diff_tiled(int dt, const DiffArgs& a, int n_tiles, hipStream_t
 hipError_t launch_diff_merge(int dt, const DiffArgs& a, const esp_combine* jobs, int n_jobs, int n_parts, hipStream_t st);
 hipError_t diff_init_attributes();
 hipError_t diff_tiled_init_attributes();
-hipError_t launch_lowrank(int dt, const LowRankArgs& a, int n_tiles, hipStream_t st);
+hipError_t launch_lowrank(int dt, const LowRankArgs& a, int rows_per_tile, int n_tiles, hipStream_t st);
 hipError_t launch_logits(int dt, const LogitsArgs& a, int n_rows, hipStream_t st);
 hipError_t launch_history_record(const esp_logits_params* p, uint32_t* seen, int32_t* counts, const int32_t* tokens, const int32_t* slots, int n,
                                  int given, hipStream_t st);
@@ -791,8 +791,9 @@ int esp_lowrank_add(const esp_lowrank_params* p, const void* X, const void* A, c
                     char* err, size_t errlen) {
   if (int rc = check_lowrank(p, err, errlen)) return rc;
   if (n_slots < 0 || n_tiles < 0) return fail(err, errlen, ESP_EINVAL, "negative count");
-  if (p->rows_per_tile != 16) return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_lowrank_rows)", p->rows_per_tile);
+  if (p->rows_per_tile != 16 && p->rows_per_tile != 64) return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_lowrank_rows)", p->rows_per_tile);
   if (n_tiles == 0) return ESP_OK;
+  if (n_tiles > 65535) return fail(err, errlen, ESP_EUNSUPPORTED, "%d tiles (at most 65535)", n_tiles);
   if (n_slots == 0) return fail(err, errlen, ESP_EINVAL, "%d tiles without rows", n_tiles);
   if (!X || !A || !B || !scale || !Y || !order || !tiles) return fail(err, errlen, ESP_EINVAL, "X, A, B, scale, Y, order, tiles must not be NULL");
   if ((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(workspace)) % 16)
@@ -815,14 +816,14 @@ int esp_lowrank_add(const esp_lowrank_params* p, const void* X, const void* A, c
   a.x_ld = p->x_ld;
   a.y_ld = p->y_ld;
   a.n_slots = n_slots;
-  a.splits = esp::lowrank_splits(p->D, n_tiles);
+  a.splits = esp::lowrank_splits(p->D, a.n_low, p->rows_per_tile, n_tiles);
   a.chunk = esp::lowrank_chunk(p->D, a.splits);
   for (int s = 0; s < p->n_slices; ++s) {
     a.y_off[s] = p->y_off[s];
     a.width[s] = p->width[s];
     a.n_out += p->width[s];
   }
-  const hipError_t e = esp::launch_lowrank(p->dtype, a, n_tiles, static_cast<hipStream_t>(stream));
+  const hipError_t e = esp::launch_lowrank(p->dtype, a, p->rows_per_tile, n_tiles, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? ESP_OK : hip_fail(err, errlen, "lowrank launch", e);
 }
 
