@@ -62,13 +62,13 @@ __device__ __forceinline__ void record_token(uint32_t* seen, int32_t* counts, in
   if (given) atomicAdd(counts + size_t(slot) * vocab + t, 1);
 }
 
-// A workgroup of W threads takes 32 W tokens of a row at a time: a chunk of its own (SOLO = false), or all of the row's, one after
+// A workgroup of W threads takes TP W tokens of a row at a time: a chunk of its own (SOLO = false), or all of the row's, one after
 // the other, and then the row's token too (SOLO).
-template <int DT, bool OUT, int W, bool SOLO>
+template <int DT, bool OUT, int W, int TP, bool SOLO>
 __global__ __launch_bounds__(W) void logits_kernel(const LogitsArgs a) {
-  constexpr int CH = 32 * W, VT = DT == ESP_F32 ? 4 : 8, U = 32 / VT;  // tokens of a chunk, of a load, loads of a thread
+  constexpr int CH = TP * W, NW = CH / 32, VT = DT == ESP_F32 ? 4 : 8, U = TP / VT;  // tokens of a chunk, its words of bits, tokens of a load, loads of a thread
   __shared__ uint16_t list[CH];                                          // the chunk's tokens that only the penalties touch
-  __shared__ uint32_t skip_sh[W + 1], allowed_sh[W + 1], known_sh[W], given_sh[W], biased_sh[W];
+  __shared__ uint32_t skip_sh[NW + 1], allowed_sh[NW + 1], known_sh[NW], given_sh[NW], biased_sh[NW];
   __shared__ float best_sh[W / 64];
   __shared__ int n_list, token_sh;
   const int row = blockIdx.y, tid = threadIdx.x;
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(W) void logits_kernel(const LogitsArgs a) {
   for (;;) {
     const int n = min(CH, a.vocab - c0);  // the chunk's tokens
     auto bits_at = [&](const uint32_t* sh, int i) { return uint32_t((uint64_t(sh[(i >> 5) + 1]) << 32 | sh[i >> 5]) >> (i & 31)); };
-    const int w = c0 / 32 + tid, left = n - 32 * tid;
+    const int w = c0 / 32 + tid, left = tid < NW ? n - 32 * tid : 0;
     const uint32_t real = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u;
     uint32_t known = 0, given = 0, allowed = real;
     uint32_t first = ~0u;  // the thread's first bias entry
@@ -134,8 +134,8 @@ __global__ __launch_bounds__(W) void logits_kernel(const LogitsArgs a) {
       allowed &= ok;
     }
     if (tid < n_bias) first = uint32_t(bias_tokens[tid]) - uint32_t(c0);
-    biased_sh[tid] = 0;
-    if (tid == 0) n_list = 0, token_sh = INT32_MAX, skip_sh[W] = allowed_sh[W] = 0;
+    if (tid < NW) biased_sh[tid] = 0;
+    if (tid == 0) n_list = 0, token_sh = INT32_MAX, skip_sh[NW] = allowed_sh[NW] = 0;
     __syncthreads();
     if (n_bias) {  // the same for the whole workgroup
       for (int e = tid; e < n_bias; e += W) {
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(W) void logits_kernel(const LogitsArgs a) {
       }
       __syncthreads();
     }
-    {
+    if (tid < NW) {
       const uint32_t biased = biased_sh[tid];
       uint32_t mine = known & allowed & ~biased;
       allowed_sh[tid] = allowed;
@@ -291,12 +291,12 @@ template <int DT>
 static void run_logits(const LogitsArgs& a, int n_rows, bool solo, hipStream_t st) {
   if (solo) {
     const dim3 grid{1, unsigned(n_rows)}, block{kLogitsSolo};
-    if (a.out) hipLaunchKernelGGL((logits_kernel<DT, true, kLogitsSolo, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((logits_kernel<DT, false, kLogitsSolo, true>), grid, block, 0, st, a);
+    if (a.out) hipLaunchKernelGGL((logits_kernel<DT, true, kLogitsSolo, 32, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((logits_kernel<DT, false, kLogitsSolo, 32, true>), grid, block, 0, st, a);
   } else {
-    const dim3 grid{unsigned(logits_chunks(a.vocab)), unsigned(n_rows)}, block{kLogitsChunk / 32};
-    if (a.out) hipLaunchKernelGGL((logits_kernel<DT, true, kLogitsChunk / 32, false>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((logits_kernel<DT, false, kLogitsChunk / 32, false>), grid, block, 0, st, a);
+    const dim3 grid{unsigned(logits_chunks(a.vocab)), unsigned(n_rows)}, block{256};
+    if (a.out) hipLaunchKernelGGL((logits_kernel<DT, true, 256, kLogitsChunk / 256, false>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((logits_kernel<DT, false, 256, kLogitsChunk / 256, false>), grid, block, 0, st, a);
   }
 }
 

@@ -33,7 +33,7 @@ constexpr int lowrank_low_groups(int n_low) { return ((n_low + 15) / 16 + lowran
 // How many ways D is split, with 128 dims or more each: of few rows so often that the first launch has two workgroups for every
 // compute unit, of many eight times, once for each XCD.
 inline int lowrank_splits(int D, int n_low, int rows_per_tile, int n_tiles) {
-  const int wgs = std::max(1, n_tiles * lowrank_low_groups(n_low)), want = rows_per_tile == 16 ? std::min(16, (512 + wgs - 1) / wgs) : 8;
+  const int wgs = std::max(1, n_tiles * lowrank_low_groups(n_low)), want = rows_per_tile == 16 ? std::min(8, (512 + wgs - 1) / wgs) : 8;
   return std::max(1, std::min(D / 128, want));
 }
 // Whether one launch does both products, each workgroup of it the first one for itself.
@@ -41,12 +41,16 @@ inline bool lowrank_fused(int D, int rank, int n_slices, const int32_t* width, i
   int64_t wgs = 0;
   for (int s = 0; s < n_slices; ++s) wgs += (width[s] + 1023) / 1024;
   wgs *= n_tiles;
-  return rank <= 64 && (wgs + 255) / 256 * rank * D <= 32 * 1024;
+  return rank <= 32 && (wgs + 255) / 256 * rank * D <= 32 * 1024;
+}
+// Blocks of columns that a workgroup of the second launch takes one after the other, with one sum of its tile's splits.
+constexpr int lowrank_blocks_each(int row_blocks, int n_tiles, int blocks) {
+  return row_blocks == 1 ? 1 : std::max(1, std::min(8, int(int64_t(n_tiles) * blocks / 512)));
 }
 constexpr int lowrank_rows(int n_rows) { return n_rows <= 0 ? 0 : n_rows <= 128 ? 16 : 64; }
 inline size_t lowrank_workspace(const esp_lowrank_params& p, int n_tiles, int n_slots) {
   return size_t(lowrank_splits(p.D, p.n_slices * p.rank, p.rows_per_tile, n_tiles)) * size_t(n_slots) * size_t(p.n_slices * p.rank) * sizeof(float);
 }
-inline int lowrank_chunk(int D, int splits) { return ((D + splits - 1) / splits + 31) / 32 * 32; }
+inline int lowrank_chunk(int D, int splits) { return ((D + splits - 1) / splits + 127) / 128 * 128; }
 
 }  // namespace esp
