@@ -871,7 +871,7 @@ int esp_logits_process(const esp_logits_params* p, const void* logits, float* ou
   a.seen = seen;
   a.counts = counts;
   a.part_v = static_cast<float*>(workspace);
-  a.part_t = static_cast<int32_t*>(workspace) + size_t(esp::logits_chunks(p->vocab)) * size_t(n_rows);
+  a.part_t = static_cast<int32_t*>(workspace) + size_t(esp::logits_shape(p->vocab, n_rows).chunks) * size_t(n_rows);
   a.vocab = p->vocab;
   a.words = esp::logits_words(p->vocab);
   a.in_ld = p->in_ld;

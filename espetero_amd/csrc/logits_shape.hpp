@@ -9,9 +9,6 @@
 
 namespace esp {
 
-constexpr int kLogitsChunk = 8192;  // tokens of a workgroup where several share a row
-constexpr int kLogitsSolo = 1024;   // threads of a workgroup that has a row to itself
-
 struct LogitsArgs {
   const void* logits;
   float* out;
@@ -28,10 +25,15 @@ struct LogitsArgs {
 };
 
 constexpr int logits_words(int vocab) { return (vocab + 31) / 32; }
-constexpr int logits_chunks(int vocab) { return (vocab + kLogitsChunk - 1) / kLogitsChunk; }
-// Whether a workgroup has a row to itself. A row's token joins a history that other rows may name too only when all rows have been
-// read: with several rows that is the second launch's work.
-constexpr bool logits_solo(int vocab, int n_rows, bool record) { return vocab <= 65536 && (n_rows == 1 || !record); }
-constexpr size_t logits_workspace(int vocab, int n_rows) { return size_t(logits_chunks(vocab)) * size_t(n_rows) * 8; }
+// Tokens of a thread and the chunks of 256 times as many that a row becomes: a small pass has as many workgroups as it can, a large one
+// less to do for each beside its tokens.
+struct LogitsShape {
+  int tokens, chunks;
+};
+inline LogitsShape logits_shape(int vocab, int n_rows) {
+  const int tokens = int64_t(vocab) * n_rows <= 12 << 20 ? 8 : 16;
+  return {tokens, (vocab + 256 * tokens - 1) / (256 * tokens)};
+}
+inline size_t logits_workspace(int vocab, int n_rows) { return size_t(logits_shape(vocab, n_rows).chunks) * size_t(n_rows) * 8; }
 
 }  // namespace esp
