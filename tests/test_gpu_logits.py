@@ -213,3 +213,29 @@ def test_a_captured_step_goes_on_from_the_history_it_leaves():
         for r, t in zip(c.rows, tokens):
             c.counts[r["slot"], t] += 1
     assert (c.dcounts.cpu().numpy() == c.counts).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_a_pass_of_many_tokens(dtype):
+    Case(97, 131001, dtype, seed=9, bias=300, in_ld=131003, out_ld=131002).check()
+
+
+@pytest.mark.parametrize("share", [0.0, 0.5, 1.0])
+def test_histories_from_empty_to_every_token(share):
+    for dtype in (BF16, F32):
+        c = Case(4, 4099, dtype, seed=10, bias=400)
+        rng = np.random.default_rng(11)
+        c.prompt = rng.random(c.prompt.shape) < share
+        c.counts = np.where(rng.random(c.counts.shape) < share, c.counts + 1, 0).astype(np.int32)
+        c.check()
+
+
+def test_bits_behind_the_vocabulary_are_not_looked_at():
+    c = Case(3, 1001, F32, seed=12)
+    want, tokens = c.expected()
+    c.prepare()
+    for words_ in (c.seen.view(-1, c.seen.shape[-1]), c.masks):
+        words_[:, -1] |= -(1 << (1001 % 32))
+    c.run()
+    torch.cuda.synchronize()
+    assert np.array_equal(c.out.cpu().numpy(), want) and (c.tokens.cpu().numpy() == tokens).all()

@@ -103,6 +103,22 @@ def test_prompts(counts, dtype):
     Case(rng.permutation(adapter), 320, 8, QKV, dtype, 3, seed=3).check()   # rows of one adapter anywhere in the batch
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D,rank,slices,counts,y_ld", [
+    (1000, 128, [(7, 300), (320, 5)], [150, 3], 331), (264, 24, [(0, 1)], [130], 1), (40, 64, [(1, 2), (3, 1), (10, 129)], [129, 64, 65], 139),
+    (8, 8, [(0, 127), (130, 129)], [200, 1], 261), (512, 16, [(0, 2048), (2048, 513)], [1500, 1400], 2561), (2560, 16, [(5, 260)], [63, 129, 128], 400)])
+def test_tiles_of_64_rows(D, rank, slices, counts, y_ld, dtype):
+    adapter = np.random.default_rng(D).permutation(np.concatenate([np.full(n, a) for a, n in enumerate(counts)] + [[-1]]))
+    Case(adapter, D, rank, slices, dtype, len(counts), seed=D, y_ld=y_ld).check()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D,rank", [(8, 8), (24, 16), (32, 24), (56, 8), (520, 32), (2048, 16), (4096, 8)])
+def test_one_launch_for_little_of_a(D, rank, dtype):
+    for adapter in ([0], [1] * 16 + [0] * 3):
+        Case(adapter, D, rank, [(3, 1030), (1040, 1), (1050, 17)], dtype, 2, seed=D, y_ld=1067).check()
+
+
 def test_many_adapters_and_strides():
     rng = np.random.default_rng(0)
     Case(rng.integers(-1, 40, 100), 512, 16, QKV, BF16, 40, seed=4, x_ld=520, y_ld=391).check()
@@ -113,16 +129,20 @@ def test_intermediates_outside_the_range_of_fp16():
         Case([0, 1, 0, -1], 512, 16, QKV, F16, 2, seed=5, x_scale=x).check()
     for x in (1e20, 1e-20):
         Case([0, 1, 0, -1], 512, 16, QKV, BF16, 2, seed=6, x_scale=x).check()
+    for dtype, x in ((F16, 3000.0), (F16, 1e-6), (BF16, 1e20), (BF16, 1e-20)):
+        Case([0] * 5, 4096, 16, QKV, dtype, 1, seed=5, x_scale=x).check()
+        Case([0, 1] * 70, 512, 16, QKV, dtype, 2, seed=5, x_scale=x).check()
 
 
-def test_a_row_of_infinities_stays_in_its_row():
-    c = Case([0] * 20, 256, 16, QKV, BF16, 1, seed=7)
+@pytest.mark.parametrize("n,D,rank", [(20, 256, 16), (20, 2048, 40), (150, 256, 16)])
+def test_a_row_of_infinities_stays_in_its_row(n, D, rank):
+    c = Case([0] * n, D, rank, QKV, BF16, 1, seed=7)
     clean = c.check()
     c.X[3, 7], c.X[11, 9] = 0x7F80, 0x7FC0
     c.prepare().run()
     torch.cuda.synchronize()
     got = c.dY.cpu().numpy()
-    keep = [r for r in range(20) if r not in (3, 11)]
+    keep = [r for r in range(n) if r not in (3, 11)]
     assert (got[keep] == clean[keep]).all()
     assert not np.isfinite(got[3]).any() and np.isnan(got[11]).all()
 

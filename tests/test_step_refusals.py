@@ -164,6 +164,48 @@ def test_lowrank_plan():
     assert m.value == len(tiles)
 
 
+@pytest.mark.parametrize("window", [0, 200])
+@pytest.mark.parametrize("heads", [(8, 4), (32, 4), (64, 2)])
+@pytest.mark.parametrize("seqs", [[(0, 1)], [(900, 1), (5000, 1), (17, 1)], [(3000, 5)] * 3, [(0, 700), (40, 33), (2000, 129)], [(12000, 500)], [(0, 1), (30000, 64)]])
+def test_diff_plans_cover_every_key_once(seqs, heads, window):
+    p = synth.make_params(*heads, 128, abi.ESP_F16, 16, window=window, rows_per_tile=1)
+    p.rows_per_tile = device.attn_diff_rows(p, max(M for _, M in seqs))
+    trees, at, used = np.zeros(len(seqs), abi.TREE_DT), 0, 0
+    for i, (P, M) in enumerate(seqs):
+        trees[i] = (at, P, used, M)
+        at, used = at + M, used + -(-(P + M) // 16)
+    pos = np.zeros((at, 4), np.int32)
+    for b, P, _, M in trees:
+        pos[b:b + M, :3] = (P + np.arange(M))[:, None]
+    for resident in (64, 256, 4096):
+        tiles, jobs, n_parts = host.plan_tiles(trees, abi.PlanGroups(heads[1] // 2, p, diff=True), window, pos if window else None,
+                                               host.options_mi355x(p.rows_per_tile, resident))
+        device.validate(p, tiles, trees, jobs, n_parts, at, np.arange(used, dtype=np.int32), used, diff=True)
+        rows = set()
+        for tree in range(len(seqs)):
+            base, P, _, M = trees[tree]
+            mine = tiles[tiles["tree"] == tree]
+            for r0 in set(mine["r0"]):
+                part = np.sort(mine[mine["r0"] == r0], order="k0")
+                n = min(p.rows_per_tile, base + M - r0)
+                rows |= set(range(r0, r0 + n))
+                first, last = P + (r0 - base), P + (r0 - base) + n - 1     # the positions of the tile's rows
+                assert (part["k0"][1:] == part["k1"][:-1]).all() and part["k0"][0] <= (max(0, first - window + 1) if window else 0)
+                assert part["last"].sum() <= 1 and part["k1"][-1] >= min(P, last + 1)
+        assert rows == set(range(at))
+        parts = tiles["part"][tiles["part"] >= 0]
+        assert len(set(parts)) == len(parts) == n_parts == jobs["nparts"].sum()
+        if p.rows_per_tile * heads[0] // heads[1] > 8 and not window:              # many packed rows: dispatched from the end, the longest parts first
+            keys, order = {}, []
+            for x in tiles:
+                at_tile = (int(x["tree"]), int(x["r0"]))
+                order += [] if at_tile in keys else [at_tile]
+                n = min(p.rows_per_tile, trees["base"][at_tile[0]] + trees["M"][at_tile[0]] - at_tile[1])
+                keys.setdefault(at_tile, []).append(int(x["k1"] - x["k0"]) + int(x["last"]) * int(at_tile[1] - trees["base"][at_tile[0]] + n))
+            mean = [sum(keys[k]) // len(keys[k]) for k in order]
+            assert all(y >= x - 1 for x, y in zip(mean, mean[1:]))
+
+
 # ---- logits
 def logits_args(p, **kw):
     a = dict(L=X, out=X + 64, tokens=X, rows=X, n=2, bt=X, bv=X, masks=X, seen=X, counts=X, record=0, ws=X, nbytes=1 << 20)
