@@ -107,12 +107,13 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
       for (int e = 0; e < 4; ++e) s[c][e] = map ? of[1][e] : of[0][e];
     }
   };
-  // Online softmax over scores x (log2 units, -inf where masked), then O^T += V^T . P^T; P in the storage type, which is what the
-  // matrix product takes, its sum in fp32. p: the weights before that rounding.
+  // Online softmax over scores x (log2 units, -inf where masked), then O^T += V^T . P^T. The matrix product takes P in the storage
+  // type: as the sum of two such numbers, 16 bits or more, since one alone makes the output 1.4 times as inexact as its own rounding
+  // does and the second product waits for memory anyway. p: the weights before that.
   auto softmax_pv = [&](const DiffUnit& U, const f32x4 (&x)[NC], f32x4 (&p)[NC]) {
     bool any_change = false;
     float corr[NC];
-    u32x2 pb[NC];
+    u32x2 pb[NC], pl[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       float mx = fmaxf(fmaxf(x[c][0], x[c][1]), fmaxf(x[c][2], x[c][3]));
@@ -127,6 +128,8 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
       for (int e = 0; e < 4; ++e) p[c][e] = fast_exp2(x[c][e] - m_safe);
       l_run[c] = l_run[c] * corr[c] + (p[c][0] + p[c][1] + p[c][2] + p[c][3]);
       pb[c] = u32x2{pack2<DT>(p[c][0], p[c][1]), pack2<DT>(p[c][2], p[c][3])};
+      pl[c] = u32x2{pack2<DT>(p[c][0] - unpack_lo<DT>(pb[c].x), p[c][1] - unpack_hi<DT>(pb[c].x)),
+                    pack2<DT>(p[c][2] - unpack_lo<DT>(pb[c].y), p[c][3] - unpack_hi<DT>(pb[c].y))};
     }
     if (__any(any_change)) {
 #pragma unroll
@@ -137,7 +140,10 @@ __global__ __launch_bounds__(256, 1) void attn_diff_stream_kernel(const DiffArgs
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int c = 0; c < NC; ++c) acc[c][mt] = mfma16x16<DT>(U.v[mt], pb[c], acc[c][mt]);
+      for (int c = 0; c < NC; ++c) {
+        acc[c][mt] = mfma16x16<DT>(U.v[mt], pb[c], acc[c][mt]);
+        acc[c][mt] = mfma16x16<DT>(U.v[mt], pl[c], acc[c][mt]);
+      }
   };
   auto interior = [&](const DiffUnit& U) {
     f32x4 s[NC], p[NC];
