@@ -7,13 +7,22 @@
 //   S^T[32 keys][32 rows] = K_map . Q_map^T      A = K from LDS, B = Q^T in registers
 //   P^T = exp2(S^T - m)                          registers; the D layout of S^T is the B layout of P^T
 //   O^T[256][32 rows]    += V^T . P^T            A = V^T from LDS, both maps read the same values
-// with v_mfma_f32_32x32x16 and P . V one stage behind S. After the last key the second map's wavefronts hand their output over
-// through LDS, and the first map's take the difference, the norm and the one rounding.
+// with v_mfma_f32_32x32x16 and P . V one stage behind S: 24 products of 32 cycles a wavefront and stage. P is rounded to the storage
+// type, what the product takes, and summed as rounded: the output's error against 64 bits is 1.5 times that of its own rounding (bf16
+// 0.0026, fp16 0.00031 of the output's size). The rest of P as a second operand, which costs the streaming kernel nothing, would be 40
+// products here. After the last key the second map's wavefronts hand their output over through LDS, and the first map's take the
+// difference, the norm and the one rounding of the output.
 //
-// LDS: a ring of 4 stages of 32 keys, 32 KB each: K of both heads, V^T of both heads, loaded straight from the pool
-// (global_load_lds) three stages ahead. K: the 16-byte chunk c of row r lies at c ^ (pi(r) & 15), pi swapping bits 2 and 3;
-// V^T: per sub-block of 16 keys and group of 32 dims [half of the keys][32 dims][8 keys], the order in which the lanes of a P . V
-// operand read it. Neither side has bank conflicts.
+// LDS: a ring of 4 stages of 32 keys, 32 KB each: K of both heads, V^T of both heads, loaded straight from the pool (global_load_lds)
+// by wavefronts 0 .. 3 (K, three stages ahead) and 4 .. 7 (V^T, two ahead), a run of 4 KB each. K: the 16-byte chunk c of row r lies at
+// c ^ (pi(r) & 15), pi swapping bits 2 and 3; V^T: per sub-block of 16 keys and group of 32 dims [half of the keys][32 dims][8 keys], the
+// order in which the lanes of a P . V operand read it. Neither side has bank conflicts. A SIMD has one wavefront of either group; they
+// run half a turn apart, so that one's softmax lies under the other's products, and meet at one barrier a turn. Nothing in the loop may
+// load from memory but the stages (any such load's wait is a wait for them), nor spill.
+//
+// 2048 rows behind 12000 keys, 40 / 8 heads, bf16: 800 us, 1.02 PFLOP/s of visible work, where a plain 8192^3 product of the library
+// reaches 1.20; 1.15 where the tiles fill the chip evenly. Ragged fresh prompts of 40 .. 800 rows: 48 us, bound by the longest tile's 25
+// stages of 1.4 us each and the turns before and after them.
 #include "diff_math.hpp"
 #include "lds_direct.hpp"
 
@@ -136,8 +145,8 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   u32x4 P[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
 
   f32x16 s{};
-  // Matrix work of a turn, and the request of stage `next` (-1: none) between it: P . V of stage h - 1 and the scores of stage h, a score product in front of every two of P . V so that neither
-  // waits for its own last result; operands are read two groups of three ahead.
+  // Matrix work of a turn, and the request of stage `next` (-1: none) between it: P . V of stage h - 1 and the scores of stage h, a score
+  // product in front of every two of P . V so that neither waits for its own last result; operands are read two groups of three ahead.
   auto products = [&](int h, int next) __attribute__((always_inline)) {
     u32x4 v[3][2], k[3];
     const uint32_t ka = k_at + uint32_t(h & (kRing - 1)) * kStage;

@@ -384,7 +384,8 @@ int esp_head_gate(const esp_gate_params* p, void* O, const void* X, const void* 
  * Pool, records, planner and append are those of esp_attn_forward without Kb / Vb: the pass's rows are in the pool
  * (esp_attn_prep with a row_table, or esp_kv_save), row j of a tree at position P + j of its own block list or ring.
  * Rows are plain causal: row j sees the keys 0 .. P + j, of them the last `window` where window > 0. Softmax, difference
- * and norm are held in fp32; the probabilities are rounded to the storage type before P.V, O once at the end. */
+ * and norm are held in fp32; the probabilities enter P.V in the storage type (as one number in passes of many rows, as the
+ * sum of two in passes of few), O is rounded once at the end. */
 typedef struct esp_diff_params {
   const float* weight; /* [H / 2] fp32, device memory */
   const float* norm_w; /* [2 * head_dim] fp32, device memory; NULL: no norm (eps is then not read) */
@@ -400,8 +401,8 @@ int esp_attn_diff_hint(const esp_attn_params* p, int device, int32_t* workgroups
 /* Bytes of workspace for a plan of n_parts partial records. Host-only arithmetic. */
 size_t esp_attn_diff_workspace_bytes(const esp_attn_params* p, int32_t n_parts);
 /* Of p: head_dim 128, H and Hkv even, no gate, no bidi; kv_ld is not read. Q and O [n_rows][q_ld], O's pair i at column
- * 2 * head_dim * i; rows outside the tiles are left as they are. Tiles, trees and jobs as planned by esp_plan_tiles;
- * what the records have to promise is what esp_attn_validate_for(ESP_PASS_DIFF) checks. Tiles with k1 = INT32_MAX end at
+ * 2 * head_dim * i; rows outside the tiles are left as they are. Tiles, trees and jobs as planned by esp_plan_tiles_diff
+ * (include/espetero_engine.h; a plan of esp_plan_tiles runs too, slower); what the records have to promise is what esp_attn_validate_for(ESP_PASS_DIFF) checks. Tiles with k1 = INT32_MAX end at
  * the tree's cached length as it is when the kernel runs (decode chains). */
 int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void* Q, const void* kv_pool, const int32_t* blocks, void* O,
                   const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees, int32_t n_trees, const esp_combine* jobs, int32_t n_jobs,
