@@ -769,7 +769,7 @@ static int check_lowrank(const esp_lowrank_params* p, char* err, size_t errlen) 
     for (int q = 0; q < s; ++q)
       if (p->y_off[s] < p->y_off[q] + p->width[q] && p->y_off[q] < p->y_off[s] + p->width[s])
         return fail(err, errlen, ESP_EINVAL, "slices %d and %d overlap", q, s);
-    blocks += (p->width[s] + 255) / 256;
+    blocks += (int64_t(p->width[s]) + 255) / 256;
     out += p->width[s];
   }
   if (blocks > 65535 || out > INT32_MAX) return fail(err, errlen, ESP_EUNSUPPORTED, "%lld columns in the slices", (long long)out);
@@ -794,6 +794,10 @@ int esp_lowrank_add(const esp_lowrank_params* p, const void* X, const void* A, c
   if (p->rows_per_tile != 16 && p->rows_per_tile != 64) return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_lowrank_rows)", p->rows_per_tile);
   if (n_tiles == 0) return ESP_OK;
   if (n_tiles > 65535) return fail(err, errlen, ESP_EUNSUPPORTED, "%d tiles (at most 65535)", n_tiles);
+  int64_t columns = 0;  // in blocks of 128
+  for (int s = 0; s < p->n_slices; ++s) columns += (int64_t(p->width[s]) + 127) / 128;
+  if ((int64_t(n_tiles) + 7) / 8 * 8 * columns >= 1 << 24)
+    return fail(err, errlen, ESP_EUNSUPPORTED, "%d tiles of %lld blocks of columns: more workgroups than a launch has", n_tiles, (long long)columns);
   if (n_slots == 0) return fail(err, errlen, ESP_EINVAL, "%d tiles without rows", n_tiles);
   if (!X || !A || !B || !scale || !Y || !order || !tiles) return fail(err, errlen, ESP_EINVAL, "X, A, B, scale, Y, order, tiles must not be NULL");
   if ((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(workspace)) % 16)

@@ -673,18 +673,27 @@ struct LowRankPlan {
 inline int plan_lowrank(LowRankPlan& plan, const int32_t* adapter, int n_rows, int n_adapters, int rows_per_tile) {
   plan.order.clear();
   plan.tiles.clear();
-  std::vector<int> first(size_t(n_adapters) + 1, 0);
   for (int r = 0; r < n_rows; ++r) {
     if (adapter[r] < -1 || adapter[r] >= n_adapters) return r;
-    if (adapter[r] >= 0) ++first[size_t(adapter[r]) + 1];
+    if (adapter[r] >= 0) plan.order.push_back(r);
   }
-  for (int a = 0; a < n_adapters; ++a) first[size_t(a) + 1] += first[size_t(a)];
-  plan.order.resize(size_t(first[size_t(n_adapters)]));
-  for (int a = 0; a < n_adapters; ++a)
-    for (int at = first[size_t(a)]; at < first[size_t(a) + 1]; at += rows_per_tile)
-      plan.tiles.push_back({a, at, std::min(rows_per_tile, first[size_t(a) + 1] - at), 0});
-  for (int r = 0; r < n_rows; ++r)
-    if (adapter[r] >= 0) plan.order[size_t(first[size_t(adapter[r])]++)] = r;
+  const size_t n = plan.order.size();
+  if (size_t(n_adapters) <= 4 * n + 1024) {  // counted, or sorted where the table of adapters is longer than the pass
+    std::vector<int> next(size_t(n_adapters) + 1, 0);
+    for (int r : plan.order) ++next[size_t(adapter[r]) + 1];
+    for (int a = 0; a < n_adapters; ++a) next[size_t(a) + 1] += next[size_t(a)];
+    for (int r = 0; r < n_rows; ++r)
+      if (adapter[r] >= 0) plan.order[size_t(next[size_t(adapter[r])]++)] = r;
+  } else {
+    std::stable_sort(plan.order.begin(), plan.order.end(), [&](int x, int y) { return adapter[x] < adapter[y]; });
+  }
+  for (size_t at = 0; at < n;) {
+    const int a = adapter[plan.order[at]];
+    size_t to = at;
+    while (to < n && to - at < size_t(rows_per_tile) && adapter[plan.order[to]] == a) ++to;
+    plan.tiles.push_back({a, int32_t(at), int32_t(to - at), 0});
+    at = to;
+  }
   return -1;
 }
 

@@ -141,6 +141,28 @@ def test_lowrank_refuses_arguments(a, rc):
     assert call("esp_lowrank_add", *lowrank_args(lowrank_params(), n_tiles=0, X=None))[0] == 0
 
 
+@pytest.mark.parametrize("n_adapters", [7, 5000, 2**31 - 1])
+@pytest.mark.parametrize("rows_per_tile", [1, 16, 2**31 - 1])
+def test_lowrank_plans_of_any_table_and_tile(n_adapters, rows_per_tile):
+    a = np.random.default_rng(1).integers(-1, min(n_adapters, 40), 300).astype(np.int32)
+    a[::50] = n_adapters - 1
+    order, tiles = host.plan_lowrank(lowrank_params(n_adapters=n_adapters, rows_per_tile=rows_per_tile), a)
+    assert (order == sorted(np.flatnonzero(a >= 0), key=lambda r: (a[r], r))).all()
+    assert (tiles["first"] == np.cumsum(tiles["count"]) - tiles["count"]).all() and tiles["count"].sum() == len(order)
+    for t in tiles:
+        assert 0 < t["count"] <= rows_per_tile and (a[order[t["first"]:t["first"] + t["count"]]] == t["adapter"]).all()
+    for x, y in zip(tiles, tiles[1:]):
+        assert x["adapter"] < y["adapter"] or (x["adapter"] == y["adapter"] and x["count"] == rows_per_tile)
+
+
+def test_lowrank_refuses_more_workgroups_than_a_launch_has():
+    p = lowrank_params(y_ld=1 << 22)
+    p.y_off[0], p.width[0], p.y_off[1], p.width[1] = 0, 1 << 21, 1 << 21, 64
+    rc, msg = call("esp_lowrank_add", *lowrank_args(p, n_tiles=65535, n_slots=65535, nbytes=1 << 40))
+    assert rc == 2 and "workgroups" in msg, msg
+    assert call("esp_lowrank_add", *lowrank_args(p, n_tiles=65536))[0] == 2
+
+
 def test_lowrank_plan():
     p = lowrank_params(rows_per_tile=2)
     order, tiles = host.plan_lowrank(p, [1, 0, -1, 1, 1, 2, -1, 0])
