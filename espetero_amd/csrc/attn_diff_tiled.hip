@@ -2,15 +2,16 @@
 //
 // Bound by the matrix cores: 1536 operations for every pair of query heads, row and visible key. One workgroup is one tile and one KV
 // pair; the tile's rows times the G query pairs of the KV pair are up to 128 packed rows (row in tile * G + query pair), so that
-// K and V are staged once for all of them and a causal tile's rows lie close together. 8 wavefronts: wavefront w works on map w % 2
-// of the 32 packed rows w / 2. Per 32 keys it computes
+// K and V are staged once for all of them and a causal tile's rows lie close together. 8 wavefronts, two for each 32 packed rows, one a
+// map. Per 32 keys it computes
 //   S^T[32 keys][32 rows] = K_map . Q_map^T      A = K from LDS, B = Q^T in registers
 //   P^T = exp2(S^T - m)                          registers; the D layout of S^T is the B layout of P^T
 //   O^T[256][32 rows]    += V^T . P^T            A = V^T from LDS, both maps read the same values
-// with v_mfma_f32_32x32x16 and P . V one stage behind S: 24 products of 32 cycles a wavefront and stage. P is rounded to the storage
-// type, what the product takes, and summed as rounded: the output's error against 64 bits is 1.5 times that of its own rounding (bf16
-// 0.0026, fp16 0.00031 of the output's size). The rest of P as a second operand, which costs the streaming kernel nothing, would be 40
-// products here. After the last key the second map's wavefronts hand their output over through LDS, and the first map's take the
+// with v_mfma_f32_32x32x16 and P . V one stage behind S. The product takes P in the storage type. The first map's enters as the sum of
+// two such numbers, the second's, which counts by its weight, as one: 40 and 24 products of 32 cycles a stage, and every SIMD has one
+// wavefront of either map. So the output's error against 64 bits is 1.15 times that of its own rounding (bf16 0.0019, fp16 0.00024 of
+// its size). One number for both: 0.0026, 0.00031, and the two cases below in 800 and 48 us; two for both: no more than the rounding,
+// in 1165 and 64 us. After the last key the second map's wavefronts hand their output over through LDS, and the first map's take the
 // difference, the norm and the one rounding of the output.
 //
 // LDS: a ring of 4 stages of 32 keys, 32 KB each: K of both heads, V^T of both heads, loaded straight from the pool (global_load_lds)
@@ -20,9 +21,9 @@
 // run half a turn apart, so that one's softmax lies under the other's products, and meet at one barrier a turn. Nothing in the loop may
 // load from memory but the stages (any such load's wait is a wait for them), nor spill.
 //
-// 2048 rows behind 12000 keys, 40 / 8 heads, bf16: 800 us, 1.02 PFLOP/s of visible work, where a plain 8192^3 product of the library
-// reaches 1.20; 1.15 where the tiles fill the chip evenly. Ragged fresh prompts of 40 .. 800 rows: 48 us, bound by the longest tile's 25
-// stages of 1.4 us each and the turns before and after them.
+// 2048 rows behind 12000 keys, 40 / 8 heads, bf16: 1020 us, 0.80 PFLOP/s of visible work and 1.07 with the second numbers, where a
+// plain 8192^3 product of the library reaches 1.20. Ragged fresh prompts of 40 .. 800 rows, 32 / 8, fp16: 53 us, bound by the longest tile's 25 stages and
+// the turns before and after them.
 #include "diff_math.hpp"
 #include "lds_direct.hpp"
 
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   const uint32_t lds_base = uint32_t(uintptr_t(lds));
   const int j = blockIdx.x;  // KV pair
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int l32 = lane & 31, hb = lane >> 5, map = wave & 1, col0 = 32 * (wave >> 1);
+  const int l32 = lane & 31, hb = lane >> 5, map = (wave ^ (wave >> 2)) & 1, col0 = 32 * (wave >> 1);
   const esp_tile tile = a.tiles[gridDim.y - 1 - blockIdx.y];  // last to first: a causal pass's longest tiles start first
   const esp_tree tree = a.trees[tile.tree];
   const int table = tile.pad > 0 ? tile.pad - 1 : tree.table;
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   float m_ref = -INFINITY, l_run = 0.0f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) acc[nt] = f32x16{};
-  u32x4 P[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+  u32x4 P[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}}, rest[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};  // rest: the first map's, what P's rounding left
 
   f32x16 s{};
   // Matrix work of a turn, and the request of stage `next` (-1: none) between it: P . V of stage h - 1 and the scores of stage h, a score
@@ -166,6 +167,10 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
       s = mfma32x16<DT>(k[g % 3], qf[g], s);
 #pragma unroll
       for (int i = 0; i < 2; ++i) acc[(2 * g + i) & 7] = mfma32x16<DT>(v[g % 3][i], P[g >> 2], acc[(2 * g + i) & 7]);
+      if (map == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[(2 * g + i) & 7] = mfma32x16<DT>(v[g % 3][i], rest[g >> 2], acc[(2 * g + i) & 7]);
+      }
       if (g == 3 && next >= 0) request(next);
       if (g == 5 && next >= 0) advance();
       __builtin_amdgcn_sched_barrier(0);
@@ -281,8 +286,10 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int at = 8 * sb + 2 * e;
-        P[sb][e] = pack2<DT>(fast_exp2(s[at] * a.scale_log2 - off), fast_exp2(s[at + 1] * a.scale_log2 - off));
-        (sb ? lx : l_run) = sum2<DT>(P[sb][e], sb ? lx : l_run);  // of the weights as the product takes them
+        const float p0 = fast_exp2(s[at] * a.scale_log2 - off), p1 = fast_exp2(s[at + 1] * a.scale_log2 - off);
+        P[sb][e] = pack2<DT>(p0, p1);
+        rest[sb][e] = pack2<DT>(p0 - unpack_lo<DT>(P[sb][e]), p1 - unpack_hi<DT>(P[sb][e]));
+        (sb ? lx : l_run) += p0 + p1;
       }
     l_run += lx;
   };
