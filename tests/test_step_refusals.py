@@ -203,29 +203,33 @@ def test_diff_plans_cover_every_key_once(seqs, heads, window):
         tiles, jobs, n_parts = host.plan_tiles(trees, abi.PlanGroups(heads[1] // 2, p, diff=True), window, pos if window else None,
                                                host.options_mi355x(p.rows_per_tile, resident))
         device.validate(p, tiles, trees, jobs, n_parts, at, np.arange(used, dtype=np.int32), used, diff=True)
-        rows = set()
+        rows, length, order = set(), {}, []
         for tree in range(len(seqs)):
             base, P, _, M = trees[tree]
             mine = tiles[tiles["tree"] == tree]
             for r0 in set(mine["r0"]):
-                part = np.sort(mine[mine["r0"] == r0], order="k0")
                 n = min(p.rows_per_tile, base + M - r0)
                 rows |= set(range(r0, r0 + n))
-                first, last = P + (r0 - base), P + (r0 - base) + n - 1     # the positions of the tile's rows
-                assert (part["k0"][1:] == part["k1"][:-1]).all() and part["k0"][0] <= (max(0, first - window + 1) if window else 0)
-                assert part["last"].sum() <= 1 and part["k1"][-1] >= min(P, last + 1)
+                first, end = P + r0 - base, P + r0 - base + n              # the tile's rows see keys up to their own, [.., end) of them
+                spans = []
+                for x in mine[mine["r0"] == r0]:                             # a part's keys: cached ones, and rows of the pass behind them
+                    lo, hi = int(x["k0"]), min(int(x["k1"]), P)
+                    if x["last"]:
+                        lo = P + int(x["b0"]) if hi <= lo else lo
+                        hi = min(end, P + int(x["last"]) - 1) if x["last"] >= 2 else end
+                    spans.append((lo, max(lo, hi)))
+                spans.sort()
+                assert spans[0][0] <= (max(0, first - window + 1) if window else 0) and spans[-1][1] == end
+                assert all(x[1] == y[0] for x, y in zip(spans, spans[1:]))
+                length[(tree, int(r0))] = sum(y - x for x, y in spans) // len(spans)
         assert rows == set(range(at))
         parts = tiles["part"][tiles["part"] >= 0]
         assert len(set(parts)) == len(parts) == n_parts == jobs["nparts"].sum()
-        if p.rows_per_tile * heads[0] // heads[1] > 8 and not window:              # many packed rows: dispatched from the end, the longest parts first
-            keys, order = {}, []
+        if p.rows_per_tile * heads[0] // heads[1] > 16 and not window:             # many packed rows: dispatched from the end, the longest parts first
             for x in tiles:
-                at_tile = (int(x["tree"]), int(x["r0"]))
-                order += [] if at_tile in keys else [at_tile]
-                n = min(p.rows_per_tile, trees["base"][at_tile[0]] + trees["M"][at_tile[0]] - at_tile[1])
-                keys.setdefault(at_tile, []).append(int(x["k1"] - x["k0"]) + int(x["last"]) * int(at_tile[1] - trees["base"][at_tile[0]] + n))
-            mean = [sum(keys[k]) // len(keys[k]) for k in order]
-            assert all(y >= x - 1 for x, y in zip(mean, mean[1:]))
+                key = (int(x["tree"]), int(x["r0"]))
+                order += [] if key in order else [key]
+            assert all(length[y] >= length[x] - 1 for x, y in zip(order, order[1:]))
 
 
 # ---- logits
