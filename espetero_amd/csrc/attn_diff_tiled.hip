@@ -10,8 +10,8 @@
 // with v_mfma_f32_32x32x16 and P . V one stage behind S. The product takes P in the storage type. The first map's enters as the sum of
 // two such numbers, the second's, which counts by its weight, as one: 40 and 24 products of 32 cycles a stage, and every SIMD has one
 // wavefront of either map. So the output's error against 64 bits is 1.15 times that of its own rounding (bf16 0.0019, fp16 0.00024 of
-// its size). One number for both: 0.0026, 0.00031, and the two cases below in 800 and 48 us where these took 1020 and 53; two for both: no
-// more than the rounding, in 1165 and 64 us. After the last key the second map's wavefronts hand their output over through LDS, and the first map's take the
+// its size). One number for both: 0.0026, 0.00031, and the two cases below in 800 and 48 us; two for both: no more than the rounding, in
+// 1165 and 64 us. After the last key the second map's wavefronts hand their output over through LDS, and the first map's take the
 // difference, the norm and the one rounding of the output.
 //
 // LDS: a ring of 4 stages of 32 keys, 32 KB each: K of both heads, V^T of both heads, loaded straight from the pool (global_load_lds)
@@ -21,9 +21,9 @@
 // run half a turn apart, so that one's softmax lies under the other's products, and meet at one barrier a turn. Nothing in the loop may
 // load from memory but the stages (any such load's wait is a wait for them), nor spill.
 //
-// 2048 rows behind 12000 keys, 40 / 8 heads, bf16: 990 us, 0.83 PFLOP/s of visible work and 1.10 with the second numbers, where a
-// plain 8192^3 product of the library reaches 1.20. Ragged fresh prompts of 40 .. 800 rows, 32 / 8, fp16: 52 us, bound by the longest tile's 25 stages and
-// the turns before and after them.
+// 2048 rows behind 12000 keys, 40 / 8 heads, bf16: 990 to 1030 us, 0.81 PFLOP/s of visible work and 1.08 with the second numbers,
+// where a plain 8192^3 product of the library reaches 1.20. Ragged fresh prompts of 40 .. 800 rows, 32 / 8, fp16: 52 us, bound by the
+// longest tile's 25 stages and the turns before and after them.
 #include "diff_math.hpp"
 #include "lds_direct.hpp"
 
