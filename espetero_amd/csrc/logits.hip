@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) void logits_kernel(const LogitsArgs a) {
     }
   }
   if constexpr (OUT) __syncthreads();  // what follows writes over some of these
-  // The others; past the list's end the last again.
+  // The others; past the list's end the last again, read but not written: in place it may have its penalty by then.
   Best other{-INFINITY, INT32_MAX};
   auto bit_of = [&](const uint32_t* sh, int i) { return (sh[i >> 5] >> (i & 31) & 1) != 0; };
   auto given_times = [&](int i) { return counts[bit_of(given_sh, i) ? uint32_t(i) : 0u]; };
@@ -209,7 +209,8 @@ __global__ __launch_bounds__(256) void logits_kernel(const LogitsArgs a) {
 #pragma unroll
     for (int j = 0; j < B; ++j) v[j] = logit_at<DT>(in, uint32_t(i[j])), times[j] = given_times(i[j]);
 #pragma unroll
-    for (int j = 0; j < B; ++j) done(i[j], penalty(v[j], i[j], true, times[j]));
+    for (int j = 0; j < B; ++j)
+      if (k + j * W < listed) done(i[j], penalty(v[j], i[j], true, times[j]));
   }
   for (int e = tid; e < n_bias; e += W) {
     const uint32_t t = e == tid ? first : uint32_t(bias_tokens[e]) - uint32_t(c0);

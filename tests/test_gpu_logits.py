@@ -119,6 +119,24 @@ def test_strides_and_rows_without_anything():
         Case(3, 4099, dtype, seed=2, n_slots=0, n_masks=0, bias=0).check()
 
 
+@pytest.mark.parametrize("seen", [0.004, 0.05, 0.3, 0.95])
+def test_in_place_every_token_is_penalised_once(seen):
+    """Lists of a few tokens a chunk up to all of them, in many workgroups: no wavefront takes what another has written for a logit."""
+    c = Case(192, 20011, F32, seed=29, n_masks=1, bias=40)
+    rng = np.random.default_rng(31)
+    c.prompt = rng.random(c.prompt.shape) < seen
+    c.counts[:] = np.where(rng.random(c.counts.shape) < seen / 4, 3, 0)
+    c.rows["repetition"], c.rows["mask"] = 1.5, -1
+    want, tokens = c.expected()
+    c.prepare()
+    for _ in range(5):
+        c.out = c.L.cuda()
+        c.dL = c.out
+        c.run()
+        torch.cuda.synchronize()
+        assert np.array_equal(c.out.cpu().numpy(), want) and (c.tokens.cpu().numpy() == tokens).all()
+
+
 def test_alone_in_place_and_only_tokens():
     c = Case(4, 3001, F32, seed=3)
     want, tokens = c.expected()
