@@ -911,7 +911,7 @@ int esp_logits_validate(const esp_logits_params* p, const esp_logits_row* rows, 
 
 static int check_history(const esp_logits_params* p, const uint32_t* seen, const int32_t* counts, const int32_t* slots, int32_t n, char* err, size_t errlen) {
   if (int rc = check_logits(p, err, errlen)) return rc;
-  if (n < 0) return fail(err, errlen, ESP_EINVAL, "negative count");
+  if (n < 0 || n > INT32_MAX - 65536) return fail(err, errlen, ESP_EINVAL, "%d entries", n);
   if (n && (!seen || !counts || !slots)) return fail(err, errlen, ESP_EINVAL, "seen, counts and slots must not be NULL");
   return ESP_OK;
 }

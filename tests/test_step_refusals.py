@@ -265,7 +265,8 @@ def test_logits_refuses_arguments(a, rc):
 
 def test_histories_refuse():
     p = logits_params()
-    for kw in ((X, X, X, X, -1, 0), (None, X, X, X, 1, 0), (X, None, X, X, 1, 0), (X, X, None, X, 1, 0), (X, X, X, None, 1, 0), (X, X, X, X, 1, 2)):
+    for kw in ((X, X, X, X, -1, 0), (None, X, X, X, 1, 0), (X, None, X, X, 1, 0), (X, X, None, X, 1, 0), (X, X, X, None, 1, 0), (X, X, X, X, 1, 2),
+               (X, X, X, X, 2**31 - 1, 1)):
         assert call("esp_history_record", C.byref(p), *kw, None)[0] == 1
     assert call("esp_history_record", C.byref(p), None, None, None, None, 0, 1, None)[0] == 0
     for kw in ((X, X, X, -1), (None, X, X, 1), (X, None, X, 1), (X, X, None, 1), (X, X, X, 65536)):
