@@ -402,8 +402,9 @@ int esp_attn_diff_hint(const esp_attn_params* p, int device, int32_t* workgroups
 size_t esp_attn_diff_workspace_bytes(const esp_attn_params* p, int32_t n_parts);
 /* Of p: head_dim 128, H and Hkv even, no gate, no bidi; kv_ld is not read. Q and O [n_rows][q_ld], O's pair i at column
  * 2 * head_dim * i; rows outside the tiles are left as they are. Tiles, trees and jobs as planned by esp_plan_tiles_diff
- * (include/espetero_engine.h; a plan of esp_plan_tiles runs too, slower); what the records have to promise is what esp_attn_validate_for(ESP_PASS_DIFF) checks. Tiles with k1 = INT32_MAX end at
- * the tree's cached length as it is when the kernel runs (decode chains). */
+ * (include/espetero_engine.h; a plan of esp_plan_tiles runs too, slower); what the records have to promise is what
+ * esp_attn_validate_for(ESP_PASS_DIFF) checks. Tiles with k1 = INT32_MAX end at the tree's cached length as it is when the
+ * kernel runs (decode chains). */
 int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void* Q, const void* kv_pool, const int32_t* blocks, void* O,
                   const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees, int32_t n_trees, const esp_combine* jobs, int32_t n_jobs,
                   int32_t n_parts, int32_t n_rows, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen);
