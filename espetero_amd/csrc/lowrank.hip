@@ -3,7 +3,7 @@
 //   down  low[split][slot][slices * rank] = x . A^T over the split's share of D, fp32 partial sums in the workspace
 //   up    the splits' sums in split order, times B, onto Y
 // or one that does both where there is little of A. Prompts are bound by Y, read and written once: 3679 rows of 7168 columns, rank 16,
-// D 5120 take 53 us, 4.7 TB/s. A decode batch is bound by the hops from record to row number to element, about a microsecond each, and by
+// D 5120 take 51 us, 4.9 TB/s. A decode batch is bound by the hops from record to row number to element, about a microsecond each, and by
 // the second launch: 48 requests of 20 adapters, rank 16, D 5120 take 11 us (4 + 6 in the kernels), of which its 16 MB are 3.
 // Every product of two 16-bit elements is exact in fp32 and summed there; the intermediate keeps its 24 bits on its way into the
 // second matrix product, which takes 16-bit operands, as the sum of three bf16 or two fp16 numbers.

@@ -32,13 +32,13 @@ constexpr int lowrank_low_blocks(int n_low) {
 constexpr int lowrank_low_groups(int n_low) { return ((n_low + 15) / 16 + lowrank_low_blocks(n_low) - 1) / lowrank_low_blocks(n_low); }
 // How many ways D is split, with 128 dims or more each. Eight: a share for each XCD's L2, and what the second launch has on its way at
 // once of a few rows. Four where that leaves enough workgroups, since every block of columns sums the splits again (3679 rows, rank 64,
-// D 5120: 63 us, 67 with eight; 500 rows, rank 16, D 4096: 17 us, 15 with eight).
+// D 5120: 62 us, 67 with eight; 500 rows, rank 16, D 4096: 17 us, 15 with eight).
 inline int lowrank_splits(int D, int n_low, int rows_per_tile, int n_tiles) {
   const int wgs = std::max(1, n_tiles * lowrank_low_groups(n_low));
   return std::max(1, std::min(D / 128, rows_per_tile == 16 ? std::min(8, (512 + wgs - 1) / wgs) : wgs < 128 ? 8 : 4));
 }
 // Whether one launch does both products, each workgroup the first one for itself: one launch less, and the slice's A read by every
-// block of 1024 columns at what one compute unit draws. bf16, one request, D 2048, rank 16: 6.6 us; D 4096, rank 16: 8.9 us, 8.0 as two
+// block of 1024 columns at what one compute unit draws. bf16, one request, D 2048, rank 16: 6.5 us; D 4096, rank 16: 8.9 us, 8.0 as two
 // launches; 48 requests of 20 adapters, D 5120, rank 16: 12.7 us, 10.9 as two.
 inline bool lowrank_fused(int D, int rank, int n_slices, const int32_t* width, int n_tiles) {
   int64_t wgs = 0;
@@ -47,9 +47,10 @@ inline bool lowrank_fused(int D, int rank, int n_slices, const int32_t* width, i
   return rank <= 32 && (wgs + 255) / 256 * rank * D <= 32 * 1024;
 }
 // Blocks of 128 columns that a workgroup of the second launch takes one after the other, with one sum of its tile's splits, as long as
-// that leaves one and a half workgroups for every compute unit (2065 rows, rank 128: 55 us, 68 with half as many blocks each).
+// that leaves one and a quarter workgroups for every compute unit (2065 rows, rank 128, D 5120, 7168 columns: 58 us; 68 with one and a
+// half, 66 with one or three. D 4096, 6144 columns: 50, 50, 58, 54).
 constexpr int lowrank_blocks_each(int row_blocks, int n_tiles, int blocks) {
-  return row_blocks == 1 ? 1 : std::max(1, std::min(8, int(int64_t(n_tiles) * blocks / 384)));
+  return row_blocks == 1 ? 1 : std::max(1, std::min(8, int(int64_t(n_tiles) * blocks / 320)));
 }
 // Rows of a tile: a decode batch has few of each adapter.
 constexpr int lowrank_rows(int n_rows) { return n_rows <= 0 ? 0 : n_rows <= 128 ? 16 : 64; }
