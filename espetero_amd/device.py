@@ -257,9 +257,11 @@ class LowRankPass:
     """Which rows of a pass take which adapter, planned and resident on the device."""
 
     def __init__(self, params, adapter, device="cuda"):
-        """adapter: int32 per row, -1 for a row without one. Sets params.rows_per_tile."""
+        """adapter: int32 per row, -1 for a row without one. params: a layer's record may serve any number of passes. Each keeps a copy,
+        with the rows_per_tile that its own tiles were planned with."""
         lib = abi.attn_lib()
         n_rows = len(adapter)
+        params = abi.LowRankParams.from_buffer_copy(params)
         params.rows_per_tile = lib.esp_lowrank_rows(C.byref(params), max(n_rows, 1))
         if params.rows_per_tile <= 0:
             raise abi.EspError("parameters that esp_lowrank_add does not serve")

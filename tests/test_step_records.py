@@ -1,0 +1,23 @@
+"""What the passes of the operators around a decode step keep of a caller's parameter record, host-side checks of their records and the
+sizes of their workspaces. No GPU: records are built in host memory and every call is refused."""
+import pytest
+
+from espetero_amd import abi, device
+
+
+# ---- one record, several passes
+@pytest.mark.parametrize("first,second", [(200, 20), (20, 200), (1000, 4)])
+def test_lowrank_passes_of_one_record_keep_their_own_tiles(first, second):
+    """A prompt's pass and a decode step's pass of one layer: the record is the layer's, the tiles are each pass's own."""
+    p = device.lowrank_params(256, 16, [(0, 64), (64, 32)], abi.ESP_F16, 256, 96, 2)
+    before = bytes(p)
+    a = device.LowRankPass(p, [0] * first, device="cpu")
+    of_a = bytes(a.params)
+    b = device.LowRankPass(p, [1] * second, device="cpu")
+    assert bytes(p) == before and bytes(a.params) == of_a
+    for x, n in ((a, first), (b, second)):
+        assert x.params.rows_per_tile == (16 if n <= 128 else 64)
+        tiles = x.tiles.numpy().view(abi.LOWRANK_TILE_DT)
+        assert tiles["count"].max() == min(n, x.params.rows_per_tile) and tiles["count"].sum() == n
+    p.D = 8                                                          # nor does a later change of the record reach them
+    assert a.params.D == b.params.D == 256
