@@ -30,10 +30,13 @@ constexpr int logits_words(int vocab) { return (vocab + 31) / 32; }
 struct LogitsShape {
   int tokens, chunks;
 };
+constexpr int kLogitsTokensLeast = 8;
+constexpr int logits_chunks(int vocab, int tokens) { return (vocab + 256 * tokens - 1) / (256 * tokens); }
 inline LogitsShape logits_shape(int vocab, int n_rows) {
-  const int tokens = int64_t(vocab) * n_rows <= 12 << 20 ? 8 : 16;
-  return {tokens, (vocab + 256 * tokens - 1) / (256 * tokens)};
+  const int tokens = int64_t(vocab) * n_rows <= 12 << 20 ? kLogitsTokensLeast : 16;
+  return {tokens, logits_chunks(vocab, tokens)};
 }
-inline size_t logits_workspace(int vocab, int n_rows) { return size_t(logits_shape(vocab, n_rows).chunks) * size_t(n_rows) * 8; }
+// A best token of every chunk. As if the chunks were always the small ones: what serves a pass serves every smaller one.
+inline size_t logits_workspace(int vocab, int n_rows) { return size_t(logits_chunks(vocab, kLogitsTokensLeast)) * size_t(n_rows) * 8; }
 
 }  // namespace esp

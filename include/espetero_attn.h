@@ -476,6 +476,7 @@ typedef struct esp_logits_row {
   int32_t pad;
 } esp_logits_row;
 
+/* Never less for more rows: what serves a pass serves every smaller one. */
 size_t esp_logits_workspace_bytes(const esp_logits_params* p, int32_t n_rows);
 /* logits [n_rows][in_ld]; out [n_rows][out_ld] fp32 or NULL (it may be the logits themselves where those are fp32 and
  * out_ld == in_ld); tokens [n_rows] or NULL (then record is 0). rows: n_rows records. masks [n_masks][ceil(vocab / 32)]:

@@ -1,5 +1,7 @@
 """What the passes of the operators around a decode step keep of a caller's parameter record, host-side checks of their records and the
 sizes of their workspaces. No GPU: records are built in host memory and every call is refused."""
+import ctypes as C
+
 import pytest
 
 from espetero_amd import abi, device
@@ -21,3 +23,14 @@ def test_lowrank_passes_of_one_record_keep_their_own_tiles(first, second):
         assert tiles["count"].max() == min(n, x.params.rows_per_tile) and tiles["count"].sum() == n
     p.D = 8                                                          # nor does a later change of the record reach them
     assert a.params.D == b.params.D == 256
+
+
+# ---- a workspace sized for the largest pass serves the smaller ones
+@pytest.mark.parametrize("dtype", [abi.ESP_F16, abi.ESP_BF16, abi.ESP_F32])
+@pytest.mark.parametrize("vocab", [1, 2048, 50257, 128256, 250000])
+def test_logits_workspace_grows_with_the_rows(vocab, dtype):
+    p = device.logits_params(vocab, dtype, 1)
+    sizes = [abi.attn_lib().esp_logits_workspace_bytes(C.byref(p), n) for n in range(1, 1200)]
+    assert sizes[0] > 0 and sizes == sorted(sizes)
+    bigger = device.logits_params(vocab + 7, dtype, 1)
+    assert all(abi.attn_lib().esp_logits_workspace_bytes(C.byref(bigger), n) >= x for n, x in enumerate(sizes, 1))
