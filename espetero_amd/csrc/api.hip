@@ -783,7 +783,7 @@ int32_t esp_lowrank_rows(const esp_lowrank_params* p, int32_t n_rows) {
 
 size_t esp_lowrank_workspace_bytes(const esp_lowrank_params* p, int32_t n_tiles, int32_t n_slots) {
   if (check_lowrank(p, nullptr, 0) != ESP_OK || n_tiles <= 0 || n_slots <= 0) return 0;
-  return esp::lowrank_workspace(*p, n_tiles, n_slots);
+  return esp::lowrank_workspace(*p, n_slots);
 }
 
 int esp_lowrank_add(const esp_lowrank_params* p, const void* X, const void* A, const void* B, const float* scale, float* Y, const int32_t* order,
@@ -802,7 +802,7 @@ int esp_lowrank_add(const esp_lowrank_params* p, const void* X, const void* A, c
   if (!X || !A || !B || !scale || !Y || !order || !tiles) return fail(err, errlen, ESP_EINVAL, "X, A, B, scale, Y, order, tiles must not be NULL");
   if ((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(workspace)) % 16)
     return fail(err, errlen, ESP_EINVAL, "X, A, B and the workspace must be 16-byte aligned");
-  const size_t need = esp::lowrank_workspace(*p, n_tiles, n_slots);
+  const size_t need = esp::lowrank_workspace(*p, n_slots);
   if (!workspace || workspace_bytes < need) return fail(err, errlen, ESP_EWORKSPACE, "workspace %zu bytes, %zu needed", workspace ? workspace_bytes : size_t(0), need);
   esp::LowRankArgs a{};
   a.X = static_cast<const uint16_t*>(X);

@@ -30,12 +30,13 @@ constexpr int lowrank_low_blocks(int n_low) {
   return (all + groups - 1) / groups;
 }
 constexpr int lowrank_low_groups(int n_low) { return ((n_low + 15) / 16 + lowrank_low_blocks(n_low) - 1) / lowrank_low_blocks(n_low); }
+constexpr int kLowRankSplits = 8;  // at most
 // How many ways D is split, with 128 dims or more each. Eight: a share for each XCD's L2, and what the second launch has on its way at
 // once of a few rows. Four where that leaves enough workgroups, since every block of columns sums the splits again (3679 rows, rank 64,
 // D 5120: 62 us, 67 with eight; 500 rows, rank 16, D 4096: 17 us, 15 with eight).
 inline int lowrank_splits(int D, int n_low, int rows_per_tile, int n_tiles) {
   const int wgs = std::max(1, n_tiles * lowrank_low_groups(n_low));
-  return std::max(1, std::min(D / 128, rows_per_tile == 16 ? std::min(8, (512 + wgs - 1) / wgs) : wgs < 128 ? 8 : 4));
+  return std::max(1, std::min(D / 128, rows_per_tile == 16 ? std::min(kLowRankSplits, (512 + wgs - 1) / wgs) : wgs < 128 ? kLowRankSplits : 4));
 }
 // Whether one launch does both products, each workgroup the first one for itself: one launch less, and the slice's A read by every
 // block of 1024 columns at what one compute unit draws. bf16, one request, D 2048, rank 16: 6.5 us; D 4096, rank 16: 8.9 us, 8.0 as two
@@ -54,8 +55,10 @@ constexpr int lowrank_blocks_each(int row_blocks, int n_tiles, int blocks) {
 }
 // Rows of a tile: a decode batch has few of each adapter.
 constexpr int lowrank_rows(int n_rows) { return n_rows <= 0 ? 0 : n_rows <= 128 ? 16 : 64; }
-inline size_t lowrank_workspace(const esp_lowrank_params& p, int n_tiles, int n_slots) {
-  return size_t(lowrank_splits(p.D, p.n_slices * p.rank, p.rows_per_tile, n_tiles)) * size_t(n_slots) * size_t(p.n_slices * p.rank) * sizeof(float);
+// The intermediate of every split, as if there were always the most of them: what serves a pass serves every one of as many slots or
+// fewer, whatever its tiles.
+inline size_t lowrank_workspace(const esp_lowrank_params& p, int n_slots) {
+  return size_t(std::max(1, std::min(p.D / 128, kLowRankSplits))) * size_t(n_slots) * size_t(p.n_slices * p.rank) * sizeof(float);
 }
 inline int lowrank_chunk(int D, int splits) { return ((D + splits - 1) / splits + 127) / 128 * 128; }
 

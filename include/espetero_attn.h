@@ -437,6 +437,8 @@ typedef struct esp_lowrank_tile {
 
 /* The rows_per_tile to plan a pass of n_rows rows with, or 0 for parameters that esp_lowrank_add refuses. */
 int32_t esp_lowrank_rows(const esp_lowrank_params* p, int32_t n_rows);
+/* Never less for more slots, and alike for any number of tiles (0 of none) and either rows_per_tile: what serves a pass serves every
+ * smaller one of the same D, rank and slices. */
 size_t esp_lowrank_workspace_bytes(const esp_lowrank_params* p, int32_t n_tiles, int32_t n_slots);
 /* X [rows][x_ld]; A [n_adapters][n_slices * rank][D]; B [n_adapters][sum of the widths][rank]; scale [n_adapters] fp32;
  * Y [rows][y_ld] fp32. order [n_slots], tiles: device copies of what esp_plan_lowrank (include/espetero_engine.h) made,

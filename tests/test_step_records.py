@@ -34,3 +34,17 @@ def test_logits_workspace_grows_with_the_rows(vocab, dtype):
     assert sizes[0] > 0 and sizes == sorted(sizes)
     bigger = device.logits_params(vocab + 7, dtype, 1)
     assert all(abi.attn_lib().esp_logits_workspace_bytes(C.byref(bigger), n) >= x for n, x in enumerate(sizes, 1))
+
+
+@pytest.mark.parametrize("D,rank,n_slices", [(8, 8, 1), (256, 8, 2), (5120, 16, 3), (4096, 64, 3), (2560, 128, 4)])
+def test_lowrank_workspace_grows_with_tiles_and_rows(D, rank, n_slices):
+    p = device.lowrank_params(D, rank, [(64 * i, 64) for i in range(n_slices)], abi.ESP_BF16, D, 256, 100)
+    tiles, slots = (1, 2, 7, 8, 9, 63, 64, 65, 127, 128, 129, 600, 4000), (1, 16, 128, 129, 4096, 65535)
+    sizes = {}
+    for p.rows_per_tile in (16, 64):
+        for t in tiles:
+            for n in slots:
+                sizes[p.rows_per_tile, t, n] = abi.attn_lib().esp_lowrank_workspace_bytes(C.byref(p), t, n)
+    for (r, t, n), x in sizes.items():
+        assert x >= 4 * n * rank * n_slices
+        assert all(x <= y for (_, t2, n2), y in sizes.items() if t2 >= t and n2 >= n), (r, t, n)
