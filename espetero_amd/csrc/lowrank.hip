@@ -5,8 +5,10 @@
 // or one that does both where there is little of A. Prompts are bound by Y, read and written once: 3679 rows of 7168 columns, rank 16,
 // D 5120 take 51 us, 4.9 TB/s. A decode batch is bound by the hops from record to row number to element, about a microsecond each, and by
 // the second launch: 48 requests of 20 adapters, rank 16, D 5120 take 11 us (4 + 6 in the kernels), of which its 16 MB are 3.
-// Every product of two 16-bit elements is exact in fp32 and summed there; the intermediate keeps its 24 bits on its way into the
-// second matrix product, which takes 16-bit operands, as the sum of three bf16 or two fp16 numbers.
+// Every product of two 16-bit elements is exact in fp32 and summed there. On its way into the second matrix product, which takes 16-bit
+// operands, an intermediate becomes the sum of three bf16 numbers, which keep its 24 bits, or of two fp16 ones. Those keep it to 2^-23
+// of itself, or to 2^-39 of the row's largest where that is more (a number of 2^-16 of the largest or less). A third would keep the
+// last bit too and cost half as many products again.
 #include "common.hpp"
 #include "lowrank_shape.hpp"
 
@@ -14,12 +16,10 @@
 
 namespace esp {
 
-// An fp16 term holds no more than 65504 and loses bits below 2^-14: a row of the intermediate is taken relative to the power of two
-// at its largest element, whose bits these are. 0 for a row of zeros or infinities, or one whose reciprocal leaves the range.
-__device__ __forceinline__ int power_of(uint32_t most) {
-  const int e = int(most >> 23) - 127;
-  return e < -120 || e > 127 ? 0 : min(e, 126);
-}
+// An fp16 term holds no more than 65504 and loses bits below 2^-14: a row of the intermediate is taken relative to a power of two that
+// puts its largest element, whose bits these are, at 2^14 .. 2^15, as far from the loss as there is room. (Rows of zeros and infinities
+// stay what they are; two_to has the power and its reciprocal.)
+__device__ __forceinline__ int power_of(uint32_t most) { return max(-112, min(int(most >> 23) - 127, 127)) - 14; }
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 
 // Four numbers as T terms of 16 bits, `apart` elements from one term to the next.

@@ -415,7 +415,8 @@ int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void
  *   Y[row, y_off[s] + c] += scale[a] * sum_k B[a][c of slice s][k] * (A[a][s * rank + k] . X[row])
  * for the slices s of the fused projection (queries, keys, values, ...; columns outside the slices are not touched).
  * Rows without an adapter are in no tile and stay as they are. An adapter of a smaller rank is stored with zeros in the
- * rows of A and columns of B that it lacks. The sums and the intermediate are held in fp32. */
+ * rows of A and columns of B that it lacks. The sums are held in fp32, and so is the intermediate but for its way into the second
+ * product with fp16 operands: there it is exact to 2^-23 of itself or to 2^-39 of the largest of its row and slice, whichever is more. */
 enum { ESP_LOWRANK_SLICES = 4 };
 typedef struct esp_lowrank_params {
   int32_t D;             /* width of X, a multiple of 8 */
