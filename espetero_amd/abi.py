@@ -133,6 +133,7 @@ ATTN_SYMBOLS = {
     "esp_lowrank_rows": (C.c_int32, (C.POINTER(LowRankParams), C.c_int32)),
     "esp_lowrank_workspace_bytes": (C.c_size_t, (C.POINTER(LowRankParams), C.c_int32, C.c_int32)),
     "esp_lowrank_add": (C.c_int, (C.POINTER(LowRankParams), _V, _V, _V, _V, _V, _V, C.c_int32, _V, C.c_int32, _V, C.c_size_t, _V) + _ERR),
+    "esp_lowrank_validate": (C.c_int, (C.POINTER(LowRankParams), _V, C.c_int32, _V, C.c_int32, C.c_int32) + _ERR),
     "esp_logits_workspace_bytes": (C.c_size_t, (C.POINTER(LogitsParams), C.c_int32)),
     "esp_logits_process": (C.c_int, (C.POINTER(LogitsParams), _V, _V, _V, _V, C.c_int32, _V, _V, _V, _V, _V, C.c_int32, _V, C.c_size_t, _V) + _ERR),
     "esp_logits_validate": (C.c_int, (C.POINTER(LogitsParams), _V, C.c_int32, _V) + _ERR),

@@ -5,7 +5,9 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <mutex>
+#include <utility>
 #include <vector>
 
 #include "common.hpp"
@@ -829,6 +831,36 @@ int esp_lowrank_add(const esp_lowrank_params* p, const void* X, const void* A, c
   }
   const hipError_t e = esp::launch_lowrank(p->dtype, a, p->rows_per_tile, n_tiles, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? ESP_OK : hip_fail(err, errlen, "lowrank launch", e);
+}
+
+int esp_lowrank_validate(const esp_lowrank_params* p, const int32_t* order, int32_t n_slots, const esp_lowrank_tile* tiles, int32_t n_tiles,
+                         int32_t n_rows, char* err, size_t errlen) {
+  if (int rc = check_lowrank(p, err, errlen)) return rc;
+  if (n_slots < 0 || n_tiles < 0 || n_rows < 0) return fail(err, errlen, ESP_EINVAL, "negative count");
+  if ((n_slots && !order) || (n_tiles && !tiles)) return fail(err, errlen, ESP_EINVAL, "order or tiles is NULL");
+  if (p->rows_per_tile != 16 && p->rows_per_tile != 64) return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_lowrank_rows)", p->rows_per_tile);
+  std::vector<std::pair<int32_t, int32_t>> rows;  // and the tile that names each
+  try {
+    for (int32_t i = 0; i < n_tiles; ++i) {
+      const esp_lowrank_tile& t = tiles[i];
+      if (t.adapter < 0 || t.adapter >= p->n_adapters) return fail(err, errlen, ESP_EINVAL, "tile %d: adapter %d of %d", i, t.adapter, p->n_adapters);
+      if (t.count < 0 || t.count > p->rows_per_tile) return fail(err, errlen, ESP_EINVAL, "tile %d: %d rows, rows_per_tile is %d", i, t.count, p->rows_per_tile);
+      if (t.first < 0 || int64_t(t.first) + t.count > n_slots)
+        return fail(err, errlen, ESP_EINVAL, "tile %d: slots [%d, %d + %d) of %d", i, t.first, t.first, t.count, n_slots);
+      for (int32_t s = t.first; s < t.first + t.count; ++s) {
+        if (order[s] < 0 || order[s] >= n_rows) return fail(err, errlen, ESP_EINVAL, "tile %d: row %d of %d", i, order[s], n_rows);
+        rows.emplace_back(order[s], i);
+      }
+      if (rows.size() > size_t(n_rows)) break;  // one of them comes twice
+    }
+    std::sort(rows.begin(), rows.end());
+  } catch (const std::exception& e) {
+    return fail(err, errlen, ESP_EINVAL, "%s", e.what());
+  }
+  for (size_t i = 1; i < rows.size(); ++i)
+    if (rows[i].first == rows[i - 1].first)
+      return fail(err, errlen, ESP_EINVAL, "tile %d: row %d is named twice (also by tile %d)", rows[i].second, rows[i].first, rows[i - 1].second);
+  return ESP_OK;
 }
 
 // ---- logits ------------------------------------------------------------------------

@@ -253,6 +253,15 @@ def lowrank_params(D, rank, slices, dtype, x_ld, y_ld, n_adapters):
     return p
 
 
+def validate_lowrank(params, order, tiles, n_rows):
+    """Host-side bounds check of a pass's records (numpy arrays) that the caller made or kept. Raises EspError. What
+    host.plan_lowrank returns for n_rows rows passes."""
+    order, tiles = np.ascontiguousarray(order, dtype=np.int32), np.ascontiguousarray(tiles, dtype=abi.LOWRANK_TILE_DT)
+    err = C.create_string_buffer(_ERRLEN)
+    abi.check(abi.attn_lib().esp_lowrank_validate(C.byref(params), order.ctypes.data, len(order), tiles.ctypes.data, len(tiles), n_rows, err, _ERRLEN),
+              err)
+
+
 class LowRankPass:
     """Which rows of a pass take which adapter, planned and resident on the device."""
 

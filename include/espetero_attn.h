@@ -447,6 +447,10 @@ size_t esp_lowrank_workspace_bytes(const esp_lowrank_params* p, int32_t n_tiles,
 int esp_lowrank_add(const esp_lowrank_params* p, const void* X, const void* A, const void* B, const float* scale, float* Y, const int32_t* order,
                     int32_t n_slots, const esp_lowrank_tile* tiles, int32_t n_tiles, void* workspace, size_t workspace_bytes, void* stream,
                     char* err, size_t errlen);
+/* Host-side check of a pass's records before they are uploaded (host pointers): adapters inside their table, tiles of at most
+ * rows_per_tile rows inside `order`, whose rows are below n_rows and in one tile each. Without it such records are read as they are. */
+int esp_lowrank_validate(const esp_lowrank_params* p, const int32_t* order, int32_t n_slots, const esp_lowrank_tile* tiles, int32_t n_tiles,
+                         int32_t n_rows, char* err, size_t errlen);
 
 /* ---- the logits at the end of a decode step ----------------------------------------
  * No counterpart in the reference's kernels (it samples on the host; its chains take the argmax on the GPU,

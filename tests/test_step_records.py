@@ -2,9 +2,10 @@
 sizes of their workspaces. No GPU: records are built in host memory and every call is refused."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
-from espetero_amd import abi, device
+from espetero_amd import abi, device, host
 
 
 # ---- one record, several passes
@@ -48,3 +49,49 @@ def test_lowrank_workspace_grows_with_tiles_and_rows(D, rank, n_slices):
     for (r, t, n), x in sizes.items():
         assert x >= 4 * n * rank * n_slices
         assert all(x <= y for (_, t2, n2), y in sizes.items() if t2 >= t and n2 >= n), (r, t, n)
+
+
+# ---- the adapters' records before they are uploaded
+def planned(n=40, rows_per_tile=16):
+    p = device.lowrank_params(64, 8, [(0, 64)], abi.ESP_F16, 64, 64, 3)
+    p.rows_per_tile = rows_per_tile
+    order, tiles = host.plan_lowrank(p, np.arange(n) % 4 - 1)
+    return p, order, tiles
+
+
+@pytest.mark.parametrize("rows_per_tile", [16, 64])
+@pytest.mark.parametrize("n", [0, 1, 40, 1000])
+def test_lowrank_validate_passes_what_the_planner_made(n, rows_per_tile):
+    p, order, tiles = planned(n, rows_per_tile)
+    device.validate_lowrank(p, order, tiles, n)
+    if len(tiles):
+        tiles["count"][0] = 0                                         # a tile without rows does nothing
+        device.validate_lowrank(p, order, tiles, n)
+
+
+@pytest.mark.parametrize("field,value,word", [("adapter", 3, "adapter"), ("adapter", -1, "adapter"), ("count", 17, "rows_per_tile"), ("count", -1, "rows"),
+                                              ("first", -1, "slots"), ("first", 25, "slots"), ("first", 2**31 - 1, "slots"), ("first", 1, "twice")])
+def test_lowrank_validate_refuses_tiles(field, value, word):
+    p, order, tiles = planned()
+    tiles[-1][field] = value
+    with pytest.raises(abi.EspError, match=word):
+        device.validate_lowrank(p, order, tiles, 40)
+
+
+def test_lowrank_validate_refuses_rows_and_arguments():
+    p, order, tiles = planned()
+    with pytest.raises(abi.EspError, match="row 39 of 39"):
+        device.validate_lowrank(p, order, tiles, 39)
+    for row, word in ((-1, "row -1"), (int(order[5]), "twice")):
+        bad = order.copy()
+        bad[0] = row
+        with pytest.raises(abi.EspError, match=word):
+            device.validate_lowrank(p, bad, tiles, 40)
+    with pytest.raises(abi.EspError, match="twice"):
+        device.validate_lowrank(p, order, np.concatenate([tiles, tiles]), 40)
+    err = C.create_string_buffer(256)
+    for args in ((None, 1, tiles.ctypes.data, 1, 40), (order.ctypes.data, 1, None, 1, 40), (None, -1, None, 0, 40), (None, 0, None, -1, 40), (None, 0, None, 0, -1)):
+        assert abi.attn_lib().esp_lowrank_validate(C.byref(p), *args, err, 256) == 1
+    p.rows_per_tile = 17
+    assert abi.attn_lib().esp_lowrank_validate(C.byref(p), None, 0, None, 0, 40, err, 256) == 2
+    assert abi.attn_lib().esp_lowrank_validate(None, None, 0, None, 0, 40, err, 256) == 1
