@@ -224,10 +224,11 @@ class DiffPass:
     """One planned pass of differential attention resident on the device (the rows of the pass are in the pool when it runs)."""
 
     def __init__(self, params, diff, trees, tiles, jobs, n_parts, n_rows, blocks, device="cuda", pool_blocks=None):
-        """pool_blocks: blocks in the pool; when given, the records are checked on the host before the upload."""
+        """pool_blocks: blocks in the pool; when given, the records are checked on the host before the upload. params stays the caller's
+        record, read by every run; passes of another rows_per_tile need one of their own."""
         if pool_blocks is not None:
             validate(params, tiles, trees, jobs, n_parts, n_rows, blocks, pool_blocks, diff=True)
-        self.params, self.diff = params, diff
+        self.params, self.diff, self.rows_per_tile = params, diff, params.rows_per_tile
         self.n_trees, self.n_tiles, self.n_jobs = len(trees), len(tiles), len(jobs)
         self.n_parts, self.n_rows = n_parts, n_rows
         self.trees = to_dev(np.ascontiguousarray(trees, dtype=abi.TREE_DT), device)
@@ -238,6 +239,8 @@ class DiffPass:
         self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
     def run(self, Q, pool, O, stream=None):
+        if self.params.rows_per_tile != self.rows_per_tile:
+            raise abi.EspError(f"rows_per_tile {self.params.rows_per_tile}: this pass was planned with {self.rows_per_tile} (one record for each)")
         ws = self.workspace
         _calls.attn_diff(self.params, self.diff, Q, pool, self.blocks, O, self.tiles, self.n_tiles, self.trees, self.n_trees, self.jobs, self.n_jobs,
                          self.n_parts, self.n_rows, ws, ws.nbytes, _stream(stream))

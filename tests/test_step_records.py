@@ -4,8 +4,9 @@ import ctypes as C
 
 import numpy as np
 import pytest
+import torch
 
-from espetero_amd import abi, device, host
+from espetero_amd import abi, device, host, synth
 
 
 # ---- one record, several passes
@@ -24,6 +25,24 @@ def test_lowrank_passes_of_one_record_keep_their_own_tiles(first, second):
         assert tiles["count"].max() == min(n, x.params.rows_per_tile) and tiles["count"].sum() == n
     p.D = 8                                                          # nor does a later change of the record reach them
     assert a.params.D == b.params.D == 256
+
+
+def test_a_diff_pass_refuses_to_run_with_other_tiles_than_its_own():
+    """The record stays the caller's, who may move its pool's region; the tiles are planned for one rows_per_tile."""
+    p = synth.make_params(8, 4, 128, abi.ESP_F16, 16, rows_per_tile=1)
+    none = torch.zeros(4)
+    passes = []
+    for M in (100, 1):
+        p.rows_per_tile = device.attn_diff_rows(p, M)
+        trees = np.array([(0, 0, 0, M)], abi.TREE_DT)
+        tiles, jobs, parts = host.plan_tiles(trees, abi.PlanGroups(2, p, diff=True), 0, None, host.options_mi355x(p.rows_per_tile, 4))
+        passes.append(device.DiffPass(p, device.diff_params(none, None, 0.0, 1.0), trees, tiles, jobs, parts, M, np.arange(7, dtype=np.int32), device="cpu",
+                                      pool_blocks=7))
+    with pytest.raises(abi.EspError, match="rows_per_tile"):
+        passes[0].run(none, none, none)
+    p.rows_per_tile = 64
+    with pytest.raises(abi.EspError, match="rows_per_tile"):
+        passes[1].run(none, none, none)
 
 
 # ---- a workspace sized for the largest pass serves the smaller ones
