@@ -315,7 +315,8 @@ class LogitsPass:
         self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
     def run(self, logits, out, tokens, bias_tokens, bias_values, masks, seen, counts, record=False, stream=None):
-        """Device tensors; out or tokens may be None, and so may what no row names. record: the tokens join their slots' histories."""
+        """Device tensors; out or tokens may be None, and so may the arrays of which params counts 0 (histories, masks, bias entries).
+        record: the tokens join their slots' histories."""
         ws = self.workspace
         _calls.logits_process(self.params, logits, out, tokens, self.rows, self.n_rows, bias_tokens, bias_values, masks, seen, counts, int(record), ws,
                               ws.nbytes, _stream(stream))

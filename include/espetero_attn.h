@@ -488,8 +488,9 @@ size_t esp_logits_workspace_bytes(const esp_logits_params* p, int32_t n_rows);
 /* logits [n_rows][in_ld]; out [n_rows][out_ld] fp32 or NULL (it may be the logits themselves where those are fp32 and
  * out_ld == in_ld); tokens [n_rows] or NULL (then record is 0). rows: n_rows records. masks [n_masks][ceil(vocab / 32)]:
  * bit t % 32 of word t / 32 set where token t is allowed. Histories: seen [n_slots][2][ceil(vocab / 32)], bits of the
- * tokens of the prompt and of those given out; counts [n_slots][vocab], how often each was given out. Arrays that no row
- * names may be NULL. All device memory. Slots, masks and entries outside their arrays count as none. */
+ * tokens of the prompt and of those given out; counts [n_slots][vocab], how often each was given out. seen
+ * and counts may be NULL where n_slots is 0, masks where n_masks is, bias_tokens and bias_values where n_bias is, whatever the rows
+ * name. All device memory. Slots, masks and entries outside their arrays count as none. */
 int esp_logits_process(const esp_logits_params* p, const void* logits, float* out, int32_t* tokens, const esp_logits_row* rows, int32_t n_rows,
                        const int32_t* bias_tokens, const float* bias_values, const uint32_t* masks, uint32_t* seen, int32_t* counts,
                        int32_t record, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen);

@@ -114,3 +114,19 @@ def test_lowrank_validate_refuses_rows_and_arguments():
     p.rows_per_tile = 17
     assert abi.attn_lib().esp_lowrank_validate(C.byref(p), None, 0, None, 0, 40, err, 256) == 2
     assert abi.attn_lib().esp_lowrank_validate(None, None, 0, None, 0, 40, err, 256) == 1
+
+
+# ---- the logits' arrays that may be NULL
+@pytest.mark.parametrize("count,arrays", [("n_slots", ("seen", "counts")), ("n_masks", ("masks",)), ("n_bias", ("bias_tokens", "bias_values"))])
+def test_logits_arrays_may_be_null_where_they_are_counted_as_empty(count, arrays):
+    """As the header says: by the count in the parameters, not by what the rows in device memory name. The last check of a call, the
+    workspace's, is reached where the arrays are accepted."""
+    at = {k: 0x1000 for k in ("bias_tokens", "bias_values", "masks", "seen", "counts")}
+    err = C.create_string_buffer(256)
+    for n, rc in ((0, 4), (2, 1)):
+        p = device.logits_params(100, abi.ESP_F16, 2, 2, 2)
+        setattr(p, count, n)
+        for missing in [(a,) for a in arrays] + [arrays]:
+            a = {k: None if k in missing else v for k, v in at.items()}
+            assert abi.attn_lib().esp_logits_process(C.byref(p), 0x1000, None, 0x1000, 0x1000, 3, a["bias_tokens"], a["bias_values"], a["masks"], a["seen"],
+                                                     a["counts"], 0, None, 0, None, err, 256) == rc, (n, missing, err.value)
