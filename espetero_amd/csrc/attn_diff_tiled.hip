@@ -22,8 +22,9 @@
 // load from memory but the stages (any such load's wait is a wait for them), nor spill.
 //
 // 2048 rows behind 12000 keys, 40 / 8 heads, bf16: 990 to 1030 us, 0.81 PFLOP/s of visible work and 1.08 with the second numbers,
-// where a plain 8192^3 product of the library reaches 1.20. Ragged fresh prompts of 40 .. 800 rows, 32 / 8, fp16: 52 us, bound by the
-// longest tile's 25 stages and the turns before and after them.
+// where a plain 8192^3 product of the library reaches 1.20. A SIMD's matrix core is busy 63 % of the time that a workgroup is there (other
+// vector work beside it for 42 % of that), and one is there 83 % of the pass. Ragged fresh prompts of 40 .. 800 rows, 32 / 8, fp16: 52 us, the
+// longest tile's 25 stages and the turns before and after them, in which the matrix cores are busy 37 %.
 #include "diff_math.hpp"
 #include "lds_direct.hpp"
 

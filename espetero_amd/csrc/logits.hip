@@ -3,8 +3,9 @@
 //
 // Bound by HBM: a logit is read once and, where the caller wants them back, written once; the histories' two bits a token come
 // with them. The counts behind the bits are read only where a bit is set, and then cost a line each: 192 fp32 rows of 250000 tokens with
-// up to 6000 seen move 309 MB in 47 us, 6.6 TB/s, 74 MB of it for counts. Small passes are bound by the hops to a row's record, its
-// words and its counts, and by the second launch: 48 bf16 rows of 50257 take 11 us (8 + 2 in the kernels), one fp32 row of 32000 takes 7.
+// up to 6000 seen move 309 MB in 47 us, 6.6 TB/s, 74 MB of it for counts (50 to 58 us with the second launch, 107 where the logits are
+// wanted back, another 192 MB). Small passes are bound by the hops to a row's record, its words and its counts, and by the second launch:
+// 48 bf16 rows of 50257 take 11 to 13 us (8 + 3 in the kernels), one fp32 row of 32000 takes 7 to 8.5.
 #include "common.hpp"
 #include "logits_shape.hpp"
 
@@ -66,7 +67,7 @@ __device__ __forceinline__ void record_token(uint32_t* seen, int32_t* counts, in
 // grid: (chunks of 256 TP tokens, rows). The penalties touch few of the tokens, and so do the biases: their bits are gathered first,
 // and a chunk's tokens then go two ways. The many that nothing but the mask touches are passed on and compared as they come. The few
 // others become a list in LDS that all lanes share, whichever thread's they were, since a lane that found one among its own would hold
-// up 63 that found none: done in place, with the counts behind it, 192 rows of 250000 took 126 us where they now take 50.
+// up 63 that found none: done in place, with the counts behind it, 192 rows of 250000 took 126 us where they now take 50 to 58.
 template <int DT, bool OUT, int TP>
 __global__ __launch_bounds__(256) void logits_kernel(const LogitsArgs a) {
   constexpr int W = 256, CH = TP * W, NW = CH / 32;                  // threads, tokens of a chunk, its words of bits

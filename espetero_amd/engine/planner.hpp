@@ -79,7 +79,10 @@ struct PlanOptions {
     return o;
   }
   // These options where the tiled differential attention kernel runs the pass: what mi355x() takes for a streaming pass by its rows is
-  // planned by the hand-out of workgroups to slots like any tiled pass. Set fields stay.
+  // planned by the hand-out of workgroups to slots like any tiled pass. Set fields stay, and so do the 512 and 1024 that mi355x() gives
+  // tiles of more than 32 rows: groups of one to three query pairs (900 fresh rows at 8 / 8, 12 / 4 and 16 / 8 heads: 52 us, uncut on 32 to
+  // 60 workgroups, where 32 / 8 take 44; 100 rows over 1000 keys: 33 to 35 and 36). The steps' prices are the plain tiled kernel's, and so
+  // is the end of its candidates at eight parts.
   PlanOptions for_diff_tiled() const {
     const PlanOptions had = mi355x(1, groups_target), tiled = mi355x(64, groups_target);
     PlanOptions o = *this;

@@ -69,7 +69,8 @@ int esp_plan_tiles_for(const esp_attn_params* p, const esp_tree* trees, int32_t 
 /* The same for a pass of esp_attn_diff (p: its parameters; groups: what esp_attn_diff_hint reports). Options as from
  * esp_plan_options_mi355x: where the tiled kernel serves p, those of a streaming pass (its tiles may have few rows, by which that
  * function tells the two apart) become its own, the pass's own rows are cut like cached keys (cut_batch), and its tiles come longest
- * last, which is the order the kernel starts them in, reversed. Fields that do not hold what that function gave them stay as they are. */
+ * last, which is the order the kernel starts them in, reversed. Fields that do not hold what that function gives a streaming pass stay as
+ * they are, those of options for more than 32 rows among them (min_chunk 512, min_span 1024). */
 int esp_plan_tiles_diff(const esp_attn_params* p, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
                         const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                         int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen);
