@@ -7,12 +7,13 @@
 //   S^T[32 keys][32 rows] = K_map . Q_map^T      A = K from LDS, B = Q^T in registers
 //   P^T = exp2(S^T - m)                          registers; the D layout of S^T is the B layout of P^T
 //   O^T[256][32 rows]    += V^T . P^T            A = V^T from LDS, both maps read the same values
-// with v_mfma_f32_32x32x16 and P . V one stage behind S. The product takes P in the storage type. The first map's enters as the sum of
-// two such numbers, the second's, which counts by its weight, as one: 40 and 24 products of 32 cycles a stage, and every SIMD has one
-// wavefront of either map. So the output's error against 64 bits is 1.15 times that of its own rounding (bf16 0.0019, fp16 0.00024 of
-// its size). One number for both: 0.0026, 0.00031, and the two cases below in 800 and 48 us; two for both: no more than the rounding, in
-// 1165 and 64 us. After the last key the second map's wavefronts hand their output over through LDS, and the first map's take the
-// difference, the norm and the one rounding of the output.
+// with v_mfma_f32_32x32x16 and P . V one stage behind S. The product takes P in the storage type, as the sum of two such numbers, 16 bits
+// or more: 40 products of 32 cycles a stage. So the output's error against 64 bits is that of its own rounding (bf16 0.0017, fp16 0.00021
+// of its size), also where the two maps are nearly alike and most of them goes in the difference. One number for both maps: 0.0026 and
+// 0.00031, the two cases below in 800 and 48 us. Two for the first and one for the second: 0.0019 and 0.00024 for maps that have nothing in
+// common, in 990 and 52 us, but 0.0064 for equal ones at weight 0.8 and 0.029 at 0.95, since what the second loses is not lost by the first
+// too. After the last key the second map's wavefronts hand their output over through LDS, and the first map's take the difference, the norm and
+// the one rounding of the output.
 //
 // LDS: a ring of 4 stages of 32 keys, 32 KB each: K of both heads, V^T of both heads, loaded straight from the pool (global_load_lds)
 // by wavefronts 0 .. 3 (K, three stages ahead) and 4 .. 7 (V^T, two ahead), a run of 4 KB each. K: the 16-byte chunk c of row r lies at
@@ -21,10 +22,10 @@
 // run half a turn apart, so that one's softmax lies under the other's products, and meet at one barrier a turn. Nothing in the loop may
 // load from memory but the stages (any such load's wait is a wait for them), nor spill.
 //
-// 2048 rows behind 12000 keys, 40 / 8 heads, bf16: 990 to 1030 us, 0.81 PFLOP/s of visible work and 1.08 with the second numbers,
-// where a plain 8192^3 product of the library reaches 1.20. A SIMD's matrix core is busy 63 % of the time that a workgroup is there (other
-// vector work beside it for 42 % of that), and one is there 83 % of the pass. Ragged fresh prompts of 40 .. 800 rows, 32 / 8, fp16: 52 us, the
-// longest tile's 25 stages and the turns before and after them, in which the matrix cores are busy 37 %.
+// 2048 rows behind 12000 keys, 40 / 8 heads, bf16: 1110 us, 0.74 PFLOP/s of visible work and 1.23 with the second numbers, where a
+// plain 8192^3 product of the library reaches 1.20. A SIMD's matrix core is busy 75 % of the time that a workgroup is there (other vector
+// work beside it for 43 % of that), and one is there 83 % of the pass. Ragged fresh prompts of 40 .. 800 rows, 32 / 8, fp16: 56 us, the
+// longest tile's 25 stages and the turns before and after them, in which the matrix cores are busy 45 %.
 #include "diff_math.hpp"
 #include "lds_direct.hpp"
 
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
   float m_ref = -INFINITY, l_run = 0.0f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) acc[nt] = f32x16{};
-  u32x4 P[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}}, rest[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};  // rest: the first map's, what P's rounding left
+  u32x4 P[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}}, rest[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};  // rest: what P's rounding left
 
   f32x16 s{};
   // Matrix work of a turn, and the request of stage `next` (-1: none) between it: P . V of stage h - 1 and the scores of stage h, a score
@@ -168,10 +169,8 @@ __global__ __launch_bounds__(512, 2) void attn_diff_tiled_kernel(const DiffArgs 
       s = mfma32x16<DT>(k[g % 3], qf[g], s);
 #pragma unroll
       for (int i = 0; i < 2; ++i) acc[(2 * g + i) & 7] = mfma32x16<DT>(v[g % 3][i], P[g >> 2], acc[(2 * g + i) & 7]);
-      if (map == 0) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) acc[(2 * g + i) & 7] = mfma32x16<DT>(v[g % 3][i], rest[g >> 2], acc[(2 * g + i) & 7]);
-      }
+      for (int i = 0; i < 2; ++i) acc[(2 * g + i) & 7] = mfma32x16<DT>(v[g % 3][i], rest[g >> 2], acc[(2 * g + i) & 7]);
       if (g == 3 && next >= 0) request(next);
       if (g == 5 && next >= 0) advance();
       __builtin_amdgcn_sched_barrier(0);

@@ -80,18 +80,18 @@ struct PlanOptions {
   }
   // These options where the tiled differential attention kernel runs the pass: what mi355x() takes for a streaming pass by its rows is
   // planned by the hand-out of workgroups to slots like any tiled pass. Set fields stay, and so do the 512 and 1024 that mi355x() gives
-  // tiles of more than 32 rows: groups of one to three query pairs (900 fresh rows at 8 / 8, 12 / 4 and 16 / 8 heads: 52 us, uncut on 32 to
-  // 60 workgroups, where 32 / 8 take 44; 100 rows over 1000 keys: 33 to 35 and 36). The steps' prices are the plain tiled kernel's, and so
+  // tiles of more than 32 rows: groups of one to three query pairs (900 fresh rows at 8 / 8, 12 / 4 and 16 / 8 heads: 53 to 54 us, uncut on 32
+  // to 60 workgroups, where 32 / 8 take 45; 100 rows over 1000 keys: 34 to 35 and 36). The steps' prices are the plain tiled kernel's, and so
   // is the end of its candidates at eight parts.
   PlanOptions for_diff_tiled() const {
     const PlanOptions had = mi355x(1, groups_target), tiled = mi355x(64, groups_target);
     PlanOptions o = *this;
     if (!o.balanced) return o;
     o.by_length = true;
-    o.cut_batch = true;  // (the rows are read like any key; 8 / 2 heads, 1500 fresh rows: 75 us without, 40 so; 32 / 8, 900: 51 and 43)
+    o.cut_batch = true;  // (the rows are read like any key; 8 / 2 heads, 1500 fresh rows: 79 us without, 41 so; 32 / 8, 900: 53 and 46)
     auto turn = [](int& field, int from, int to) { field = field == from ? to : field; };
     turn(o.granule, had.granule, tiled.granule);
-    turn(o.min_chunk, had.min_chunk, 128);  // (100 rows over 1000 keys, 32 / 8 heads: 51 us at 512 and 1024, 35 so; fresh prompts alike)
+    turn(o.min_chunk, had.min_chunk, 128);  // (100 rows over 1000 keys, 32 / 8 heads: 63 us uncut, 38 at 512 and 1024, 36 so)
     turn(o.min_span, had.min_span, 256);
     turn(o.item_steps, had.item_steps, tiled.item_steps);
     turn(o.part_steps, had.part_steps, tiled.part_steps);

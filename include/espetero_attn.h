@@ -384,8 +384,8 @@ int esp_head_gate(const esp_gate_params* p, void* O, const void* X, const void* 
  * Pool, records, planner and append are those of esp_attn_forward without Kb / Vb: the pass's rows are in the pool
  * (esp_attn_prep with a row_table, or esp_kv_save), row j of a tree at position P + j of its own block list or ring.
  * Rows are plain causal: row j sees the keys 0 .. P + j, of them the last `window` where window > 0. Softmax, difference
- * and norm are held in fp32; the probabilities enter P.V as the sum of two numbers of the storage type (the second map's, in
- * passes of many rows, as one), O is rounded once at the end. */
+ * and norm are held in fp32; the probabilities enter P.V as the sum of two numbers of the storage type, O is rounded once at
+ * the end. */
 typedef struct esp_diff_params {
   const float* weight; /* [H / 2] fp32, device memory */
   const float* norm_w; /* [2 * head_dim] fp32, device memory; NULL: no norm (eps is then not read) */
