@@ -22,9 +22,9 @@
 // run half a turn apart, so that one's softmax lies under the other's products, and meet at one barrier a turn. Nothing in the loop may
 // load from memory but the stages (any such load's wait is a wait for them), nor spill.
 //
-// 2048 rows behind 12000 keys, 40 / 8 heads, bf16: 1110 us, 0.74 PFLOP/s of visible work and 1.23 with the second numbers, where a
-// plain 8192^3 product of the library reaches 1.20. A SIMD's matrix core is busy 75 % of the time that a workgroup is there (other vector
-// work beside it for 43 % of that), and one is there 83 % of the pass. Ragged fresh prompts of 40 .. 800 rows, 32 / 8, fp16: 56 us, the
+// 2048 rows behind 12000 keys, 40 / 8 heads, bf16: 1110 to 1150 us, 0.71 to 0.74 PFLOP/s of visible work and 1.19 to 1.23 with the second
+// numbers, where a plain 8192^3 product of the library reaches 1.20. A SIMD's matrix core is busy 75 % of the time that a workgroup is there (other vector
+// work beside it for 43 % of that), and one is there 83 % of the pass. Ragged fresh prompts of 40 .. 800 rows, 32 / 8, fp16: 56 to 57 us, the
 // longest tile's 25 stages and the turns before and after them, in which the matrix cores are busy 45 %.
 #include "diff_math.hpp"
 #include "lds_direct.hpp"
