@@ -75,6 +75,12 @@ class LogitsParams(C.Structure):
                 ("n_masks", C.c_int32), ("n_bias", C.c_int32), ("pad", C.c_int32)]
 
 
+class LinearParams(C.Structure):
+    _fields_ = [("H", C.c_int32), ("Hk", C.c_int32), ("dk", C.c_int32), ("dv", C.c_int32), ("dtype", C.c_int32), ("q_ld", C.c_int32),
+                ("k_ld", C.c_int32), ("v_ld", C.c_int32), ("o_ld", C.c_int32), ("decay_ld", C.c_int32), ("n_states", C.c_int32),
+                ("scale", C.c_float)]
+
+
 TREE_DT = np.dtype([("base", "<i4"), ("P", "<i4"), ("table", "<i4"), ("M", "<i4")])
 TILE_DT = np.dtype([("tree", "<i4"), ("r0", "<i4"), ("k0", "<i4"), ("k1", "<i4"),
                     ("part", "<i4"), ("last", "<i4"), ("b0", "<i4"), ("pad", "<i4")])
@@ -83,6 +89,9 @@ KVSAVE_DT = np.dtype([("src_row", "<i4"), ("block", "<i4"), ("pos", "<i4"), ("pa
 LOWRANK_TILE_DT = np.dtype([("adapter", "<i4"), ("first", "<i4"), ("count", "<i4"), ("pad", "<i4")])
 LOGITS_ROW_DT = np.dtype([("slot", "<i4"), ("mask", "<i4"), ("bias0", "<i4"), ("n_bias", "<i4"), ("repetition", "<f4"),
                           ("frequency", "<f4"), ("presence", "<f4"), ("pad", "<i4")])
+LINEAR_SEQ_DT = np.dtype([("base", "<i4"), ("rows", "<i4"), ("src", "<i4"), ("dst", "<i4")])
+LINEAR_TILE_DT = np.dtype([("row0", "<i4"), ("rows", "<i4"), ("src", "<i4"), ("dst", "<i4"), ("part", "<i4"), ("before", "<i4"),
+                           ("after", "<i4"), ("pad", "<i4")])
 
 assert C.sizeof(Tree) == TREE_DT.itemsize == 16
 assert C.sizeof(Tile) == TILE_DT.itemsize == 32
@@ -95,6 +104,7 @@ assert C.sizeof(DiffParams) == 24
 assert C.sizeof(LowRankParams) == 64
 assert C.sizeof(LogitsParams) == 32
 assert LOWRANK_TILE_DT.itemsize == 16 and LOGITS_ROW_DT.itemsize == 32
+assert C.sizeof(LinearParams) == 48 and LINEAR_SEQ_DT.itemsize == 16 and LINEAR_TILE_DT.itemsize == 32
 
 # name -> (restype, argtypes); every symbol the header declares.
 _P = C.POINTER(AttnParams)
@@ -139,6 +149,11 @@ ATTN_SYMBOLS = {
     "esp_logits_validate": (C.c_int, (C.POINTER(LogitsParams), _V, C.c_int32, _V) + _ERR),
     "esp_history_record": (C.c_int, (C.POINTER(LogitsParams), _V, _V, _V, _V, C.c_int32, C.c_int32, _V) + _ERR),
     "esp_history_clear": (C.c_int, (C.POINTER(LogitsParams), _V, _V, _V, C.c_int32, _V) + _ERR),
+    "esp_linear_hint": (C.c_int, (C.POINTER(LinearParams), C.c_int, C.POINTER(C.c_int32)) + _ERR),
+    "esp_linear_workspace_bytes": (C.c_size_t, (C.POINTER(LinearParams), C.c_int32)),
+    "esp_linear_attn": (C.c_int, (C.POINTER(LinearParams), _V, _V, _V, _V, _V, _V, _V, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _V, C.c_size_t,
+                                  _V) + _ERR),
+    "esp_linear_validate": (C.c_int, (C.POINTER(LinearParams), _V, C.c_int32, C.c_int32, C.c_int32, C.c_int32) + _ERR),
     "esp_attn_prep": (C.c_int, (C.POINTER(PrepParams), _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, _V, C.c_int32, _V) + _ERR),
 }
 

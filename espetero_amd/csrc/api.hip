@@ -12,6 +12,7 @@
 
 #include "common.hpp"
 #include "diff_math.hpp"
+#include "linear_shape.hpp"
 #include "logits_shape.hpp"
 #include "lowrank_shape.hpp"
 
@@ -43,6 +44,8 @@ hipError_t launch_diff_tiled(int dt, const DiffArgs& a, int n_tiles, hipStream_t
 hipError_t launch_diff_merge(int dt, const DiffArgs& a, const esp_combine* jobs, int n_jobs, int n_parts, hipStream_t st);
 hipError_t diff_init_attributes();
 hipError_t diff_tiled_init_attributes();
+hipError_t launch_linear(int dt, const LinearArgs& a, int n_few, int n_chunked, bool split, hipStream_t st);
+hipError_t linear_init_attributes();
 hipError_t launch_lowrank(int dt, const LowRankArgs& a, int rows_per_tile, int n_tiles, hipStream_t st);
 hipError_t launch_logits(int dt, const LogitsArgs& a, int n_rows, hipStream_t st);
 hipError_t launch_history_record(const esp_logits_params* p, uint32_t* seen, int32_t* counts, const int32_t* tokens, const int32_t* slots, int n,
@@ -172,6 +175,7 @@ int device_state(DeviceState** out, char* err, size_t errlen) {
     if ((e = esp::gate_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (head gate)", e);
     if ((e = esp::diff_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (differential attention)", e);
     if ((e = esp::diff_tiled_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (tiled differential attention)", e);
+    if ((e = esp::linear_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (linear attention)", e);
     d.scratch = static_cast<unsigned char*>(ps);
     d.ready = true;
   }
@@ -965,6 +969,130 @@ int esp_history_clear(const esp_logits_params* p, uint32_t* seen, int32_t* count
   if (n == 0) return ESP_OK;
   const hipError_t e = esp::launch_history_clear(p, seen, counts, slots, n, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? ESP_OK : hip_fail(err, errlen, "history_clear launch", e);
+}
+
+// ---- linear attention --------------------------------------------------------------
+static int check_linear(const esp_linear_params* p, char* err, size_t errlen) {
+  if (!p) return fail(err, errlen, ESP_EINVAL, "params is NULL");
+  if (p->dtype != ESP_F16 && p->dtype != ESP_BF16) return fail(err, errlen, ESP_EINVAL, "dtype %d", p->dtype);
+  if (p->Hk <= 0 || p->H <= 0 || p->H % p->Hk || p->H > 4096)
+    return fail(err, errlen, ESP_EINVAL, "H=%d Hk=%d: H must be a positive multiple of Hk, at most 4096", p->H, p->Hk);
+  if (!esp::linear_dims(p->dk, p->dv)) return fail(err, errlen, ESP_EUNSUPPORTED, "dk %d (64 or 128), dv %d (a multiple of 64, at most 512)", p->dk, p->dv);
+  if (p->q_ld < p->Hk * p->dk || p->k_ld < p->Hk * p->dk || p->v_ld < p->H * p->dv || p->o_ld < p->H * p->dv)
+    return fail(err, errlen, ESP_EINVAL, "q_ld %d, k_ld %d, v_ld %d, o_ld %d: a row has %d, %d, %d and %d elements", p->q_ld, p->k_ld, p->v_ld, p->o_ld,
+                p->Hk * p->dk, p->Hk * p->dk, p->H * p->dv, p->H * p->dv);
+  if ((p->q_ld | p->k_ld | p->v_ld | p->o_ld) % 8) return fail(err, errlen, ESP_EINVAL, "row strides must be multiples of 8");
+  if (p->decay_ld != 0 && p->decay_ld < p->H) return fail(err, errlen, ESP_EINVAL, "decay_ld %d (0, or at least H = %d)", p->decay_ld, p->H);
+  if (p->n_states < 0) return fail(err, errlen, ESP_EINVAL, "n_states %d", p->n_states);
+  if (!std::isfinite(p->scale)) return fail(err, errlen, ESP_EINVAL, "scale is not finite");
+  return ESP_OK;
+}
+
+int esp_linear_hint(const esp_linear_params* p, int device, int32_t* workgroups, char* err, size_t errlen) {
+  if (int rc = check_linear(p, err, errlen)) return rc;
+  if (!workgroups) return fail(err, errlen, ESP_EINVAL, "NULL output");
+  int cus = 0;
+  const hipError_t e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
+  if (e != hipSuccess) return hip_fail(err, errlen, "hipDeviceGetAttribute", e);
+  *workgroups = cus * esp::linear_workgroups_per_cu(p->dk, p->dv);
+  return ESP_OK;
+}
+
+size_t esp_linear_workspace_bytes(const esp_linear_params* p, int32_t n_parts) {
+  if (check_linear(p, nullptr, 0) != ESP_OK) return 0;
+  return esp::carve_linear(p->H, p->dk, p->dv, n_parts).total;
+}
+
+int esp_linear_attn(const esp_linear_params* p, const void* Q, const void* K, const void* V, const float* decay, float* states, void* O,
+                    const esp_linear_tile* tiles, int32_t n_tiles, int32_t n_few, int32_t n_parts, int32_t n_rows, void* workspace,
+                    size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  if (int rc = check_linear(p, err, errlen)) return rc;
+  if (n_tiles < 0 || n_few < 0 || n_few > n_tiles || n_parts < 0 || n_rows < 0) return fail(err, errlen, ESP_EINVAL, "counts");
+  if (n_tiles == 0) return ESP_OK;
+  if (!tiles || !decay) return fail(err, errlen, ESP_EINVAL, "tiles and decay must not be NULL");
+  if (n_rows > 0 && (!Q || !K || !V || !O)) return fail(err, errlen, ESP_EINVAL, "Q, K, V and O must not be NULL");
+  if (p->n_states > 0 && !states) return fail(err, errlen, ESP_EINVAL, "states is NULL");
+  if ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V) | reinterpret_cast<uintptr_t>(O) |
+       reinterpret_cast<uintptr_t>(states) | reinterpret_cast<uintptr_t>(workspace)) % 16)
+    return fail(err, errlen, ESP_EINVAL, "Q, K, V, O, states and workspace must be 16-byte aligned");
+  if (n_few > 65535 || n_tiles - n_few > 65535) return fail(err, errlen, ESP_EUNSUPPORTED, "%d and %d tiles in one pass: at most 65535 of each kind", n_few, n_tiles - n_few);
+  const esp::LinearCarve c = esp::carve_linear(p->H, p->dk, p->dv, n_parts);
+  if (n_parts > 0 && (!workspace || workspace_bytes < c.total))
+    return fail(err, errlen, ESP_EWORKSPACE, "workspace %zu bytes, %zu needed", workspace ? workspace_bytes : size_t(0), c.total);
+  DeviceState* dev = nullptr;
+  if (int rc = device_state(&dev, err, errlen)) return rc;
+  esp::LinearArgs a{};
+  a.Q = static_cast<const uint16_t*>(Q);
+  a.K = static_cast<const uint16_t*>(K);
+  a.V = static_cast<const uint16_t*>(V);
+  a.decay = decay;
+  a.states = states;
+  a.O = static_cast<uint16_t*>(O);
+  a.tiles = tiles;
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + c.states);
+  a.part_totals = reinterpret_cast<double*>(static_cast<char*>(workspace) + c.totals);
+  a.H = p->H;
+  a.group = p->H / p->Hk;
+  a.dk = p->dk;
+  a.dv = p->dv;
+  a.q_ld = p->q_ld;
+  a.k_ld = p->k_ld;
+  a.v_ld = p->v_ld;
+  a.o_ld = p->o_ld;
+  a.decay_ld = p->decay_ld;
+  a.scale = p->scale;
+  const hipError_t e = esp::launch_linear(p->dtype, a, n_few, n_tiles - n_few, n_parts > 0, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? ESP_OK : hip_fail(err, errlen, "linear_attn launch", e);
+}
+
+int esp_linear_validate(const esp_linear_params* p, const esp_linear_tile* tiles, int32_t n_tiles, int32_t n_few, int32_t n_parts, int32_t n_rows,
+                        char* err, size_t errlen) {
+  if (int rc = check_linear(p, err, errlen)) return rc;
+  if (n_tiles < 0 || n_few < 0 || n_few > n_tiles || n_parts < 0 || n_rows < 0) return fail(err, errlen, ESP_EINVAL, "counts");
+  if (n_tiles && !tiles) return fail(err, errlen, ESP_EINVAL, "NULL record array");
+  try {
+    std::vector<char> row(size_t(n_rows), 0), part(size_t(n_parts), 0);
+    std::vector<int32_t> writer(size_t(p->n_states), -1), reader(size_t(p->n_states), -1);  // sequences, named by their first tile
+    int first = 0;
+    for (int i = 0; i < n_tiles; ++i) {
+      const esp_linear_tile& t = tiles[i];
+      if (t.rows < 0 || t.row0 < 0 || int64_t(t.row0) + t.rows > n_rows)
+        return fail(err, errlen, ESP_EINVAL, "tile %d: rows [%d, %d + %d) outside the pass's %d rows", i, t.row0, t.row0, t.rows, n_rows);
+      if (i < n_few && t.rows > esp::kLinearFew) return fail(err, errlen, ESP_EINVAL, "tile %d: %d rows among those of few (at most %d)", i, t.rows, esp::kLinearFew);
+      for (int r = t.row0; r < t.row0 + t.rows; ++r)
+        if (row[size_t(r)]++) return fail(err, errlen, ESP_EINVAL, "tile %d: row %d is in another tile too", i, r);
+      if (t.src < -1 || t.src >= p->n_states || t.dst < -1 || t.dst >= p->n_states)
+        return fail(err, errlen, ESP_EINVAL, "tile %d: slots %d and %d of %d", i, t.src, t.dst, p->n_states);
+      if (t.before < 0 || t.after < 0 || t.part < -1) return fail(err, errlen, ESP_EINVAL, "tile %d: segments or record negative", i);
+      if ((t.before > 0 || t.after > 0) != (t.part >= 0) || (t.part >= 0 && i < n_few))
+        return fail(err, errlen, ESP_EINVAL, "tile %d: %d segments in front, %d behind, first record %d", i, t.before, t.after, t.part);
+      if (t.part >= 0 && int64_t(t.part) + t.before + t.after + 1 > n_parts)
+        return fail(err, errlen, ESP_EINVAL, "tile %d: records [%d, %d + %d) of %d", i, t.part, t.part, t.before + t.after + 1, n_parts);
+      if (t.before == 0) {
+        first = i;
+        if (t.src >= 0) reader[size_t(t.src)] = reader[size_t(t.src)] == -1 || reader[size_t(t.src)] == i ? i : -2;
+        for (int q = t.part; t.part >= 0 && q <= t.part + t.after; ++q)
+          if (part[size_t(q)]++) return fail(err, errlen, ESP_EINVAL, "tile %d: record %d is another sequence's too", i, q);
+      } else {
+        const esp_linear_tile& u = tiles[i - 1];
+        if (i == 0 || i == n_few || u.before + 1 != t.before || u.after - 1 != t.after || u.part != t.part || u.src != t.src || u.row0 + u.rows != t.row0)
+          return fail(err, errlen, ESP_EINVAL, "tile %d does not go on where the one in front of it ends", i);
+      }
+      if (t.after > 0 && (i + 1 >= n_tiles || tiles[i + 1].before != t.before + 1))
+        return fail(err, errlen, ESP_EINVAL, "tile %d: the segment behind it is missing", i);
+      if (t.after > 0 && t.dst >= 0) return fail(err, errlen, ESP_EINVAL, "tile %d: dst %d in front of its sequence's end", i, t.dst);
+      if (t.dst >= 0) {
+        if (writer[size_t(t.dst)] != -1) return fail(err, errlen, ESP_EINVAL, "tile %d: slot %d is another sequence's too", i, t.dst);
+        writer[size_t(t.dst)] = first;
+      }
+    }
+    for (int s = 0; s < p->n_states; ++s)
+      if (writer[size_t(s)] != -1 && reader[size_t(s)] != -1 && reader[size_t(s)] != writer[size_t(s)])
+        return fail(err, errlen, ESP_EINVAL, "slot %d is read by another sequence than the one that leaves its state there", s);
+  } catch (const std::exception& e) {
+    return fail(err, errlen, ESP_EINVAL, "%s", e.what());
+  }
+  return ESP_OK;
 }
 
 }  // extern "C"

@@ -328,3 +328,46 @@ def history_record(params, seen, counts, tokens, slots, n, given, stream=None):
 
 def history_clear(params, seen, counts, slots, n, stream=None):
     _calls.history_clear(params, seen, counts, slots, n, _stream(stream))
+
+
+def linear_params(H, Hk, dk, dv, dtype, scale, n_states, row_decay=False, q_ld=None, k_ld=None, v_ld=None, o_ld=None, decay_ld=None):
+    """row_decay: log decays [n_rows][H] (rows decay_ld apart) instead of [H]. Strides in elements, of rows without gaps by default."""
+    return abi.LinearParams(H, Hk, dk, dv, dtype, q_ld or Hk * dk, k_ld or Hk * dk, v_ld or H * dv, o_ld or H * dv,
+                            (decay_ld or H) if row_decay else 0, n_states, scale)
+
+
+def validate_linear(params, tiles, n_few, n_parts, n_rows):
+    """Host-side bounds check of a pass's records (numpy array) that the caller made or kept. Raises EspError. What
+    host.plan_linear returns for n_rows rows passes."""
+    tiles = np.ascontiguousarray(tiles, dtype=abi.LINEAR_TILE_DT)
+    err = C.create_string_buffer(_ERRLEN)
+    abi.check(abi.attn_lib().esp_linear_validate(C.byref(params), tiles.ctypes.data, len(tiles), n_few, n_parts, n_rows, err, _ERRLEN), err)
+
+
+def linear_hint(params, device=0):
+    """Workgroups of linear attention's chunked kernel that the device holds at once: what a pass is planned for."""
+    err = C.create_string_buffer(_ERRLEN)
+    n = C.c_int32(0)
+    abi.check(abi.attn_lib().esp_linear_hint(C.byref(params), device, C.byref(n), err, _ERRLEN), err)
+    return n.value
+
+
+class LinearPass:
+    """The sequences of a pass of linear attention, planned and resident on the device."""
+
+    def __init__(self, params, seqs, n_rows, workgroups=None, device="cuda"):
+        """seqs: LINEAR_SEQ_DT. params: a layer's record may serve any number of passes; each keeps a copy."""
+        self.params, self.n_rows = abi.LinearParams.from_buffer_copy(params), n_rows
+        if workgroups is None:
+            workgroups = linear_hint(params, torch.device(device).index or 0)
+        tiles, self.n_few, self.n_parts = host.plan_linear(params, seqs, n_rows, workgroups)
+        self.n_tiles = len(tiles)
+        self.tiles = to_dev(tiles, device) if self.n_tiles else None
+        nbytes = abi.attn_lib().esp_linear_workspace_bytes(C.byref(params), self.n_parts)
+        self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+    def run(self, Q, K, V, decay, states, O, stream=None):
+        """Device tensors; Q, K, V may be slices of one projection's rows (their strides in params). states are updated in place."""
+        ws = self.workspace
+        _calls.linear_attn(self.params, Q, K, V, decay, states, O, self.tiles, self.n_tiles, self.n_few, self.n_parts, self.n_rows, ws, ws.nbytes,
+                           _stream(stream))

@@ -134,6 +134,57 @@ int esp_plan_lowrank(const esp_lowrank_params* p, const int32_t* adapter, int32_
   }
 }
 
+int esp_plan_linear(const esp_linear_params* p, const esp_linear_seq* seqs, int32_t n_seqs, int32_t n_rows, int32_t workgroups, esp_linear_tile* tiles,
+                    int32_t tiles_cap, int32_t* n_tiles, int32_t* n_few, int32_t* n_parts, char* err, size_t errlen) {
+  if (!p || !n_tiles || !n_few || !n_parts || (n_seqs > 0 && !seqs)) return put_err(err, errlen, ESP_EINVAL, "NULL argument");
+  if (n_seqs < 0 || n_rows < 0 || workgroups <= 0 || tiles_cap < 0) return put_err(err, errlen, ESP_EINVAL, "counts / workgroups");
+  if (p->H <= 0 || p->n_states < 0 || !esp::linear_dims(p->dk, p->dv)) return put_err(err, errlen, ESP_EINVAL, "H / n_states / dk / dv");
+  try {
+    char msg[128];
+    std::vector<int32_t> owner(size_t(n_rows), -1), writer(size_t(p->n_states), -1);
+    for (int i = 0; i < n_seqs; ++i) {
+      const esp_linear_seq& q = seqs[i];
+      if (q.rows < 0 || q.base < 0 || int64_t(q.base) + q.rows > n_rows) {
+        snprintf(msg, sizeof msg, "sequence %d: rows [%d, %d + %d) outside the pass's %d rows", i, q.base, q.base, q.rows, n_rows);
+        return put_err(err, errlen, ESP_EINVAL, msg);
+      }
+      if (q.src < -1 || q.src >= p->n_states || q.dst < -1 || q.dst >= p->n_states) {
+        snprintf(msg, sizeof msg, "sequence %d: slots %d and %d of %d", i, q.src, q.dst, p->n_states);
+        return put_err(err, errlen, ESP_EINVAL, msg);
+      }
+      for (int r = q.base; r < q.base + q.rows; ++r) {
+        if (owner[size_t(r)] >= 0) {
+          snprintf(msg, sizeof msg, "row %d is in sequences %d and %d", r, owner[size_t(r)], i);
+          return put_err(err, errlen, ESP_EINVAL, msg);
+        }
+        owner[size_t(r)] = i;
+      }
+      if (q.dst >= 0) {
+        if (writer[size_t(q.dst)] >= 0) {
+          snprintf(msg, sizeof msg, "slot %d is left by sequences %d and %d", q.dst, writer[size_t(q.dst)], i);
+          return put_err(err, errlen, ESP_EINVAL, msg);
+        }
+        writer[size_t(q.dst)] = i;
+      }
+    }
+    for (int i = 0; i < n_seqs; ++i)
+      if (seqs[i].src >= 0 && writer[size_t(seqs[i].src)] >= 0 && writer[size_t(seqs[i].src)] != i) {
+        snprintf(msg, sizeof msg, "slot %d is read by sequence %d and left by sequence %d", seqs[i].src, i, writer[size_t(seqs[i].src)]);
+        return put_err(err, errlen, ESP_EINVAL, msg);
+      }
+    LinearPlan plan;
+    plan_linear(plan, *p, seqs, n_seqs, workgroups);
+    *n_tiles = int32_t(plan.tiles.size());
+    *n_few = plan.few;
+    *n_parts = plan.parts;
+    if (*n_tiles > tiles_cap || (!tiles && *n_tiles > 0)) return put_err(err, errlen, ESP_EWORKSPACE, "tiles capacity too small");
+    if (!plan.tiles.empty()) memcpy(tiles, plan.tiles.data(), plan.tiles.size() * sizeof(esp_linear_tile));
+    return ESP_OK;
+  } catch (const std::exception& e) {
+    return put_err(err, errlen, ESP_EINVAL, e.what());
+  }
+}
+
 esp_engine* esp_engine_create(int32_t n_blocks, int32_t bt, int32_t n_slots, int32_t max_ctx) {
   try {
     return new esp_engine(n_blocks, bt, n_slots, max_ctx);

@@ -30,6 +30,7 @@
 
 #include "../../include/espetero_attn.h"
 #include "../csrc/launch_shape.hpp"
+#include "../csrc/linear_shape.hpp"
 
 namespace espetero::engine {
 
@@ -699,6 +700,66 @@ inline int plan_lowrank(LowRankPlan& plan, const int32_t* adapter, int n_rows, i
     at = to;
   }
   return -1;
+}
+
+// Which tiles esp_linear_attn runs.
+struct LinearPlan {
+  std::vector<esp_linear_tile> tiles;  // sequences of few rows first
+  int few = 0, parts = 0;
+};
+
+// Sequences that esp_linear_attn's chunked kernel takes are cut into segments where a pass has fewer workgroups than the chip holds. A
+// segment's state is made by a launch in front, which reads K and V once more; what comes of that is worked out in chunks of
+// the kernel, for the segments of every length: the longest tile against an even share of all of them.
+inline void plan_linear(LinearPlan& plan, const esp_linear_params& p, const esp_linear_seq* seqs, int n_seqs, int workgroups) {
+  plan.tiles.clear();
+  plan.few = plan.parts = 0;
+  std::vector<int> many;
+  int longest = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    const esp_linear_seq& q = seqs[i];
+    if (q.rows > esp::kLinearFew) {
+      many.push_back(i);
+      longest = std::max(longest, (q.rows + esp::kLinearChunk - 1) / esp::kLinearChunk);
+    } else if (q.rows > 0 || q.src != q.dst) {
+      plan.tiles.push_back({q.rows > 0 ? q.base : 0, q.rows, q.src, q.dst, -1, 0, 0, 0});
+    }
+  }
+  plan.few = int(plan.tiles.size());
+  auto chunks = [&](int i) { return (seqs[i].rows + esp::kLinearChunk - 1) / esp::kLinearChunk; };
+  const double groups = double(p.H) * (p.dv / esp::linear_cols(p.dv)), slots = std::max(1, workgroups);
+  // Of a cut into segments of `most` chunks: a workgroup's set-up 1, a chunk 1, or half of one where only the state is made; a record read
+  // half a chunk, the launch in front 4.
+  auto cost = [&](int most) {
+    double all = 0, state = 0, top = 0, top_state = 0;
+    for (int i : many) {
+      const int c = chunks(i), n = (c + most - 1) / most, each = (c + n - 1) / n;
+      all += c + n + 0.25 * n * (n - 1);
+      top = std::max(top, each + 1 + 0.5 * (n - 1));
+      if (n > 1) {
+        state += 0.5 * (c - each) + (n - 1);
+        top_state = std::max(top_state, 0.5 * each + 1);
+      }
+    }
+    const double t = std::max(top, all * groups / slots);
+    return state == 0 ? t : t + std::max(top_state, state * groups / slots) + 4;
+  };
+  int most = std::max(1, longest);
+  double best = cost(most);
+  for (int n = 2; n <= 64 && (longest + n - 1) / n >= 2; ++n) {
+    const int m = (longest + n - 1) / n;
+    const double t = cost(m);
+    if (t < best) best = t, most = m;
+  }
+  for (int i : many) {
+    const esp_linear_seq& q = seqs[i];
+    const int c = chunks(i), n = (c + most - 1) / most, each = (c + n - 1) / n, real = (c + each - 1) / each;
+    for (int k = 0; k < real; ++k) {
+      const int r0 = k * each * esp::kLinearChunk, r1 = std::min(q.rows, (k + 1) * each * esp::kLinearChunk);
+      plan.tiles.push_back({q.base + r0, r1 - r0, q.src, k + 1 == real ? q.dst : -1, real > 1 ? plan.parts : -1, k, real - 1 - k, 0});
+    }
+    plan.parts += real > 1 ? real : 0;
+  }
 }
 
 }  // namespace espetero::engine

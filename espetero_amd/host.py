@@ -57,6 +57,7 @@ ENGINE_SYMBOLS = {
     "esp_engine_pass_pos": (C.c_int, (_V, _V)),
     "esp_engine_pass_table": (C.c_int, (_V, _V)),
     "esp_engine_pass_saves": (C.c_int, (_V, _V)),
+    "esp_plan_linear": (C.c_int, (C.POINTER(abi.LinearParams), _V, _I, _I, _I, _V, _I, _IP, _IP, _IP) + _ERR),
     "esp_engine_pass_cow": (C.c_int, (_V, _V)),
     "esp_engine_pass_rings": (C.c_int, (_V, _I, _I, _V, _V, _I, _IP, _V, _I, _IP) + _ERR),
     "esp_slot_file_save": (C.c_int, (C.c_char_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_uint64, _V)),
@@ -130,6 +131,24 @@ def plan_tiles(trees, groups, window, pos, options):
         n_tiles, n_jobs = max(n_tiles, nt.value), max(n_jobs, nj.value)
     abi.check(rc, err)
     return tiles[:nt.value].copy(), jobs[:nj.value].copy(), npart.value
+
+
+def plan_linear(params, seqs, n_rows, workgroups):
+    """seqs: LINEAR_SEQ_DT array. Returns (tiles LINEAR_TILE_DT, tiles of sequences of few rows at their front, parts)."""
+    lib = engine_lib()
+    seqs = np.ascontiguousarray(seqs, dtype=abi.LINEAR_SEQ_DT)
+    err = C.create_string_buffer(256)
+    nt, nf, np_ = C.c_int32(0), C.c_int32(0), C.c_int32(0)
+    room = len(seqs) + 64
+    while True:
+        tiles = np.empty(room, abi.LINEAR_TILE_DT)
+        rc = lib.esp_plan_linear(C.byref(params), seqs.ctypes.data, len(seqs), n_rows, workgroups, tiles.ctypes.data, room, C.byref(nt), C.byref(nf),
+                                 C.byref(np_), err, 256)
+        if rc != abi.ESP_EWORKSPACE or nt.value <= room:
+            break
+        room = nt.value
+    abi.check(rc, err)
+    return tiles[:nt.value].copy(), nf.value, np_.value
 
 
 def plan_lowrank(params, adapter):

@@ -506,6 +506,60 @@ int esp_history_record(const esp_logits_params* p, uint32_t* seen, int32_t* coun
 int esp_history_clear(const esp_logits_params* p, uint32_t* seen, int32_t* counts, const int32_t* slots, int32_t n, void* stream, char* err,
                       size_t errlen);
 
+/* ---- linear attention with a decay for each head ------------------------------------
+ * No counterpart among the reference's paged attention. A layer that keeps a state in place of a cache: per head h, of dk x dv numbers,
+ *   S_t = exp(d) S_{t-1} + k_t^T v_t        O_t = scale q_t S_t
+ * over the rows t of a sequence, with the log decay d of the head, or of the row and head. H heads of values, outputs and
+ * states; Hk of queries and keys, of which head h takes h / (H / Hk). States live in slots, fp32 [n_states][H][dk][dv]; a sequence goes on
+ * from one slot's state (or from zeros) and leaves its own in another, the same one, or nowhere. Chunks of a prompt, drafts whose states are
+ * kept apart until they are accepted, and forks are sequences like any. States and sums are held in fp32 (how the kernel's products keep
+ * that, and what they scale with fp16 operands, is at the kernel); O is rounded once. Log decays above 0 count as 0, below -138 as
+ * a factor of 0. An infinite or NaN value shows in its own row and the ones behind it only. */
+typedef struct esp_linear_params {
+  int32_t H;        /* heads of V, O and the states */
+  int32_t Hk;       /* heads of Q and K; H % Hk == 0 */
+  int32_t dk;       /* dims of a query or key head: 64 or 128 */
+  int32_t dv;       /* dims of a value head: a multiple of 64, at most 512 */
+  int32_t dtype;    /* ESP_F16 | ESP_BF16: Q, K, V and O */
+  int32_t q_ld, k_ld, v_ld, o_ld; /* row strides, elements, multiples of 8 */
+  int32_t decay_ld; /* 0: decay [H], one for every row; else decay [n_rows][decay_ld] */
+  int32_t n_states; /* slots */
+  float scale;      /* multiplies q */
+} esp_linear_params;
+
+/* Rows [base, base + rows) of a pass, in order: they go on from the state in slot src (-1: zeros) and leave theirs in slot dst (-1:
+ * nowhere). Without rows the state of src is copied, or dst cleared. */
+typedef struct esp_linear_seq {
+  int32_t base, rows, src, dst;
+} esp_linear_seq;
+
+/* A sequence, or a segment of one, as esp_plan_linear (include/espetero_engine.h) makes them. */
+typedef struct esp_linear_tile {
+  int32_t row0, rows;
+  int32_t src;    /* the sequence's first state, wherever the segment lies */
+  int32_t dst;    /* where the state behind it goes: the last segment's, else -1 */
+  int32_t part;   /* first of the workspace's records of its sequence, one a segment; -1: a sequence in one piece */
+  int32_t before; /* segments of the sequence in front of it */
+  int32_t after;  /* and behind it */
+  int32_t pad;
+} esp_linear_tile;
+
+/* Workgroups of a sequence in one piece that the device holds at once: what esp_plan_linear cuts a pass up to. */
+int esp_linear_hint(const esp_linear_params* p, int device, int32_t* workgroups, char* err, size_t errlen);
+/* Never less for more parts. Host-only arithmetic. */
+size_t esp_linear_workspace_bytes(const esp_linear_params* p, int32_t n_parts);
+/* Q [n_rows][q_ld], K [n_rows][k_ld], V [n_rows][v_ld], O [n_rows][o_ld], 16-byte aligned like the workspace and the states; head h of V
+ * and O at column h * dv, head i of Q and K at i * dk. tiles: device copies of esp_plan_linear's, n_few of them in front for the kernel that
+ * takes sequences of few rows. Rows in no tile and slots that are no tile's dst are left as they are. O must not overlap Q, K or V. */
+int esp_linear_attn(const esp_linear_params* p, const void* Q, const void* K, const void* V, const float* decay, float* states, void* O,
+                    const esp_linear_tile* tiles, int32_t n_tiles, int32_t n_few, int32_t n_parts, int32_t n_rows, void* workspace,
+                    size_t workspace_bytes, void* stream, char* err, size_t errlen);
+/* Host-side check of a pass's records before they are uploaded (host pointers): rows inside the pass and in one tile each, slots inside
+ * the states, no slot that one sequence leaves its state in read or written by another, segments of a sequence in order, each with records
+ * of its own. Without it such records are read as they are. */
+int esp_linear_validate(const esp_linear_params* p, const esp_linear_tile* tiles, int32_t n_tiles, int32_t n_few, int32_t n_parts, int32_t n_rows,
+                        char* err, size_t errlen);
+
 #ifdef __cplusplus
 }
 #endif

@@ -82,6 +82,13 @@ int esp_plan_tiles_diff(const esp_attn_params* p, const esp_tree* trees, int32_t
 int esp_plan_lowrank(const esp_lowrank_params* p, const int32_t* adapter, int32_t n_rows, int32_t* order, int32_t* n_slots, esp_lowrank_tile* tiles,
                      int32_t tiles_cap, int32_t* n_tiles, char* err, size_t errlen);
 
+/* The tiles of a pass of esp_linear_attn: sequences of few rows first (n_few of them, those without rows among them), then the others,
+ * cut into segments of whole chunks of rows where the pass has fewer workgroups than `workgroups` (esp_linear_hint's). ESP_EINVAL for a
+ * sequence with rows outside the pass or in another sequence, slots outside the states, or a slot that another sequence leaves its state
+ * in. On ESP_EWORKSPACE (tiles' capacity too small) the counts are still written. */
+int esp_plan_linear(const esp_linear_params* p, const esp_linear_seq* seqs, int32_t n_seqs, int32_t n_rows, int32_t workgroups, esp_linear_tile* tiles,
+                    int32_t tiles_cap, int32_t* n_tiles, int32_t* n_few, int32_t* n_parts, char* err, size_t errlen);
+
 /* ---- KV engine: pool + slots + pass builder ---- */
 typedef struct esp_engine esp_engine;
 
