@@ -13,7 +13,7 @@ ESP_F16, ESP_BF16, ESP_F32 = 0, 1, 2
 ESP_EWORKSPACE = 4
 ESP_LAYOUT_REFERENCE, ESP_LAYOUT_NATIVE = 0, 1
 ESP_ABI_VERSION = 3
-ESP_PASS_FUSED, ESP_PASS_ROWS_IN_POOL, ESP_PASS_DIFF = 1, 2, 4
+ESP_PASS_FUSED, ESP_PASS_ROWS_IN_POOL, ESP_PASS_DIFF, ESP_PASS_SHAPED = 1, 2, 4, 8
 ESP_LOWRANK_SLICES = 4
 ESP_STATIC_SCRATCH_BYTES = 32 << 20
 
@@ -75,6 +75,10 @@ class LogitsParams(C.Structure):
                 ("n_masks", C.c_int32), ("n_bias", C.c_int32), ("pad", C.c_int32)]
 
 
+class ShapeParams(C.Structure):
+    _fields_ = [("slopes", C.c_void_p), ("spans", C.c_void_p), ("cap", C.c_float), ("pad", C.c_int32)]
+
+
 class LinearParams(C.Structure):
     _fields_ = [("H", C.c_int32), ("Hk", C.c_int32), ("dk", C.c_int32), ("dv", C.c_int32), ("dtype", C.c_int32), ("q_ld", C.c_int32),
                 ("k_ld", C.c_int32), ("v_ld", C.c_int32), ("o_ld", C.c_int32), ("decay_ld", C.c_int32), ("n_states", C.c_int32),
@@ -104,6 +108,7 @@ assert C.sizeof(DiffParams) == 24
 assert C.sizeof(LowRankParams) == 64
 assert C.sizeof(LogitsParams) == 32
 assert LOWRANK_TILE_DT.itemsize == 16 and LOGITS_ROW_DT.itemsize == 32
+assert C.sizeof(ShapeParams) == 24
 assert C.sizeof(LinearParams) == 48 and LINEAR_SEQ_DT.itemsize == 16 and LINEAR_TILE_DT.itemsize == 32
 
 # name -> (restype, argtypes); every symbol the header declares.
@@ -149,6 +154,11 @@ ATTN_SYMBOLS = {
     "esp_logits_validate": (C.c_int, (C.POINTER(LogitsParams), _V, C.c_int32, _V) + _ERR),
     "esp_history_record": (C.c_int, (C.POINTER(LogitsParams), _V, _V, _V, _V, C.c_int32, C.c_int32, _V) + _ERR),
     "esp_history_clear": (C.c_int, (C.POINTER(LogitsParams), _V, _V, _V, C.c_int32, _V) + _ERR),
+    "esp_attn_shaped_rows": (C.c_int32, (_P, C.c_int32)),
+    "esp_attn_shaped_hint": (C.c_int, (_P, C.c_int, C.POINTER(C.c_int32), C.POINTER(C.c_int32)) + _ERR),
+    "esp_attn_shaped_workspace_bytes": (C.c_size_t, (_P, C.c_int32)),
+    "esp_attn_shaped": (C.c_int, (_P, C.POINTER(ShapeParams), _V, _V, _V, _V, _V, C.c_int32, _V, C.c_int32, _V, C.c_int32, C.c_int32, C.c_int32,
+                                  _V, C.c_size_t, _V) + _ERR),
     "esp_linear_hint": (C.c_int, (C.POINTER(LinearParams), C.c_int, C.POINTER(C.c_int32)) + _ERR),
     "esp_linear_workspace_bytes": (C.c_size_t, (C.POINTER(LinearParams), C.c_int32)),
     "esp_linear_attn": (C.c_int, (C.POINTER(LinearParams), _V, _V, _V, _V, _V, _V, _V, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _V, C.c_size_t,
@@ -164,13 +174,13 @@ class EspError(RuntimeError):
 
 class PlanGroups(int):
     """Workgroups per tile, as plan_hint reports them: a plain count, which also knows the layer it was asked for, so that the
-    planner needs no argument of its own for that. A count worked out otherwise is planned for any layer. diff: as
-    attn_diff_hint reports them."""
+    planner needs no argument of its own for that. A count worked out otherwise is planned for any layer. diff, shaped: as
+    attn_diff_hint and attn_shaped_hint report them."""
 
-    def __new__(cls, value, params=None, diff=False):
+    def __new__(cls, value, params=None, diff=False, shaped=False):
         g = super().__new__(cls, value)
         layer = None if params is None else (params.H, params.Hkv, params.head_dim)
-        g.layer, g.diff = (None, layer) if diff else (layer, None)
+        g.layer, g.diff, g.shaped = (None if diff or shaped else layer), (layer if diff else None), (layer if shaped else None)
         return g
 
 

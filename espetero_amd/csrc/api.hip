@@ -15,6 +15,7 @@
 #include "linear_shape.hpp"
 #include "logits_shape.hpp"
 #include "lowrank_shape.hpp"
+#include "shaped_math.hpp"
 
 namespace esp {
 hipError_t launch_stream(int dt, int HD, int NC, const KArgs& a, const PrepArgs* pa, int n_tiles, hipStream_t st);
@@ -44,6 +45,11 @@ hipError_t launch_diff_tiled(int dt, const DiffArgs& a, int n_tiles, hipStream_t
 hipError_t launch_diff_merge(int dt, const DiffArgs& a, const esp_combine* jobs, int n_jobs, int n_parts, hipStream_t st);
 hipError_t diff_init_attributes();
 hipError_t diff_tiled_init_attributes();
+hipError_t launch_shaped_stream(int dt, int HD, const ShapedArgs& a, int n_tiles, hipStream_t st);
+hipError_t launch_shaped_tiled(int dt, int HD, const ShapedArgs& a, int n_tiles, hipStream_t st);
+hipError_t launch_shaped_merge(int dt, int HD, const ShapedArgs& a, const esp_combine* jobs, int n_jobs, int n_parts, hipStream_t st);
+hipError_t shaped_init_attributes();
+hipError_t shaped_tiled_init_attributes();
 hipError_t launch_linear(int dt, const LinearArgs& a, int n_few, int n_chunked, bool split, hipStream_t st);
 hipError_t linear_init_attributes();
 hipError_t launch_lowrank(int dt, const LowRankArgs& a, int rows_per_tile, int n_tiles, hipStream_t st);
@@ -106,6 +112,16 @@ int check_diff(const esp_attn_params* p, char* err, size_t errlen) {
   if (p->H % 2 || p->Hkv % 2) return fail(err, errlen, ESP_EINVAL, "H=%d Hkv=%d: heads work in pairs", p->H, p->Hkv);
   if (p->gate || p->bidi) return fail(err, errlen, ESP_EUNSUPPORTED, "differential attention takes neither a gate nor bidirectional rows");
   if (!(p->scale > 0.0f)) return fail(err, errlen, ESP_EINVAL, "scale must be positive");
+  return ESP_OK;
+}
+
+// What attention with shaped scores asks of a layer's parameters beyond check_params.
+int check_shaped(const esp_attn_params* p, char* err, size_t errlen) {
+  if (int rc = check_params(p, err, errlen)) return rc;
+  if (p->head_dim != 128 && p->head_dim != 256) return fail(err, errlen, ESP_EUNSUPPORTED, "head_dim %d: attention with shaped scores serves 128 and 256", p->head_dim);
+  if (p->H / p->Hkv > 128) return fail(err, errlen, ESP_EUNSUPPORTED, "%d query heads to a KV head (at most 128)", p->H / p->Hkv);
+  if (p->gate || p->bidi) return fail(err, errlen, ESP_EUNSUPPORTED, "attention with shaped scores takes neither a gate nor bidirectional rows");
+  if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return fail(err, errlen, ESP_EINVAL, "scale must be positive and finite");
   return ESP_OK;
 }
 
@@ -175,6 +191,8 @@ int device_state(DeviceState** out, char* err, size_t errlen) {
     if ((e = esp::gate_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (head gate)", e);
     if ((e = esp::diff_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (differential attention)", e);
     if ((e = esp::diff_tiled_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (tiled differential attention)", e);
+    if ((e = esp::shaped_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (attention with shaped scores)", e);
+    if ((e = esp::shaped_tiled_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (tiled attention with shaped scores)", e);
     if ((e = esp::linear_init_attributes()) != hipSuccess) return hip_fail(err, errlen, "hipFuncSetAttribute (linear attention)", e);
     d.scratch = static_cast<unsigned char*>(ps);
     d.ready = true;
@@ -416,12 +434,20 @@ int esp_attn_validate_for(const esp_attn_params* p, int32_t mode, const esp_tile
   if (int rc = esp_attn_validate(p, tiles, n_tiles, trees, n_trees, jobs, n_jobs, n_parts, n_rows, blocks, n_block_entries, pool_blocks,
                                  err, errlen))
     return rc;
-  if (mode & ~(ESP_PASS_FUSED | ESP_PASS_ROWS_IN_POOL | ESP_PASS_DIFF)) return fail(err, errlen, ESP_EINVAL, "mode %d", mode);
+  if (mode & ~(ESP_PASS_FUSED | ESP_PASS_ROWS_IN_POOL | ESP_PASS_DIFF | ESP_PASS_SHAPED)) return fail(err, errlen, ESP_EINVAL, "mode %d", mode);
   if (mode & ESP_PASS_DIFF) {
     if (mode != ESP_PASS_DIFF) return fail(err, errlen, ESP_EINVAL, "mode %d: a pass of differential attention has no other form", mode);
     if (int rc = check_diff(p, err, errlen)) return rc;
     if (!esp::diff_family(p->rows_per_tile, p->H / p->Hkv))
       return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_attn_diff_rows)", p->rows_per_tile);
+  }
+  if (mode & ESP_PASS_SHAPED) {
+    if (mode != ESP_PASS_SHAPED) return fail(err, errlen, ESP_EINVAL, "mode %d: a pass of attention with shaped scores has no other form", mode);
+    if (int rc = check_shaped(p, err, errlen)) return rc;
+    if (!esp::shaped_family(p->head_dim, p->rows_per_tile, p->H / p->Hkv))
+      return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_attn_shaped_rows)", p->rows_per_tile);
+  }
+  if (mode & (ESP_PASS_DIFF | ESP_PASS_SHAPED)) {
     for (int i = 0; i < n_tiles; ++i) {
       const esp_tile& t = tiles[i];
       const int32_t P = trees[t.tree].P, k1 = std::min(t.k1, P);
@@ -444,7 +470,7 @@ int esp_attn_validate_for(const esp_attn_params* p, int32_t mode, const esp_tile
         return fail(err, errlen, ESP_EINVAL, "tile %d: first row %d is not its tree's first row %d (a fused pass has one tile group per tree)", i,
                     tiles[i].r0, trees[tiles[i].tree].base);
   }
-  if (mode & (ESP_PASS_ROWS_IN_POOL | ESP_PASS_DIFF)) {
+  if (mode & (ESP_PASS_ROWS_IN_POOL | ESP_PASS_DIFF | ESP_PASS_SHAPED)) {
     // Row j of a tree is read at position P + j of the tree's own block list (or ring).
     const int64_t bt = p->bt;
     for (int i = 0; i < n_trees; ++i) {
@@ -754,6 +780,86 @@ int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void
   if (n_jobs > 0) {
     e = esp::launch_diff_merge(p->dtype, a, jobs, n_jobs, n_parts, st);
     if (e != hipSuccess) return hip_fail(err, errlen, "attn_diff_merge launch", e);
+  }
+  return ESP_OK;
+}
+
+// ---- attention with shaped scores ------------------------------------------------
+int32_t esp_attn_shaped_rows(const esp_attn_params* p, int32_t rows) {
+  if (check_shaped(p, nullptr, 0) != ESP_OK || rows <= 0) return 0;
+  return esp::shaped_rows(rows, p->H / p->Hkv);
+}
+
+int esp_attn_shaped_hint(const esp_attn_params* p, int device, int32_t* workgroups, int32_t* groups_per_tile, char* err, size_t errlen) {
+  if (int rc = check_shaped(p, err, errlen)) return rc;
+  const int fam = esp::shaped_family(p->head_dim, p->rows_per_tile, p->H / p->Hkv);
+  if (!workgroups || !groups_per_tile) return fail(err, errlen, ESP_EINVAL, "NULL output");
+  if (!fam) return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_attn_shaped_rows)", p->rows_per_tile);
+  int cus = 0;
+  const hipError_t e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device);
+  if (e != hipSuccess) return hip_fail(err, errlen, "hipDeviceGetAttribute", e);
+  *workgroups = cus * esp::shaped_workgroups_per_cu(p->head_dim, fam);
+  *groups_per_tile = p->Hkv;
+  return ESP_OK;
+}
+
+size_t esp_attn_shaped_workspace_bytes(const esp_attn_params* p, int32_t n_parts) {
+  if (!p || p->Hkv <= 0 || p->H <= 0 || p->head_dim <= 0 || p->rows_per_tile <= 0) return 0;
+  return esp::carve_shaped(p->H, p->head_dim, p->rows_per_tile, n_parts).total;
+}
+
+int esp_attn_shaped(const esp_attn_params* p, const esp_shape_params* shape, const void* Q, const void* kv_pool, const int32_t* blocks, void* O,
+                    const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees, int32_t n_trees, const esp_combine* jobs, int32_t n_jobs,
+                    int32_t n_parts, int32_t n_rows, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen) {
+  if (int rc = check_shaped(p, err, errlen)) return rc;
+  if (!shape) return fail(err, errlen, ESP_EINVAL, "shape is NULL");
+  if (!(shape->cap >= 0.0f) || !std::isfinite(shape->cap)) return fail(err, errlen, ESP_EINVAL, "cap must be 0 or positive, and finite");
+  if (n_tiles < 0 || n_trees < 0 || n_jobs < 0 || n_parts < 0 || n_rows < 0) return fail(err, errlen, ESP_EINVAL, "negative count");
+  if (n_tiles == 0) return ESP_OK;
+  if (!Q || !O || !tiles || !trees || !kv_pool) return fail(err, errlen, ESP_EINVAL, "Q, O, tiles, trees, kv_pool must not be NULL");
+  if (n_trees == 0 || n_rows == 0) return fail(err, errlen, ESP_EINVAL, "%d tiles without trees or rows", n_tiles);
+  if (!p->ring && !blocks) return fail(err, errlen, ESP_EINVAL, "blocks is NULL on a layer without rings");
+  if (n_jobs > 0 && !jobs) return fail(err, errlen, ESP_EINVAL, "jobs is NULL");
+  if ((n_jobs > 0) != (n_parts > 0)) return fail(err, errlen, ESP_EINVAL, "%d merge jobs with %d partial records", n_jobs, n_parts);
+  const int fam = esp::shaped_family(p->head_dim, p->rows_per_tile, p->H / p->Hkv);
+  if (!fam) return fail(err, errlen, ESP_EUNSUPPORTED, "rows_per_tile %d (see esp_attn_shaped_rows)", p->rows_per_tile);
+  if (n_tiles > 65535 || n_jobs > 65535) return fail(err, errlen, ESP_EUNSUPPORTED, "%d tiles, %d jobs in one pass: at most 65535", n_tiles, n_jobs);
+  const esp::DiffCarve c = esp::carve_shaped(p->H, p->head_dim, p->rows_per_tile, n_parts);
+  if (n_parts > 0 && (!workspace || workspace_bytes < c.total))
+    return fail(err, errlen, ESP_EWORKSPACE, "workspace %zu bytes, %zu needed", workspace ? workspace_bytes : size_t(0), c.total);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(err, errlen, ESP_EINVAL, "workspace must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(shape->spans) % 8) return fail(err, errlen, ESP_EINVAL, "spans must be 8-byte aligned");
+  DeviceState* dev = nullptr;
+  if (int rc = device_state(&dev, err, errlen)) return rc;
+  esp::ShapedArgs a{};
+  a.Q = static_cast<const uint16_t*>(Q);
+  a.pool = static_cast<const uint16_t*>(kv_pool);
+  a.blocks = blocks;
+  a.O = static_cast<uint16_t*>(O);
+  a.tiles = tiles;
+  a.trees = trees;
+  a.parts_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + c.parts_o);
+  a.parts_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + c.parts_ml);
+  a.slopes = shape->slopes;
+  a.spans = reinterpret_cast<const int2*>(shape->spans);
+  a.H = p->H;
+  a.Hkv = p->Hkv;
+  a.G = p->H / p->Hkv;
+  a.q_ld = p->q_ld;
+  a.bt = p->bt;
+  a.window = p->window;
+  a.ring = p->ring;
+  a.R = p->rows_per_tile;
+  a.cols = a.R * a.G;
+  a.scale_log2 = shape->cap > 0.0f ? float(2.0 * double(p->scale) * 1.4426950408889634 / double(shape->cap)) : p->scale * esp::kLog2e;
+  a.cap_log2 = shape->cap * esp::kLog2e;
+  a.kv_base = p->kv_base;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e = fam > 0 ? esp::launch_shaped_stream(p->dtype, p->head_dim, a, n_tiles, st) : esp::launch_shaped_tiled(p->dtype, p->head_dim, a, n_tiles, st);
+  if (e != hipSuccess) return hip_fail(err, errlen, "attn_shaped launch", e);
+  if (n_jobs > 0) {
+    e = esp::launch_shaped_merge(p->dtype, p->head_dim, a, jobs, n_jobs, n_parts, st);
+    if (e != hipSuccess) return hip_fail(err, errlen, "attn_shaped_merge launch", e);
   }
   return ESP_OK;
 }

@@ -75,4 +75,24 @@ constexpr DiffCarve carve_diff(int H, int rows_per_tile, int64_t n_parts) {
   return c;
 }
 
+// Attention with shaped scores: 1 or 2, the streaming kernel with that many column tiles; -1, the tiled one, up to 128 packed rows; 0, no
+// kernel.
+constexpr int shaped_family(int head_dim, int rows_per_tile, int G) {
+  if (rows_per_tile <= 0 || G <= 0 || rows_per_tile > 128 / G) return 0;
+  const int nc = (rows_per_tile * G + 15) / 16;
+  return nc == 1 || (nc == 2 && head_dim == 128) ? nc : -1;
+}
+constexpr int shaped_rows(int rows, int G) { return rows < 128 / G ? rows : 128 / G; }
+constexpr int shaped_workgroups_per_cu(int head_dim, int family) { return family > 0 ? stream_occ(head_dim, family) : tiled_occ(head_dim); }
+
+// Its partial records.
+constexpr DiffCarve carve_shaped(int H, int head_dim, int rows_per_tile, int64_t n_parts) {
+  const size_t recs = size_t(n_parts > 0 ? n_parts : 0) * size_t(H) * size_t(rows_per_tile);
+  DiffCarve c{};
+  c.parts_o = 0;
+  c.parts_ml = (recs * size_t(head_dim) * sizeof(float) + 255) & ~size_t(255);
+  c.total = c.parts_ml + recs * 2 * sizeof(float);
+  return c;
+}
+
 }  // namespace esp

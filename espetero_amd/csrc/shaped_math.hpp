@@ -1,0 +1,75 @@
+// What the kernels of attention with shaped scores share: their argument block, what a row sees, how a product becomes a score, and
+// which keys a tile scans.
+#pragma once
+
+#include "common.hpp"
+#include "diff_math.hpp"
+
+namespace esp {
+
+// Everything a kernel of attention with shaped scores reads, passed by value.
+struct ShapedArgs {
+  const uint16_t* Q;
+  const uint16_t* pool;
+  const int32_t* blocks;
+  uint16_t* O;
+  const esp_tile* tiles;
+  const esp_tree* trees;
+  float* parts_o;   // [part][Hkv][cols][head_dim]  unnormalised
+  float* parts_ml;  // [part][Hkv][cols][2]         running max (log2 units), sum
+  const float* slopes;  // [H], or null
+  const int2* spans;    // [n_rows] (first key, end of what is seen whichever way round), or null
+  int32_t H, Hkv, G, q_ld, bt, window, ring, R, cols;
+  float scale_log2;  // without a cap: scale in log2 units; with one: 2 scale log2(e) / cap
+  float cap_log2;    // cap in log2 units
+  uint64_t kv_base;
+};
+
+__device__ __forceinline__ int shaped_block(const ShapedArgs& a, int table, int bi) {
+  using const_i32 = const int32_t __attribute__((address_space(4)));  // read only: scalar loads
+  return a.ring ? table + bi % a.ring : ((const_i32*)a.blocks)[table + bi];
+}
+
+// The keys [from, end) that a row at position q sees of a tree with n_keys.
+struct Sight {
+  int from, end;
+};
+__device__ __forceinline__ Sight shaped_sight(const ShapedArgs& a, int row, int q, int n_keys) {
+  Sight s{0, q + 1};
+  if (a.spans) {
+    const int2 span = a.spans[row];
+    s.end = min(max(q + 1, span.y), n_keys);
+    s.from = min(max(span.x, 0), s.end);  // (a row that sees nothing: no number that later sums could carry past 32 bits)
+  }
+  if (a.window > 0) s.from = max(s.from, q - a.window + 1);
+  return s;
+}
+
+// x = scale q.k through the cap, in log2 units: cap tanh(x / cap) = cap (1 - 2 / (exp(2 x / cap) + 1)), which holds for infinite x too.
+template <bool CAP>
+__device__ __forceinline__ float shaped_score(const ShapedArgs& a, float dot) {
+  if constexpr (CAP) {
+    return a.cap_log2 - 2.0f * a.cap_log2 * __builtin_amdgcn_rcpf(fast_exp2(dot * a.scale_log2) + 1.0f);
+  } else {
+    return dot * a.scale_log2;
+  }
+}
+
+// The keys a tile scans, [lo, hi) in cache positions, of those that its rows see at all, [from, end): its cached range and, on a `last` tile,
+// the rows of the pass behind it, which lie in the pool at positions P + row - up to `end` where the tile's range of them is open. Both at once
+// only where they meet.
+__device__ __forceinline__ Sight shaped_range(const esp_tile& t, const esp_tree& tr, int from, int end) {
+  const int k1 = min(t.k1, tr.P);  // INT32_MAX: up to the tree's cached length as it is now
+  Sight d{t.k0, k1};
+  if (t.last) {
+    if (k1 <= t.k0) d.from = tr.P + t.b0;
+    d.end = t.last >= 2 ? tr.P + t.last - 1 : INT32_MAX;
+  }
+  d.from = max(d.from, from);
+  d.end = max(min(d.end, end), d.from);
+  return d;
+}
+
+__device__ __forceinline__ float shaped_inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }  // 0: a row that has seen no key; NaN stays
+
+}  // namespace esp

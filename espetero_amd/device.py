@@ -77,18 +77,19 @@ def forward_static(params, Q, Kb, Vb, pool, blocks, desc, pos, O, tiles, n_tiles
                                _stream(stream))
 
 
-def validate(params, tiles, trees, jobs, n_parts, n_rows, blocks, pool_blocks, fused=False, rows_in_pool=False, diff=False):
+def validate(params, tiles, trees, jobs, n_parts, n_rows, blocks, pool_blocks, fused=False, rows_in_pool=False, diff=False, shaped=False):
     """Host-side bounds check of a pass's records (numpy arrays) before they are uploaded. Raises EspError.
     fused: the pass goes to esp_attn_decode_fused (also: one tile group per tree, trees of at most rows_per_tile rows).
     rows_in_pool: the pass runs without Kb / Vb (also: block lists that reach P + M, P - base a multiple of 16 on the tiled kernel).
-    diff: the pass goes to esp_attn_diff (also: block lists that reach P + M)."""
+    diff, shaped: the pass goes to esp_attn_diff, or esp_attn_shaped (also: block lists that reach P + M)."""
     tiles = np.ascontiguousarray(tiles, dtype=abi.TILE_DT)
     trees = np.ascontiguousarray(trees, dtype=abi.TREE_DT)
     jobs = np.ascontiguousarray(jobs, dtype=abi.COMBINE_DT)
     blocks = None if blocks is None else np.ascontiguousarray(blocks, dtype=np.int32)
     hp = lambda a: None if a is None or a.size == 0 else a.ctypes.data  # noqa: E731
     err = C.create_string_buffer(_ERRLEN)
-    mode = (abi.ESP_PASS_FUSED if fused else 0) | (abi.ESP_PASS_ROWS_IN_POOL if rows_in_pool else 0) | (abi.ESP_PASS_DIFF if diff else 0)
+    mode = (abi.ESP_PASS_FUSED if fused else 0) | (abi.ESP_PASS_ROWS_IN_POOL if rows_in_pool else 0) | (abi.ESP_PASS_DIFF if diff else 0) | \
+        (abi.ESP_PASS_SHAPED if shaped else 0)
     rc = abi.attn_lib().esp_attn_validate_for(C.byref(params), mode, hp(tiles), len(tiles), hp(trees), len(trees), hp(jobs), len(jobs),
                                               n_parts, n_rows, hp(blocks), 0 if blocks is None else len(blocks), pool_blocks, err, _ERRLEN)
     abi.check(rc, err)
@@ -244,6 +245,62 @@ class DiffPass:
         ws = self.workspace
         _calls.attn_diff(self.params, self.diff, Q, pool, self.blocks, O, self.tiles, self.n_tiles, self.trees, self.n_trees, self.jobs, self.n_jobs,
                          self.n_parts, self.n_rows, ws, ws.nbytes, _stream(stream))
+
+
+def shape_params(cap=0.0, slopes=None):
+    """slopes fp32 [H] or None: a device tensor, kept alive by the record."""
+    s = abi.ShapeParams(_ptr(slopes), None, cap, 0)
+    s._keep = slopes
+    return s
+
+
+def attn_shaped_rows(params, rows):
+    """rows_per_tile to plan a pass of attention with shaped scores with whose trees have at most `rows` rows."""
+    r = abi.attn_lib().esp_attn_shaped_rows(C.byref(params), rows)
+    if r <= 0:
+        raise abi.EspError("parameters or rows that esp_attn_shaped does not serve")
+    return r
+
+
+def attn_shaped_hint(params, device=0):
+    """(workgroups resident at once, workgroups per tile) of the kernel of attention with shaped scores serving `params`."""
+    err = C.create_string_buffer(_ERRLEN)
+    n, g = C.c_int32(0), C.c_int32(0)
+    abi.check(abi.attn_lib().esp_attn_shaped_hint(C.byref(params), device, C.byref(n), C.byref(g), err, _ERRLEN), err)
+    return n.value, abi.PlanGroups(g.value, params, shaped=True)
+
+
+class ShapedPass:
+    """One planned pass of attention with shaped scores resident on the device (the rows of the pass are in the pool when it runs)."""
+
+    def __init__(self, params, shape, trees, tiles, jobs, n_parts, n_rows, blocks, spans=None, device="cuda", pool_blocks=None):
+        """spans: int32 [n_rows][2], what each row sees (first key of its document, end of what is seen whichever way round), or None. The pass
+        keeps copies of the records, with the spans that it was given. pool_blocks: blocks in the pool; when given, the records
+        are checked on the host before the upload."""
+        if pool_blocks is not None:
+            validate(params, tiles, trees, jobs, n_parts, n_rows, blocks, pool_blocks, shaped=True)
+        self.params, self.shape = abi.AttnParams.from_buffer_copy(params), abi.ShapeParams.from_buffer_copy(shape)
+        self._keep = getattr(shape, "_keep", None)
+        self.spans = None
+        if spans is not None:
+            spans = np.ascontiguousarray(spans, dtype=np.int32)
+            if spans.shape != (n_rows, 2):
+                raise abi.EspError(f"spans of shape {spans.shape}, {n_rows} rows of 2 expected")
+            self.spans = to_dev(spans, device)
+        self.shape.spans = _ptr(self.spans)
+        self.n_trees, self.n_tiles, self.n_jobs = len(trees), len(tiles), len(jobs)
+        self.n_parts, self.n_rows = n_parts, n_rows
+        self.trees = to_dev(np.ascontiguousarray(trees, dtype=abi.TREE_DT), device)
+        self.tiles = to_dev(np.ascontiguousarray(tiles, dtype=abi.TILE_DT), device)
+        self.jobs = to_dev(np.ascontiguousarray(jobs, dtype=abi.COMBINE_DT), device) if len(jobs) else None
+        self.blocks = to_dev(np.ascontiguousarray(blocks, dtype=np.int32), device) if blocks is not None else None
+        nbytes = abi.attn_lib().esp_attn_shaped_workspace_bytes(C.byref(self.params), n_parts)
+        self.workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+    def run(self, Q, pool, O, stream=None):
+        ws = self.workspace
+        _calls.attn_shaped(self.params, self.shape, Q, pool, self.blocks, O, self.tiles, self.n_tiles, self.trees, self.n_trees, self.jobs, self.n_jobs,
+                           self.n_parts, self.n_rows, ws, ws.nbytes, _stream(stream))
 
 
 def lowrank_params(D, rank, slices, dtype, x_ld, y_ld, n_adapters):

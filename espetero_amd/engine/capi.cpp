@@ -71,7 +71,8 @@ int esp_plan_tiles(const esp_tree* trees, int32_t n_trees, int32_t groups, int32
   return esp_plan_tiles_for(nullptr, trees, n_trees, groups, window, pos, o, tiles, tiles_cap, n_tiles, jobs, jobs_cap, n_jobs, n_parts, err, errlen);
 }
 
-static int plan_pass(const esp_attn_params* p, bool diff, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
+enum class Pass { plain, diff, shaped };
+static int plan_pass(const esp_attn_params* p, Pass kind, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
                      const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                      int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen) {
   if (!o || (n_trees > 0 && !trees) || !n_tiles || !n_jobs || !n_parts) return put_err(err, errlen, ESP_EINVAL, "NULL argument");
@@ -83,8 +84,11 @@ static int plan_pass(const esp_attn_params* p, bool diff, const esp_tree* trees,
   try {
     AttnPlan A;
     A.trees.assign(trees, trees + n_trees);
-    const bool tiled = diff && esp::diff_family(o->rows_per_tile, p->H / p->Hkv) < 0;
-    plan_tiles(A, groups, window, pos, tiled ? to_cpp(*o).for_diff_tiled() : to_cpp(*o), diff ? nullptr : p);
+    // The tiled kernels of differential attention and of shaped scores are planned for as such, shaped scores' streaming kernel as the one it is like.
+    const int family = kind == Pass::diff     ? esp::diff_family(o->rows_per_tile, p->H / p->Hkv)
+                       : kind == Pass::shaped ? esp::shaped_family(p->head_dim, o->rows_per_tile, p->H / p->Hkv)
+                                              : 1;
+    plan_tiles(A, groups, window, pos, family < 0 ? to_cpp(*o).for_diff_tiled() : to_cpp(*o), kind == Pass::diff || family < 0 ? nullptr : p);
     *n_tiles = int32_t(A.tiles.size());
     *n_jobs = int32_t(A.combine.size());
     *n_parts = A.parts;
@@ -102,14 +106,21 @@ static int plan_pass(const esp_attn_params* p, bool diff, const esp_tree* trees,
 int esp_plan_tiles_for(const esp_attn_params* p, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
                        const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                        int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen) {
-  return plan_pass(p, false, trees, n_trees, groups, window, pos, o, tiles, tiles_cap, n_tiles, jobs, jobs_cap, n_jobs, n_parts, err, errlen);
+  return plan_pass(p, Pass::plain, trees, n_trees, groups, window, pos, o, tiles, tiles_cap, n_tiles, jobs, jobs_cap, n_jobs, n_parts, err, errlen);
 }
 
 int esp_plan_tiles_diff(const esp_attn_params* p, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
                         const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                         int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen) {
   if (!p || p->H <= 0 || p->Hkv <= 0 || p->H % p->Hkv) return put_err(err, errlen, ESP_EINVAL, "H / Hkv");
-  return plan_pass(p, true, trees, n_trees, groups, window, pos, o, tiles, tiles_cap, n_tiles, jobs, jobs_cap, n_jobs, n_parts, err, errlen);
+  return plan_pass(p, Pass::diff, trees, n_trees, groups, window, pos, o, tiles, tiles_cap, n_tiles, jobs, jobs_cap, n_jobs, n_parts, err, errlen);
+}
+
+int esp_plan_tiles_shaped(const esp_attn_params* p, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
+                          const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
+                          int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen) {
+  if (!p || p->H <= 0 || p->Hkv <= 0 || p->H % p->Hkv) return put_err(err, errlen, ESP_EINVAL, "H / Hkv");
+  return plan_pass(p, Pass::shaped, trees, n_trees, groups, window, pos, o, tiles, tiles_cap, n_tiles, jobs, jobs_cap, n_jobs, n_parts, err, errlen);
 }
 
 int esp_plan_lowrank(const esp_lowrank_params* p, const int32_t* adapter, int32_t n_rows, int32_t* order, int32_t* n_slots, esp_lowrank_tile* tiles,

@@ -57,6 +57,7 @@ ENGINE_SYMBOLS = {
     "esp_engine_pass_pos": (C.c_int, (_V, _V)),
     "esp_engine_pass_table": (C.c_int, (_V, _V)),
     "esp_engine_pass_saves": (C.c_int, (_V, _V)),
+    "esp_plan_tiles_shaped": (C.c_int, (_AP, _V, _I, _I, _I, _V, _PO, _V, _I, _IP, _V, _I, _IP, _IP) + _ERR),
     "esp_plan_linear": (C.c_int, (C.POINTER(abi.LinearParams), _V, _I, _I, _I, _V, _I, _IP, _IP, _IP) + _ERR),
     "esp_engine_pass_cow": (C.c_int, (_V, _V)),
     "esp_engine_pass_rings": (C.c_int, (_V, _I, _I, _V, _V, _I, _IP, _V, _I, _IP) + _ERR),
@@ -102,14 +103,14 @@ def options_mi355x(rows, workgroups):
 
 
 def plan_tiles(trees, groups, window, pos, options):
-    """trees: TREE_DT array. groups: plan_hint's, which plans for that layer (attn_diff_hint's: for differential attention on it), or a
-    number, which plans for any. Returns (tiles TILE_DT, jobs COMBINE_DT, n_parts)."""
+    """trees: TREE_DT array. groups: plan_hint's, which plans for that layer (attn_diff_hint's: for differential attention on it, attn_shaped_hint's:
+    for attention with shaped scores), or a number, which plans for any. Returns (tiles TILE_DT, jobs COMBINE_DT, n_parts)."""
     lib = engine_lib()
     trees = np.ascontiguousarray(trees, dtype=abi.TREE_DT)
     pos_a = None if pos is None else np.ascontiguousarray(pos, dtype=np.int32)
-    diff = getattr(groups, "diff", None)
-    layer = diff or getattr(groups, "layer", None)
-    plan = lib.esp_plan_tiles_diff if diff else lib.esp_plan_tiles_for
+    diff, shaped = getattr(groups, "diff", None), getattr(groups, "shaped", None)
+    layer = diff or shaped or getattr(groups, "layer", None)
+    plan = lib.esp_plan_tiles_diff if diff else lib.esp_plan_tiles_shaped if shaped else lib.esp_plan_tiles_for
     p = None
     if layer is not None:
         p = abi.AttnParams()

@@ -207,9 +207,10 @@ int esp_attn_validate(const esp_attn_params* p, const esp_tile* tiles, int32_t n
  *                          P + j of the tree's own block list, which must reach that far; on the tiled kernel P - base
  *                          is a multiple of 16; on ring layers a tree's rows must not overwrite keys its first rows see;
  *   ESP_PASS_DIFF          the pass goes to esp_attn_diff: rows in the pool as above (any P - base), a tile that has both
- *                          cached keys and rows of the pass has the former up to P and the latter from row 0 on.
+ *                          cached keys and rows of the pass has the former up to P and the latter from row 0 on;
+ *   ESP_PASS_SHAPED        the same for a pass of esp_attn_shaped.
  * Same arguments as esp_attn_validate otherwise. Host pointers; touches no device. */
-enum { ESP_PASS_FUSED = 1, ESP_PASS_ROWS_IN_POOL = 2, ESP_PASS_DIFF = 4 };
+enum { ESP_PASS_FUSED = 1, ESP_PASS_ROWS_IN_POOL = 2, ESP_PASS_DIFF = 4, ESP_PASS_SHAPED = 8 };
 int esp_attn_validate_for(const esp_attn_params* p, int32_t mode, const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees,
                           int32_t n_trees, const esp_combine* jobs, int32_t n_jobs, int32_t n_parts, int32_t n_rows, const int32_t* blocks,
                           int32_t n_block_entries, int32_t pool_blocks, char* err, size_t errlen);
@@ -408,6 +409,38 @@ size_t esp_attn_diff_workspace_bytes(const esp_attn_params* p, int32_t n_parts);
 int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void* Q, const void* kv_pool, const int32_t* blocks, void* O,
                   const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees, int32_t n_trees, const esp_combine* jobs, int32_t n_jobs,
                   int32_t n_parts, int32_t n_rows, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen);
+
+/* ---- attention with shaped scores over the paged pool ------------------------------
+ * No counterpart in the reference. Query head h of a row at cache position p weighs the key at position j of its tree by the softmax of
+ *   x = scale q.k;   x = cap tanh(x / cap) where cap > 0;   x -= slopes[h] |p - j| where there are slopes
+ * over the keys that the row sees: with span (first, prefix) of the row those with first <= j and (j <= p or j < prefix), of them
+ * the last `window` (p - j < window) where window > 0. So `first` is where the row's document starts in a sequence of several, and keys in
+ * front of `prefix` are seen by the rows in front of them too (an image, an instruction). Without spans rows are plain causal. Any numbers may
+ * stand in a span; a row that sees nothing gets zeros. Pool, records and append are those of esp_attn_diff: the pass's rows are in the
+ * pool, row j of a tree at position P + j of its own block list or ring, and all of them are there before the call, also those that only rows
+ * in front of them see. Softmax and sums are held in fp32; the probabilities enter P.V in the storage type (as the sum of two such
+ * numbers in passes of few rows), O is rounded once at the end. */
+typedef struct esp_shape_params {
+  const float* slopes;  /* [H] fp32, device memory; NULL: no bias */
+  const int32_t* spans; /* int32[2] per row of the pass, device memory; NULL: plain causal rows */
+  float cap;            /* 0: none */
+  int32_t pad;
+} esp_shape_params;
+
+/* The rows_per_tile to plan a pass with whose trees have at most `rows` rows, or 0 for parameters that
+ * esp_attn_shaped refuses. Host-only arithmetic. */
+int32_t esp_attn_shaped_rows(const esp_attn_params* p, int32_t rows);
+/* As esp_attn_plan_hint, of the kernel that serves p->rows_per_tile. */
+int esp_attn_shaped_hint(const esp_attn_params* p, int device, int32_t* workgroups, int32_t* groups_per_tile, char* err, size_t errlen);
+/* Bytes of workspace for a plan of n_parts partial records. Host-only arithmetic. */
+size_t esp_attn_shaped_workspace_bytes(const esp_attn_params* p, int32_t n_parts);
+/* Of p: head_dim 128 or 256, H / Hkv at most 128, no gate, no bidi; kv_ld is not read. Q and O [n_rows][q_ld]; rows outside the tiles are left as
+ * they are. Tiles, trees and jobs as planned by esp_plan_tiles_shaped (include/espetero_engine.h; a plan of esp_plan_tiles runs too, slower);
+ * what the records have to promise is what esp_attn_validate_for(ESP_PASS_SHAPED) checks. Tiles with k1 = INT32_MAX end at the tree's
+ * cached length as it is when the kernel runs (decode chains). */
+int esp_attn_shaped(const esp_attn_params* p, const esp_shape_params* shape, const void* Q, const void* kv_pool, const int32_t* blocks, void* O,
+                    const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees, int32_t n_trees, const esp_combine* jobs, int32_t n_jobs,
+                    int32_t n_parts, int32_t n_rows, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen);
 
 /* ---- low-rank adapters of many requests beside a shared projection -----------------
  * No counterpart in the reference. Every row adds its own adapter's product to the fp32 projection that esp_attn_prep

@@ -75,6 +75,12 @@ int esp_plan_tiles_diff(const esp_attn_params* p, const esp_tree* trees, int32_t
                         const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                         int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen);
 
+/* And for a pass of esp_attn_shaped (p: its parameters; groups: what esp_attn_shaped_hint reports), by the same rules: passes of the streaming
+ * kernel as esp_plan_tiles_for plans them, those of the tiled one as esp_plan_tiles_diff. */
+int esp_plan_tiles_shaped(const esp_attn_params* p, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
+                          const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
+                          int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen);
+
 /* The tiles of a pass of esp_lowrank_add: the rows that have an adapter, grouped by it (adapters ascending, rows ascending within
  * one), in tiles of p->rows_per_tile rows and fewer at an adapter's end. adapter[n_rows]: each row's, -1 for none; ESP_EINVAL for one
  * that p->n_adapters does not hold. order (room for n_rows) and tiles (capacity given) out; on ESP_EWORKSPACE the counts are still
