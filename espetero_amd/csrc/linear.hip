@@ -106,6 +106,8 @@ __global__ __launch_bounds__(256) void linear_few_kernel(const LinearArgs a) {
 // the sequence's), and the segments then start from the sum of those in front of them, each decayed over the segments between.
 
 using lds_u32x4 = const __attribute__((address_space(3))) u32x4;
+using lds_u32x4_out = __attribute__((address_space(3))) u32x4;
+using lds_u32x2_out = __attribute__((address_space(3))) u32x2;
 
 constexpr int kPBytes = 32 * 64 + 32 * 128;  // rows 0 .. 31 of P have no weights behind column 31
 
@@ -130,7 +132,7 @@ template <int DK>
 __device__ __forceinline__ int row_part(int r, int c) {
   return r * (DK * 2) + ((DK == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7)) << 4);
 }
-__device__ __forceinline__ int col_part(int r, int c) { return r * 128 + ((c ^ (((r >> 1) + (r >> 4)) & 7)) << 4); }
+__device__ __forceinline__ int col_part(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7) ^ ((r >> 3) & 2)) << 4); }
 
 __device__ __forceinline__ int p_part(int r, int c) {
   return r < 32 ? r * 64 + ((c ^ ((r >> 2) & 3)) << 4) : 2048 + (r - 32) * 128 + ((c ^ ((r >> 1) & 7)) << 4);
@@ -170,7 +172,7 @@ __device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&out)[N]) {
 __device__ __forceinline__ float abs_max_halves(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
 
 template <int DT, int DK, int DVB, bool STATE>
-__global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearArgs a) {
+__global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linear_chunk_kernel(const LinearArgs a) {
   constexpr int NW = DVB / 32, T = 64 * NW, KT = DK / 32, NV = DT == ESP_F16 ? 2 : 3;
   using L = ChunkLds<DK, DVB, STATE>;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -273,20 +275,32 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
     for (int i = 0; i < 4; ++i)
       if (r + i >= n) x[i] = u32x4{0, 0, 0, 0};
   };
-  // 4 rows of 8 columns as 8 columns of 4 rows, into a [columns][64 rows] array.
-  auto turn = [&](const u32x4 (&x)[4], char* to, int group, int part) __attribute__((always_inline)) {
+  // Operands' places: one address each, the parts of a row by turning bits of it, tiles behind each other as the instruction's own offset.
+  // Worked out again in every chunk: kept for the next they would be spilled.
+  const uint32_t base = uint32_t(uintptr_t(lds));
+  auto place = [&](int at) {
+    uint32_t x = base + uint32_t(at);
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  auto read = [&](uint32_t at) { return *reinterpret_cast<lds_u32x4*>(at); };
+  // 4 rows of 8 columns, rows 4 group .. + 3 and their part: as they come, and as 8 columns of 4 rows into a [columns][64 rows] array.
+  auto put_rows = [&](const u32x4 (&x)[4], int to, int group, int part) __attribute__((always_inline)) {
+    const uint32_t at = place(to + row_part<DK>(4 * group, part));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<lds_u32x4_out*>((at ^ ((DK == 128 ? j : j >> 1) << 4)) + j * (DK * 2)) = x[j];
+  };
+  auto put_columns = [&](const u32x4 (&x)[4], int to, int group, int part) __attribute__((always_inline)) {
+    const uint32_t at = place(to + col_part(8 * part, group >> 1) + 8 * (group & 1));
 #pragma unroll
     for (int p = 0; p < 4; ++p)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const uint32_t sel = s ? 0x07060302u : 0x05040100u;
-        const int r = 8 * part + 2 * p + s;
-        *reinterpret_cast<u32x2*>(to + col_part(r, group >> 1) + 8 * (group & 1)) =
+        *reinterpret_cast<lds_u32x2_out*>((at ^ (p << 4)) + (2 * p + s) * 128) =
             u32x2{__builtin_amdgcn_perm(x[1][p], x[0][p], sel), __builtin_amdgcn_perm(x[3][p], x[2][p], sel)};
       }
   };
-  const uint32_t base = uint32_t(uintptr_t(lds));
-  auto read = [&](int at) { return *reinterpret_cast<lds_u32x4*>(base + uint32_t(at)); };
 
   if (n_chunks > 0) fetch(0);
   double so_far = 0.0;
@@ -307,13 +321,10 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
       if (STATE && it >= 2 * DK) break;
       const bool isK = STATE || it < 2 * DK;
       const int b = isK ? it : it - 2 * DK;
-      if (!STATE) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(lds + (isK ? L::kK : L::kQ) + row_part<DK>(4 * (b / kParts) + j, b % kParts)) = kq[i][j];
-      }
-      if (isK) turn(kq[i], lds + L::kKT, b / kParts, b % kParts);
+      if (!STATE) put_rows(kq[i], isK ? L::kK : L::kQ, b / kParts, b % kParts);
+      if (isK) put_columns(kq[i], L::kKT, b / kParts, b % kParts);
     }
-    turn(vv, lds + L::kVT, tid / vParts, tid % vParts);
+    put_columns(vv, L::kVT, tid / vParts, tid % vParts);
     double cl;  // C, in every wavefront
     {
       double s;
@@ -337,7 +348,7 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
     }
     so_far += cl;
     __syncthreads();
-    if (c + 1 < n_chunks) fetch(c + 1);
+    if (STATE && c + 1 < n_chunks) fetch(c + 1);
 
     f32x16 O[2];
     float s_down = 1.0f;
@@ -349,8 +360,9 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
         const int rt = NW == 4 ? wave : half ? 3 - wave : wave;
         const int row = 16 * rt + l16;
         u32x4 qf[DK / 32];
+        const uint32_t q_at = place(L::kQ + row_part<DK>(row, q4)), k_at = place(L::kK + row_part<DK>(l16, q4));
 #pragma unroll
-        for (int kk = 0; kk < DK / 32; ++kk) qf[kk] = read(L::kQ + row_part<DK>(row, 4 * kk + q4));
+        for (int kk = 0; kk < DK / 32; ++kk) qf[kk] = read(q_at ^ (kk << 6));
         const double ci = cum[row];
         float x[4][4], mx = 0.0f;
 #pragma unroll
@@ -360,7 +372,7 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
           if (jt > rt) continue;
           f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-          for (int kk = 0; kk < DK / 32; ++kk) acc = mfma16x32<DT>(read(L::kK + row_part<DK>(16 * jt + l16, 4 * kk + q4)), qf[kk], acc);
+          for (int kk = 0; kk < DK / 32; ++kk) acc = mfma16x32<DT>(read((k_at ^ (kk << 6)) + jt * (32 * DK)), qf[kk], acc);
           mfma_settle(acc);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -413,6 +425,7 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
         for (int x = 1; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
         scale_for(mx, kOutputScale, s_up, s_down);
       }
+      const uint32_t q_at = place(L::kQ + row_part<DK>(l32, hb));
 #pragma unroll
       for (int ks = 0; ks < DK / 16; ++ks) {
         float x[8];
@@ -422,16 +435,22 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
         split8<DT, 2>(x, sp);
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-          const u32x4 q = read(L::kQ + row_part<DK>(32 * rt + l32, 2 * ks + hb));
+          const u32x4 q = read((q_at ^ (ks << 5)) + rt * (64 * DK));
           O[rt] = mfma32x16<DT>(sp[0], q, O[rt]);
           O[rt] = mfma32x16<DT>(sp[1], q, O[rt]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
+      if (c + 1 < n_chunks) fetch(c + 1);
       __syncthreads();  // P is there, and nobody reads Q and K any more
     }
     u32x4 vr[4];
+    auto read_v = [&] {
+      const uint32_t v_at = place(L::kVT + col_part(32 * wave + l32, hb));
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) vr[ks] = read(L::kVT + col_part(32 * wave + l32, 2 * ks + hb));
+      for (int ks = 0; ks < 4; ++ks) vr[ks] = read(v_at ^ (ks << 5));
+    };
+    read_v();
     if constexpr (!STATE) {
       // An infinite or NaN value may not reach the rows in front of its own, whose weight of it is zero.
       float nf = 0.0f;
@@ -440,17 +459,14 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
 #pragma unroll
         for (int e = 0; e < 4; ++e) nf = fmaf(unpack_lo<DT>(vr[ks][e]), 0.0f, fmaf(unpack_hi<DT>(vr[ks][e]), 0.0f, nf));
       const bool odd = __any(nf != 0.0f);
-      u32x4 vp[4];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) vp[ks] = vr[ks];
       if (__builtin_expect(odd, 0)) {
         constexpr uint32_t ex = DT == ESP_F16 ? 0x7c00u : 0x7f80u;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t w = vp[ks][e];
-            vp[ks][e] = w & (((w & ex) == ex ? 0u : 0xffffu) | ((w >> 16 & ex) == ex ? 0u : 0xffff0000u));
+            const uint32_t w = vr[ks][e];
+            vr[ks][e] = w & (((w & ex) == ex ? 0u : 0xffffu) | ((w >> 16 & ex) == ex ? 0u : 0xffff0000u));
           }
       }
 #pragma unroll
@@ -466,27 +482,31 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
         } else {
           O[rt] *= f;
         }
+        const uint32_t p_at = place(L::kP + p_part(row, hb));
 #pragma unroll
         for (int ks = 0; ks < 2 + 2 * rt; ++ks) {
-          const int at = L::kP + p_part(row, 2 * ks + hb);
-          O[rt] = mfma32x16<DT>(vp[ks], read(at), O[rt]);
-          O[rt] = mfma32x16<DT>(vp[ks], read(at + kPBytes), O[rt]);
+          O[rt] = mfma32x16<DT>(vr[ks], read(p_at ^ (ks << 5)), O[rt]);
+          O[rt] = mfma32x16<DT>(vr[ks], read((p_at ^ (ks << 5)) + kPBytes), O[rt]);
         }
         mfma_settle(O[rt]);
         if (__builtin_expect(odd, 0)) {
+          // Rows 8 (e / 4) + 4 hb + e % 4 of the wavefront's part of V^T: their turns differ by constants.
+#pragma unroll 1
           for (int j = 0; j <= row; ++j) {
-            const uint16_t pw = *reinterpret_cast<const uint16_t*>(lds + L::kP + p_part(row, j >> 3) + 2 * (j & 7));
-            const float p = unpack_lo<DT>(pw);
+            const float p = unpack_lo<DT>(*reinterpret_cast<const uint16_t*>(lds + L::kP + p_part(row, j >> 3) + 2 * (j & 7)));
+            const uint32_t at = place(L::kVT + (32 * wave + 4 * hb) * 128 + (((j >> 3) ^ (2 * hb)) << 4) + 2 * (j & 7));
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const int d = 32 * wave + 8 * (e >> 2) + 4 * hb + (e & 3);
-              const float v = unpack_lo<DT>(*reinterpret_cast<const uint16_t*>(lds + L::kVT + col_part(d, j >> 3) + 2 * (j & 7)));
+              constexpr auto turn = [](int d) { return ((d >> 1) & 7) ^ ((d >> 3) & 2); };
+              const int d = 8 * (e >> 2) + (e & 3);
+              const float v = unpack_lo<DT>(*reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>((at ^ (turn(d) << 4)) + d * 128));
               if (!(fabsf(v) < INFINITY)) O[rt][e] += p * v;
             }
           }
         }
         O[rt] *= DT == ESP_F16 ? pinv[row] * a.scale : a.scale;
       }
+      if (__builtin_expect(odd, 0)) read_v();
       // Through LDS, where Q and K were, a wavefront's 64 rows of 64 bytes each; 16-byte parts turned by the row.
       char* const mine = lds + L::kQ + wave * 4096;
       auto part_at = [&](int r, int p) { return mine + r * 64 + ((p ^ ((r >> 2) & 3)) << 4); };
@@ -508,36 +528,43 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
     // S = exp(C) S + K^T V'. (The state behind the segment is of use only where somebody reads it.)
     if (STATE || c + 1 < n_chunks || tile.dst >= 0) {
       const float f = *total;
-      float x[4][8];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
+      const uint32_t k_at = place(L::kKT + col_part(swap23(l32), hb));
+      auto weighted = [&](int ks, float (&x)[8]) __attribute__((always_inline)) {
+        const f32x4 w0 = *reinterpret_cast<const f32x4*>(left + 16 * ks + 8 * hb), w1 = *reinterpret_cast<const f32x4*>(left + 16 * ks + 8 * hb + 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[ks][2 * e] = unpack_lo<DT>(vr[ks][e]) * left[16 * ks + 8 * hb + 2 * e];
-          x[ks][2 * e + 1] = unpack_hi<DT>(vr[ks][e]) * left[16 * ks + 8 * hb + 2 * e + 1];
+          x[2 * e] = unpack_lo<DT>(vr[ks][e]) * (e < 2 ? w0 : w1)[2 * (e & 1)];
+          x[2 * e + 1] = unpack_hi<DT>(vr[ks][e]) * (e < 2 ? w0 : w1)[2 * (e & 1) + 1];
         }
+      };
       if constexpr (DT == ESP_F16) {
         float mx = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
+        for (int ks = 0; ks < 4; ++ks) {
+          float x[8];
+          weighted(ks, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[ks][e]));
+          for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+        }
         mx = abs_max_halves(mx);
         float up, down;
         scale_for(mx, 126, up, down);
         u32x4 vs[4][NV];
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
+          float x[8];
+          weighted(ks, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[ks][e] *= up;
-          split8<DT, NV>(x[ks], vs[ks]);
+          for (int e = 0; e < 8; ++e) x[e] *= up;
+          split8<DT, NV>(x, vs[ks]);
+          __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           f32x16 d{};
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
-            const u32x4 k = read(L::kKT + col_part(32 * t + swap23(l32), 2 * ks + hb));
+            const u32x4 k = read((k_at ^ (ks << 5)) + t * 4096);
 #pragma unroll
             for (int v = 0; v < NV; ++v) d = mfma32x16<DT>(k, vs[ks][v], d);
           }
@@ -550,14 +577,17 @@ __global__ __launch_bounds__(2 * DVB, 2) void linear_chunk_kernel(const LinearAr
         for (int t = 0; t < KT; ++t) S[t] *= f;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
+          float x[8];
+          weighted(ks, x);
           u32x4 vs[NV];
-          split8<DT, NV>(x[ks], vs);
+          split8<DT, NV>(x, vs);
 #pragma unroll
           for (int t = 0; t < KT; ++t) {
-            const u32x4 k = read(L::kKT + col_part(32 * t + swap23(l32), 2 * ks + hb));
+            const u32x4 k = read((k_at ^ (ks << 5)) + t * 4096);
 #pragma unroll
             for (int v = 0; v < NV; ++v) S[t] = mfma32x16<DT>(k, vs[v], S[t]);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int t = 0; t < KT; ++t) mfma_settle(S[t]);
