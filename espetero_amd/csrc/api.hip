@@ -1088,6 +1088,8 @@ static int check_linear(const esp_linear_params* p, char* err, size_t errlen) {
     return fail(err, errlen, ESP_EINVAL, "q_ld %d, k_ld %d, v_ld %d, o_ld %d: a row has %d, %d, %d and %d elements", p->q_ld, p->k_ld, p->v_ld, p->o_ld,
                 p->Hk * p->dk, p->Hk * p->dk, p->H * p->dv, p->H * p->dv);
   if ((p->q_ld | p->k_ld | p->v_ld | p->o_ld) % 8) return fail(err, errlen, ESP_EINVAL, "row strides must be multiples of 8");
+  if (std::max(std::max(p->q_ld, p->k_ld), std::max(p->v_ld, p->o_ld)) > 1 << 24)  // 64 rows of it in 32 bits of bytes
+    return fail(err, errlen, ESP_EUNSUPPORTED, "row strides of more than %d elements", 1 << 24);
   if (p->decay_ld != 0 && p->decay_ld < p->H) return fail(err, errlen, ESP_EINVAL, "decay_ld %d (0, or at least H = %d)", p->decay_ld, p->H);
   if (p->n_states < 0) return fail(err, errlen, ESP_EINVAL, "n_states %d", p->n_states);
   if (!std::isfinite(p->scale)) return fail(err, errlen, ESP_EINVAL, "scale is not finite");

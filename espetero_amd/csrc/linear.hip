@@ -119,12 +119,14 @@ struct ChunkLds {
   static constexpr int kKT = STATE ? 0 : 2 * 64 * DK * 2;
   static constexpr int kVT = kKT + 64 * DK * 2;
   static constexpr int kP = kVT + 64 * DVB * 2;             // two numbers for each weight
-  static constexpr int kCum = kP + (STATE ? 0 : 2 * kPBytes);  // double[64]: c
-  static constexpr int kLeft = kCum + 512;                  // float[64]: exp(C - c_j)
-  static constexpr int kRowF = kLeft + 256;                 // float[64]: exp(c_i)
-  static constexpr int kPInv = kRowF + 256;                 // float[64]: what undoes P's scale
-  static constexpr int kTotal = kPInv + 256;                // float: exp(C)
-  static constexpr int kBytes = kTotal + 256;
+  static constexpr int kLeft = kP + (STATE ? 0 : 2 * kPBytes);  // float[64]: exp(C - c_j)
+  static constexpr int kRowF = kLeft + 256;                 // float[64]: scale exp(c_i)
+  static constexpr int kTotal = kRowF + 256;                // float: exp(C)
+  static constexpr int kColF = kTotal + 16;                 // float[4][64]: exp(b_t - c_j), b_t the sum in front of row 16 t, of the rows there
+  static constexpr int kSince = kColF + (STATE ? 0 : 1024); // float[64][2]: c_i - b of the row's tile, in two numbers
+  static constexpr int kPInv = kSince + (STATE ? 0 : 512);  // float[64]: what undoes P's scale
+  static constexpr int kNone = kPInv + (STATE ? 0 : 256);               // where what has no place in P goes, a wavefront's over another's
+  static constexpr int kBytes = kNone + (STATE ? 0 : 512);
 };
 
 // Parts of rows of DK numbers and of rows of 64 (K^T, V^T, P): where part c of row r lies.
@@ -151,9 +153,24 @@ __device__ __forceinline__ void scale_for(float largest, int most, float& up, fl
 // step, and the other half of the sums, which takes the same scale, stays far from fp32's largest.
 constexpr int kOutputScale = 60;
 
-// 8 numbers as N numbers of 16 bits each.
+// 8 numbers times `by` (1 for bf16) as N numbers of 16 bits each.
 template <int DT, int N>
-__device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&out)[N]) {
+__device__ __forceinline__ void split8(const float (&x)[8], float by, u32x4 (&out)[N]) {
+  if constexpr (DT == ESP_F16) {
+    static_assert(N == 2);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f16x2 a, b;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // (an instruction each, which rounds its product or difference to fp16)
+        a[i] = (_Float16)__builtin_fmaf(x[2 * e + i], by, 0.0f);
+        b[i] = (_Float16)__builtin_fmaf(x[2 * e + i], by, -float(a[i]));
+      }
+      out[0][e] = __builtin_bit_cast(uint32_t, a);
+      out[1][e] = __builtin_bit_cast(uint32_t, b);
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     float lo = x[2 * e], hi = x[2 * e + 1];
@@ -169,7 +186,59 @@ __device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&out)[N]) {
   }
 }
 
+// acc + the two storage elements of a dword times zero: NaN where one of them is not finite.
+template <int DT>
+__device__ __forceinline__ float times_zero2(uint32_t w, float acc) {
+  if constexpr (DT == ESP_F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0u), acc, false);
+  else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0u), acc, false);
+}
+
+// Sums over the lanes up to and with this one, in 64 bits: within rows of 16 lanes, then the rows' last lanes to the rows behind.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_from(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b)), CTRL, ROWS, 0xf, false));
+  const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b >> 32)), CTRL, ROWS, 0xf, false));
+  return x + __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ double scan64(double x) {
+  x = add_from<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x = add_from<0x112, 0xf>(x);
+  x = add_from<0x114, 0xf>(x);
+  x = add_from<0x118, 0xf>(x);
+  x = add_from<0x142, 0xa>(x);  // row_bcast 15, to rows 1 and 3
+  return add_from<0x143, 0xc>(x);  // row_bcast 31, to rows 2 and 3
+}
+__device__ __forceinline__ double lane_of(double x, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b)), lane)), hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b >> 32)), lane));
+  return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+
+// All wavefronts of the workgroup are here and their LDS accesses done. Loads from memory on their way stay there, for which __syncthreads
+// would wait: the next chunk's rows.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// The maximum over the wavefront, of numbers of 0 or more.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float max_from(float x) {
+  return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = max_from<0x111, 0xf>(x);
+  x = max_from<0x112, 0xf>(x);
+  x = max_from<0x114, 0xf>(x);
+  x = max_from<0x118, 0xf>(x);
+  x = max_from<0x142, 0xa>(x);
+  x = max_from<0x143, 0xc>(x);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
 __device__ __forceinline__ float abs_max_halves(float x) { return fmaxf(x, __shfl_xor(x, 32)); }
+
+// mfma_settle for several results at once.
+__device__ __forceinline__ void settle(f32x16 (&x)[2]) { asm volatile("s_nop 15\n\ts_nop 15" : "+v"(x[0]), "+v"(x[1])); }
+__device__ __forceinline__ void settle(f32x16 (&x)[4]) { asm volatile("s_nop 15\n\ts_nop 15" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3])); }
 
 template <int DT, int DK, int DVB, bool STATE>
 __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linear_chunk_kernel(const LinearArgs a) {
@@ -185,7 +254,8 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
   const int kh = h / a.group;
   const int col = blk * DVB + 32 * wave + l32;  // this lane's column of the state
   const size_t slot = size_t(a.H) * DK * a.dv;
-  double* const cum = reinterpret_cast<double*>(lds + L::kCum);
+  float* const colf = reinterpret_cast<float*>(lds + L::kColF);
+  float2* const since = reinterpret_cast<float2*>(lds + L::kSince);
   float* const left = reinterpret_cast<float*>(lds + L::kLeft);
   float* const rowf = reinterpret_cast<float*>(lds + L::kRowF);
   float* const pinv = reinterpret_cast<float*>(lds + L::kPInv);
@@ -251,23 +321,54 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
   const float g_const = a.decay_ld ? 0.0f : decay_log2(a.decay[h]);
   float g_row = 0.0f;
   const int n_chunks = (tile.rows + 63) >> 6;
-  auto fetch = [&](int c) __attribute__((always_inline)) {
-    const int r0 = tile.row0 + 64 * c, last = tile.row0 + tile.rows - 1;
+  const char *from_kq[NI], *from_v;  // the lane's first row of each piece in the next chunk
+  uint32_t ld_kq[NI];
+  const uint32_t ld_v = uint32_t(2 * a.v_ld);
 #pragma unroll
-    for (int n = 0; n < NI; ++n) {
-      const int it = tid + T * n;
-      if (STATE && it >= 2 * DK) break;
-      const bool isK = STATE || it < 2 * DK;
-      const int b = isK ? it : it - 2 * DK, r = r0 + 4 * (b / kParts), part = b % kParts;
-      const uint16_t* from = (isK ? a.K : a.Q) + size_t(kh) * DK + 8 * part;
-      const size_t ld = isK ? a.k_ld : a.q_ld;
+  for (int p = 0; p < NI; ++p) {
+    const int it = tid + T * p;
+    const bool isK = STATE || it < 2 * DK;  // (alike in a wavefront)
+    const int b = (isK ? it : it - 2 * DK) % (2 * DK);
+    ld_kq[p] = uint32_t(__builtin_amdgcn_readfirstlane(2 * (isK ? a.k_ld : a.q_ld)));
+    from_kq[p] = reinterpret_cast<const char*>((isK ? a.K : a.Q) + size_t(kh) * DK) + (size_t(tile.row0) + 4 * (b / kParts)) * ld_kq[p] + 16 * (b % kParts);
+  }
+  from_v = reinterpret_cast<const char*>(a.V + dv0) + (size_t(tile.row0) + 4 * (tid / vParts)) * ld_v + 16 * (tid % vParts);
+  // Row i of piece p (of NI: V's) of the next chunk; in the segment's last one rows behind the last are read as that one.
+  auto fetch_row = [&](int p, int i) __attribute__((always_inline)) {
+    if (p < NI) kq[p < NI ? p : 0][i] = *reinterpret_cast<const u32x4*>(from_kq[p < NI ? p : 0] + size_t(i) * ld_kq[p < NI ? p : 0]);
+    else vv[i] = *reinterpret_cast<const u32x4*>(from_v + size_t(i) * ld_v);
+  };
+  auto fetch_last = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) kq[n][i] = *reinterpret_cast<const u32x4*>(from + size_t(min(r + i, last)) * ld);
+    for (int p = 0; p < NI; ++p) {
+      const int r = 4 * (((tid + T * p) % (2 * DK)) / kParts);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kq[p][i] = *reinterpret_cast<const u32x4*>(from_kq[p] + int64_t(min(r + i, n - 1) - r) * int64_t(ld_kq[p]));
     }
-    const int r = r0 + 4 * (tid / vParts), part = tid % vParts;
+    const int r = 4 * (tid / vParts);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vv[i] = *reinterpret_cast<const u32x4*>(a.V + size_t(min(r + i, last)) * a.v_ld + dv0 + 8 * part);
-    if (a.decay_ld) g_row = decay_log2(a.decay[size_t(min(r0 + lane, last)) * a.decay_ld + h]);
+    for (int i = 0; i < 4; ++i) vv[i] = *reinterpret_cast<const u32x4*>(from_v + int64_t(min(r + i, n - 1) - r) * int64_t(ld_v));
+  };
+  auto fetch_decay = [&](int c) __attribute__((always_inline)) {  // (as it is: working on it here would be a wait)
+    if (a.decay_ld) g_row = a.decay[(size_t(tile.row0) + min(64 * c + lane, tile.rows - 1)) * a.decay_ld + h];
+  };
+  auto fetch_on = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < NI; ++p) from_kq[p] += 64 * size_t(ld_kq[p]);
+    from_v += 64 * size_t(ld_v);
+  };
+  auto fetch_all = [&](int c) __attribute__((always_inline)) {
+    const int n = tile.rows - 64 * c;
+    if (n >= 64) {
+#pragma unroll
+      for (int p = 0; p <= NI; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fetch_row(p, i);
+    } else {
+      fetch_last(n);
+    }
+    fetch_on();
+    fetch_decay(c);
   };
   // Rows behind the segment's last are zeros in K and V.
   auto clear_past = [&](u32x4 (&x)[4], int r, int n) {
@@ -302,12 +403,10 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
       }
   };
 
-  if (n_chunks > 0) fetch(0);
+  if (n_chunks > 0) fetch_all(0);
   double so_far = 0.0;
   for (int c = 0; c < n_chunks; ++c) {
-    const int n = min(64, tile.rows - 64 * c);
-    if (c > 0) __syncthreads();  // everybody is done with the chunk in front of this one
-    if (n < 64) {
+    const int n = min(64, tile.rows - 64 * c);    if (c > 0) lds_barrier();  // everybody is done with the chunk in front of this one    if (n < 64) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int it = tid + T * i;
@@ -324,127 +423,160 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
       if (!STATE) put_rows(kq[i], isK ? L::kK : L::kQ, b / kParts, b % kParts);
       if (isK) put_columns(kq[i], L::kKT, b / kParts, b % kParts);
     }
-    put_columns(vv, L::kVT, tid / vParts, tid % vParts);
-    double cl;  // C, in every wavefront
-    {
-      double s;
-      if (a.decay_ld) {
-        s = lane < n ? double(g_row) : 0.0;
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) {
-          const double up = __shfl_up(s, x);
-          s += lane >= x ? up : 0.0;
-        }
-      } else {
-        s = double(g_const) * min(lane + 1, n);
-      }
-      cl = __shfl(s, 63);
-      if (wave == 0) {
-        cum[lane] = s;
-        left[lane] = lane < n ? fast_exp2(float(cl - s)) : 0.0f;
-        rowf[lane] = fast_exp2(float(s));
+    put_columns(vv, L::kVT, tid / vParts, tid % vParts);    // What the chunk's decays come to. Of a head's own they are those of the chunk before, but for the first and the last.
+    if (a.decay_ld || c == 0 || n < 64) {
+      const double s = a.decay_ld ? scan64(lane < n ? double(decay_log2(g_row)) : 0.0) : double(g_const) * min(lane + 1, n);
+      const double cl = lane_of(s, 63);
+      so_far = STATE ? so_far + cl : 0.0;
+      if (wave == 0) left[lane] = lane < n ? fast_exp2(float(cl - s)) : 0.0f;
+      if (wave == NW - 1) {
+        rowf[lane] = a.scale * fast_exp2(float(s));
         if (lane == 0) *total = fast_exp2(float(cl));
       }
+      if (!STATE) {
+#pragma unroll
+        for (int i = 0; i < 4 / NW; ++i) {
+          const int t = i ? 3 - wave : wave;
+          const double b = t ? lane_of(s, 16 * t - 1) : 0.0;
+          colf[64 * t + lane] = lane < 16 * t ? fast_exp2(float(b - s)) : 0.0f;
+          const float hi = float(s - b);
+          if (lane >> 4 == t) since[lane] = float2{hi, float(s - b - double(hi))};
+        }
+      }
+    } else if (STATE) {
+      so_far += double(g_const) * 64.0;
     }
-    so_far += cl;
-    __syncthreads();
-    if (STATE && c + 1 < n_chunks) fetch(c + 1);
+    lds_barrier();    if (STATE && c + 1 < n_chunks) fetch_all(c + 1);
 
     f32x16 O[2];
     float s_down = 1.0f;
     if constexpr (!STATE) {
-      // P^T, 16 x 16 at a time: lane l has row 16 rt + l % 16 and columns 16 jt + 4 (l / 16) .. + 3.
+      // P^T, 16 x 16 at a time: lane l has row 16 rt + l % 16 and columns 16 jt + 4 (l / 16) .. + 3. Every wavefront makes all four
+      // tiles of its rows (the last one needs them all): without branches the rest can be laid under the next product.
       const int l16 = lane & 15, q4 = lane >> 4;
-#pragma unroll
-      for (int half = 0; half < (NW == 4 ? 1 : 2); ++half) {
-        const int rt = NW == 4 ? wave : half ? 3 - wave : wave;
-        const int row = 16 * rt + l16;
-        u32x4 qf[DK / 32];
+      int rt, row;
+      f32x4 x[4];
+      float row_scale, mx, p_up;
+      f32x4 diagonal;
+      auto make_p = [&](int which) __attribute__((always_inline)) {
+        rt = which, row = 16 * rt + l16;
         const uint32_t q_at = place(L::kQ + row_part<DK>(row, q4)), k_at = place(L::kK + row_part<DK>(l16, q4));
+        u32x4 qf[DK / 32];
 #pragma unroll
         for (int kk = 0; kk < DK / 32; ++kk) qf[kk] = read(q_at ^ (kk << 6));
-        const double ci = cum[row];
-        float x[4][4], mx = 0.0f;
+        // Weights: within the diagonal tile exp(c_i - c_j), left of it the product of what lies before and behind the tile's first row.
+        const float2 ci = since[row];
+        row_scale = a.scale * fast_exp2(ci.x + ci.y);
 #pragma unroll
-        for (int jt = 0; jt < 4; ++jt) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[jt][e] = 0.0f;
-          if (jt > rt) continue;
-          f32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-          for (int kk = 0; kk < DK / 32; ++kk) acc = mfma16x32<DT>(read((k_at ^ (kk << 6)) + jt * (32 * DK)), qf[kk], acc);
-          mfma_settle(acc);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = 16 * jt + 4 * q4 + e;
-            const float w = fast_exp2(float(ci - cum[j]));
-            x[jt][e] = j <= row ? acc[e] * w : 0.0f;
-            mx = fmaxf(mx, fabsf(x[jt][e]));
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float2 cj = since[16 * rt + 4 * q4 + e];
+          diagonal[e] = a.scale * fast_exp2((ci.x - cj.x) + (ci.y - cj.y));
         }
+        mx = 0.0f;
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt) x[jt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int kk = 0; kk < DK / 32; ++kk)
+#pragma unroll
+          for (int jt = 0; jt < 4; ++jt) x[jt] = mfma16x32<DT>(read((k_at ^ (kk << 6)) + jt * (32 * DK)), qf[kk], x[jt]);
+      };
+      auto weigh_p = [&](int jt) __attribute__((always_inline)) {
+        const f32x4 before = *reinterpret_cast<const f32x4*>(colf + 64 * rt + 16 * jt + 4 * q4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float y = x[jt][e] * (jt == rt ? diagonal[e] : row_scale * before[e]);
+          asm("" : "+v"(y));  // (left alone the compiler branches around the work of each masked weight)
+          x[jt][e] = 16 * jt + 4 * q4 + e <= row ? y : 0.0f;
+          mx = fmaxf(mx, fabsf(x[jt][e]));
+        }
+      };
+      auto scale_p = [&]() __attribute__((always_inline)) {
         if constexpr (DT == ESP_F16) {
           mx = fmaxf(mx, __shfl_xor(mx, 16));
           mx = fmaxf(mx, __shfl_xor(mx, 32));
-          float up, down;
-          scale_for(mx, kOutputScale, up, down);
-#pragma unroll
-          for (int jt = 0; jt < 4; ++jt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[jt][e] *= up;
-          if (q4 == 0) pinv[row] = down;
+          float down;
+          scale_for(mx, kOutputScale, p_up, down);
+          pinv[row] = down;  // (four lanes with the same)
         }
+      };
+      auto put_p = [&](int jt) __attribute__((always_inline)) {
+        if constexpr (DT == ESP_F16) x[jt] *= p_up;
+        const uint32_t w0 = pack2<DT>(x[jt][0], x[jt][1]), w1 = pack2<DT>(x[jt][2], x[jt][3]);
+        const uint32_t r0 = pack2<DT>(x[jt][0] - unpack_lo<DT>(w0), x[jt][1] - unpack_hi<DT>(w0));
+        const uint32_t r1 = pack2<DT>(x[jt][2] - unpack_lo<DT>(w1), x[jt][3] - unpack_hi<DT>(w1));
+        // Rows 0 .. 31 have no place for columns 32 .. 63, all of them zeros.
+        const bool real = jt <= (rt | 1);
+        const uint32_t to = base + uint32_t(real ? L::kP + p_part(row, 2 * jt + (q4 >> 1)) + 8 * (q4 & 1) : L::kNone + 8 * lane);
+        *reinterpret_cast<lds_u32x2_out*>(to) = u32x2{w0, w1};
+        *reinterpret_cast<lds_u32x2_out*>(to + (real ? kPBytes : 0)) = u32x2{r0, r1};
+      };
+      if constexpr (NW == 2) {
+        make_p(3 - wave);
 #pragma unroll
-        for (int jt = 0; jt < 4; ++jt) {
-          if (jt > (rt | 1)) continue;  // (the product reads columns in groups of 32)
-          const uint32_t w0 = pack2<DT>(x[jt][0], x[jt][1]), w1 = pack2<DT>(x[jt][2], x[jt][3]);
-          const uint32_t r0 = pack2<DT>(x[jt][0] - unpack_lo<DT>(w0), x[jt][1] - unpack_hi<DT>(w0));
-          const uint32_t r1 = pack2<DT>(x[jt][2] - unpack_lo<DT>(w1), x[jt][3] - unpack_hi<DT>(w1));
-          const int to = L::kP + p_part(row, 2 * jt + (q4 >> 1)) + 8 * (q4 & 1);
-          *reinterpret_cast<u32x2*>(lds + to) = u32x2{w0, w1};
-          *reinterpret_cast<u32x2*>(lds + to + kPBytes) = u32x2{r0, r1};
-        }
+        for (int jt = 0; jt < 4; ++jt) weigh_p(jt);
+        scale_p();
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt) put_p(jt);
       }
-      // (Q S)^T
+      make_p(wave);      // (Q S)^T, a step of 16 dims at a time; the next step's part of S is split, and P's weights are worked out, under the products.
       O[0] = f32x16{};
       O[1] = f32x16{};
       float s_up = 1.0f;
       if constexpr (DT == ESP_F16) {
-        float mx = 0.0f;
+        float sx = 0.0f;
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fabsf(S[t][e]));
-        if (__builtin_expect(__any(mx == INFINITY), 0)) {  // infinities are not what the others are scaled by
-          mx = 0.0f;
+          for (int e = 0; e < 16; ++e) sx = fmaxf(sx, fabsf(S[t][e]));
+        if (__builtin_expect(__any(sx == INFINITY), 0)) {  // infinities are not what the others are scaled by
+          sx = 0.0f;
 #pragma unroll
           for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fabsf(S[t][e]) < INFINITY ? fmaxf(mx, fabsf(S[t][e])) : mx;
+            for (int e = 0; e < 16; ++e) sx = fabsf(S[t][e]) < INFINITY ? fmaxf(sx, fabsf(S[t][e])) : sx;
         }
+        sx = wave_max(sx);
+        scale_for(sx, kOutputScale, s_up, s_down);
 #pragma unroll
-        for (int x = 1; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-        scale_for(mx, kOutputScale, s_up, s_down);
+        for (int jt = 0; jt < 4; ++jt) mfma_settle(x[jt]);
       }
       const uint32_t q_at = place(L::kQ + row_part<DK>(l32, hb));
+      constexpr int NS = DK / 16, PER = 8 / NS;  // steps; of the eight pieces of P's work how many go with each
+      u32x4 sp[2][2], q[2][2];
+      auto step_in = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
-      for (int ks = 0; ks < DK / 16; ++ks) {
-        float x[8];
+        for (int r = 0; r < 2; ++r) q[ks & 1][r] = read((q_at ^ (ks << 5)) + r * (64 * DK));
+      };
+      auto step_split = [&](int ks) __attribute__((always_inline)) {
+        float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = DT == ESP_F16 ? S[ks >> 1][8 * (ks & 1) + e] * s_up : S[ks >> 1][8 * (ks & 1) + e];
-        u32x4 sp[2];
-        split8<DT, 2>(x, sp);
+        for (int e = 0; e < 8; ++e) y[e] = S[ks >> 1][8 * (ks & 1) + e];
+        split8<DT, 2>(y, s_up, sp[ks & 1]);
+      };
+      step_in(0);
+      step_split(0);
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
-          const u32x4 q = read((q_at ^ (ks << 5)) + rt * (64 * DK));
-          O[rt] = mfma32x16<DT>(sp[0], q, O[rt]);
-          O[rt] = mfma32x16<DT>(sp[1], q, O[rt]);
+      for (int ks = 0; ks < NS; ++ks) {
+        if (ks + 1 < NS) step_in(ks + 1);
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) O[r] = mfma32x16<DT>(sp[ks & 1][v], q[ks & 1][r], O[r]);
+        if (ks + 1 < NS) step_split(ks + 1);
+#pragma unroll
+        for (int y = ks * PER; y < (ks + 1) * PER; ++y) {
+          if (y < 4) weigh_p(y);
+          if (y == 3) scale_p();
+          if (y >= 4) put_p(y - 4);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 16, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-      }
-      if (c + 1 < n_chunks) fetch(c + 1);
-      __syncthreads();  // P is there, and nobody reads Q and K any more
-    }
-    u32x4 vr[4];
+      }      if (c + 1 < n_chunks) fetch_all(c + 1);      lds_barrier();  // P is there, and nobody reads Q and K any more
+    }    u32x4 vr[4];
     auto read_v = [&] {
       const uint32_t v_at = place(L::kVT + col_part(32 * wave + l32, hb));
 #pragma unroll
@@ -457,7 +589,7 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) nf = fmaf(unpack_lo<DT>(vr[ks][e]), 0.0f, fmaf(unpack_hi<DT>(vr[ks][e]), 0.0f, nf));
+        for (int e = 0; e < 4; ++e) nf = times_zero2<DT>(vr[ks][e], nf);
       const bool odd = __any(nf != 0.0f);
       if (__builtin_expect(odd, 0)) {
         constexpr uint32_t ex = DT == ESP_F16 ? 0x7c00u : 0x7f80u;
@@ -468,27 +600,42 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
             const uint32_t w = vr[ks][e];
             vr[ks][e] = w & (((w & ex) == ex ? 0u : 0xffffu) | ((w >> 16 & ex) == ex ? 0u : 0xffff0000u));
           }
-      }
+      }      const uint32_t p_at[2] = {place(L::kP + p_part(l32, hb)), place(L::kP + p_part(32 + l32, hb))};
+      u32x4 pq[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pq[i] = read(p_at[i & 1] + (i >> 1) * kPBytes);
+      settle(O);
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt) {
-        const int row = 32 * rt + l32;
-        mfma_settle(O[rt]);
-        float f = rowf[row];
+        float f = rowf[32 * rt + l32];
         if constexpr (DT == ESP_F16) {
-          const float d = pinv[row];  // (a power of two)
           f *= s_down;
           O[rt] *= f;
-          O[rt] *= 1.0f / d;
+          O[rt] *= 1.0f / pinv[32 * rt + l32];  // (a power of two)
         } else {
           O[rt] *= f;
         }
-        const uint32_t p_at = place(L::kP + p_part(row, hb));
+      }
+      // Twelve products: of both halves of the rows in turn as long as there are two.
+      auto which = [](int i) { return i < 8 ? i >> 2 : 2 + ((i - 8) >> 1); };   // 16 columns
+      auto of_rows = [](int i) { return i < 8 ? i & 1 : 1; };
+      auto p_in = [&](int i) {
+        const int v = i < 8 ? (i >> 1) & 1 : i & 1;
+        return read((p_at[of_rows(i)] ^ (which(i) << 5)) + v * kPBytes);
+      };
 #pragma unroll
-        for (int ks = 0; ks < 2 + 2 * rt; ++ks) {
-          O[rt] = mfma32x16<DT>(vr[ks], read(p_at ^ (ks << 5)), O[rt]);
-          O[rt] = mfma32x16<DT>(vr[ks], read((p_at ^ (ks << 5)) + kPBytes), O[rt]);
+      for (int i = 0; i < 12; ++i) {
+        if (i % 4 == 0 && i < 8) {
+#pragma unroll
+          for (int y = i + 4; y < i + 8; ++y) pq[y & 7] = p_in(y);
         }
-        mfma_settle(O[rt]);
+        O[of_rows(i)] = mfma32x16<DT>(vr[which(i)], pq[i & 7], O[of_rows(i)]);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      settle(O);
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) {
+        const int row = 32 * rt + l32;
         if (__builtin_expect(odd, 0)) {
           // Rows 8 (e / 4) + 4 hb + e % 4 of the wavefront's part of V^T: their turns differ by constants.
 #pragma unroll 1
@@ -504,9 +651,10 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
             }
           }
         }
-        O[rt] *= DT == ESP_F16 ? pinv[row] * a.scale : a.scale;
+        if constexpr (DT == ESP_F16) O[rt] *= pinv[row];
       }
-      if (__builtin_expect(odd, 0)) read_v();
+      if (__builtin_expect(odd, 0)) read_v();      char* const o0 = reinterpret_cast<char*>(a.O + (size_t(tile.row0) + 64 * size_t(c)) * a.o_ld + dv0 + 32 * wave);
+      const uint32_t at_o = uint32_t(lane >> 2) * uint32_t(2 * a.o_ld) + 16 * (lane & 3);
       // Through LDS, where Q and K were, a wavefront's 64 rows of 64 bytes each; 16-byte parts turned by the row.
       char* const mine = lds + L::kQ + wave * 4096;
       auto part_at = [&](int r, int p) { return mine + r * 64 + ((p ^ ((r >> 2) & 3)) << 4); };
@@ -522,10 +670,9 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
       for (int i = 0; i < 4; ++i) {
         const int r = 16 * i + (lane >> 2), p = lane & 3;
         const u32x4 x = *reinterpret_cast<const u32x4*>(part_at(r, p));
-        if (r < n) *reinterpret_cast<u32x4*>(a.O + size_t(tile.row0 + 64 * c + r) * a.o_ld + dv0 + 32 * wave + 8 * p) = x;
+        if (r < n) *reinterpret_cast<u32x4*>(o0 + i * (32 * size_t(a.o_ld)) + at_o) = x;
       }
-    }
-    // S = exp(C) S + K^T V'. (The state behind the segment is of use only where somebody reads it.)
+    }    // S = exp(C) S + K^T V'. (The state behind the segment is of use only where somebody reads it.)
     if (STATE || c + 1 < n_chunks || tile.dst >= 0) {
       const float f = *total;
       const uint32_t k_at = place(L::kKT + col_part(swap23(l32), hb));
@@ -554,43 +701,58 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
         for (int ks = 0; ks < 4; ++ks) {
           float x[8];
           weighted(ks, x);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= up;
-          split8<DT, NV>(x, vs[ks]);
-          __builtin_amdgcn_sched_barrier(0);
+          split8<DT, NV>(x, up, vs[ks]);
         }
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          f32x16 d{};
+        f32x16 d[2];
+        auto product = [&](int t) __attribute__((always_inline)) {
+          d[t & 1] = f32x16{};
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
             const u32x4 k = read((k_at ^ (ks << 5)) + t * 4096);
 #pragma unroll
-            for (int v = 0; v < NV; ++v) d = mfma32x16<DT>(k, vs[ks][v], d);
+            for (int v = 0; v < NV; ++v) d[t & 1] = mfma32x16<DT>(k, vs[ks][v], d[t & 1]);
           }
-          mfma_settle(d);
+        };
+        product(0);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) S[t][e] = __builtin_fmaf(d[e], down, S[t][e] * f);
+        for (int t = 0; t < KT; ++t) {
+          if (t + 1 < KT) product(t + 1);
+          mfma_settle(d[t & 1]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) S[t][e] = __builtin_fmaf(d[t & 1][e], down, S[t][e] * f);
         }
       } else {
 #pragma unroll
         for (int t = 0; t < KT; ++t) S[t] *= f;
+        // The next 16 rows' values are weighed and split under the products of these.
+        u32x4 vs[2][NV], k[2][KT];
+        auto step_in = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
+          for (int t = 0; t < KT; ++t) k[ks & 1][t] = read((k_at ^ (ks << 5)) + t * 4096);
+        };
+        auto step_split = [&](int ks) __attribute__((always_inline)) {
           float x[8];
           weighted(ks, x);
-          u32x4 vs[NV];
-          split8<DT, NV>(x, vs);
+          split8<DT, NV>(x, 1.0f, vs[ks & 1]);
+        };
+        step_in(0);
+        step_split(0);
 #pragma unroll
-          for (int t = 0; t < KT; ++t) {
-            const u32x4 k = read((k_at ^ (ks << 5)) + t * 4096);
+        for (int ks = 0; ks < 4; ++ks) {
+          if (ks < 3) step_in(ks + 1);
 #pragma unroll
-            for (int v = 0; v < NV; ++v) S[t] = mfma32x16<DT>(k, vs[v], S[t]);
+          for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int t = 0; t < KT; ++t) S[t] = mfma32x16<DT>(k[ks & 1][t], vs[ks & 1][v], S[t]);
+          if (ks < 3) step_split(ks + 1);
+#pragma unroll
+          for (int y = 0; y < NV * KT; ++y) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 84 / (NV * KT), 0);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int t = 0; t < KT; ++t) mfma_settle(S[t]);
+        settle(S);
       }
     }
   }
