@@ -176,7 +176,8 @@ __device__ __forceinline__ void split8(const float (&x)[8], float by, u32x4 (&ou
     float lo = x[2 * e], hi = x[2 * e + 1];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const uint32_t w = pack2<DT>(lo, hi);
+      uint32_t w = pack2<DT>(lo, hi);
+      if (n + 1 < N) asm("" : "+v"(w));  // (left alone the compiler converts the lower one once more instead of shifting it out)
       out[n][e] = w;
       if (n + 1 < N) {
         lo -= unpack_lo<DT>(w);
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
   const int n_chunks = (tile.rows + 63) >> 6;
   const char *from_kq[NI], *from_v;  // the lane's first row of each piece in the next chunk
   uint32_t ld_kq[NI];
-  const uint32_t ld_v = uint32_t(2 * a.v_ld);
+  uint32_t ld_v = uint32_t(2 * a.v_ld);
 #pragma unroll
   for (int p = 0; p < NI; ++p) {
     const int it = tid + T * p;
@@ -338,24 +339,25 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
     if (p < NI) kq[p < NI ? p : 0][i] = *reinterpret_cast<const u32x4*>(from_kq[p < NI ? p : 0] + size_t(i) * ld_kq[p < NI ? p : 0]);
     else vv[i] = *reinterpret_cast<const u32x4*>(from_v + size_t(i) * ld_v);
   };
-  auto fetch_last = [&](int n) __attribute__((always_inline)) {
+  // The n < 64 rows that start `ahead` rows behind the pointers' chunk.
+  auto fetch_last = [&](int n, int ahead) __attribute__((always_inline)) {
 #pragma unroll
     for (int p = 0; p < NI; ++p) {
       const int r = 4 * (((tid + T * p) % (2 * DK)) / kParts);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) kq[p][i] = *reinterpret_cast<const u32x4*>(from_kq[p] + int64_t(min(r + i, n - 1) - r) * int64_t(ld_kq[p]));
+      for (int i = 0; i < 4; ++i) kq[p][i] = *reinterpret_cast<const u32x4*>(from_kq[p] + int64_t(ahead + min(r + i, n - 1) - r) * int64_t(ld_kq[p]));
     }
     const int r = 4 * (tid / vParts);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vv[i] = *reinterpret_cast<const u32x4*>(from_v + int64_t(min(r + i, n - 1) - r) * int64_t(ld_v));
+    for (int i = 0; i < 4; ++i) vv[i] = *reinterpret_cast<const u32x4*>(from_v + int64_t(ahead + min(r + i, n - 1) - r) * int64_t(ld_v));
   };
   auto fetch_decay = [&](int c) __attribute__((always_inline)) {  // (as it is: working on it here would be a wait)
     if (a.decay_ld) g_row = a.decay[(size_t(tile.row0) + min(64 * c + lane, tile.rows - 1)) * a.decay_ld + h];
   };
-  auto fetch_on = [&]() __attribute__((always_inline)) {
+  auto fetch_on = [&](uint32_t rows) __attribute__((always_inline)) {
 #pragma unroll
-    for (int p = 0; p < NI; ++p) from_kq[p] += 64 * size_t(ld_kq[p]);
-    from_v += 64 * size_t(ld_v);
+    for (int p = 0; p < NI; ++p) from_kq[p] += size_t(rows) * ld_kq[p];
+    from_v += size_t(rows) * ld_v;
   };
   auto fetch_all = [&](int c) __attribute__((always_inline)) {
     const int n = tile.rows - 64 * c;
@@ -365,9 +367,8 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
 #pragma unroll
         for (int i = 0; i < 4; ++i) fetch_row(p, i);
     } else {
-      fetch_last(n);
+      fetch_last(n, 0);
     }
-    fetch_on();
     fetch_decay(c);
   };
   // Rows behind the segment's last are zeros in K and V.
@@ -404,9 +405,20 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
   };
 
   if (n_chunks > 0) fetch_all(0);
+  if (!STATE && tile.rows < 64) {  // no whole chunk that could be read again: the first row stands for it
+#pragma unroll
+    for (int p = 0; p < NI; ++p) {
+      from_kq[p] -= size_t(4 * (((tid + T * p) % (2 * DK)) / kParts)) * ld_kq[p];
+      ld_kq[p] = 0;
+    }
+    from_v -= size_t(4 * (tid / vParts)) * ld_v;
+    ld_v = 0;
+  }
   double so_far = 0.0;
   for (int c = 0; c < n_chunks; ++c) {
-    const int n = min(64, tile.rows - 64 * c);    if (c > 0) lds_barrier();  // everybody is done with the chunk in front of this one    if (n < 64) {
+    const int n = min(64, tile.rows - 64 * c);
+    if (c > 0) lds_barrier();  // everybody is done with the chunk in front of this one
+    if (n < 64) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int it = tid + T * i;
@@ -423,7 +435,8 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
       if (!STATE) put_rows(kq[i], isK ? L::kK : L::kQ, b / kParts, b % kParts);
       if (isK) put_columns(kq[i], L::kKT, b / kParts, b % kParts);
     }
-    put_columns(vv, L::kVT, tid / vParts, tid % vParts);    // What the chunk's decays come to. Of a head's own they are those of the chunk before, but for the first and the last.
+    put_columns(vv, L::kVT, tid / vParts, tid % vParts);
+    // What the chunk's decays come to. Of a head's own they are those of the chunk before, but for the first and the last.
     if (a.decay_ld || c == 0 || n < 64) {
       const double s = a.decay_ld ? scan64(lane < n ? double(decay_log2(g_row)) : 0.0) : double(g_const) * min(lane + 1, n);
       const double cl = lane_of(s, 63);
@@ -446,7 +459,11 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
     } else if (STATE) {
       so_far += double(g_const) * 64.0;
     }
-    lds_barrier();    if (STATE && c + 1 < n_chunks) fetch_all(c + 1);
+    lds_barrier();
+    if (STATE && c + 1 < n_chunks) {
+      fetch_on(64);
+      fetch_all(c + 1);
+    }
 
     f32x16 O[2];
     float s_down = 1.0f;
@@ -501,7 +518,8 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
       };
       auto put_p = [&](int jt) __attribute__((always_inline)) {
         if constexpr (DT == ESP_F16) x[jt] *= p_up;
-        const uint32_t w0 = pack2<DT>(x[jt][0], x[jt][1]), w1 = pack2<DT>(x[jt][2], x[jt][3]);
+        uint32_t w0 = pack2<DT>(x[jt][0], x[jt][1]), w1 = pack2<DT>(x[jt][2], x[jt][3]);
+        asm("" : "+v"(w0), "+v"(w1));
         const uint32_t r0 = pack2<DT>(x[jt][0] - unpack_lo<DT>(w0), x[jt][1] - unpack_hi<DT>(w0));
         const uint32_t r1 = pack2<DT>(x[jt][2] - unpack_lo<DT>(w1), x[jt][3] - unpack_hi<DT>(w1));
         // Rows 0 .. 31 have no place for columns 32 .. 63, all of them zeros.
@@ -518,7 +536,8 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
 #pragma unroll
         for (int jt = 0; jt < 4; ++jt) put_p(jt);
       }
-      make_p(wave);      // (Q S)^T, a step of 16 dims at a time; the next step's part of S is split, and P's weights are worked out, under the products.
+      make_p(wave);
+      // (Q S)^T, a step of 16 dims at a time; the next step's part of S is split, and P's weights are worked out, under the products.
       O[0] = f32x16{};
       O[1] = f32x16{};
       float s_up = 1.0f;
@@ -553,11 +572,18 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
         for (int e = 0; e < 8; ++e) y[e] = S[ks >> 1][8 * (ks & 1) + e];
         split8<DT, 2>(y, s_up, sp[ks & 1]);
       };
+      // The next chunk's rows are asked for here, a few a step: all at once they stand in line for a quarter of the chunk's time. Without
+      // another whole chunk it is the last whole one's rows once more, and the rest of the segment's are asked for behind.
+      const bool next_whole = tile.rows - 64 * (c + 1) >= 64;
+      fetch_on(next_whole ? 64 : 0);
+      constexpr int LOADS = 4 * (NI + 1), LPS = (LOADS + NS - 1) / NS;
       step_in(0);
       step_split(0);
 #pragma unroll
       for (int ks = 0; ks < NS; ++ks) {
         if (ks + 1 < NS) step_in(ks + 1);
+#pragma unroll
+        for (int y = ks * LPS; y < (ks + 1) * LPS && y < LOADS; ++y) fetch_row(y >> 2, y & 3);
 #pragma unroll
         for (int v = 0; v < 2; ++v)
 #pragma unroll
@@ -575,8 +601,14 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
           __builtin_amdgcn_sched_group_barrier(0x002, 16, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-      }      if (c + 1 < n_chunks) fetch_all(c + 1);      lds_barrier();  // P is there, and nobody reads Q and K any more
-    }    u32x4 vr[4];
+      }
+      if (c + 1 < n_chunks && !next_whole) {
+        fetch_last(tile.rows - 64 * (c + 1), 64);
+      }
+      if (c + 1 < n_chunks) fetch_decay(c + 1);
+      lds_barrier();  // P is there, and nobody reads Q and K any more
+    }
+    u32x4 vr[4];
     auto read_v = [&] {
       const uint32_t v_at = place(L::kVT + col_part(32 * wave + l32, hb));
 #pragma unroll
@@ -600,7 +632,8 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
             const uint32_t w = vr[ks][e];
             vr[ks][e] = w & (((w & ex) == ex ? 0u : 0xffffu) | ((w >> 16 & ex) == ex ? 0u : 0xffff0000u));
           }
-      }      const uint32_t p_at[2] = {place(L::kP + p_part(l32, hb)), place(L::kP + p_part(32 + l32, hb))};
+      }
+      const uint32_t p_at[2] = {place(L::kP + p_part(l32, hb)), place(L::kP + p_part(32 + l32, hb))};
       u32x4 pq[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) pq[i] = read(p_at[i & 1] + (i >> 1) * kPBytes);
@@ -653,7 +686,8 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
         }
         if constexpr (DT == ESP_F16) O[rt] *= pinv[row];
       }
-      if (__builtin_expect(odd, 0)) read_v();      char* const o0 = reinterpret_cast<char*>(a.O + (size_t(tile.row0) + 64 * size_t(c)) * a.o_ld + dv0 + 32 * wave);
+      if (__builtin_expect(odd, 0)) read_v();
+      char* const o0 = reinterpret_cast<char*>(a.O + (size_t(tile.row0) + 64 * size_t(c)) * a.o_ld + dv0 + 32 * wave);
       const uint32_t at_o = uint32_t(lane >> 2) * uint32_t(2 * a.o_ld) + 16 * (lane & 3);
       // Through LDS, where Q and K were, a wavefront's 64 rows of 64 bytes each; 16-byte parts turned by the row.
       char* const mine = lds + L::kQ + wave * 4096;
@@ -672,7 +706,8 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
         const u32x4 x = *reinterpret_cast<const u32x4*>(part_at(r, p));
         if (r < n) *reinterpret_cast<u32x4*>(o0 + i * (32 * size_t(a.o_ld)) + at_o) = x;
       }
-    }    // S = exp(C) S + K^T V'. (The state behind the segment is of use only where somebody reads it.)
+    }
+    // S = exp(C) S + K^T V'. (The state behind the segment is of use only where somebody reads it.)
     if (STATE || c + 1 < n_chunks || tile.dst >= 0) {
       const float f = *total;
       const uint32_t k_at = place(L::kKT + col_part(swap23(l32), hb));
