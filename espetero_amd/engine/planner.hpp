@@ -708,9 +708,13 @@ struct LinearPlan {
   int few = 0, parts = 0;
 };
 
-// Sequences that esp_linear_attn's chunked kernel takes are cut into segments where a pass has fewer workgroups than the chip holds. A
-// segment's state is made by a launch in front, which reads K and V once more; what comes of that is worked out in chunks of
-// the kernel, for the segments of every length: the longest tile against an even share of all of them.
+// Sequences that esp_linear_attn's chunked kernel takes are cut into segments where a pass has fewer workgroups than the chip holds, or
+// longer ones than its share. A segment's state is made by a launch in front, which reads K and V once more. What comes of a cut
+// is worked out by handing its workgroups to the chip's slots, two to a compute unit, in the order of the tiles; all figures in
+// microseconds, of heads of 128 x 128 (64 x 128 take a tenth less): a chunk 4.5 alone on a compute unit, 6.9 beside another (2.5 and 3.6
+// where only the state is made), 7 for a workgroup's set-up and end, 0.9 for a record summed up, 3 for the launch in front. (One prompt of 2000
+// rows, 32 heads, in segments of 2, 4, 8, 16 and 32 chunks: 55, 45, 63, 111 and 146 us; 16000 rows, 32 heads of 64 x 128, 4, 8, 16, 32: 229,
+// 165, 156, 197; four of 2048 rows, 40 heads, 4, 8, 11, 16, 32: 168, 152, 146, 183, 154.)
 inline void plan_linear(LinearPlan& plan, const esp_linear_params& p, const esp_linear_seq* seqs, int n_seqs, int workgroups) {
   plan.tiles.clear();
   plan.few = plan.parts = 0;
@@ -727,33 +731,62 @@ inline void plan_linear(LinearPlan& plan, const esp_linear_params& p, const esp_
   }
   plan.few = int(plan.tiles.size());
   auto chunks = [&](int i) { return (seqs[i].rows + esp::kLinearChunk - 1) / esp::kLinearChunk; };
-  const double groups = double(p.H) * (p.dv / esp::linear_cols(p.dv)), slots = std::max(1, workgroups);
-  // Of a cut into segments of `most` chunks: a workgroup's set-up 1, a chunk 1, or half of one where only the state is made; a record read
-  // half a chunk, the launch in front 4.
-  auto cost = [&](int most) {
-    double all = 0, state = 0, top = 0, top_state = 0;
-    for (int i : many) {
-      const int c = chunks(i), n = (c + most - 1) / most, each = (c + n - 1) / n;
-      all += c + n + 0.25 * n * (n - 1);
-      top = std::max(top, each + 1 + 0.5 * (n - 1));
-      if (n > 1) {
-        state += 0.5 * (c - each) + (n - 1);
-        top_state = std::max(top_state, 0.5 * each + 1);
+  const long long groups = (long long)p.H * (p.dv / esp::linear_cols(p.dv));
+  const int slots = std::max(2, workgroups);
+  struct Work {
+    int chunks, records;
+  };
+  using Free = std::pair<double, long long>;  // (when, how many slots)
+  auto finish = [&](const std::vector<Work>& work, double alone, double shared) {
+    const bool few = groups * (long long)work.size() <= slots / 2;
+    std::priority_queue<Free, std::vector<Free>, std::greater<Free>> free_at;
+    free_at.push({0.0, few ? slots / 2 : slots});
+    double end = 0;
+    for (const Work& w : work) {
+      const double cost = 7 + 0.9 * w.records + w.chunks * (few ? alone : shared);
+      for (long long left = groups; left > 0;) {
+        const Free f = free_at.top();
+        const long long take = std::min(left, f.second);
+        free_at.pop();
+        if (f.second > take) free_at.push({f.first, f.second - take});
+        free_at.push({f.first + cost, take});
+        end = std::max(end, f.first + cost);
+        left -= take;
       }
     }
-    const double t = std::max(top, all * groups / slots);
-    return state == 0 ? t : t + std::max(top_state, state * groups / slots) + 4;
+    return end;
+  };
+  // Segments of at most `most` chunks: how many of a sequence of c, each of how many.
+  auto cut = [](int c, int most) {
+    const int n = (c + most - 1) / most, each = (c + n - 1) / n;
+    return std::pair<int, int>{(c + each - 1) / each, each};
+  };
+  std::vector<Work> all, states;
+  auto cost = [&](int most) {
+    all.clear();
+    states.clear();
+    for (int i : many) {
+      const auto [n, each] = cut(chunks(i), most);
+      for (int k = 0; k < n; ++k) {
+        all.push_back({std::min(each, chunks(i) - k * each), k});
+        if (k + 1 < n) states.push_back({each, 0});
+      }
+    }
+    return finish(all, 4.5, 6.9) + (states.empty() ? 0.0 : 3 + finish(states, 2.5, 3.6));
   };
   int most = std::max(1, longest);
-  double best = cost(most);
-  for (int n = 2; n <= 64 && (longest + n - 1) / n >= 2; ++n) {
-    const int m = (longest + n - 1) / n;
-    const double t = cost(m);
-    if (t < best) best = t, most = m;
-  }
+  double best = many.empty() ? 0.0 : cost(most);
+  // Not where whole sequences fill the slots several times over: the longest then ends beside the others.
+  if (groups * (long long)many.size() < 4LL * slots)
+    for (const int n : {2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64}) {
+      if (n > longest) break;
+      const int m = (longest + n - 1) / n;
+      const double t = cost(m);
+      if (t < best) best = t, most = m;
+    }
   for (int i : many) {
     const esp_linear_seq& q = seqs[i];
-    const int c = chunks(i), n = (c + most - 1) / most, each = (c + n - 1) / n, real = (c + each - 1) / each;
+    const auto [real, each] = cut(chunks(i), most);
     for (int k = 0; k < real; ++k) {
       const int r0 = k * each * esp::kLinearChunk, r1 = std::min(q.rows, (k + 1) * each * esp::kLinearChunk);
       plan.tiles.push_back({q.base + r0, r1 - r0, q.src, k + 1 == real ? q.dst : -1, real > 1 ? plan.parts : -1, k, real - 1 - k, 0});
