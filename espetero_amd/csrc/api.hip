@@ -853,6 +853,14 @@ int esp_attn_shaped(const esp_attn_params* p, const esp_shape_params* shape, con
   a.cols = a.R * a.G;
   a.scale_log2 = shape->cap > 0.0f ? float(2.0 * double(p->scale) * 1.4426950408889634 / double(shape->cap)) : p->scale * esp::kLog2e;
   a.cap_log2 = shape->cap * esp::kLog2e;
+  if (shape->cap > 0.0f) {
+    constexpr double kTanh[5] = {0.9999985098838806, -0.33326974511146545, 0.13257454335689545, -0.050195250660181046, 0.013194181025028229};
+    const double z = double(p->scale) / double(shape->cap);
+    double power = double(p->scale) * 1.4426950408889634;
+    for (int i = 0; i < 5; ++i, power *= z * z) a.tanh_c[i] = float(kTanh[i] * power);
+    // (of caps so far from the scale that a coefficient leaves fp32 none)
+    a.tanh_below = z > 0x1p-13 && z < 0x1p10 && p->scale > 0x1p-16 && p->scale < 0x1p16 ? float(0.7 / z) : 0.0f;
+  }
   a.kv_base = p->kv_base;
   hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e = fam > 0 ? esp::launch_shaped_stream(p->dtype, p->head_dim, a, n_tiles, st) : esp::launch_shaped_tiled(p->dtype, p->head_dim, a, n_tiles, st);

@@ -6,15 +6,24 @@
 //   S^T[32 keys][32 rows] = K . Q^T      A = K from LDS, B = Q^T in registers
 //   P^T = exp2(shaped(S^T) - m)          registers; the D layout of S^T is the B layout of P^T
 //   O^T[head_dim][32 rows] += V^T . P^T  A = V^T from LDS
-// with v_mfma_f32_32x32x16 and P . V one stage behind S.
+// with v_mfma_f32_32x32x16. A turn has three stages in hand: the scores of stage h are made under the shaping of stage h - 1's and the
+// look for a new maximum, P . V of stage h - 2 under the exponentials of stage h - 1, so that matrix and vector units work beside each other
+// within a wavefront too. Turns that are not all of that - the ends of a range, masked stages, a new reference - run the three one by one.
 //
-// LDS: a ring of 4 stages of 32 keys, K and V^T, loaded straight from the pool (global_load_lds) two stages ahead: wavefronts 0 and 1 load the
-// two sub-blocks of K, 2 and 3 those of V^T. K: the 16-byte chunk c of row r lies at c ^ (pi(r) & 15), pi swapping bits 2 and 3; V^T: per
-// sub-block of 16 keys and group of 32 dims [half of the keys][32 dims][8 keys], the order in which the lanes of a P . V operand read
-// it. Neither side has bank conflicts. Nothing in the loop may load from memory but the stages (any such load's wait is a wait for them).
+// Scores: the bias is what the score product's accumulator starts from (without a cap; behind a cap it is the last step's addend). A cap
+// is tanh as an odd polynomial where all of a wavefront's scores of the stage are below 0.7 caps (six operations a score), else by an
+// exponential and a reciprocal (eleven). 2048 rows behind 8000 keys, 32 / 8 heads: ...
+//
+// LDS: a ring of 4 stages of 32 keys, K and V^T, loaded straight from the pool (global_load_lds): wavefronts 0 and 1 load the
+// two sub-blocks of K, three stages ahead of the scores, 2 and 3 those of V^T, three ahead of P . V. K: the 16-byte chunk c of row r lies at
+// c ^ (pi(r) & 15), pi swapping bits 2 and 3; V^T: per sub-block of 16 keys and group of 32 dims [half of the keys][32 dims][8 keys], the
+// order in which the lanes of a P . V operand read it. Neither side has bank conflicts. Nothing in the loop may load from memory but the
+// stages (any such load's wait is a wait for them).
 #include "lds_direct.hpp"
 #include "rows_out.hpp"
 #include "shaped_math.hpp"
+
+#include <type_traits>
 
 namespace esp {
 
@@ -38,9 +47,22 @@ __device__ __forceinline__ float max_halves(float x) {
   asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
   return fmaxf(x, y);
 }
+
+// The order of a block of N matrix instructions with operands from LDS two ahead: one, then V vector operations (exponentials among
+// them), and the operand of the one after the next.
+template <int N, int V>
+__device__ __forceinline__ void lay_out() {
+  __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+  for (int g = 0; g < N; ++g) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x402, V, 0);
+  }
+}
 }  // namespace
 
-template <int DT, int HD, bool CAP>
+template <int DT, int HD, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kernel(const ShapedArgs a) {
   using L = TiledLds<HD>;
   constexpr int NT = HD / 32, KS = HD / 16, RB = HD * 2, LOADS = L::kRun / 1024;
@@ -74,13 +96,15 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const u32x4*>(qp + 16 * ks);
     sight = shaped_sight(a, tile.r0 + pl.m, qpos, n_keys);
-    slope = a.slopes ? a.slopes[kvh * a.G + pl.hg] * kLog2e : 0.0f;
+    // In the units of the score that it is added to: the product's, or behind a cap log2 units.
+    slope = BIAS ? a.slopes[kvh * a.G + pl.hg] * (CAP ? kLog2e : kLog2e / a.scale_log2) : 0.0f;
   }
   // What some and what all of a set of rows see: of this wavefront's and of the tile's.
   struct Seen {
     int some_from, some_end, all_from, all_end;
   };
   Seen mine{}, whole{};
+  const int q_first = tree.P + rr0 + min(col0, cols_live - 1) / a.G;  // of this wavefront's rows
   if (a.spans) {
     auto reduce = [](Seen s, int lanes) {
       for (int x = 1; x < lanes; x <<= 1) {
@@ -119,7 +143,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
       v0 = (some_lo - s0) >> 5;
       v1 = (some_hi - s0 + 31) >> 5;
       f0 = (all_lo - s0 + 31) >> 5;
-      f1 = max(f0, (all_hi - s0) >> 5);
+      f1 = max(f0, ((BIAS ? min(all_hi, q_first + 1) : all_hi) - s0) >> 5);  // (behind a row's own key its bias falls again)
     }
   }
   if (n_st) {
@@ -145,7 +169,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   const char* const plane = reinterpret_cast<const char*>(a.pool + size_t(a.kv_base) + size_t(kvh) * head + (kind == 0 ? 0 : size_t(a.bt) * HD));
   const uint64_t block_bytes = uint64_t(a.Hkv) * head * 2;
   const char* next_from = nullptr;  // the run of the stage to be requested next
-  auto locate = [&](int id) {
+  auto locate = [&](int id) __attribute__((always_inline)) {
     // (t0 is a multiple of 16: a V^T sub-block starts as far behind its plane as the K row of its first token does)
     next_from = plane + uint64_t(uint32_t(id)) * block_bytes + uint32_t(next_t0 * (HD * 2));
   };
@@ -154,7 +178,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     for (int i = 0; i < LOADS; i += 4)
       load_to_lds16_x4(next_from + 1024 * i, turned(i), turned(i + 1), turned(i + 2), turned(i + 3), dst + uint32_t(h & (kRing - 1)) * L::kStage + 1024 * i);
   };
-  auto advance = [&] {
+  auto advance = [&]() __attribute__((always_inline)) {
     if (next_key + 32 <= last_sub) {
       next_key += 32;
       next_t0 += 32;
@@ -174,30 +198,112 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   float m_ref = -INFINITY, l_run = 0.0f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) acc[nt] = f32x16{};
-  u32x4 P[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+  // Scores and weights of the stage at work and of the one before, by the stage's parity.
+  f32x16 s[2] = {f32x16{}, f32x16{}};
+  u32x4 P[2][2] = {};
 
-  f32x16 s{};
-  // Matrix work of a stage: P . V of stage h - 1 and the scores of stage h, turn by turn, so that neither waits for its own last result;
-  // operands are read two ahead.
-  auto products = [&](int h, int next) __attribute__((always_inline)) {
-    u32x4 v[3], k[3];
+  // The bias of index e of this lane's half, linear in the key: right up to the row's own key.
+  auto bias_at = [&](int h) { return slope * float(s0 + 32 * h + 8 * hb - qpos); };
+  auto score_operand = [&](int h, int g) { return lds_read((k_at + uint32_t(h & (kRing - 1)) * L::kStage) ^ uint32_t(g << 5)); };
+  auto value_operand = [&](uint32_t va, int g) { return lds_read(va + (g / NT) * L::kRun + (g % NT) * 1024); };
+  auto values_of = [&](int h) {
+    uint32_t va = v_at + uint32_t(h & (kRing - 1)) * L::kStage;
+    asm("" : "+v"(va));  // one register, the operands' places as immediates
+    return va;
+  };
+  // S = K Q^T of stage h (+ bias / scale), operands read two ahead; `between` is work to be laid under it.
+  auto score = [&](int h, f32x16& to, auto between) __attribute__((always_inline)) {
+    u32x4 k[3];
     const uint32_t ka = k_at + uint32_t(h & (kRing - 1)) * L::kStage;
-    const uint32_t va = v_at + uint32_t((h - 1) & (kRing - 1)) * L::kStage;
-    auto fetch = [&](int g) {
-      k[g % 3] = lds_read(ka ^ uint32_t(g << 5));
-      v[g % 3] = lds_read(va + (g / NT) * L::kRun + (g % NT) * 1024);
-    };
-    s = f32x16{};
+    auto fetch = [&](int g) { k[g % 3] = lds_read(ka ^ uint32_t(g << 5)); };
     fetch(0);
     fetch(1);
+    if constexpr (BIAS && !CAP) {
+      const float b = bias_at(h);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) to[e] = __builtin_fmaf(slope, float(16 * (e >> 3) + (e & 7)), b);
+    } else {
+      to = f32x16{};
+    }
 #pragma unroll
     for (int g = 0; g < KS; ++g) {
       if (g + 2 < KS) fetch(g + 2);
-      s = mfma32x16<DT>(k[g % 3], qf[g], s);
-      acc[g % NT] = mfma32x16<DT>(v[g % 3], P[g / NT], acc[g % NT]);
-      if (g == KS / 2 - 1 && next >= 0) request(next);
-      if (g == KS / 2 && next >= 0) advance();
-      __builtin_amdgcn_sched_barrier(0);
+      to = mfma32x16<DT>(k[g % 3], qf[g], to);
+      between(g);
+      __builtin_amdgcn_sched_barrier(0x406);  // (vector and scalar work may cross; operands' reads and products keep their order)
+    }
+  };
+  // O^T += V^T P^T of stage h.
+  auto weigh = [&](int h, const u32x4 (&p)[2], auto between) __attribute__((always_inline)) {
+    u32x4 v[3];
+    const uint32_t va = values_of(h);
+    auto fetch = [&](int g) { v[g % 3] = value_operand(va, g); };
+    fetch(0);
+    fetch(1);
+#pragma unroll
+    for (int g = 0; g < 2 * NT; ++g) {
+      if (g + 2 < 2 * NT) fetch(g + 2);
+      acc[g % NT] = mfma32x16<DT>(v[g % 3], p[g / NT], acc[g % NT]);
+      between(g);
+      __builtin_amdgcn_sched_barrier(0x406);
+    }
+  };
+  // From products to scores in log2 units (BIAS without a cap: the bias is in already).
+  auto largest_size = [&](const f32x16& x) {
+    float m = fabsf(x[0]);
+#pragma unroll
+    for (int e = 1; e < 16; ++e) m = fmaxf(m, fabsf(x[e]));
+    return m;
+  };
+  auto shape_e = [&](float x, int e, float b, bool low) __attribute__((always_inline)) {
+    if constexpr (CAP) {
+      const float at = BIAS ? __builtin_fmaf(slope, float(16 * (e >> 3) + (e & 7)), b) : 0.0f;
+      if (low) {
+        const float u = x * x;
+        float p = __builtin_fmaf(u, a.tanh_c[4], a.tanh_c[3]);
+        p = __builtin_fmaf(u, p, a.tanh_c[2]);
+        p = __builtin_fmaf(u, p, a.tanh_c[1]);
+        p = __builtin_fmaf(u, p, a.tanh_c[0]);
+        return __builtin_fmaf(x, p, at);
+      }
+      const float r = __builtin_amdgcn_rcpf(fast_exp2(x * a.scale_log2) + 1.0f);
+      return __builtin_fmaf(-2.0f * a.cap_log2, r, a.cap_log2 + at);
+    } else {
+      return x;
+    }
+  };
+  // With a cap scores are in log2 units, else still in those of the products.
+  const float unit = CAP ? 1.0f : a.scale_log2;
+  auto exponentials = [&](const f32x16& x, u32x4 (&p)[2]) __attribute__((always_inline)) {
+    const float off = m_ref == -INFINITY ? 0.0f : m_ref;
+    float lx = 0.0f;
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = 8 * sb + 2 * e;
+        const float p0 = fast_exp2(CAP ? x[at] - off : __builtin_fmaf(x[at], unit, -off));
+        const float p1 = fast_exp2(CAP ? x[at + 1] - off : __builtin_fmaf(x[at + 1], unit, -off));
+        p[sb][e] = pack2<DT>(p0, p1);
+        (sb ? lx : l_run) = sum2<DT>(p[sb][e], sb ? lx : l_run);  // (the weights as the product takes them)
+      }
+    l_run += lx;
+  };
+  // A new reference where a score exceeds the old one by more than kSlack. What was weighed by the old one joins the accumulators
+  // first; then they go over to the new one.
+  auto move_reference = [&](float mx, bool up) __attribute__((always_inline)) {
+    const float c = m_ref == -INFINITY ? 0.0f : up ? fast_exp2(m_ref - mx) : 1.0f;
+    m_ref = up ? mx : m_ref;
+    l_run *= c;
+    return c;
+  };
+  auto follow_reference = [&](float c) __attribute__((always_inline)) {
+    // (0 where there was none: whatever the accumulators hold goes.)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      mfma_settle(acc[nt]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[nt][e] = c == 0.0f ? 0.0f : acc[nt][e] * c;
     }
   };
   // Lane l holds of S^T, at index 8 sb + i, key 16 sb + 8 hb + i of the stage.
@@ -233,7 +339,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     if (ln == 0) bad[2 * (uint32_t(h) & (kRing - 1)) + (wave & 1)] = any;
   };
   bool marked = false;
-  auto marks = [&](int h) {
+  auto marks = [&](int h, const u32x4 (&P)[2]) __attribute__((always_inline)) {
     const int ln = here(lane);
 #pragma unroll 1
     for (int w = 0; w < NT; ++w) {
@@ -262,9 +368,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     marked = true;
   };
 
-  constexpr int kAhead = 2;  // stages requested in front of the one at work
+  const int lead = kind == 0 ? 3 : 1;  // the stage requested in turn h, less h
   locate(block_id());
-  for (int h = 0; h < min(n_st, kAhead); ++h) {
+  for (int h = 0; h < min(n_st, lead); ++h) {
     request(h);
     advance();
     locate(block_id());
@@ -272,83 +378,117 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   // Q is waited for here, not at its first use in the loop: that wait would be on the counter of the stages on their way.
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
-  auto softmax = [&](int h) __attribute__((always_inline)) {
-    const float ago = float(s0 + 32 * h + 8 * hb - qpos);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = shaped_score<CAP>(a, s[e]) - slope * fabsf(ago + float(16 * (e >> 3) + (e & 7)));
-    if (uint32_t(h - f0) >= uint32_t(f1 - f0)) {
-      // The row sees the keys [from, from + n); index e of this lane's half is key 16 (e / 8) + e % 8 behind the first.
-      const int lo = max(rg.from, sight.from), n = max(0, min(rg.end, sight.end) - lo);
-      const int at = s0 + 32 * h + 8 * (here(lane) >> 5) - lo;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = uint32_t(at + 16 * (e >> 3) + (e & 7)) < uint32_t(n) ? s[e] : -INFINITY;
-    }
-    float mx = s[0];
-#pragma unroll
-    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-    mx = max_halves(mx);
-    const bool up = mx > m_ref + kSlack;  // from -inf on: the first key that the row sees
-    if (__builtin_expect(__any(up), 0)) {
-      const float c = up ? fast_exp2(m_ref - mx) : 1.0f;
-      const bool first = m_ref == -INFINITY;
-      m_ref = up ? mx : m_ref;
-      l_run *= c;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        mfma_settle(acc[nt]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[nt][e] = first ? 0.0f : acc[nt][e] * c;
-      }
-    }
-    const float off = m_ref == -INFINITY ? 0.0f : m_ref;
-    float lx = 0.0f;
-#pragma unroll
-    for (int sb = 0; sb < 2; ++sb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int at = 8 * sb + 2 * e;
-        const float p0 = fast_exp2(s[at] - off), p1 = fast_exp2(s[at + 1] - off);
-        P[sb][e] = pack2<DT>(p0, p1);
-        (sb ? lx : l_run) += p0 + p1;
-      }
-    l_run += lx;
-  };
   auto within = [](int h, int lo, int hi) { return uint32_t(h - lo) < uint32_t(hi - lo); };  // (lo <= hi)
-  for (int h = 0; h <= n_st; ++h) {
-    // All but the stage requested behind this one have landed for this wavefront.
-    if (h + 1 < n_st) {
+  const float low_below = CAP ? a.tanh_below : 0.0f;
+  // What a turn begins with. Behind barrier h, K of stage h and V of stage h - 1 have landed for everybody, and nobody reads K of stage h - 1
+  // or V of stage h - 3 any more, whose places in the ring the requests take. Returns the id of the block that is located at the turn's end.
+  auto begin = [&](int h, bool edges) __attribute__((always_inline)) {
+    const int behind = kind == 0 ? min(2, n_st - 1 - h) : min(1, n_st - h);  // stages requested behind the one that has to be there
+    if (behind >= 2) {
+      if constexpr (LOADS == 4) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    } else if (behind == 1) {
       if constexpr (LOADS == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
       else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    if (kind == 1 && h < n_st && !within(h, w0, w1)) {
-      mend(h);
+    if (edges && kind == 1 && h >= 1 && h <= n_st && !within(h - 1, w0, w1)) {
+      mend(h - 1);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    // Behind barrier h stage h has landed for everybody, and nobody reads K of stage h - 1 or V of stage h - 2 any more, whose place in
-    // the ring the request takes. On a wavefront's first stage P is zero and the V of "the stage before" whatever lies there, infinities and
-    // NaN among it: what that makes of the accumulators goes when a row's reference is first set. On its last turn the scores are not used.
-    const bool do_pv = within(h - 1, v0, v1), next_do = h + kAhead < n_st;
-    if (do_pv || within(h, v0, v1)) {
-      products(h, next_do ? h + kAhead : -1);
-    } else if (next_do) {
-      request(h + kAhead);
+    if (h + lead < n_st) {
+      request(h + lead);
       advance();
     }
-    const int id = block_id();
-    if (do_pv && !within(h - 1, w0, w1)) {
-      const int* b = bad + 2 * ((h - 1) & (kRing - 1));
-      if (__builtin_expect(__builtin_amdgcn_readfirstlane(b[0] | b[1]), 0)) marks(h - 1);
+    return block_id();
+  };
+  // A turn of whatever there is to do, one after the other: S and W are the scores and the weights of the last stage.
+  auto mixed_turn = [&](int h, f32x16& S, u32x4 (&W)[2]) __attribute__((always_inline)) {
+    const int id = begin(h, true);
+    // On a wavefront's first stage acc is whatever; it is cleared when a row's reference is first set.
+    if (within(h - 2, v0, v1)) weigh(h - 2, W, [](int) {});
+    if (within(h - 1, v0, v1)) {
+      mfma_settle(S);
+      const float b = bias_at(h - 1);
+      // (By the exponential whatever the scores: those of keys that a row does not see may be anything, and choose nothing.)
+      const int lo = max(rg.from, sight.from), n = max(0, min(rg.end, sight.end) - lo);
+      const int at0 = s0 + 32 * (h - 1) + 8 * (here(lane) >> 5), at = at0 - lo;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int k = 16 * (e >> 3) + (e & 7);
+        float x = shape_e(S[e], e, b, false);
+        if constexpr (BIAS) x -= 2.0f * slope * fmaxf(float(at0 + k - qpos), 0.0f);
+        S[e] = uint32_t(at + k) < uint32_t(n) ? x : -INFINITY;  // the row sees the keys [lo, lo + n)
+        mx = fmaxf(mx, S[e]);
+      }
+      mx = max_halves(mx) * unit;
+      const bool up = mx > m_ref + kSlack;  // from -inf on: the first key that the row sees
+      if (__any(up)) follow_reference(move_reference(mx, up));
+      exponentials(S, W);
+      if (!within(h - 1, w0, w1)) {
+        const int* f = bad + 2 * ((h - 1) & (kRing - 1));
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(f[0] | f[1]), 0)) marks(h - 1, W);
+      }
     }
     if (within(h, v0, v1)) {
-      mfma_settle(s);
-      softmax(h);
+      score(h, S, [](int) {});
+      mfma_settle(S);
     }
     locate(id);
+  };
+  // A turn with all three stages to do, the middle one seen whole by all rows of the tile: scores of stage h to `to`, those of stage h - 1 in
+  // `of`, weights of stage h - 2 in `had`, of stage h - 1 to `W`.
+  auto whole_turn = [&](int h, f32x16& to, f32x16& of, const u32x4 (&had)[2], u32x4 (&W)[2]) __attribute__((always_inline)) {
+    const int id = begin(h, false);
+    const float b = bias_at(h - 1);
+    float mx;
+    auto shaped = [&](bool low) __attribute__((always_inline)) {
+      score(h, to, [&](int g) __attribute__((always_inline)) {
+        constexpr int PER = 16 / KS;
+#pragma unroll
+        for (int e = g * PER; e < (g + 1) * PER; ++e) of[e] = shape_e(of[e], e, b, low);
+      });
+      mx = of[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, of[e]);
+      lay_out<KS, (CAP ? 8 : 1) * 16 / KS>();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) asm volatile("" : "+v"(of[e]));
+    };
+    if constexpr (CAP) {
+      if (__builtin_expect(!__any(!(largest_size(of) < low_below)), 1)) shaped(true);
+      else shaped(false);
+    } else {
+      shaped(true);
+    }
+    mx = max_halves(mx) * unit;
+    const bool up = mx > m_ref + kSlack;
+    const bool moved = __any(up);
+    float c = 1.0f;
+    if (__builtin_expect(moved, 0)) c = move_reference(mx, up);
+    weigh(h - 2, had, [](int) {});
+    exponentials(of, W);
+    lay_out<2 * NT, 52 / (2 * NT)>();
+    asm volatile("" : "+v"(W[0]), "+v"(W[1]), "+v"(l_run));  // (made here, not where the next turn first needs them)
+    if (__builtin_expect(moved, 0)) follow_reference(c);
+    locate(id);
+  };
+  if (n_st > 0) {
+    // Turns [t0, t1) are whole for this wavefront, an even number of them.
+    const int t0 = max(max(f0, w0) + 1, v0 + 2), t1 = max(t0, min(min(f1, w1) + 1, v1)) , whole_turns = (t1 - t0) & ~1;
+    int h = 0;
+    for (; h < (whole_turns ? t0 : n_st + 2); ++h) mixed_turn(h, s[0], P[0]);
+    for (const int end = h + whole_turns; h < end; h += 2) {
+      whole_turn(h, s[1], s[0], P[0], P[1]);
+      whole_turn(h + 1, s[0], s[1], P[1], P[0]);
+    }
+    mfma_settle(s[0]);
+    for (; h <= n_st + 1; ++h) mixed_turn(h, s[0], P[0]);
   }
 
   // ---- the rows' end
@@ -404,24 +544,29 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
 
 namespace {
 
-template <int DT, int HD>
-hipError_t allow_tiled() {
-  const hipError_t e = allow_dynamic_lds<attn_shaped_tiled_kernel<DT, HD, false>>(TiledLds<HD>::kBytes);
-  return e == hipSuccess ? allow_dynamic_lds<attn_shaped_tiled_kernel<DT, HD, true>>(TiledLds<HD>::kBytes) : e;
-}
-
-template <int DT, int HD, bool CAP>
-hipError_t launch_tiled_c(const ShapedArgs& a, int n_tiles, hipStream_t st) {
-  constexpr auto k = attn_shaped_tiled_kernel<DT, HD, CAP>;
+template <int DT, int HD, bool CAP, bool BIAS>
+hipError_t launch_tiled_s(const ShapedArgs& a, int n_tiles, hipStream_t st) {
+  constexpr auto k = attn_shaped_tiled_kernel<DT, HD, CAP, BIAS>;
   const hipError_t e = allow_dynamic_lds<k>(TiledLds<HD>::kBytes);
-  if (e != hipSuccess) return e;
+  if (e != hipSuccess || n_tiles == 0) return e;  // (no tiles: the limit alone)
   hipLaunchKernelGGL(k, dim3(unsigned(a.Hkv), unsigned(n_tiles)), dim3(256), size_t(TiledLds<HD>::kBytes), st, a);
   return hipGetLastError();
 }
 
 template <int DT, int HD>
 hipError_t launch_tiled_t(const ShapedArgs& a, int n_tiles, hipStream_t st) {
-  return a.cap_log2 > 0.0f ? launch_tiled_c<DT, HD, true>(a, n_tiles, st) : launch_tiled_c<DT, HD, false>(a, n_tiles, st);
+  if (a.cap_log2 > 0.0f) return a.slopes ? launch_tiled_s<DT, HD, true, true>(a, n_tiles, st) : launch_tiled_s<DT, HD, true, false>(a, n_tiles, st);
+  return a.slopes ? launch_tiled_s<DT, HD, false, true>(a, n_tiles, st) : launch_tiled_s<DT, HD, false, false>(a, n_tiles, st);
+}
+
+template <int DT, int HD>
+hipError_t allow_tiled() {
+  ShapedArgs a{};
+  hipError_t e = launch_tiled_s<DT, HD, false, false>(a, 0, nullptr);
+  if (e == hipSuccess) e = launch_tiled_s<DT, HD, false, true>(a, 0, nullptr);
+  if (e == hipSuccess) e = launch_tiled_s<DT, HD, true, false>(a, 0, nullptr);
+  if (e == hipSuccess) e = launch_tiled_s<DT, HD, true, true>(a, 0, nullptr);
+  return e;
 }
 
 }  // namespace

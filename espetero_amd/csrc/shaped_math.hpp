@@ -22,6 +22,9 @@ struct ShapedArgs {
   int32_t H, Hkv, G, q_ld, bt, window, ring, R, cols;
   float scale_log2;  // without a cap: scale in log2 units; with one: 2 scale log2(e) / cap
   float cap_log2;    // cap in log2 units
+  // cap tanh(scale q.k / cap) in log2 units as q.k times a polynomial of (q.k)^2, for |q.k| < tanh_below. tanh(z) / z fitted in z^2 for
+  // |z| < 0.7, 1.5e-7 of tanh off in fp32.
+  float tanh_c[5], tanh_below;
   uint64_t kv_base;
 };
 
