@@ -131,9 +131,17 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   }
   const Sight rg = shaped_range(tile, tree, whole.some_from, whole.some_end);
 
-  // ---- stages of 32 keys from the sub-block of the first key on; which of them this wavefront's rows see, and which whole
+  // ---- stages of 32 keys, the last ones first: a bias makes near keys' scores the largest, and taken from the far ones on every stage's would
+  // move the reference (2048 rows behind 8000 keys, 32 / 8 heads, 8 of them of slopes above 0.17: 500 us). Stage h holds the keys from
+  // key_of(h) on, the last stage's from the sub-block of the first key on. Which stages this wavefront's rows see, and which whole:
   const int s0 = rg.from & ~15;
   const int n_st = rg.end > rg.from ? (rg.end - s0 + 31) >> 5 : 0;
+  auto key_of = [&](int h) { return s0 + 32 * (n_st - 1 - h); };
+  auto turn_round = [&](int& x0, int& x1) {
+    const int y = n_st - x1;
+    x1 = n_st - x0;
+    x0 = y;
+  };
   int v0 = 0, v1 = 0, f0 = 0, f1 = 0;  // stages [v0, v1) hold keys that some row sees, [f0, f1) only keys that all see
   int w0 = 0, w1 = 0;                  // [w0, w1) only keys that all rows of the tile see
   if (n_st && col0 < cols_live) {
@@ -149,7 +157,10 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   if (n_st) {
     w0 = (max(rg.from, whole.all_from) - s0 + 31) >> 5;
     w1 = max(w0, (min(rg.end, whole.all_end) - s0) >> 5);
+    turn_round(w0, w1);
   }
+  turn_round(v0, v1);
+  turn_round(f0, f1);
 
   // ---- staging: wavefront w loads sub-block w % 2 of K or V (w / 2) of every stage
   const int kind = wave >> 1, last_sub = rg.end > rg.from ? (rg.end - 1) & ~15 : s0;
@@ -160,8 +171,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   const uint32_t from = kind == 0 ? uint32_t((lane / CPR) * RB + (((lane % CPR) ^ swap23(lane / CPR)) << 4)) : uint32_t((2 * l32 + hb) << 4);
   auto turned = [&](int i) { return kind == 0 ? from ^ uint32_t(swap23(RPL * i) << 4) : from; };
   const uint32_t dst = lds_base + wave * L::kRun;
-  // Where this wavefront's next sub-block lies; a stage further is 32 tokens further, past the range the last sub-block again.
-  int next_key = n_st > 0 ? min(s0 + 16 * (wave & 1), last_sub) : 0, next_at = next_key / a.bt, next_t0 = next_key - next_at * a.bt;
+  // Where this wavefront's next sub-block lies; a stage further is 32 tokens further down. Past the range's end the last sub-block again.
+  int next_raw = n_st > 0 ? key_of(0) + 16 * (wave & 1) : 0, next_key = min(next_raw, last_sub);
+  int next_at = next_key / a.bt, next_t0 = next_key - next_at * a.bt;
   if (a.ring) next_at %= a.ring;
   using const_i32 = const int32_t __attribute__((address_space(4)));
   const const_i32* const list = (const const_i32*)a.blocks;
@@ -173,18 +185,21 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     // (t0 is a multiple of 16: a V^T sub-block starts as far behind its plane as the K row of its first token does)
     next_from = plane + uint64_t(uint32_t(id)) * block_bytes + uint32_t(next_t0 * (HD * 2));
   };
-  auto request = [&](int h) __attribute__((always_inline)) {
+  auto request = [&](int h, int i) __attribute__((always_inline)) {
+    load_to_lds16(next_from + 1024 * i, turned(i), dst + uint32_t(h & (kRing - 1)) * L::kStage + 1024 * i);
+  };
+  auto request_all = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < LOADS; i += 4)
-      load_to_lds16_x4(next_from + 1024 * i, turned(i), turned(i + 1), turned(i + 2), turned(i + 3), dst + uint32_t(h & (kRing - 1)) * L::kStage + 1024 * i);
+    for (int i = 0; i < LOADS; ++i) request(h, i);
   };
   auto advance = [&]() __attribute__((always_inline)) {
-    if (next_key + 32 <= last_sub) {
-      next_key += 32;
-      next_t0 += 32;
-      while (next_t0 >= a.bt) {
-        next_t0 -= a.bt;
-        if (++next_at == a.ring) next_at = 0;  // (0 on a layer without rings, which it never is again)
+    if (next_raw - 32 >= s0) {
+      next_raw -= 32;
+      next_t0 -= next_key - next_raw;
+      next_key = next_raw;
+      while (next_t0 < 0) {
+        next_t0 += a.bt;
+        if (--next_at < 0) next_at = a.ring - 1;  // (a layer without rings has no blocks in front of the first key's)
       }
     }
   };
@@ -203,7 +218,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   u32x4 P[2][2] = {};
 
   // The bias of index e of this lane's half, linear in the key: right up to the row's own key.
-  auto bias_at = [&](int h) { return slope * float(s0 + 32 * h + 8 * hb - qpos); };
+  auto bias_at = [&](int h) { return slope * float(key_of(h) + 8 * hb - qpos); };
   auto score_operand = [&](int h, int g) { return lds_read((k_at + uint32_t(h & (kRing - 1)) * L::kStage) ^ uint32_t(g << 5)); };
   auto value_operand = [&](uint32_t va, int g) { return lds_read(va + (g / NT) * L::kRun + (g % NT) * 1024); };
   auto values_of = [&](int h) {
@@ -292,18 +307,18 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   // A new reference where a score exceeds the old one by more than kSlack. What was weighed by the old one joins the accumulators
   // first; then they go over to the new one.
   auto move_reference = [&](float mx, bool up) __attribute__((always_inline)) {
-    const float c = m_ref == -INFINITY ? 0.0f : up ? fast_exp2(m_ref - mx) : 1.0f;
+    const float c = m_ref == -INFINITY ? -1.0f : up ? fast_exp2(m_ref - mx) : 1.0f;
     m_ref = up ? mx : m_ref;
     l_run *= c;
     return c;
   };
   auto follow_reference = [&](float c) __attribute__((always_inline)) {
-    // (0 where there was none: whatever the accumulators hold goes.)
+    // (Below 0 where there was none: whatever the accumulators hold goes.)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       mfma_settle(acc[nt]);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[nt][e] = c == 0.0f ? 0.0f : acc[nt][e] * c;
+      for (int e = 0; e < 16; ++e) acc[nt][e] = c < 0.0f ? 0.0f : acc[nt][e] * c;
     }
   };
   // Lane l holds of S^T, at index 8 sb + i, key 16 sb + 8 hb + i of the stage.
@@ -321,7 +336,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   };
   auto mend = [&](int h) __attribute__((always_inline)) {
     uint32_t found = 0;
-    const int ln = here(lane), key0 = s0 + 32 * h + 16 * (wave & 1) + 8 * (ln >> 5);
+    const int ln = here(lane), key0 = key_of(h) + 16 * (wave & 1) + 8 * (ln >> 5);
     char* const mine_at = lds + (uint32_t(h) & (kRing - 1)) * L::kStage + wave * L::kRun + ln * 16;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
@@ -347,7 +362,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
       uint32_t found = marked ? *word : 0u;
 #pragma unroll 1
       for (int t = 0; t < 32; ++t) {
-        const int key = s0 + 32 * h + t;
+        const int key = key_of(h) + t;
         if (key < rg.from || key >= rg.end) continue;
         // The row's weight of the key: element t % 8 of P[t / 16], in the lane half (t / 8) % 2.
         uint32_t p2 = 0;
@@ -371,7 +386,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   const int lead = kind == 0 ? 3 : 1;  // the stage requested in turn h, less h
   locate(block_id());
   for (int h = 0; h < min(n_st, lead); ++h) {
-    request(h);
+    request_all(h);
     advance();
     locate(block_id());
   }
@@ -381,9 +396,10 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   auto within = [](int h, int lo, int hi) { return uint32_t(h - lo) < uint32_t(hi - lo); };  // (lo <= hi)
   const float low_below = CAP ? a.tanh_below : 0.0f;
   // What a turn begins with. Behind barrier h, K of stage h and V of stage h - 1 have landed for everybody, and nobody reads K of stage h - 1
-  // or V of stage h - 3 any more, whose places in the ring the requests take. Returns the id of the block that is located at the turn's end.
+  // or V of stage h - 3 any more, whose places in the ring the turn's requests take.
   auto begin = [&](int h, bool edges) __attribute__((always_inline)) {
-    const int behind = kind == 0 ? min(2, n_st - 1 - h) : min(1, n_st - h);  // stages requested behind the one that has to be there
+    // Stages requested behind the one that has to be there.
+    const int behind = kind == 0 ? (edges ? min(2, n_st - 1 - h) : 2) : edges ? min(1, n_st - h) : 1;
     if (behind >= 2) {
       if constexpr (LOADS == 4) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
       else asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
@@ -400,15 +416,15 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (h + lead < n_st) {
-      request(h + lead);
-      advance();
-    }
-    return block_id();
   };
   // A turn of whatever there is to do, one after the other: S and W are the scores and the weights of the last stage.
   auto mixed_turn = [&](int h, f32x16& S, u32x4 (&W)[2]) __attribute__((always_inline)) {
-    const int id = begin(h, true);
+    begin(h, true);
+    if (h + lead < n_st) {
+      request_all(h + lead);
+      advance();
+    }
+    const int id = block_id();
     // On a wavefront's first stage acc is whatever; it is cleared when a row's reference is first set.
     if (within(h - 2, v0, v1)) weigh(h - 2, W, [](int) {});
     if (within(h - 1, v0, v1)) {
@@ -416,7 +432,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
       const float b = bias_at(h - 1);
       // (By the exponential whatever the scores: those of keys that a row does not see may be anything, and choose nothing.)
       const int lo = max(rg.from, sight.from), n = max(0, min(rg.end, sight.end) - lo);
-      const int at0 = s0 + 32 * (h - 1) + 8 * (here(lane) >> 5), at = at0 - lo;
+      const int at0 = key_of(h - 1) + 8 * (here(lane) >> 5), at = at0 - lo;
       float mx = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -444,7 +460,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   // A turn with all three stages to do, the middle one seen whole by all rows of the tile: scores of stage h to `to`, those of stage h - 1 in
   // `of`, weights of stage h - 2 in `had`, of stage h - 1 to `W`.
   auto whole_turn = [&](int h, f32x16& to, f32x16& of, const u32x4 (&had)[2], u32x4 (&W)[2]) __attribute__((always_inline)) {
-    const int id = begin(h, false);
+    begin(h, false);
     const float b = bias_at(h - 1);
     float mx;
     auto shaped = [&](bool low) __attribute__((always_inline)) {
@@ -452,6 +468,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
         constexpr int PER = 16 / KS;
 #pragma unroll
         for (int e = g * PER; e < (g + 1) * PER; ++e) of[e] = shape_e(of[e], e, b, low);
+        // Requests one by one: together at the turn's beginning they stand in line behind those of the other wavefronts.
+        if (g % 2 == 1 && g < 2 * LOADS) request(h + lead, g / 2);
       });
       mx = of[0];
 #pragma unroll
@@ -466,6 +484,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     } else {
       shaped(true);
     }
+    advance();
+    const int id = block_id();
     mx = max_halves(mx) * unit;
     const bool up = mx > m_ref + kSlack;
     const bool moved = __any(up);
@@ -479,8 +499,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     locate(id);
   };
   if (n_st > 0) {
-    // Turns [t0, t1) are whole for this wavefront, an even number of them.
-    const int t0 = max(max(f0, w0) + 1, v0 + 2), t1 = max(t0, min(min(f1, w1) + 1, v1)) , whole_turns = (t1 - t0) & ~1;
+    // Turns [t0, t1) are whole for this wavefront, an even number of them, each with a stage to request.
+    const int t0 = max(max(f0, w0) + 1, v0 + 2), t1 = max(t0, min(min(min(f1, w1) + 1, v1), n_st - lead)), whole_turns = (t1 - t0) & ~1;
     int h = 0;
     for (; h < (whole_turns ? t0 : n_st + 2); ++h) mixed_turn(h, s[0], P[0]);
     for (const int end = h + whole_turns; h < end; h += 2) {
