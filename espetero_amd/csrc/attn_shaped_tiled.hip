@@ -15,7 +15,7 @@
 // exponential and a reciprocal (eleven). 2048 rows behind 8000 keys, 32 / 8 heads: ...
 //
 // LDS: a ring of 4 stages of 32 keys, K and V^T, loaded straight from the pool (global_load_lds): wavefronts 0 and 1 load the
-// two sub-blocks of K, three stages ahead of the scores, 2 and 3 those of V^T, three ahead of P . V. K: the 16-byte chunk c of row r lies at
+// two sub-blocks of K, two stages ahead of the scores, 2 and 3 those of V^T, two ahead of P . V. K: the 16-byte chunk c of row r lies at
 // c ^ (pi(r) & 15), pi swapping bits 2 and 3; V^T: per sub-block of 16 keys and group of 32 dims [half of the keys][32 dims][8 keys], the
 // order in which the lanes of a P . V operand read it. Neither side has bank conflicts. Nothing in the loop may load from memory but the
 // stages (any such load's wait is a wait for them).
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     marked = true;
   };
 
-  const int lead = kind == 0 ? 3 : 1;  // the stage requested in turn h, less h
+  const int lead = kind == 0 ? 2 : 0;  // the stage requested in turn h, less h
   locate(block_id());
   for (int h = 0; h < min(n_st, lead); ++h) {
     request_all(h);
@@ -395,22 +395,15 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
   auto within = [](int h, int lo, int hi) { return uint32_t(h - lo) < uint32_t(hi - lo); };  // (lo <= hi)
   const float low_below = CAP ? a.tanh_below : 0.0f;
-  // What a turn begins with. Behind barrier h, K of stage h and V of stage h - 1 have landed for everybody, and nobody reads K of stage h - 1
-  // or V of stage h - 3 any more, whose places in the ring the turn's requests take.
+  // Two turns between barriers: 64 keys. Behind the one in front of turns h and h + 1 (h even), K of stages h and h + 1 and V of stages h - 2
+  // and h - 1 have landed for everybody, and nobody reads K or V of the two stages in front of those any more, whose places in the
+  // ring the two turns' requests take.
   auto begin = [&](int h, bool edges) __attribute__((always_inline)) {
-    // Stages requested behind the one that has to be there.
-    const int behind = kind == 0 ? (edges ? min(2, n_st - 1 - h) : 2) : edges ? min(1, n_st - h) : 1;
-    if (behind >= 2) {
-      if constexpr (LOADS == 4) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-    } else if (behind == 1) {
-      if constexpr (LOADS == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    if (edges && kind == 1 && h >= 1 && h <= n_st && !within(h - 1, w0, w1)) {
-      mend(h - 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (edges && kind == 1) {
+#pragma unroll 1
+      for (int x = max(h - 2, 0); x < min(h, n_st); ++x)
+        if (!within(x, w0, w1)) mend(x);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
     asm volatile("" ::: "memory");
@@ -419,14 +412,19 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   };
   // A turn of whatever there is to do, one after the other: S and W are the scores and the weights of the last stage.
   auto mixed_turn = [&](int h, f32x16& S, u32x4 (&W)[2]) __attribute__((always_inline)) {
-    begin(h, true);
     if (h + lead < n_st) {
       request_all(h + lead);
       advance();
     }
     const int id = block_id();
     // On a wavefront's first stage acc is whatever; it is cleared when a row's reference is first set.
-    if (within(h - 2, v0, v1)) weigh(h - 2, W, [](int) {});
+    if (within(h - 2, v0, v1)) {
+      weigh(h - 2, W, [](int) {});
+      if (!within(h - 2, w0, w1)) {
+        const int* f = bad + 2 * ((h - 2) & (kRing - 1));
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(f[0] | f[1]), 0)) marks(h - 2, W);
+      }
+    }
     if (within(h - 1, v0, v1)) {
       mfma_settle(S);
       const float b = bias_at(h - 1);
@@ -446,10 +444,6 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
       const bool up = mx > m_ref + kSlack;  // from -inf on: the first key that the row sees
       if (__any(up)) follow_reference(move_reference(mx, up));
       exponentials(S, W);
-      if (!within(h - 1, w0, w1)) {
-        const int* f = bad + 2 * ((h - 1) & (kRing - 1));
-        if (__builtin_expect(__builtin_amdgcn_readfirstlane(f[0] | f[1]), 0)) marks(h - 1, W);
-      }
     }
     if (within(h, v0, v1)) {
       score(h, S, [](int) {});
@@ -457,10 +451,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     }
     locate(id);
   };
-  // A turn with all three stages to do, the middle one seen whole by all rows of the tile: scores of stage h to `to`, those of stage h - 1 in
+  // A turn with all three stages to do, the last two seen whole by all rows of the tile: scores of stage h to `to`, those of stage h - 1 in
   // `of`, weights of stage h - 2 in `had`, of stage h - 1 to `W`.
   auto whole_turn = [&](int h, f32x16& to, f32x16& of, const u32x4 (&had)[2], u32x4 (&W)[2]) __attribute__((always_inline)) {
-    begin(h, false);
     const float b = bias_at(h - 1);
     float mx;
     auto shaped = [&](bool low) __attribute__((always_inline)) {
@@ -499,16 +492,22 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     locate(id);
   };
   if (n_st > 0) {
-    // Turns [t0, t1) are whole for this wavefront, an even number of them, each with a stage to request.
-    const int t0 = max(max(f0, w0) + 1, v0 + 2), t1 = max(t0, min(min(min(f1, w1) + 1, v1), n_st - lead)), whole_turns = (t1 - t0) & ~1;
+    // Turns [t0, t1) are whole for this wavefront, in pairs.
+    const int t0 = (max(max(f0 + 1, w0 + 2), v0 + 2) + 1) & ~1, t1 = max(t0, min(min(f1, w1) + 1, v1) & ~1);
+    auto mixed_pair = [&](int h) __attribute__((always_inline)) {
+      begin(h, true);
+#pragma unroll 1
+      for (int x = h; x < h + 2; ++x) mixed_turn(x, s[0], P[0]);
+    };
     int h = 0;
-    for (; h < (whole_turns ? t0 : n_st + 2); ++h) mixed_turn(h, s[0], P[0]);
-    for (const int end = h + whole_turns; h < end; h += 2) {
+    for (; h < (t1 > t0 ? t0 : n_st + 2); h += 2) mixed_pair(h);
+    for (; h < t1; h += 2) {
+      begin(h, false);
       whole_turn(h, s[1], s[0], P[0], P[1]);
       whole_turn(h + 1, s[0], s[1], P[1], P[0]);
     }
     mfma_settle(s[0]);
-    for (; h <= n_st + 1; ++h) mixed_turn(h, s[0], P[0]);
+    for (; h < n_st + 2; h += 2) mixed_pair(h);
   }
 
   // ---- the rows' end
