@@ -828,7 +828,8 @@ int esp_attn_shaped(const esp_attn_params* p, const esp_shape_params* shape, con
   if (n_parts > 0 && (!workspace || workspace_bytes < c.total))
     return fail(err, errlen, ESP_EWORKSPACE, "workspace %zu bytes, %zu needed", workspace ? workspace_bytes : size_t(0), c.total);
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(err, errlen, ESP_EINVAL, "workspace must be 16-byte aligned");
-  if (reinterpret_cast<uintptr_t>(shape->spans) % 8) return fail(err, errlen, ESP_EINVAL, "spans must be 8-byte aligned");
+  if (reinterpret_cast<uintptr_t>(shape->spans) % 8 || reinterpret_cast<uintptr_t>(shape->slopes) % 4)
+    return fail(err, errlen, ESP_EINVAL, "spans must be 8-byte, slopes 4-byte aligned");
   DeviceState* dev = nullptr;
   if (int rc = device_state(&dev, err, errlen)) return rc;
   esp::ShapedArgs a{};
