@@ -48,6 +48,21 @@ __device__ __forceinline__ float max_halves(float x) {
   return fmaxf(x, y);
 }
 
+// The largest of a wavefront's numbers (none the lowest there is): over rows of 16 lanes, then from row to row.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int most_from(int x) {
+  return max(x, __builtin_amdgcn_update_dpp(INT32_MIN, x, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ int wave_most(int x) {
+  x = most_from<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x = most_from<0x112, 0xf>(x);
+  x = most_from<0x114, 0xf>(x);
+  x = most_from<0x118, 0xf>(x);
+  x = most_from<0x142, 0xa>(x);  // row_bcast 15, 31
+  x = most_from<0x143, 0xc>(x);
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // The order of a block of N matrix instructions with operands from LDS two ahead: one, then V vector operations (exponentials among
 // them), and the operand of the one after the next.
 template <int N, int V>
@@ -106,21 +121,11 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   Seen mine{}, whole{};
   const int q_first = tree.P + rr0 + min(col0, cols_live - 1) / a.G;  // of this wavefront's rows
   if (a.spans) {
-    auto reduce = [](Seen s, int lanes) {
-      for (int x = 1; x < lanes; x <<= 1) {
-        s.some_from = min(s.some_from, __shfl_xor(s.some_from, x));
-        s.some_end = max(s.some_end, __shfl_xor(s.some_end, x));
-        s.all_from = max(s.all_from, __shfl_xor(s.all_from, x));
-        s.all_end = min(s.all_end, __shfl_xor(s.all_end, x));
-      }
-      s.some_from = __builtin_amdgcn_readfirstlane(s.some_from), s.some_end = __builtin_amdgcn_readfirstlane(s.some_end);
-      s.all_from = __builtin_amdgcn_readfirstlane(s.all_from), s.all_end = __builtin_amdgcn_readfirstlane(s.all_end);
-      return s;
-    };
-    mine = reduce(Seen{sight.from, sight.end, sight.from, sight.end}, 32);
+    auto reduce = [](const Seen& s) { return Seen{-wave_most(-s.some_from), wave_most(s.some_end), wave_most(s.all_from), -wave_most(-s.all_end)}; };
+    mine = reduce(Seen{sight.from, sight.end, sight.from, sight.end});
     const int m0 = min(lane, rows - 1), m1 = min(lane + 64, rows - 1);
     const Sight s0 = shaped_sight(a, tile.r0 + m0, tree.P + rr0 + m0, n_keys), s1 = shaped_sight(a, tile.r0 + m1, tree.P + rr0 + m1, n_keys);
-    whole = reduce(Seen{min(s0.from, s1.from), max(s0.end, s1.end), max(s0.from, s1.from), min(s0.end, s1.end)}, 64);
+    whole = reduce(Seen{min(s0.from, s1.from), max(s0.end, s1.end), max(s0.from, s1.from), min(s0.end, s1.end)});
   } else {
     auto of_rows = [&](int m0, int m1) {
       const int q0 = tree.P + rr0 + m0, q1 = tree.P + rr0 + m1;
@@ -335,22 +340,36 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     return x;
   };
   auto mend = [&](int h) __attribute__((always_inline)) {
-    uint32_t found = 0;
     const int ln = here(lane), key0 = key_of(h) + 16 * (wave & 1) + 8 * (ln >> 5);
     char* const mine_at = lds + (uint32_t(h) & (kRing - 1)) * L::kStage + wave * L::kRun + ln * 16;
+    // (An exponent of ones, and only that, carries into the sign's place.)
+    constexpr uint32_t kExp = DT == ESP_F16 ? 0x7c007c00u : 0x7f807f80u, kOne = DT == ESP_F16 ? 0x04000400u : 0x00800080u;
+    uint32_t found = 0;
+    const bool cut = key_of(h) < rg.from || key_of(h) + 32 > rg.end;
+    uint32_t in[4] = {~0u, ~0u, ~0u, ~0u};
+    if (cut) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) in[e] = in_range(key0 + 2 * e);
+    }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      u32x4 v = *reinterpret_cast<const u32x4*>(mine_at + i * 1024);
+      const u32x4 v = *reinterpret_cast<const u32x4*>(mine_at + i * 1024);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] &= in_range(key0 + 2 * e);
-        const uint32_t nf = not_finite2<DT>(v[e]);
-        found |= nf;
-        v[e] &= ~nf;
-      }
-      *reinterpret_cast<u32x4*>(mine_at + i * 1024) = v;
+      for (int e = 0; e < 4; ++e) found |= (v[e] & in[e] & kExp) + kOne;
     }
-    const bool any = __any(found != 0);
+    const bool any = __any((found & 0x80008000u) != 0);
+    if (cut || any) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        u32x4 v = *reinterpret_cast<const u32x4*>(mine_at + i * 1024);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] &= in[e];
+          if (any) v[e] &= ~not_finite2<DT>(v[e]);
+        }
+        *reinterpret_cast<u32x4*>(mine_at + i * 1024) = v;
+      }
+    }
     if (ln == 0) bad[2 * (uint32_t(h) & (kRing - 1)) + (wave & 1)] = any;
   };
   bool marked = false;
