@@ -5,7 +5,8 @@
 // Streaming kernel: decode and short trees. Bound by HBM: every visible key's K and V are read once for all G query heads of a KV head and
 // all rows of the tile. One workgroup is one tile and one KV head; up to 16 packed rows (row in tile * G + head of the group) are the columns
 // of a matrix tile, NC such tiles. A wavefront takes 16-key units round robin straight from HBM with the next unit's loads in
-// flight; the four wavefronts' sums meet in LDS at the end.
+// flight; the four wavefronts' sums meet in LDS at the end. 24 sequences of 300 to 9000 keys, 32 / 8 heads of 128 dims: 89 us for 540 MB, 6.0 TB/s
+// of the 6.6 that a plain read of such pages reaches, and 5 us for the merge; two or three units ahead in place of one: 88.
 #include "shaped_math.hpp"
 
 namespace esp {

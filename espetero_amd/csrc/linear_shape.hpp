@@ -10,8 +10,10 @@
 namespace esp {
 
 constexpr int kLinearChunk = 64;  // rows that the chunked kernel takes at a time
-// Sequences of up to so many rows go through the recurrent kernel, whose time grows with every row beyond the state's own bytes.
-constexpr int kLinearFew = 16;
+// Sequences of up to so many rows go through the recurrent kernel, whose time grows with every row beyond the state's own bytes. 32 heads of
+// 128 x 128, bf16, recurrent and chunked: 64 sequences of 4 rows 46 and 56 us, of 8 56 and 56, of 12 66 and 55; one of 4 rows 5.6 and 9.3, of 8
+// 6.3 and 9.1, of 12 8.0 and 9.2.
+constexpr int kLinearFew = 8;
 
 // Columns of V that a workgroup of the chunked kernel takes.
 constexpr int linear_cols(int dv) { return dv % 128 == 0 ? 128 : 64; }
