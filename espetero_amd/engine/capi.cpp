@@ -84,11 +84,16 @@ static int plan_pass(const esp_attn_params* p, Pass kind, const esp_tree* trees,
   try {
     AttnPlan A;
     A.trees.assign(trees, trees + n_trees);
-    // The tiled kernels of differential attention and of shaped scores are planned for as such, shaped scores' streaming kernel as the one it is like.
+    // The tiled kernels of differential attention and of shaped scores are planned for as such (the latter's by a rule of its own, unless the
+    // reference's is asked for), shaped scores' streaming kernel as the one it is like.
     const int family = kind == Pass::diff     ? esp::diff_family(o->rows_per_tile, p->H / p->Hkv)
                        : kind == Pass::shaped ? esp::shaped_family(p->head_dim, o->rows_per_tile, p->H / p->Hkv)
                                               : 1;
-    plan_tiles(A, groups, window, pos, family < 0 ? to_cpp(*o).for_diff_tiled() : to_cpp(*o), kind == Pass::diff || family < 0 ? nullptr : p);
+    const PlanOptions options = to_cpp(*o);
+    if (kind == Pass::shaped && family < 0 && options.balanced)
+      plan_shaped_tiled(A, p->head_dim, p->H, esp::shaped_workgroups_per_cu(p->head_dim, family), groups, window, pos, options);
+    else
+      plan_tiles(A, groups, window, pos, family < 0 ? options.for_diff_tiled() : options, kind == Pass::diff || family < 0 ? nullptr : p);
     *n_tiles = int32_t(A.tiles.size());
     *n_jobs = int32_t(A.combine.size());
     *n_parts = A.parts;

@@ -668,6 +668,129 @@ inline void plan_tiles(AttnPlan& A, int groups, int window, const int32_t* pos, 
   }
 }
 
+// Attention with shaped scores on its tiled kernel: every tile of rows in parts of at most so many stages of 32 keys, whichever of them the cache
+// and whichever the pass itself holds. What comes of a cut is worked out by handing its workgroups to the chip's slots, longest first (as the
+// records are ordered; the kernel takes them from the end); figures in microseconds, of 128 and 256 dims: 7.7 and 9.6 for a workgroup's
+// set-up and end, 0.82 and 1.17 for a stage, 1.0 for one beside another workgroup on the compute unit, 4.7 and 5.6 for the merge, and the partial
+// records at 3 MB a microsecond. Fitted to 109 passes of 13 to 1976 rows over 0 to 16000 keys, each timed whole and in up to 24 cuts: right
+// within 11 %; what it picks takes 2.5 % longer than the best of them in geometric mean. (24 rows behind 16000 keys, 32 / 8 heads: 444 us
+// whole, 68 in 8 parts, 30 in 32; 1500 fresh rows, 8 / 4 heads of 256: 76 whole, 43 in 60 parts.) A cut has to promise a tenth: spans, which are not
+// known here, may leave a tile fewer keys than it is planned for.
+inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, int groups, int window, const int32_t* pos, const PlanOptions& o) {
+  constexpr int kStage = 32;
+  A.tiles.clear();
+  A.combine.clear();
+  A.parts = 0;
+  A.rows_per_tile = o.rows_per_tile;
+  const int R = o.rows_per_tile;
+  struct Rows {
+    int tree, r, lo, hi, stages;  // keys [lo, hi) of the tree, lo a multiple of 16
+  };
+  std::vector<Rows> tiles;
+  long long whole = 0;
+  int longest = 1;
+  for (int ti = 0; ti < int(A.trees.size()); ++ti) {
+    const esp_tree& t = A.trees[size_t(ti)];
+    for (int r = 0; r < t.M; r += R) {
+      int lo = 0;
+      if (window > 0) {
+        int first = INT32_MAX;
+        for (int i = r; i < std::min(t.M, r + R); ++i) first = std::min(first, pos[4 * (t.base + i)]);
+        lo = std::clamp(first - window + 1, 0, t.P + r) / 16 * 16;
+      }
+      const int hi = t.P + std::min(t.M, r + R), stages = (hi - lo + kStage - 1) / kStage;
+      tiles.push_back({ti, r, lo, hi, stages});
+      whole += stages;
+      longest = std::max(longest, stages);
+    }
+  }
+  const int slots = std::max(per_cu, o.groups_target), units = std::max(1, slots / per_cu);
+  const bool wide = head_dim == 256;
+  const double end = wide ? 9.6 : 7.7, alone = wide ? 1.17 : 0.82, beside = wide ? 1.19 : 1.0, merge = wide ? 5.6 : 4.7;
+  struct Cut {
+    int parts, each;
+  };
+  // (parts of two stages and more, and of no fewer keys than a caller's own limit)
+  const PlanOptions had = PlanOptions::mi355x(R, o.groups_target);
+  const int fewest = std::max(2, o.min_chunk == had.min_chunk ? 0 : o.min_chunk / kStage);
+  auto cut = [&](const Rows& t, int most) {
+    const int n = std::min({(t.stages + most - 1) / most, std::max(1, t.stages / fewest), o.max_splits});
+    const int each = (t.stages + n - 1) / n;
+    return Cut{(t.stages + each - 1) / each, each};
+  };
+  std::vector<int> lengths;
+  auto price = [&](int most) {
+    lengths.clear();
+    double records = 0;
+    for (const Rows& t : tiles) {
+      const Cut c = cut(t, most);
+      for (int k = 0; k < c.parts; ++k) lengths.push_back(std::min(c.each, t.stages - k * c.each));
+      if (c.parts > 1) records += double(c.parts) * std::min(R, A.trees[size_t(t.tree)].M - t.r);
+    }
+    std::sort(lengths.begin(), lengths.end(), std::greater<int>());
+    const long long workgroups = (long long)lengths.size() * groups;
+    const bool few = workgroups <= units;
+    using Free = std::pair<double, long long>;  // (when, how many slots)
+    std::priority_queue<Free, std::vector<Free>, std::greater<Free>> free_at;
+    free_at.push({0.0, few ? units : slots});
+    double last = 0;
+    for (const int stages : lengths) {
+      const double cost = end + stages * (few ? alone : beside);
+      for (long long left = groups; left > 0;) {
+        const Free f = free_at.top();
+        const long long take = std::min(left, f.second);
+        free_at.pop();
+        if (f.second > take) free_at.push({f.first, f.second - take});
+        free_at.push({f.first + cost, take});
+        last = std::max(last, f.first + cost);
+        left -= take;
+      }
+    }
+    return last + (records > 0 ? merge + records * heads * head_dim * 4e-6 / 3.0 : 0.0);
+  };
+  int most = longest;
+  if ((long long)tiles.size() * groups < 4LL * slots && whole > 0) {
+    double best = 0.9 * price(longest);
+    for (const int n : {2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128}) {
+      const int m = (longest + n - 1) / n;
+      if (m < fewest) break;
+      long long workgroups = 0;
+      for (const Rows& t : tiles) workgroups += (long long)cut(t, m).parts * groups;
+      if (workgroups > 4LL * slots) break;  // (so the workspace is bounded too)
+      const double t = price(m);
+      if (t < best) best = t, most = m;
+    }
+  }
+  struct Record {
+    int stages;
+    esp_tile tile;
+  };
+  std::vector<Record> records;
+  for (const Rows& rows : tiles) {
+    const esp_tree& t = A.trees[size_t(rows.tree)];
+    const Cut c = cut(rows, most);
+    const int part0 = A.parts, pad = o.balanced ? t.table + 1 : 0;
+    if (c.parts == 1) {
+      records.push_back({rows.stages, {rows.tree, t.base + rows.r, std::min(rows.lo, t.P), t.P, -1, 1, std::max(0, rows.lo - t.P), pad}});
+      continue;
+    }
+    int x = rows.lo;
+    for (int k = 0; k < c.parts; ++k) {
+      const bool is_last = k + 1 == c.parts;
+      int y = is_last ? rows.hi : rows.lo + (k + 1) * c.each * kStage;
+      if (y == t.P && !is_last) y -= 16;  // the last of the cached keys go with the pass's own: a part that ends with them may be made to grow
+      esp_tile tile{rows.tree, t.base + rows.r, std::min(x, t.P), std::min(y, t.P), A.parts++, 0, std::max(0, x - t.P), pad};
+      if (is_last) tile.last = 1;  // open: spans may reach behind the tile's own rows
+      else if (y > t.P) tile.last = y - t.P + 1;
+      records.push_back({c.each, tile});
+      x = y;
+    }
+    A.combine.push_back({t.base + rows.r, std::min(R, t.M - rows.r), part0, c.parts});
+  }
+  std::stable_sort(records.begin(), records.end(), [](const Record& a, const Record& b) { return a.stages < b.stages; });
+  for (const Record& r : records) A.tiles.push_back(r.tile);
+}
+
 // Rows grouped by their adapter, in tiles of at most rows_per_tile: which tiles esp_lowrank_add runs.
 struct LowRankPlan {
   std::vector<int32_t> order;  // row numbers, slot by slot

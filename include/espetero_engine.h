@@ -75,8 +75,10 @@ int esp_plan_tiles_diff(const esp_attn_params* p, const esp_tree* trees, int32_t
                         const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                         int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen);
 
-/* And for a pass of esp_attn_shaped (p: its parameters; groups: what esp_attn_shaped_hint reports), by the same rules: passes of the streaming
- * kernel as esp_plan_tiles_for plans them, those of the tiled one as esp_plan_tiles_diff. */
+/* And for a pass of esp_attn_shaped (p: its parameters; groups: what esp_attn_shaped_hint reports): passes of the streaming kernel as
+ * esp_plan_tiles_for plans them; on the tiled one every tile in parts of one length, cached keys and the pass's own rows alike, the length by
+ * what the hand-out of their workgroups to the chip comes to (o: rows_per_tile, groups_target, max_splits, and a min_chunk that is not
+ * esp_plan_options_mi355x's). The planner does not see the rows' spans. */
 int esp_plan_tiles_shaped(const esp_attn_params* p, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
                           const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                           int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen);
