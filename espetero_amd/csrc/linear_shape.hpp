@@ -19,9 +19,9 @@ constexpr int kLinearFew = 8;
 constexpr int linear_cols(int dv) { return dv % 128 == 0 ? 128 : 64; }
 constexpr bool linear_dims(int dk, int dv) { return (dk == 64 || dk == 128) && dv >= 64 && dv <= 512 && dv % 64 == 0; }
 
-// Resident workgroups per compute unit of the chunked kernel: two of 78 KB of LDS, wavefronts of 256 registers (dk 64: three by LDS, two
-// by registers); of half the columns, four wavefronts of two workgroups as well.
-constexpr int linear_workgroups_per_cu(int, int) { return 2; }
+// Resident workgroups per compute unit of the chunked kernel: two of 78 KB of LDS, wavefronts of 256 registers (dk 64: by registers); of 64 x 64
+// dims a third one fits, and fills what two leave.
+constexpr int linear_workgroups_per_cu(int dk, int dv) { return dk == 64 && linear_cols(dv) == 64 ? 3 : 2; }
 
 // Records of sequences cut into segments: states, then the log2 of what each segment's decays come to.
 struct LinearCarve {

@@ -831,13 +831,26 @@ struct LinearPlan {
   int few = 0, parts = 0;
 };
 
+// What the chunked kernel's workgroups take, in microseconds, by the dims of a state that a workgroup holds: a chunk on a compute unit of its
+// own and beside others (of bf16; fp16 1.2 and 1.05 times as much), where only the state is made likewise, a workgroup's set-up and end in
+// either launch, a record summed up, the launch in front. Fitted to 77 passes of 200 to 12000 rows on 5 to 40 heads, each in up to 17 cuts:
+// right within 9 %, and what it picks takes 1 % longer than the best of them.
+struct LinearPrices {
+  double alone, beside, state_alone, state_beside, end, state_end, record, front;
+};
+inline LinearPrices linear_prices(const esp_linear_params& p) {
+  const bool wide = esp::linear_cols(p.dv) == 128;
+  LinearPrices x = p.dk == 128 ? (wide ? LinearPrices{4.1, 8.1, 2.1, 2.5, 7.2, 3.0, 0.97, 0.9} : LinearPrices{4.5, 6.5, 2.2, 2.0, 5.2, 1.6, 0.49, 3.0})
+                               : (wide ? LinearPrices{3.4, 5.8, 1.4, 1.5, 3.0, 2.5, 0.38, 2.3} : LinearPrices{3.5, 5.3, 1.5, 1.7, 3.0, 1.8, 0.23, 2.8});
+  if (p.dtype == ESP_F16) x.alone *= 1.2, x.beside *= 1.05;
+  return x;
+}
+
 // Sequences that esp_linear_attn's chunked kernel takes are cut into segments where a pass has fewer workgroups than the chip holds, or
 // longer ones than its share. A segment's state is made by a launch in front, which reads K and V once more. What comes of a cut
-// is worked out by handing its workgroups to the chip's slots, two to a compute unit, in the order of the tiles; all figures in
-// microseconds, of heads of 128 x 128 (64 x 128 take a tenth less): a chunk 4.5 alone on a compute unit, 6.9 beside another (2.5 and 3.6
-// where only the state is made), 7 for a workgroup's set-up and end, 0.9 for a record summed up, 3 for the launch in front. (One prompt of 2000
-// rows, 32 heads, in segments of 2, 4, 8, 16 and 32 chunks: 55, 45, 63, 111 and 146 us; 16000 rows, 32 heads of 64 x 128, 4, 8, 16, 32: 229,
-// 165, 156, 197; four of 2048 rows, 40 heads, 4, 8, 11, 16, 32: 168, 152, 146, 183, 154.)
+// is worked out by handing its workgroups to the chip's slots in the order of the tiles, at the prices above. (One prompt of 2000 rows, 32
+// heads of 128 x 128, bf16, in segments of 2, 4, 8, 16 and 32 chunks: 51, 45, 66, 112 and 146 us; five of 785, 64 x 64, of 3, 5, 7 and
+// 13: 34, 43, 54 and 53; four of 2048, 40 heads, 128 x 128, of 4, 8, 11, 16 and 32: 166, 145, 134, 180 and 154.)
 inline void plan_linear(LinearPlan& plan, const esp_linear_params& p, const esp_linear_seq* seqs, int n_seqs, int workgroups) {
   plan.tiles.clear();
   plan.few = plan.parts = 0;
@@ -855,18 +868,19 @@ inline void plan_linear(LinearPlan& plan, const esp_linear_params& p, const esp_
   plan.few = int(plan.tiles.size());
   auto chunks = [&](int i) { return (seqs[i].rows + esp::kLinearChunk - 1) / esp::kLinearChunk; };
   const long long groups = (long long)p.H * (p.dv / esp::linear_cols(p.dv));
-  const int slots = std::max(2, workgroups);
+  const int per_cu = esp::linear_workgroups_per_cu(p.dk, p.dv), slots = std::max(per_cu, workgroups), units = slots / per_cu;
+  const LinearPrices prices = linear_prices(p);
   struct Work {
     int chunks, records;
   };
   using Free = std::pair<double, long long>;  // (when, how many slots)
-  auto finish = [&](const std::vector<Work>& work, double alone, double shared) {
-    const bool few = groups * (long long)work.size() <= slots / 2;
+  auto finish = [&](const std::vector<Work>& work, double end_of_one, double alone, double beside) {
+    const bool few = groups * (long long)work.size() <= units;
     std::priority_queue<Free, std::vector<Free>, std::greater<Free>> free_at;
-    free_at.push({0.0, few ? slots / 2 : slots});
+    free_at.push({0.0, few ? units : slots});
     double end = 0;
     for (const Work& w : work) {
-      const double cost = 7 + 0.9 * w.records + w.chunks * (few ? alone : shared);
+      const double cost = end_of_one + prices.record * w.records + w.chunks * (few ? alone : beside);
       for (long long left = groups; left > 0;) {
         const Free f = free_at.top();
         const long long take = std::min(left, f.second);
@@ -895,7 +909,8 @@ inline void plan_linear(LinearPlan& plan, const esp_linear_params& p, const esp_
         if (k + 1 < n) states.push_back({each, 0});
       }
     }
-    return finish(all, 4.5, 6.9) + (states.empty() ? 0.0 : 3 + finish(states, 2.5, 3.6));
+    const double front = states.empty() ? 0.0 : prices.front + finish(states, prices.state_end, prices.state_alone, prices.state_beside);
+    return front + finish(all, prices.end, prices.alone, prices.beside);
   };
   int most = std::max(1, longest);
   double best = many.empty() ? 0.0 : cost(most);
