@@ -139,7 +139,18 @@ template <int DK>
 __device__ __forceinline__ int row_part(int r, int c) {
   return r * (DK * 2) + ((DK == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7)) << 4);
 }
-__device__ __forceinline__ int col_part(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7) ^ ((r >> 3) & 2)) << 4); }
+__device__ __forceinline__ int col_part(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7) ^ ((r >> 3) & 2) ^ ((r >> 5) & 1)) << 4); }
+
+// Which 4 rows and which part of them piece b of a [64 rows][8 PARTS numbers] array is, such that 16 lanes one after the other hold 8 parts of
+// 8 rows: as 8 bytes each in the columns of such an array that is all of LDS's banks once.
+template <int PARTS>
+__device__ __forceinline__ int piece_group(int b) {
+  return PARTS == 16 ? ((b >> 5) << 1) | ((b >> 3) & 1) : b / PARTS;
+}
+template <int PARTS>
+__device__ __forceinline__ int piece_part(int b) {
+  return PARTS == 16 ? (b & 7) | ((b >> 1) & 8) : b % PARTS;
+}
 
 __device__ __forceinline__ int p_part(int r, int c) {
   return r < 32 ? r * 64 + ((c ^ ((r >> 2) & 3)) << 4) : 2048 + (r - 32) * 128 + ((c ^ ((r >> 1) & 7)) << 4);
@@ -336,9 +347,9 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
     const bool isK = STATE || it < 2 * DK;  // (alike in a wavefront)
     const int b = (isK ? it : it - 2 * DK) % (2 * DK);
     ld_kq[p] = uint32_t(__builtin_amdgcn_readfirstlane(2 * (isK ? a.k_ld : a.q_ld)));
-    from_kq[p] = reinterpret_cast<const char*>((isK ? a.K : a.Q) + size_t(kh) * DK) + (size_t(tile.row0) + 4 * (b / kParts)) * ld_kq[p] + 16 * (b % kParts);
+    from_kq[p] = reinterpret_cast<const char*>((isK ? a.K : a.Q) + size_t(kh) * DK) + (size_t(tile.row0) + 4 * piece_group<kParts>(b)) * ld_kq[p] + 16 * piece_part<kParts>(b);
   }
-  from_v = reinterpret_cast<const char*>(a.V + dv0) + (size_t(tile.row0) + 4 * (tid / vParts)) * ld_v + 16 * (tid % vParts);
+  from_v = reinterpret_cast<const char*>(a.V + dv0) + (size_t(tile.row0) + 4 * piece_group<vParts>(tid)) * ld_v + 16 * piece_part<vParts>(tid);
   // Row i of piece p (of NI: V's) of the next chunk; in the segment's last one rows behind the last are read as that one.
   auto fetch_row = [&](int p, int i) __attribute__((always_inline)) {
     if (p < NI) kq[p < NI ? p : 0][i] = *reinterpret_cast<const u32x4*>(from_kq[p < NI ? p : 0] + size_t(i) * ld_kq[p < NI ? p : 0]);
@@ -348,11 +359,11 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
   auto fetch_last = [&](int n, int ahead) __attribute__((always_inline)) {
 #pragma unroll
     for (int p = 0; p < NI; ++p) {
-      const int r = 4 * (((tid + T * p) % (2 * DK)) / kParts);
+      const int r = 4 * piece_group<kParts>((tid + T * p) % (2 * DK));
 #pragma unroll
       for (int i = 0; i < 4; ++i) kq[p][i] = *reinterpret_cast<const u32x4*>(from_kq[p] + int64_t(ahead + min(r + i, n - 1) - r) * int64_t(ld_kq[p]));
     }
-    const int r = 4 * (tid / vParts);
+    const int r = 4 * piece_group<vParts>(tid);
 #pragma unroll
     for (int i = 0; i < 4; ++i) vv[i] = *reinterpret_cast<const u32x4*>(from_v + int64_t(ahead + min(r + i, n - 1) - r) * int64_t(ld_v));
   };
@@ -413,10 +424,10 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
   if (!STATE && tile.rows < 64) {  // no whole chunk that could be read again: the first row stands for it
 #pragma unroll
     for (int p = 0; p < NI; ++p) {
-      from_kq[p] -= size_t(4 * (((tid + T * p) % (2 * DK)) / kParts)) * ld_kq[p];
+      from_kq[p] -= size_t(4 * piece_group<kParts>((tid + T * p) % (2 * DK))) * ld_kq[p];
       ld_kq[p] = 0;
     }
-    from_v -= size_t(4 * (tid / vParts)) * ld_v;
+    from_v -= size_t(4 * piece_group<vParts>(tid)) * ld_v;
     ld_v = 0;
   }
   double so_far = 0.0;
@@ -427,9 +438,9 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int it = tid + T * i;
-        if (STATE || it < 2 * DK) clear_past(kq[i], 4 * (it / kParts), n);
+        if (STATE || it < 2 * DK) clear_past(kq[i], 4 * piece_group<kParts>(it), n);
       }
-      clear_past(vv, 4 * (tid / vParts), n);
+      clear_past(vv, 4 * piece_group<vParts>(tid), n);
     }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -437,10 +448,10 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
       if (STATE && it >= 2 * DK) break;
       const bool isK = STATE || it < 2 * DK;
       const int b = isK ? it : it - 2 * DK;
-      if (!STATE) put_rows(kq[i], isK ? L::kK : L::kQ, b / kParts, b % kParts);
-      if (isK) put_columns(kq[i], L::kKT, b / kParts, b % kParts);
+      if (!STATE) put_rows(kq[i], isK ? L::kK : L::kQ, piece_group<kParts>(b), piece_part<kParts>(b));
+      if (isK) put_columns(kq[i], L::kKT, piece_group<kParts>(b), piece_part<kParts>(b));
     }
-    put_columns(vv, L::kVT, tid / vParts, tid % vParts);
+    put_columns(vv, L::kVT, piece_group<vParts>(tid), piece_part<vParts>(tid));
     // What the chunk's decays come to. Of a head's own they are those of the chunk before, but for the first and the last.
     if (a.decay_ld || c == 0 || n < 64) {
       const double s = a.decay_ld ? scan64(lane < n ? double(decay_log2(g_row)) : 0.0) : double(g_const) * min(lane + 1, n);
@@ -679,7 +690,7 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
 #pragma unroll 1
           for (int j = 0; j <= row; ++j) {
             const float p = unpack_lo<DT>(*reinterpret_cast<const uint16_t*>(lds + L::kP + p_part(row, j >> 3) + 2 * (j & 7)));
-            const uint32_t at = place(L::kVT + (32 * wave + 4 * hb) * 128 + (((j >> 3) ^ (2 * hb)) << 4) + 2 * (j & 7));
+            const uint32_t at = place(L::kVT + (32 * wave + 4 * hb) * 128 + (((j >> 3) ^ (2 * hb) ^ (wave & 1)) << 4) + 2 * (j & 7));
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               constexpr auto turn = [](int d) { return ((d >> 1) & 7) ^ ((d >> 3) & 2); };
@@ -748,7 +759,7 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
           d[t & 1] = f32x16{};
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
-            const u32x4 k = read((k_at ^ (ks << 5)) + t * 4096);
+            const u32x4 k = read((k_at ^ ((ks << 5) | ((t & 1) << 4))) + t * 4096);
 #pragma unroll
             for (int v = 0; v < NV; ++v) d[t & 1] = mfma32x16<DT>(k, vs[ks][v], d[t & 1]);
           }
@@ -768,7 +779,7 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
         u32x4 vs[2][NV], k[2][KT];
         auto step_in = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
-          for (int t = 0; t < KT; ++t) k[ks & 1][t] = read((k_at ^ (ks << 5)) + t * 4096);
+          for (int t = 0; t < KT; ++t) k[ks & 1][t] = read((k_at ^ ((ks << 5) | ((t & 1) << 4))) + t * 4096);
         };
         auto step_split = [&](int ks) __attribute__((always_inline)) {
           float x[8];
