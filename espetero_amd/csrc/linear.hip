@@ -139,7 +139,9 @@ template <int DK>
 __device__ __forceinline__ int row_part(int r, int c) {
   return r * (DK * 2) + ((DK == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7)) << 4);
 }
-__device__ __forceinline__ int col_part(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7) ^ ((r >> 3) & 2) ^ ((r >> 5) & 1)) << 4); }
+// (Of a read of 16 bytes a lane 16 lanes go at a time, one set those of rows 0 .. 3, 12 .. 15, 20 .. 27 of 32, the other the rest; written are eight
+// columns 8 apart. Both find different places this way.)
+__device__ __forceinline__ int col_part(int r, int c) { return r * 128 + ((c ^ ((r >> 1) & 7) ^ ((r >> 4) & 3)) << 4); }
 
 // Which 4 rows and which part of them piece b of a [64 rows][8 PARTS numbers] array is, such that 16 lanes one after the other hold 8 parts of
 // 8 rows: as 8 bytes each in the columns of such an array that is all of LDS's banks once.
@@ -690,10 +692,10 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
 #pragma unroll 1
           for (int j = 0; j <= row; ++j) {
             const float p = unpack_lo<DT>(*reinterpret_cast<const uint16_t*>(lds + L::kP + p_part(row, j >> 3) + 2 * (j & 7)));
-            const uint32_t at = place(L::kVT + (32 * wave + 4 * hb) * 128 + (((j >> 3) ^ (2 * hb) ^ (wave & 1)) << 4) + 2 * (j & 7));
+            const uint32_t at = place(L::kVT + (32 * wave + 4 * hb) * 128 + (((j >> 3) ^ (2 * hb) ^ (2 * (wave & 1))) << 4) + 2 * (j & 7));
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              constexpr auto turn = [](int d) { return ((d >> 1) & 7) ^ ((d >> 3) & 2); };
+              constexpr auto turn = [](int d) { return ((d >> 1) & 7) ^ ((d >> 4) & 1); };
               const int d = 8 * (e >> 2) + (e & 3);
               const float v = unpack_lo<DT>(*reinterpret_cast<const __attribute__((address_space(3))) uint16_t*>((at ^ (turn(d) << 4)) + d * 128));
               if (!(fabsf(v) < INFINITY)) O[rt][e] += p * v;
@@ -759,7 +761,7 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
           d[t & 1] = f32x16{};
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
-            const u32x4 k = read((k_at ^ ((ks << 5) | ((t & 1) << 4))) + t * 4096);
+            const u32x4 k = read((k_at ^ ((ks ^ (t & 1)) << 5)) + t * 4096);
 #pragma unroll
             for (int v = 0; v < NV; ++v) d[t & 1] = mfma32x16<DT>(k, vs[ks][v], d[t & 1]);
           }
@@ -779,7 +781,7 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
         u32x4 vs[2][NV], k[2][KT];
         auto step_in = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
-          for (int t = 0; t < KT; ++t) k[ks & 1][t] = read((k_at ^ ((ks << 5) | ((t & 1) << 4))) + t * 4096);
+          for (int t = 0; t < KT; ++t) k[ks & 1][t] = read((k_at ^ ((ks ^ (t & 1)) << 5)) + t * 4096);
         };
         auto step_split = [&](int ks) __attribute__((always_inline)) {
           float x[8];
