@@ -1,6 +1,7 @@
 // The C ABI (include/espetero_attn.h): argument checks, workspace carving and
 // kernel selection. Nothing here allocates device memory or synchronises.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -121,7 +122,7 @@ int check_shaped(const esp_attn_params* p, char* err, size_t errlen) {
   if (p->head_dim != 128 && p->head_dim != 256) return fail(err, errlen, ESP_EUNSUPPORTED, "head_dim %d: attention with shaped scores serves 128 and 256", p->head_dim);
   if (p->H / p->Hkv > 128) return fail(err, errlen, ESP_EUNSUPPORTED, "%d query heads to a KV head (at most 128)", p->H / p->Hkv);
   if (p->gate || p->bidi) return fail(err, errlen, ESP_EUNSUPPORTED, "attention with shaped scores takes neither a gate nor bidirectional rows");
-  if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return fail(err, errlen, ESP_EINVAL, "scale must be positive and finite");
+  if (!(p->scale >= 0x1p-64f && p->scale <= 0x1p64f)) return fail(err, errlen, ESP_EINVAL, "scale must be positive, from 2^-64 to 2^64");
   return ESP_OK;
 }
 
@@ -813,7 +814,8 @@ int esp_attn_shaped(const esp_attn_params* p, const esp_shape_params* shape, con
                     int32_t n_parts, int32_t n_rows, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen) {
   if (int rc = check_shaped(p, err, errlen)) return rc;
   if (!shape) return fail(err, errlen, ESP_EINVAL, "shape is NULL");
-  if (!(shape->cap >= 0.0f) || !std::isfinite(shape->cap)) return fail(err, errlen, ESP_EINVAL, "cap must be 0 or positive, and finite");
+  if (!(shape->cap >= 0.0f) || (shape->cap > 0.0f && !(shape->cap >= p->scale * 0x1p-60f && shape->cap <= 0x1p120f)))
+    return fail(err, errlen, ESP_EINVAL, "cap must be 0, or from 2^-60 of the scale to 2^120");
   if (n_tiles < 0 || n_trees < 0 || n_jobs < 0 || n_parts < 0 || n_rows < 0) return fail(err, errlen, ESP_EINVAL, "negative count");
   if (n_tiles == 0) return ESP_OK;
   if (!Q || !O || !tiles || !trees || !kv_pool) return fail(err, errlen, ESP_EINVAL, "Q, O, tiles, trees, kv_pool must not be NULL");
@@ -855,12 +857,21 @@ int esp_attn_shaped(const esp_attn_params* p, const esp_shape_params* shape, con
   a.scale_log2 = shape->cap > 0.0f ? float(2.0 * double(p->scale) * 1.4426950408889634 / double(shape->cap)) : p->scale * esp::kLog2e;
   a.cap_log2 = shape->cap * esp::kLog2e;
   if (shape->cap > 0.0f) {
-    constexpr double kTanh[5] = {0.9999985098838806, -0.33326974511146545, 0.13257454335689545, -0.050195250660181046, 0.013194181025028229};
+    // Behind |z| = t the terms from i on are more than 2^-25 of the sum: where a cap is so far from the scale that fp32 does not hold their
+    // coefficients, the polynomial ends in front of them (huge caps), or is not used (tiny ones).
+    constexpr double kTanh[5] = {0.9999996972994237, -0.33330212938002485, 0.13281112912937199, -0.050836244052251026, 0.013773716642020806};
+    constexpr double kUntil[5] = {0.0, 3e-4, 0.021, 0.09, 0.19};
     const double z = double(p->scale) / double(shape->cap);
-    double power = double(p->scale) * 1.4426950408889634;
-    for (int i = 0; i < 5; ++i, power *= z * z) a.tanh_c[i] = float(kTanh[i] * power);
-    // (of caps so far from the scale that a coefficient leaves fp32 none)
-    a.tanh_below = z > 0x1p-13 && z < 0x1p10 && p->scale > 0x1p-16 && p->scale < 0x1p16 ? float(0.7 / z) : 0.0f;
+    double power = double(p->scale) * 1.4426950408889634, until = 0.7;
+    int terms = 0;
+    for (; terms < 5; ++terms, power *= z * z) {
+      const double c = kTanh[terms] * power;
+      if (std::fabs(c) > FLT_MAX) until = 0.0;
+      if (std::fabs(c) > FLT_MAX || std::fabs(c) < FLT_MIN) break;
+      a.tanh_c[terms] = float(c);
+    }
+    if (terms < 5) until = std::min(until, kUntil[terms]);
+    a.tanh_below = float(std::min(until / z, double(FLT_MAX)));
   }
   a.kv_base = p->kv_base;
   hipStream_t st = static_cast<hipStream_t>(stream);

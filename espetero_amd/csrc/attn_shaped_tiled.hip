@@ -13,9 +13,9 @@
 // Scores: the bias is what the score product's accumulator starts from (without a cap; behind a cap it is the last step's addend). A cap
 // is tanh as an odd polynomial where all of a wavefront's scores of the stage are below 0.7 caps (six operations a score), else by an
 // exponential and a reciprocal (eleven). 2048 rows behind 8000 keys, 32 / 8 heads of 128 dims, bf16, 303 billion operations: plain 342 us, with
-// slopes 332, with a cap 405, with both 445 (680 TFLOP/s): there the vector units are busy for six sevenths of the loop. Short ranges are bound
-// by their ends: three prompts of 500 to 2000 rows in six documents each take 57 us, of which a tile's seven stages are a third, its first
-// loads from memory another.
+// slopes 332, with a cap 405, with both 400 to 450 by the card's clock (0.67 to 0.76 PFLOP/s): there the vector units are busy for six sevenths of
+// the loop. Short ranges are bound by their ends: three prompts of 500 to 2000 rows in six documents each take 52 to 57 us, of which a tile's
+// seven stages are a third, its first loads from memory another.
 //
 // P enters its product as one number of the storage type, as is usual: an output's error is then at most 1.4 times what its own rounding
 // makes it. As the sum of two, as in the streaming kernel, which waits for memory anyway, P . V would be twice the matrix work here.
@@ -230,7 +230,6 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
 
   // The bias of index e of this lane's half, linear in the key: right up to the row's own key.
   auto bias_at = [&](int h) { return slope * float(key_of(h) + 8 * hb - qpos); };
-  auto score_operand = [&](int h, int g) { return lds_read((k_at + uint32_t(h & (kRing - 1)) * L::kStage) ^ uint32_t(g << 5)); };
   auto value_operand = [&](uint32_t va, int g) { return lds_read(va + (g / NT) * L::kRun + (g % NT) * 1024); };
   auto values_of = [&](int h) {
     uint32_t va = v_at + uint32_t(h & (kRing - 1)) * L::kStage;
@@ -281,22 +280,10 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     for (int e = 1; e < 16; ++e) m = fmaxf(m, fabsf(x[e]));
     return m;
   };
+  auto bias_e = [&](int e, float b) { return BIAS ? __builtin_fmaf(slope, float(16 * (e >> 3) + (e & 7)), b) : 0.0f; };
   auto shape_e = [&](float x, int e, float b, bool low) __attribute__((always_inline)) {
-    if constexpr (CAP) {
-      const float at = BIAS ? __builtin_fmaf(slope, float(16 * (e >> 3) + (e & 7)), b) : 0.0f;
-      if (low) {
-        const float u = x * x;
-        float p = __builtin_fmaf(u, a.tanh_c[4], a.tanh_c[3]);
-        p = __builtin_fmaf(u, p, a.tanh_c[2]);
-        p = __builtin_fmaf(u, p, a.tanh_c[1]);
-        p = __builtin_fmaf(u, p, a.tanh_c[0]);
-        return __builtin_fmaf(x, p, at);
-      }
-      const float r = __builtin_amdgcn_rcpf(fast_exp2(x * a.scale_log2) + 1.0f);
-      return __builtin_fmaf(-2.0f * a.cap_log2, r, a.cap_log2 + at);
-    } else {
-      return x;
-    }
+    if constexpr (!CAP) return x;
+    return low ? shaped_tanh_low(a, x, bias_e(e, b)) : shaped_tanh_high(a, x, bias_e(e, b));
   };
   // With a cap scores are in log2 units, else still in those of the products.
   const float unit = CAP ? 1.0f : a.scale_log2;
@@ -453,14 +440,14 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     if (within(h - 1, v0, v1)) {
       mfma_settle(S);
       const float b = bias_at(h - 1);
-      // (By the exponential whatever the scores: those of keys that a row does not see may be anything, and choose nothing.)
+      // (Each score by its own size: those of keys that a row does not see may be anything, and choose nothing for the others.)
       const int lo = max(rg.from, sight.from), n = max(0, min(rg.end, sight.end) - lo);
       const int at0 = key_of(h - 1) + 8 * (here(lane) >> 5), at = at0 - lo;
       float mx = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int k = 16 * (e >> 3) + (e & 7);
-        float x = shape_e(S[e], e, b, false);
+        float x = CAP ? shaped_score<CAP>(a, S[e]) + bias_e(e, b) : S[e];
         if constexpr (BIAS) x -= 2.0f * slope * fmaxf(float(at0 + k - qpos), 0.0f);
         S[e] = uint32_t(at + k) < uint32_t(n) ? x : -INFINITY;  // the row sees the keys [lo, lo + n)
         mx = fmaxf(mx, S[e]);

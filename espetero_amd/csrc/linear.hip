@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void linear_few_kernel(const LinearArgs a) {
   __shared__ __attribute__((aligned(16))) float out[kLinearFew][4][DVB];
   const int blocks = a.dv / DVB, h = blockIdx.x / blocks, c0 = (blockIdx.x - h * blocks) * DVB;
   const esp_linear_tile tile = a.tiles[blockIdx.y];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = min(tile.rows, kLinearFew);
   const int col = c0 + 4 * int(threadIdx.x % LPR), g = threadIdx.x / LPR;
   const size_t at = size_t(h) * DK * a.dv + col, slot = size_t(a.H) * DK * a.dv;
   f32x4 s[NK];
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void linear_few_kernel(const LinearArgs a) {
     for (int i = 0; i < NK; ++i) s[i] = f32x4{0, 0, 0, 0};
   }
   const int kh = h / a.group;
-  for (int i = threadIdx.x; i < tile.rows * (DK / 2); i += 256) {
+  for (int i = threadIdx.x; i < rows * (DK / 2); i += 256) {
     const int m = i / (DK / 2), d = 2 * (i - m * (DK / 2));
     const uint32_t q = *reinterpret_cast<const uint32_t*>(a.Q + size_t(tile.row0 + m) * a.q_ld + size_t(kh) * DK + d);
     const uint32_t k = *reinterpret_cast<const uint32_t*>(a.K + size_t(tile.row0 + m) * a.k_ld + size_t(kh) * DK + d);
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void linear_few_kernel(const LinearArgs a) {
     qk[1][m][d + 1] = unpack_hi<DT>(k);
   }
   __syncthreads();
-  for (int m = 0; m < tile.rows; ++m) {
+  for (int m = 0; m < rows; ++m) {
     const int row = tile.row0 + m;
     const float f = fast_exp2(decay_log2(a.decay[size_t(row) * a.decay_ld + h]));
     const u32x2 vb = *reinterpret_cast<const u32x2*>(a.V + size_t(row) * a.v_ld + size_t(h) * a.dv + col);
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void linear_few_kernel(const LinearArgs a) {
     for (int i = 0; i < NK; ++i) *reinterpret_cast<f32x4*>(to + size_t(g + RG * i) * a.dv) = s[i];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < tile.rows * LPR; i += 256) {
+  for (int i = threadIdx.x; i < rows * LPR; i += 256) {
     const int m = i / LPR, c = 4 * (i - m * LPR);
     f32x4 o = *reinterpret_cast<const f32x4*>(&out[m][0][c]);
 #pragma unroll

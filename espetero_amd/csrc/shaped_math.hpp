@@ -23,7 +23,7 @@ struct ShapedArgs {
   float scale_log2;  // without a cap: scale in log2 units; with one: 2 scale log2(e) / cap
   float cap_log2;    // cap in log2 units
   // cap tanh(scale q.k / cap) in log2 units as q.k times a polynomial of (q.k)^2, for |q.k| < tanh_below. tanh(z) / z fitted in z^2 for
-  // |z| < 0.7, 1.5e-7 of tanh off in fp32.
+  // |z| < 0.7: six steps of 2^-24 of tanh off in fp32. 0, or fewer terms and a nearer bound, where fp32 does not hold the coefficients.
   float tanh_c[5], tanh_below;
   uint64_t kv_base;
 };
@@ -48,14 +48,24 @@ __device__ __forceinline__ Sight shaped_sight(const ShapedArgs& a, int row, int 
   return s;
 }
 
-// x = scale q.k through the cap, in log2 units: cap tanh(x / cap) = cap (1 - 2 / (exp(2 x / cap) + 1)), which holds for infinite x too.
+// x = scale q.k through the cap, in log2 units. cap tanh(x / cap) = cap (1 - 2 / (exp(2 x / cap) + 1)) holds for infinite x too, but is off by as
+// many steps of the cap as of x: small x go through the polynomial.
+__device__ __forceinline__ float shaped_tanh_low(const ShapedArgs& a, float dot, float add) {
+  const float u = dot * dot;
+  float p = __builtin_fmaf(u, a.tanh_c[4], a.tanh_c[3]);
+  p = __builtin_fmaf(u, p, a.tanh_c[2]);
+  p = __builtin_fmaf(u, p, a.tanh_c[1]);
+  p = __builtin_fmaf(u, p, a.tanh_c[0]);
+  return __builtin_fmaf(dot, p, add);
+}
+__device__ __forceinline__ float shaped_tanh_high(const ShapedArgs& a, float dot, float add) {
+  return __builtin_fmaf(-2.0f * a.cap_log2, __builtin_amdgcn_rcpf(fast_exp2(dot * a.scale_log2) + 1.0f), a.cap_log2 + add);
+}
 template <bool CAP>
 __device__ __forceinline__ float shaped_score(const ShapedArgs& a, float dot) {
-  if constexpr (CAP) {
-    return a.cap_log2 - 2.0f * a.cap_log2 * __builtin_amdgcn_rcpf(fast_exp2(dot * a.scale_log2) + 1.0f);
-  } else {
-    return dot * a.scale_log2;
-  }
+  if constexpr (!CAP) return dot * a.scale_log2;
+  const float high = shaped_tanh_high(a, dot, 0.0f), low = shaped_tanh_low(a, dot, 0.0f);
+  return fabsf(dot) < a.tanh_below ? low : high;
 }
 
 // The keys a tile scans, [lo, hi) in cache positions, of those that its rows see at all, [from, end): its cached range and, on a `last` tile,

@@ -81,13 +81,16 @@ class ShapedCase:
         """(O, how far from it an output may be) in float64, [n_rows][H * hd] with NaN in rows of no sequence.
 
         A score is off by e = 2^-24 ((hd + 4) scale max sum |q| |k|, the products' sum and its factor; 6 |x|, the operations on it and its
-        distance to the row's reference in log2 units; 8 cap, the cap's exponential, sum, reciprocal and product; 2 |bias|), the weight by a
+        distance to the row's reference in log2 units; 16 max |x| for a polynomial within 6 steps and its operations, or where scores of the case come
+        to 0.69 caps 8 cap, the cap's exponential, sum, reciprocal and product; 2 |bias|), the weight by a
         factor of 1 + d, |d| <= u + 2 e with u half a step of the storage type for its own rounding; sums over n keys in fp32 add n 2^-24
         (weights half of that again). With A = sum p |v| the output is off by (u + 2 e + 1.5 n 2^-24) A and its rounding u |O|. A row that
         sees nothing gets zeros."""
         G, hd, u = self.H // self.Hkv, self.hd, HALF[self.dtype]
         f = lambda x: ob.to_f32(x, self.dtype).astype(np.float64)  # noqa: E731
         Q = f(self.Q)[:, :self.H * hd].reshape(-1, self.H, hd)
+        live = np.isfinite(Q[:, 0, 0])
+        largest = max(np.abs(np.einsum("khd,rhd->rkh", np.repeat(f(K), G, 1), np.nan_to_num(Q[live]))).max() for K in self.K) * self.scale if self.cap else 0
         O = np.full((self.n_rows, self.H, hd), np.nan)
         tol = np.full_like(O, np.nan)
         for i, (P, M) in enumerate(self.seqs):
@@ -105,8 +108,8 @@ class ShapedCase:
                     x = k @ q * self.scale
                     e = (hd + 4) * self.scale * (np.abs(k) @ np.abs(q)).max()
                     if self.cap:
+                        e += 8 * self.cap if largest >= 0.69 * self.cap else 16 * np.abs(x).max()
                         x = self.cap * np.tanh(x / self.cap)
-                        e += 8 * self.cap
                     if self.slopes is not None:
                         b = float(self.slopes[h]) * ago
                         x = x - b

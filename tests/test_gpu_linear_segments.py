@@ -101,3 +101,17 @@ def test_states_of_few_sizes_across_segments(dtype):
         V[128:] *= second
         c.V = ob.from_f32(V.reshape(-1), dtype).reshape(256, -1)
         check(c, cut(Run(c), 1)())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,r0", [(7, 3), (300, 37), (300, 64), (300, 200)])
+def test_a_decay_that_is_no_number_stays_behind_its_row(rows, r0, dtype):
+    """NaN as a row's log decay: that row and those behind it, of that head, have no value; the others keep their bits."""
+    c = LinearCase(2, 2, 64, 64, dtype, [(rows, 0, 0), (rows, 1, 1)], seed=37, row_decay=True)
+    run = (lambda: Run(c)()) if rows < 9 else (lambda: cut(Run(c), 2)())
+    clean, clean_states = run()
+    c.decay[r0, 1] = np.nan
+    bits, states = run()
+    assert (bits[:r0] == clean[:r0]).all() and (bits[rows:] == clean[rows:]).all() and (bits[:, :64] == clean[:, :64]).all()
+    assert np.isnan(ob.to_f32(bits[r0:rows, 64:], dtype)).all() and np.isnan(states[0, 1]).all()
+    assert (states[0, 0] == clean_states[0, 0]).all() and (states[1] == clean_states[1]).all()

@@ -132,6 +132,14 @@ def test_sharp_softmax_and_large_caps():
         check(c, Run(c)())
 
 
+@pytest.mark.parametrize("cap", [2.0 ** 120, 1e30, 1e12, 1e8, 1e5, 1000.0, 0.1, 1e-4, 1e-12])
+def test_caps_far_from_the_scale(cap):
+    """Of a cap far above the scores nothing is left but the scores, of one far below their signs."""
+    for hd, seqs in ((128, [(300, 1), (40, 3)]), (256, [(90, 60), (0, 33)]), (128, [(50, 150)])):
+        c = ShapedCase(8, 2, hd, F16, 16, seqs, seed=18, cap=cap, bias=hd == 256)
+        check(c, Run(c)())
+
+
 def test_rows_outside_the_trees_and_wide_strides():
     for hd in (128, 256):
         c = ShapedCase(8, 2, hd, BF16, 32, [(70, 2), (0, 40)], seed=6, q_ld=8 * hd + 24, base_gap=5, cap=10.0)

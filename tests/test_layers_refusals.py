@@ -188,7 +188,7 @@ S = abi.ShapeParams(None, None, 0.0, 0)
     (dict(head_dim=512, q_ld=4096, kv_ld=2048), 2, "head_dim"), (dict(head_dim=64), 2, "head_dim"), (dict(H=7), 1, "multiple"), (dict(dtype=2), 1, "dtype"),
     (dict(bt=24), 1, "bt"), (dict(q_ld=8), 1, "q_ld"), (dict(q_ld=1028), 1, "q_ld"), (dict(kv_base=4), 1, "kv_base"), (dict(gate=X), 2, "gate"),
     (dict(bidi=1), 2, "bidirectional"), (dict(scale=0.0), 1, "scale"), (dict(scale=-1.0), 1, "scale"), (dict(scale=float("nan")), 1, "scale"),
-    (dict(scale=float("inf")), 1, "scale"), (dict(window=-1), 1, "window"), (dict(H=258, Hkv=2, q_ld=258 * 128), 2, "128"), (dict(rows_per_tile=0), 2, "rows_per_tile"),
+    (dict(scale=float("inf")), 1, "scale"), (dict(scale=1e-30), 1, "scale"), (dict(scale=1e30), 1, "scale"), (dict(window=-1), 1, "window"), (dict(H=258, Hkv=2, q_ld=258 * 128), 2, "128"), (dict(rows_per_tile=0), 2, "rows_per_tile"),
     (dict(rows_per_tile=65), 2, "rows_per_tile"), (dict(rows_per_tile=BIG), 2, "rows_per_tile")])
 def test_shaped_refuses_parameters(p, rc, word):
     got = call("esp_attn_shaped", *shaped_args(shaped_params(**p), S))
@@ -213,7 +213,7 @@ def test_shaped_refuses_arguments(a, rc, word):
 
 
 def test_shaped_refuses_shapes():
-    for cap in (-1.0, float("nan"), float("inf"), float("-inf")):
+    for cap in (-1.0, float("nan"), float("inf"), float("-inf"), 3e38, 1e-30):
         got = call("esp_attn_shaped", *shaped_args(shaped_params(), abi.ShapeParams(None, None, cap, 0)))
         assert got[0] == 1 and "cap" in got[1], got
     got = call("esp_attn_shaped", *shaped_args(shaped_params(), abi.ShapeParams(None, X + 4, 0.0, 0)))
