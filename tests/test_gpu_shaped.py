@@ -126,6 +126,42 @@ def test_spans_of_any_numbers_and_rows_that_see_nothing(hd, rows_per_tile):
         assert (bits[[2, 3]] == 0).all()
 
 
+def cut(r, each):
+    """Run r's pass with every tile in parts of `each` stages of 32 keys, cached ones and the pass's own alike."""
+    c, p = r.case, r.p
+    tiles, jobs, parts = [], [], 0
+    for i, (base, P, table, M) in enumerate(c.trees.tolist()):
+        for m in range(0, M, p.rows_per_tile):
+            lo = max(0, P + m - c.window + 1) // 16 * 16 if c.window else 0
+            hi = P + min(M, m + p.rows_per_tile)
+            n = -(-(hi - lo) // (32 * each))
+            if n > 1:
+                jobs.append((base + m, min(M - m, p.rows_per_tile), parts, n))
+            for k in range(n):
+                x, y, end = lo + 32 * each * k, lo + 32 * each * (k + 1), k + 1 == n
+                last = 1 if end else y - P + 1 if y > P else 0
+                tiles.append((i, base + m, min(x, P), P if end else min(y, P), parts + k if n > 1 else -1, last, max(0, x - P), 0))
+            parts += n if n > 1 else 0
+    tiles, jobs = np.array(tiles, abi.TILE_DT), np.array(jobs, abi.COMBINE_DT) if jobs else np.zeros(0, abi.COMBINE_DT)
+    device.validate(p, tiles, c.trees, jobs, parts, c.n_rows, c.block_list, c.n_blocks, shaped=True)
+    r.sp.tiles, r.sp.n_tiles, r.sp.jobs, r.sp.n_jobs, r.sp.n_parts = device.to_dev(tiles), len(tiles), device.to_dev(jobs) if len(jobs) else None, len(jobs), parts
+    nbytes = abi.attn_lib().esp_attn_shaped_workspace_bytes(C.byref(p), parts)
+    r.sp.workspace = torch.full((max(nbytes, 16),), 0xff, dtype=torch.uint8, device="cuda")    # NaN: nothing is merged that was not written
+    return r
+
+
+@pytest.mark.parametrize("hd,heads", [(128, (8, 2)), (256, (4, 2)), (128, (7, 1))])
+@pytest.mark.parametrize("window,ring", [(0, False), (60, False), (60, True)])
+@pytest.mark.parametrize("each", [1, 2, 5])
+def test_any_parts(each, window, ring, hd, heads):
+    """Parts that some rows, or all, see nothing of among them: spans leave them other keys."""
+    seqs = [(100, 70), (0, 90), (31, 20), (16, 40)] if not ring else [(100, 20), (0, 24), (31, 20)]
+    spans = [documents(P, M, [0, 40, 64, 80], 50) if i % 2 == 0 else [(3, P + M)] * M for i, (P, M) in enumerate(seqs)]
+    for sp in (None, spans):
+        c = ShapedCase(*heads, hd, BF16, 16, seqs, window=window, ring=ring, spans=sp, cap=20.0, bias=True, seed=19)
+        check(c, cut(Run(c), each)())
+
+
 def test_sharp_softmax_and_large_caps():
     for cap in (0.0, 1.0, 200.0):
         c = ShapedCase(8, 2, 128, F16, 16, [(500, 1), (90, 3), (60, 70)], seed=5, sharp=12.0, cap=cap)
