@@ -10,7 +10,8 @@
 // look for a new maximum, P . V of stage h - 2 under the exponentials of stage h - 1, so that matrix and vector units work beside each other
 // within a wavefront too. Turns that are not all of that - the ends of a range, masked stages - run the three one by one.
 //
-// Scores: the bias is what the score product's accumulator starts from (without a cap; behind a cap it is the last step's addend). A cap
+// Scores: the bias is what the score product's accumulator starts from (without a cap; behind a cap it is the last step's addend), but for
+// what it has of the stage, which is taken from the reference. A cap
 // is tanh as an odd polynomial where all of a wavefront's scores of the stage are below 0.7 caps (six operations a score), else by an
 // exponential and a reciprocal (eleven). 2048 rows behind 8000 keys, 32 / 8 heads of 128 dims, bf16, 303 billion operations: plain 342 us, with
 // slopes 332, with a cap 405, with both 400 to 450 by the card's clock (0.67 to 0.76 PFLOP/s): there the vector units are busy for six sevenths of
@@ -228,32 +229,32 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   f32x16 s[2] = {f32x16{}, f32x16{}};
   u32x4 P[2][2] = {};
 
-  // The bias of index e of this lane's half, linear in the key: right up to the row's own key.
-  auto bias_at = [&](int h) { return slope * float(key_of(h) + 8 * hb - qpos); };
+  // The bias of index e of this lane's half, linear in the key: right up to the row's own key. A part for the index, which never changes, and
+  // one for the stage, which joins the scores where they are taken from the reference.
+  auto bias_at = [&](int h) { return BIAS ? slope * float(key_of(h) + 8 * hb - qpos) : 0.0f; };
+  f32x16 bias;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    bias[e] = BIAS ? slope * float(16 * (e >> 3) + (e & 7)) : 0.0f;
+    if constexpr (BIAS && HD == 128) asm("" : "+v"(bias[e]));
+  }
   auto value_operand = [&](uint32_t va, int g) { return lds_read(va + (g / NT) * L::kRun + (g % NT) * 1024); };
   auto values_of = [&](int h) {
     uint32_t va = v_at + uint32_t(h & (kRing - 1)) * L::kStage;
     asm("" : "+v"(va));  // one register, the operands' places as immediates
     return va;
   };
-  // S = K Q^T of stage h (+ bias / scale), operands read two ahead; `between` is work to be laid under it.
+  // S = K Q^T of stage h (+ the indexes' bias / scale), operands read two ahead; `between` is work to be laid under it.
   auto score = [&](int h, f32x16& to, auto between) __attribute__((always_inline)) {
     u32x4 k[3];
     const uint32_t ka = k_at + uint32_t(h & (kRing - 1)) * L::kStage;
     auto fetch = [&](int g) { k[g % 3] = lds_read(ka ^ uint32_t(g << 5)); };
     fetch(0);
     fetch(1);
-    if constexpr (BIAS && !CAP) {
-      const float b = bias_at(h);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) to[e] = __builtin_fmaf(slope, float(16 * (e >> 3) + (e & 7)), b);
-    } else {
-      to = f32x16{};
-    }
 #pragma unroll
     for (int g = 0; g < KS; ++g) {
       if (g + 2 < KS) fetch(g + 2);
-      to = mfma32x16<DT>(k[g % 3], qf[g], to);
+      to = mfma32x16<DT>(k[g % 3], qf[g], g > 0 ? to : BIAS && !CAP ? bias : f32x16{});
       between(g);
       __builtin_amdgcn_sched_barrier(0x406);  // (vector and scalar work may cross; operands' reads and products keep their order)
     }
@@ -280,15 +281,14 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     for (int e = 1; e < 16; ++e) m = fmaxf(m, fabsf(x[e]));
     return m;
   };
-  auto bias_e = [&](int e, float b) { return BIAS ? __builtin_fmaf(slope, float(16 * (e >> 3) + (e & 7)), b) : 0.0f; };
-  auto shape_e = [&](float x, int e, float b, bool low) __attribute__((always_inline)) {
+  auto shape_e = [&](float x, int e, bool low) __attribute__((always_inline)) {
     if constexpr (!CAP) return x;
-    return low ? shaped_tanh_low(a, x, bias_e(e, b)) : shaped_tanh_high(a, x, bias_e(e, b));
+    return low ? shaped_tanh_low(a, x, bias[e]) : shaped_tanh_high(a, x, bias[e]);
   };
   // With a cap scores are in log2 units, else still in those of the products.
   const float unit = CAP ? 1.0f : a.scale_log2;
-  auto exponentials = [&](const f32x16& x, u32x4 (&p)[2]) __attribute__((always_inline)) {
-    const float off = m_ref == -INFINITY ? 0.0f : m_ref;
+  auto exponentials = [&](const f32x16& x, u32x4 (&p)[2], float stage) __attribute__((always_inline)) {  // stage: the stage's bias, log2 units
+    const float off = (m_ref == -INFINITY ? 0.0f : m_ref) - stage;
     float lx = 0.0f;
 #pragma unroll
     for (int sb = 0; sb < 2; ++sb)
@@ -447,15 +447,15 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int k = 16 * (e >> 3) + (e & 7);
-        float x = CAP ? shaped_score<CAP>(a, S[e]) + bias_e(e, b) : S[e];
-        if constexpr (BIAS) x -= 2.0f * slope * fmaxf(float(at0 + k - qpos), 0.0f);
+        float x = CAP ? shaped_score<CAP>(a, S[e]) + bias[e] : S[e];
+        if constexpr (BIAS) x += b - 2.0f * slope * fmaxf(float(at0 + k - qpos), 0.0f);
         S[e] = uint32_t(at + k) < uint32_t(n) ? x : -INFINITY;  // the row sees the keys [lo, lo + n)
         mx = fmaxf(mx, S[e]);
       }
       mx = max_halves(mx) * unit;
       const bool up = mx > m_ref + kSlack;  // from -inf on: the first key that the row sees
       if (__any(up)) follow_reference(move_reference(mx, up));
-      exponentials(S, W);
+      exponentials(S, W, 0.0f);
     }
     if (within(h, v0, v1)) {
       score(h, S, [](int) {});
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
       score(h, to, [&](int g) __attribute__((always_inline)) {
         constexpr int PER = 16 / KS;
 #pragma unroll
-        for (int e = g * PER; e < (g + 1) * PER; ++e) of[e] = shape_e(of[e], e, b, low);
+        for (int e = g * PER; e < (g + 1) * PER; ++e) of[e] = shape_e(of[e], e, low);
         // Requests one by one: together at the turn's beginning they stand in line behind those of the other wavefronts.
         if (g % 2 == 1 && g < 2 * LOADS) request(h + lead, g / 2);
       });
@@ -491,13 +491,13 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     }
     advance();
     const int id = block_id();
-    mx = max_halves(mx) * unit;
+    mx = max_halves(mx + b) * unit;
     const bool up = mx > m_ref + kSlack;
     const bool moved = __any(up);
     float c = 1.0f;
     if (__builtin_expect(moved, 0)) c = move_reference(mx, up);
     weigh(h - 2, had, [](int) {});
-    exponentials(of, W);
+    exponentials(of, W, b * unit);
     lay_out<2 * NT, 52 / (2 * NT)>();
     asm volatile("" : "+v"(W[0]), "+v"(W[1]), "+v"(l_run));  // (made here, not where the next turn first needs them)
     if (__builtin_expect(moved, 0)) follow_reference(c);
