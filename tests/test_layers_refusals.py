@@ -303,6 +303,28 @@ def test_shaped_plans_cover_every_key_once(pairs, heads, window):
         assert len(set(parts)) == len(parts) == n_parts == jobs["nparts"].sum()
 
 
+@pytest.mark.parametrize("heads", [(32, 1, 256), (128, 1, 128)])
+@pytest.mark.parametrize("P", [0, 1, 15, 16, 31, 32, 64, 96, 128, 500, 512, 4096, 16000])
+def test_shaped_plans_grow_with_a_chain(P, heads):
+    """Single tokens on the tiled kernel: open-ended tiles cover every key once, however far the chain has moved on."""
+    p = synth.make_params(*heads, abi.ESP_F16, 16, rows_per_tile=1)
+    trees = np.array([(0, P, 0, 1), (1, P // 2, P // 16 + 4, 1)], abi.TREE_DT)
+    for resident in (8, 256, 5000):
+        tiles, jobs, n_parts = host.plan_tiles(trees, abi.PlanGroups(1, p, shaped=True), 0, None, host.options_mi355x(1, resident))
+        tiles = host.open_ended(tiles, trees)
+        assert P < 4096 or resident < 256 or n_parts > 2
+        for s in (0, 1, 2, 15, 16, 17, 100):
+            for i, t in enumerate(trees):
+                now, spans = int(t["P"]) + s, []
+                for x in tiles[tiles["tree"] == i]:                           # what the kernel makes of a record
+                    k1 = min(int(x["k1"]), now)
+                    lo = now + int(x["b0"]) if x["last"] and k1 <= x["k0"] else int(x["k0"])
+                    hi = k1 if not x["last"] else now + int(x["last"]) - 1 if x["last"] >= 2 else now + 1
+                    spans.append((lo, min(hi, now + 1)))
+                spans.sort()
+                assert spans[0][0] == 0 and spans[-1][1] == now + 1 and all(a[1] == b[0] for a, b in zip(spans, spans[1:])), (s, spans)
+
+
 def test_shaped_pass_refuses_spans_of_another_shape():
     p = shaped_params()
     trees, tiles = np.array([(0, 40, 0, 1)], abi.TREE_DT), np.array([(0, 0, 0, 40, -1, 1, 0, 1)], abi.TILE_DT)
