@@ -309,19 +309,40 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
         }
     }
   } else if (!STATE) {
-    double since = 0.0;  // log2 of the decays of the segments between
-    for (int j = tile.before; j >= 1; --j) {
-      const float f = fast_exp2(float(since));
-      const float* from = record(tile.part + j);
+    // Lane k: what the decays of the k segments between come to. (64 segments at a time; half a record is on its way while the one in
+    // front of it joins.)
+    constexpr int HT = KT / 2;
+    f32x4 x[2][HT][4];
+    auto load = [&](int k, int half) __attribute__((always_inline)) {
+      const float* from = record(tile.part + tile.before - k) + half * (HT * 1024);
 #pragma unroll
-      for (int t = 0; t < KT; ++t)
+      for (int t = 0; t < HT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(from + (t * 4 + i) * 256);
+        for (int i = 0; i < 4; ++i) x[half][t][i] = *reinterpret_cast<const f32x4*>(from + (t * 4 + i) * 256);
+    };
+    auto join = [&](float f, int half) __attribute__((always_inline)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) S[t][4 * i + e] = __builtin_fmaf(x[e], f, S[t][4 * i + e]);
-        }
-      since += a.part_totals[size_t(tile.part + j) * a.H + h];
+      for (int t = 0; t < HT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[half * HT + t][4 * i + e] = __builtin_fmaf(x[half][t][i][e], f, S[half * HT + t][4 * i + e]);
+    };
+    double front = 0.0;
+    load(0, 0);
+    for (int k0 = 0; k0 < tile.before; k0 += 64) {
+      const int k = k0 + lane - 1;
+      const double sums = front + scan64(k >= 0 && k < tile.before ? a.part_totals[size_t(tile.part + tile.before - k) * a.H + h] : 0.0);
+      const int fs = __builtin_bit_cast(int, fast_exp2(float(sums)));
+      front = lane_of(sums, 63);
+#pragma unroll 1
+      for (int i = 0; i < min(64, tile.before - k0); ++i) {
+        const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(fs, i));
+        load(k0 + i, 1);
+        join(f, 0);
+        load(min(k0 + i + 1, tile.before - 1), 0);
+        join(f, 1);
+      }
     }
   }
   auto keep_record = [&](int r) {

@@ -38,6 +38,14 @@ def test_any_segments(each, dims, dtype):
     check(c, cut(Run(c), each)())
 
 
+@pytest.mark.parametrize("dims", [(64, 64), (128, 128)])
+def test_more_segments_than_lanes(dims):
+    """135 and 130 segments of a chunk each, whose decays a wavefront sums up 64 at a time."""
+    for dtype, rows in ((F16, 64 * 135 - 3), (BF16, 64 * 130)):
+        c = LinearCase(1, 1, *dims, dtype, [(rows, 0, 0)], seed=38, decay=-0.002)
+        check(c, cut(Run(c), 1)())
+
+
 @pytest.mark.parametrize("decay", [0.0, -1e-4, -3.0, -60.0, -200.0, float("-inf"), 1.0])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_decays_across_segments(decay, dtype):
