@@ -37,6 +37,7 @@ namespace esp {
 namespace {
 constexpr int kRing = 4;
 constexpr float kSlack = 8.0f;  // a row's reference moves when a score exceeds it by more (log2 units): P stays below 2^8
+constexpr float kMost = 256.0f; // and where that is not looked for, when a lane's weights of a stage come to more
 
 template <int HD>
 struct TiledLds {
@@ -287,8 +288,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   };
   // With a cap scores are in log2 units, else still in those of the products.
   const float unit = CAP ? 1.0f : a.scale_log2;
-  auto exponentials = [&](const f32x16& x, u32x4 (&p)[2], float stage) __attribute__((always_inline)) {  // stage: the stage's bias, log2 units
-    const float off = (m_ref == -INFINITY ? 0.0f : m_ref) - stage;
+  auto exponentials = [&](const f32x16& x, u32x4 (&p)[2]) __attribute__((always_inline)) {
+    const float off = m_ref == -INFINITY ? 0.0f : m_ref;
     float lx = 0.0f;
 #pragma unroll
     for (int sb = 0; sb < 2; ++sb)
@@ -455,7 +456,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
       mx = max_halves(mx) * unit;
       const bool up = mx > m_ref + kSlack;  // from -inf on: the first key that the row sees
       if (__any(up)) follow_reference(move_reference(mx, up));
-      exponentials(S, W, 0.0f);
+      exponentials(S, W);
     }
     if (within(h, v0, v1)) {
       score(h, S, [](int) {});
@@ -464,10 +465,22 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     locate(id);
   };
   // A turn with all three stages to do, the last two seen whole by all rows of the tile: scores of stage h to `to`, those of stage h - 1 in
-  // `of`, weights of stage h - 2 in `had`, of stage h - 1 to `W`.
+  // `of`, weights of stage h - 2 in `had`, of stage h - 1 to `W`. No maximum is taken: all weights are positive, so a lane's sum bounds them, and only
+  // where one is too large (or the row has no reference yet) does the reference move and the stage's weights are made again.
   auto whole_turn = [&](int h, f32x16& to, f32x16& of, const u32x4 (&had)[2], u32x4 (&W)[2]) __attribute__((always_inline)) {
-    const float b = bias_at(h - 1);
-    float mx;
+    const float stage = bias_at(h - 1) * unit;
+    float off = m_ref - stage, sum[2] = {0.0f, 0.0f};
+    auto weights = [&](int sb) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = 8 * sb + 2 * e;
+        const float p0 = fast_exp2(CAP ? of[at] - off : __builtin_fmaf(of[at], unit, -off));
+        const float p1 = fast_exp2(CAP ? of[at + 1] - off : __builtin_fmaf(of[at + 1], unit, -off));
+        W[sb][e] = pack2<DT>(p0, p1);
+        sum[sb] = sum2<DT>(W[sb][e], sum[sb]);  // (the weights as the product takes them)
+      }
+    };
+    // Under the score products: the scores' shape, or without a cap half of the weights.
     auto shaped = [&](bool low) __attribute__((always_inline)) {
       score(h, to, [&](int g) __attribute__((always_inline)) {
         constexpr int PER = 16 / KS;
@@ -476,12 +489,11 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
         // Requests one by one: together at the turn's beginning they stand in line behind those of the other wavefronts.
         if (g % 2 == 1 && g < 2 * LOADS) request(h + lead, g / 2);
       });
-      mx = of[0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, of[e]);
-      lay_out<KS, (CAP ? 8 : 1) * 16 / KS>();
+      if constexpr (!CAP) weights(0);
+      lay_out<KS, (CAP ? 8 * 16 : 28) / KS>();
 #pragma unroll
       for (int e = 0; e < 16; ++e) asm volatile("" : "+v"(of[e]));
+      if constexpr (!CAP) asm volatile("" : "+v"(W[0]), "+v"(sum[0]));
     };
     if constexpr (CAP) {
       if (__builtin_expect(!__any(!(largest_size(of) < low_below)), 1)) shaped(true);
@@ -491,16 +503,23 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     }
     advance();
     const int id = block_id();
-    mx = max_halves(mx + b) * unit;
-    const bool up = mx > m_ref + kSlack;
-    const bool moved = __any(up);
-    float c = 1.0f;
-    if (__builtin_expect(moved, 0)) c = move_reference(mx, up);
     weigh(h - 2, had, [](int) {});
-    exponentials(of, W, b * unit);
-    lay_out<2 * NT, 52 / (2 * NT)>();
-    asm volatile("" : "+v"(W[0]), "+v"(W[1]), "+v"(l_run));  // (made here, not where the next turn first needs them)
-    if (__builtin_expect(moved, 0)) follow_reference(c);
+    if constexpr (CAP) weights(0);
+    weights(1);
+    lay_out<2 * NT, (CAP ? 52 : 28) / (2 * NT)>();
+    asm volatile("" : "+v"(W[0]), "+v"(W[1]), "+v"(sum[0]), "+v"(sum[1]));  // (made here, not where the next turn first needs them)
+    if (__builtin_expect(__any(!(sum[0] + sum[1] <= kMost)), 0)) {
+      float mx = of[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, of[e]);
+      mx = max_halves(__builtin_fmaf(mx, unit, stage));
+      follow_reference(move_reference(mx, mx > m_ref));
+      off = (m_ref == -INFINITY ? 0.0f : m_ref) - stage;
+      sum[0] = sum[1] = 0.0f;
+      weights(0);
+      weights(1);
+    }
+    l_run += sum[0] + sum[1];
     locate(id);
   };
   if (n_st > 0) {
