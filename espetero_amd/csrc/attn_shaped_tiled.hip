@@ -6,17 +6,17 @@
 //   S^T[32 keys][32 rows] = K . Q^T      A = K from LDS, B = Q^T in registers
 //   P^T = exp2(shaped(S^T) - m)          registers; the D layout of S^T is the B layout of P^T
 //   O^T[head_dim][32 rows] += V^T . P^T  A = V^T from LDS
-// with v_mfma_f32_32x32x16. A turn has three stages in hand: the scores of stage h are made under the shaping of stage h - 1's and the
-// look for a new maximum, P . V of stage h - 2 under the exponentials of stage h - 1, so that matrix and vector units work beside each other
+// with v_mfma_f32_32x32x16. A turn has three stages in hand: the scores of stage h are made under the caps of stage h - 1's (without a cap: under
+// half of its exponentials), P . V of stage h - 2 under the exponentials of stage h - 1, so that matrix and vector units work beside each other
 // within a wavefront too. Turns that are not all of that - the ends of a range, masked stages - run the three one by one.
 //
 // Scores: the bias is what the score product's accumulator starts from (without a cap; behind a cap it is the last step's addend), but for
-// what it has of the stage, which is taken from the reference. A cap
-// is tanh as an odd polynomial where all of a wavefront's scores of the stage are below 0.7 caps (six operations a score), else by an
-// exponential and a reciprocal (eleven). 2048 rows behind 8000 keys, 32 / 8 heads of 128 dims, bf16, 303 billion operations: plain 342 us, with
-// slopes 332, with a cap 405, with both 400 to 450 by the card's clock (0.67 to 0.76 PFLOP/s): there the vector units are busy for six sevenths of
-// the loop. Short ranges are bound by their ends: three prompts of 500 to 2000 rows in six documents each take 52 to 57 us, of which a tile's
-// seven stages are a third, its first loads from memory another.
+// what it has of the stage, which is taken from the reference. A cap is tanh as an odd polynomial where all of a wavefront's scores of the
+// stage are below 0.7 caps (six operations a score), else by an exponential and a reciprocal (eleven). 2048 rows behind 8000 keys, 32 / 8
+// heads of 128 dims, bf16, 303 billion operations, by the card's clock: plain 310 to 350 us, with slopes 295 to 335, with a cap 390 to 410, with
+// both 365 to 425 (0.72 to 0.83 PFLOP/s), where the vector units issue in two thirds of the clocks. Short ranges are bound by their ends: three
+// prompts of 500 to 2000 rows in six documents each take 52 to 57 us, of which a tile's seven stages are a third, its first loads from
+// memory another.
 //
 // P enters its product as one number of the storage type, as is usual: an output's error is then at most 1.4 times what its own rounding
 // makes it. As the sum of two, as in the streaming kernel, which waits for memory anyway, P . V would be twice the matrix work here.
