@@ -647,6 +647,21 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
       if (c + 1 < n_chunks) fetch_decay(c + 1);
       lds_barrier();  // P is there, and nobody reads Q and K any more
     }
+    // Rows of O leave through LDS, where Q and K were, a wavefront's 64 rows of 64 bytes each, 16-byte parts turned by the row; written behind
+    // the products, read and stored under those of the state.
+    auto row_at = [&](int r, int p) { return lds + L::kQ + wave * 4096 + r * 64 + ((p ^ ((r >> 2) & 3)) << 4); };
+    u32x4 rows_out[4];
+    auto read_rows = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 4 && !STATE; ++i) rows_out[i] = *reinterpret_cast<const u32x4*>(row_at(16 * i + (lane >> 2), lane & 3));
+    };
+    auto store_rows = [&]() __attribute__((always_inline)) {
+      char* const to = reinterpret_cast<char*>(a.O + (size_t(tile.row0) + 64 * size_t(c)) * a.o_ld + dv0 + 32 * wave) +
+                       uint32_t(lane >> 2) * uint32_t(2 * a.o_ld) + 16 * (lane & 3);
+#pragma unroll
+      for (int i = 0; i < 4 && !STATE; ++i)
+        if (16 * i + (lane >> 2) < n) *reinterpret_cast<u32x4*>(to + i * (32 * size_t(a.o_ld))) = rows_out[i];
+    };
     u32x4 vr[4];
     auto read_v = [&] {
       const uint32_t v_at = place(L::kVT + col_part(32 * wave + l32, hb));
@@ -726,25 +741,14 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
         if constexpr (DT == ESP_F16) O[rt] *= pinv[row];
       }
       if (__builtin_expect(odd, 0)) read_v();
-      char* const o0 = reinterpret_cast<char*>(a.O + (size_t(tile.row0) + 64 * size_t(c)) * a.o_ld + dv0 + 32 * wave);
-      const uint32_t at_o = uint32_t(lane >> 2) * uint32_t(2 * a.o_ld) + 16 * (lane & 3);
-      // Through LDS, where Q and K were, a wavefront's 64 rows of 64 bytes each; 16-byte parts turned by the row.
-      char* const mine = lds + L::kQ + wave * 4096;
-      auto part_at = [&](int r, int p) { return mine + r * 64 + ((p ^ ((r >> 2) & 3)) << 4); };
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<u32x2*>(part_at(32 * rt + l32, i) + 8 * hb) =
+          *reinterpret_cast<u32x2*>(row_at(32 * rt + l32, i) + 8 * hb) =
               u32x2{pack2<DT>(O[rt][4 * i], O[rt][4 * i + 1]), pack2<DT>(O[rt][4 * i + 2], O[rt][4 * i + 3])};
       __builtin_amdgcn_wave_barrier();
       asm volatile("" ::: "memory");
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * i + (lane >> 2), p = lane & 3;
-        const u32x4 x = *reinterpret_cast<const u32x4*>(part_at(r, p));
-        if (r < n) *reinterpret_cast<u32x4*>(o0 + i * (32 * size_t(a.o_ld)) + at_o) = x;
-      }
     }
     // S = exp(C) S + K^T V'. (The state behind the segment is of use only where somebody reads it.)
     if (STATE || c + 1 < n_chunks || tile.dst >= 0) {
@@ -787,7 +791,9 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
             for (int v = 0; v < NV; ++v) d[t & 1] = mfma32x16<DT>(k, vs[ks][v], d[t & 1]);
           }
         };
+        read_rows();
         product(0);
+        store_rows();
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           if (t + 1 < KT) product(t + 1);
@@ -811,6 +817,7 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
         };
         step_in(0);
         step_split(0);
+        read_rows();
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           if (ks < 3) step_in(ks + 1);
@@ -825,9 +832,13 @@ __global__ __launch_bounds__(2 * DVB, DK == 128 && DVB == 64 ? 1 : 2) void linea
             __builtin_amdgcn_sched_group_barrier(0x002, 84 / (NV * KT), 0);
           }
           __builtin_amdgcn_sched_barrier(0);
+          if (ks == 0) store_rows();
         }
         settle(S);
       }
+    } else {
+      read_rows();
+      store_rows();
     }
   }
 
