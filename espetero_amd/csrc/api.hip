@@ -1137,8 +1137,9 @@ int esp_linear_attn(const esp_linear_params* p, const void* Q, const void* K, co
   if (int rc = check_linear(p, err, errlen)) return rc;
   if (n_tiles < 0 || n_few < 0 || n_few > n_tiles || n_parts < 0 || n_rows < 0) return fail(err, errlen, ESP_EINVAL, "counts");
   if (n_tiles == 0) return ESP_OK;
-  if (!tiles || !decay) return fail(err, errlen, ESP_EINVAL, "tiles and decay must not be NULL");
-  if (n_rows > 0 && (!Q || !K || !V || !O)) return fail(err, errlen, ESP_EINVAL, "Q, K, V and O must not be NULL");
+  if (!tiles) return fail(err, errlen, ESP_EINVAL, "tiles must not be NULL");
+  if ((n_rows > 0 || n_few < n_tiles) && (!Q || !K || !V || !O || !decay))  // (without rows states are copied or cleared)
+    return fail(err, errlen, ESP_EINVAL, "Q, K, V, O and decay must not be NULL");
   if (p->n_states > 0 && !states) return fail(err, errlen, ESP_EINVAL, "states is NULL");
   if ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V) | reinterpret_cast<uintptr_t>(O) |
        reinterpret_cast<uintptr_t>(states) | reinterpret_cast<uintptr_t>(workspace)) % 16)

@@ -66,6 +66,7 @@ def test_linear_refuses_arguments(a, rc, word):
 def test_linear_without_tiles_does_nothing():
     assert call("esp_linear_attn", *linear_args(linear_params(), n_tiles=0, n_few=0, tiles=None, Q=None, states=None))[0] == 0
     assert call("esp_linear_attn", *linear_args(None))[0] == 1
+    assert "decay" in call("esp_linear_attn", *linear_args(linear_params(), n_rows=0, decay=None))[1]        # the second tile is the chunked kernel's
     assert call("esp_linear_hint", C.byref(linear_params()), 0, None)[0] == 1
 
 
