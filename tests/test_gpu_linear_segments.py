@@ -17,7 +17,7 @@ def cut(r, each):
     """Run r's pass with each sequence in segments of `each` chunks."""
     c, tiles, parts = r.case, [], 0
     for base, rows, src, dst in c.records.tolist():
-        n = -(-rows // (64 * each))
+        n = max(1, -(-rows // (64 * each)))
         for k in range(n):
             at, end = 64 * each * k, min(rows, 64 * each * (k + 1))
             tiles.append((base + at, end - at, src, dst if k + 1 == n else -1, parts if n > 1 else -1, k, n - 1 - k, 0))
