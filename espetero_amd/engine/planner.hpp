@@ -670,12 +670,13 @@ inline void plan_tiles(AttnPlan& A, int groups, int window, const int32_t* pos, 
 
 // Attention with shaped scores on its tiled kernel: every tile of rows in parts of at most so many stages of 32 keys, whichever of them the cache
 // and whichever the pass itself holds. What comes of a cut is worked out by handing its workgroups to the chip's slots, longest first (as the
-// records are ordered; the kernel takes them from the end); figures in microseconds, of 128 and 256 dims: 7.7 and 9.6 for a workgroup's
-// set-up and end, 0.82 and 1.17 for a stage, 1.0 for one beside another workgroup on the compute unit, 4.7 and 5.6 for the merge, and the partial
-// records at 3 MB a microsecond. Fitted to 109 passes of 13 to 1976 rows over 0 to 16000 keys, each timed whole and in up to 24 cuts: right
-// within 11 %; what it picks takes 2.5 % longer than the best of them in geometric mean. (24 rows behind 16000 keys, 32 / 8 heads: 444 us
-// whole, 68 in 8 parts, 30 in 32; 1500 fresh rows, 8 / 4 heads of 256: 76 whole, 43 in 60 parts.) A cut has to promise a tenth: spans, which are not
-// known here, may leave a tile fewer keys than it is planned for.
+// records are ordered; the kernel takes them from the end); figures in microseconds, of 128 and 256 dims: 7.5 and 8.6 for a workgroup's
+// set-up and end, 1.05 and 1.76 for each of its first six stages (masked ones, turns not yet full), 0.75 and 1.05 for the others, 1.21 times as
+// much beside another workgroup on the compute unit, 4.9 and 5.0 for the merge, and the partial records at 3 MB a microsecond. Fitted to 109
+// passes of 13 to 1976 rows over 0 to 16000 keys, each timed whole and in up to 24 cuts: right within 12 %; what it picks takes 1.5 % longer
+// than the best of them in geometric mean. (24 rows behind 16000 keys, 32 / 8 heads: 400 us whole, 63 in 8 parts, 29 in 32; 1500 fresh rows,
+// 8 / 4 heads of 256: 73 whole, 41 in 60 parts.) A cut has to promise a tenth: spans, which are not known here, may leave a tile fewer keys than it
+// is planned for.
 inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, int groups, int window, const int32_t* pos, const PlanOptions& o) {
   constexpr int kStage = 32;
   A.tiles.clear();
@@ -706,7 +707,7 @@ inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, 
   }
   const int slots = std::max(per_cu, o.groups_target), units = std::max(1, slots / per_cu);
   const bool wide = head_dim == 256;
-  const double end = wide ? 9.6 : 7.7, alone = wide ? 1.17 : 0.82, beside = wide ? 1.19 : 1.0, merge = wide ? 5.6 : 4.7;
+  const double end = wide ? 8.6 : 7.5, first = wide ? 1.76 : 1.05, further = wide ? 1.05 : 0.75, merge = wide ? 5.0 : 4.9;
   struct Cut {
     int parts, each;
   };
@@ -735,7 +736,7 @@ inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, 
     free_at.push({0.0, few ? units : slots});
     double last = 0;
     for (const int stages : lengths) {
-      const double cost = end + stages * (few ? alone : beside);
+      const double cost = end + (std::min(stages, 6) * first + std::max(stages - 6, 0) * further) * (few || per_cu == 1 ? 1.0 : 1.21);
       for (long long left = groups; left > 0;) {
         const Free f = free_at.top();
         const long long take = std::min(left, f.second);
