@@ -414,6 +414,8 @@ hipError_t launch_stream_t(const ShapedArgs& a, int n_tiles, hipStream_t st) {
   return a.cap_log2 > 0.0f ? launch_stream_c<DT, HD, NC, true>(a, n_tiles, st) : launch_stream_c<DT, HD, NC, false>(a, n_tiles, st);
 }
 
+// Pass and merge with one wavefront an output and with four, us: 16 parts of one tile 9.0 and 8.0, 63 of one 23.6 and 17.6 (of 24 rows 32.5 and 28), 64 of
+// eight 30.3 and 29.2, 57 of eighteen 83.8 and 84.9. (2048 workgroups of four wavefronts are what the chip holds.)
 template <int DT, int HD>
 void launch_merge_t(const ShapedArgs& a, const esp_combine* jobs, int n_jobs, int n_parts, hipStream_t st) {
   const unsigned outs = unsigned(a.R * a.H), jobs_n = unsigned(n_jobs);
