@@ -872,6 +872,12 @@ int esp_attn_shaped(const esp_attn_params* p, const esp_shape_params* shape, con
     }
     if (terms < 5) until = std::min(until, kUntil[terms]);
     a.tanh_below = float(std::min(until / z, double(FLT_MAX)));
+    if (terms == 5) {
+      constexpr double kShort[3] = {0.9999998947913661, -0.33328590898156374, 0.13015407522207817};
+      power = double(p->scale) * 1.4426950408889634;
+      for (int i = 0; i < 3; ++i, power *= z * z) a.tanh_s[i] = float(kShort[i] * power);
+      a.tanh_short = float(0.2 / z);
+    }
   }
   a.kv_base = p->kv_base;
   hipStream_t st = static_cast<hipStream_t>(stream);

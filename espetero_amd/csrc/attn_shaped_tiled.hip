@@ -12,11 +12,11 @@
 //
 // Scores: the bias is what the score product's accumulator starts from (without a cap; behind a cap it is the last step's addend), but for
 // what it has of the stage, which is taken from the reference. A cap is tanh as an odd polynomial where all of a wavefront's scores of the
-// stage are below 0.7 caps (six operations a score), else by an exponential and a reciprocal (eleven). 2048 rows behind 8000 keys, 32 / 8
-// heads of 128 dims, bf16, 303 billion operations, by the card's clock: plain 310 to 350 us, with slopes 295 to 335, with a cap 390 to 410, with
-// both 365 to 425 (0.72 to 0.83 PFLOP/s), where the vector units issue in two thirds of the clocks. Short ranges are bound by their ends: three
-// prompts of 500 to 2000 rows in six documents each take 52 to 57 us, of which a tile's seven stages are a third, its first loads from
-// memory another.
+// stage are below 0.2 caps (four operations a score) or 0.7 (six), else by an exponential and a reciprocal (eleven). 2048 rows behind 8000 keys,
+// 32 / 8 heads of 128 dims, bf16, 303 billion operations, by the card's clock: plain 310 to 350 us, with slopes 295 to 335, with a cap 370 (scores
+// below 0.2 caps; else 395), with both 395 (425), 0.72 to 0.77 PFLOP/s, where the vector units issue in two thirds of the clocks. Short ranges are
+// bound by their ends: three prompts of 500 to 2000 rows in six documents each take 52 to 57 us, of which a tile's seven stages are a third, its first
+// loads from memory another.
 //
 // P enters its product as one number of the storage type, as is usual: an output's error is then at most 1.4 times what its own rounding
 // makes it. As the sum of two, as in the streaming kernel, which waits for memory anyway, P . V would be twice the matrix work here.
@@ -293,9 +293,11 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     for (int e = 1; e < 16; ++e) m = fmaxf(m, fabsf(x[e]));
     return m;
   };
-  auto shape_e = [&](float x, int e, bool low) __attribute__((always_inline)) {
+  auto shape_e = [&](float x, int e, auto terms) __attribute__((always_inline)) {  // terms of the polynomial; 0: the exponential
     if constexpr (!CAP) return x;
-    return low ? shaped_tanh_low(a, x, bias[e]) : shaped_tanh_high(a, x, bias[e]);
+    else if constexpr (terms == 3) return shaped_tanh_short(a, x, bias[e]);
+    else if constexpr (terms == 5) return shaped_tanh_low(a, x, bias[e]);
+    else return shaped_tanh_high(a, x, bias[e]);
   };
   // With a cap scores are in log2 units, else still in those of the products.
   const float unit = CAP ? 1.0f : a.scale_log2;
@@ -427,7 +429,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
   auto within = [](int h, int lo, int hi) { return uint32_t(h - lo) < uint32_t(hi - lo); };  // (lo <= hi)
-  const float low_below = CAP ? a.tanh_below : 0.0f;
+  const float low_below = CAP ? a.tanh_below : 0.0f, short_below = CAP ? a.tanh_short : 0.0f;
   // Two turns between barriers: 64 keys. Behind the one in front of turns h and h + 1 (h even), K of stages h and h + 1 and V of stages h - 2
   // and h - 1 have landed for everybody, and nobody reads K or V of the two stages in front of those any more, whose places in the
   // ring the two turns' requests take.
@@ -494,26 +496,31 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
         sum[sb] = sum2<DT>(W[sb][e], sum[sb]);  // (the weights as the product takes them)
       }
     };
-    // Under the score products: the scores' shape, or without a cap half of the weights.
-    auto shaped = [&](bool low) __attribute__((always_inline)) {
-      score(h, to, [&](int g) __attribute__((always_inline)) {
-        constexpr int PER = 16 / KS;
-#pragma unroll
-        for (int e = g * PER; e < (g + 1) * PER; ++e) of[e] = shape_e(of[e], e, low);
-        // Requests one by one: together at the turn's beginning they stand in line behind those of the other wavefronts.
-        if (first && g % 2 == 1 && g < 2 * LOADS) request(h + lead, g / 2, 0);
-      });
-      if constexpr (!CAP) weights(0);
-      lay_out<KS, (CAP ? 8 * 16 : 28) / KS>();
+    auto made_here = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) asm volatile("" : "+v"(of[e]));
       if constexpr (!CAP) asm volatile("" : "+v"(W[0]), "+v"(sum[0]));
     };
+    // Under the score products: the scores' shape, or without a cap half of the weights.
+    auto shaped = [&](auto terms) __attribute__((always_inline)) {
+      score(h, to, [&](int g) __attribute__((always_inline)) {
+        constexpr int PER = 16 / KS;
+#pragma unroll
+        for (int e = g * PER; e < (g + 1) * PER; ++e) of[e] = shape_e(of[e], e, terms);
+        // Requests one by one: together at the turn's beginning they stand in line behind those of the other wavefronts.
+        if (first && g % 2 == 1 && g < 2 * LOADS) request(h + lead, g / 2, 0);
+      });
+      if constexpr (!CAP) weights(0);
+      lay_out<KS, (CAP ? (terms == 3 ? 6 : 8) * 16 : 28) / KS>();
+      made_here();
+    };
     if constexpr (CAP) {
-      if (__builtin_expect(!__any(!(largest_size(of) < low_below)), 1)) shaped(true);
-      else shaped(false);
+      const float largest = largest_size(of);
+      if (__builtin_expect(!__any(!(largest < short_below)), 1)) shaped(std::integral_constant<int, 3>{});
+      else if (!__any(!(largest < low_below))) shaped(std::integral_constant<int, 5>{});
+      else shaped(std::integral_constant<int, 0>{});
     } else {
-      shaped(true);
+      shaped(std::integral_constant<int, 0>{});
     }
     look_up(first ? 0 : 1);
     weigh(h - 2, had, [&](int g) __attribute__((always_inline)) {

@@ -25,6 +25,7 @@ struct ShapedArgs {
   // cap tanh(scale q.k / cap) in log2 units as q.k times a polynomial of (q.k)^2, for |q.k| < tanh_below. tanh(z) / z fitted in z^2 for
   // |z| < 0.7: six steps of 2^-24 of tanh off in fp32. 0, or fewer terms and a nearer bound, where fp32 does not hold the coefficients.
   float tanh_c[5], tanh_below;
+  float tanh_s[3], tanh_short;  // likewise for |z| < 0.2, where three terms do
   uint64_t kv_base;
 };
 
@@ -57,6 +58,10 @@ __device__ __forceinline__ float shaped_tanh_low(const ShapedArgs& a, float dot,
   p = __builtin_fmaf(u, p, a.tanh_c[1]);
   p = __builtin_fmaf(u, p, a.tanh_c[0]);
   return __builtin_fmaf(dot, p, add);
+}
+__device__ __forceinline__ float shaped_tanh_short(const ShapedArgs& a, float dot, float add) {
+  const float u = dot * dot;
+  return __builtin_fmaf(dot, __builtin_fmaf(u, __builtin_fmaf(u, a.tanh_s[2], a.tanh_s[1]), a.tanh_s[0]), add);
 }
 __device__ __forceinline__ float shaped_tanh_high(const ShapedArgs& a, float dot, float add) {
   return __builtin_fmaf(-2.0f * a.cap_log2, __builtin_amdgcn_rcpf(fast_exp2(dot * a.scale_log2) + 1.0f), a.cap_log2 + add);
