@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
     for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = mw[w] == -INFINITY ? 0.0f : fast_exp2(mw[w] - M);
+      const float f = shaped_share(mw[w], M);
       L += f * lw[w];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) o[e] += ow[w][e] * f;
@@ -329,24 +329,31 @@ __global__ __launch_bounds__(256) void attn_shaped_merge_kernel(const ShapedArgs
     float mN[4], lN[4], oN[4][VEC];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // all loads before the first use; slots past the last record weigh nothing
-      const bool in = s + W * i < job.nparts;
-      const size_t rec = rec0 + size_t(in ? s + W * i : s) * step;
-      mN[i] = in ? a.parts_ml[rec * 2] : -INFINITY;
+      const size_t rec = rec0 + size_t(s + W * i < job.nparts ? s + W * i : s) * step;
+      mN[i] = a.parts_ml[rec * 2];
       lN[i] = a.parts_ml[rec * 2 + 1];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) oN[i][e] = a.parts_o[rec * HD + VEC * lane + e];
     }
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {  // (zeros, not a weight of zero: what is read again there may be infinite)
+      const bool in = s + W * i < job.nparts;
+      mN[i] = in ? mN[i] : -INFINITY;
+      lN[i] = in ? lN[i] : 0.0f;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) oN[i][e] = in ? oN[i][e] : 0.0f;
+    }
     float Mn = M;
 #pragma unroll
     for (int i = 0; i < 4; ++i) Mn = fmaxf(Mn, mN[i]);
-    const float c = M == -INFINITY ? 0.0f : fast_exp2(M - Mn);
+    const float c = shaped_share(M, Mn);
     L *= c;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) o[e] *= c;
     M = Mn;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float w = mN[i] == -INFINITY ? 0.0f : fast_exp2(mN[i] - Mn);
+      const float w = shaped_share(mN[i], Mn);
       L += w * lN[i];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) o[e] += oN[i][e] * w;
@@ -369,7 +376,7 @@ __global__ __launch_bounds__(256) void attn_shaped_merge_kernel(const ShapedArgs
     for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float f = ml_sh[w][0] == -INFINITY ? 0.0f : fast_exp2(ml_sh[w][0] - M);
+      const float f = shaped_share(ml_sh[w][0], M);
       L += f * ml_sh[w][1];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) o[e] += o_sh[w][VEC * lane + e] * f;

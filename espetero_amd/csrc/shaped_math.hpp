@@ -88,6 +88,10 @@ __device__ __forceinline__ Sight shaped_range(const esp_tile& t, const esp_tree&
   return d;
 }
 
+// What sums taken from reference m count for beside a reference M of m or more; m is -inf where no key has been seen. Never zero for keys that
+// have: a sum may hold an infinite value, which is no less infinite for weighing next to nothing (2^-126 of finite ones is lost in any output).
+__device__ __forceinline__ float shaped_share(float m, float M) { return m == -INFINITY ? 0.0f : fmaxf(fast_exp2(m - M), 0x1p-126f); }
+
 __device__ __forceinline__ float shaped_inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }  // 0: a row that has seen no key; NaN stays
 
 }  // namespace esp
