@@ -18,8 +18,10 @@
 // bound by their ends: three prompts of 500 to 2000 rows in six documents each take 52 to 57 us, of which a tile's seven stages are a third, its first
 // loads from memory another.
 //
-// P enters its product as one number of the storage type, as is usual: an output's error is then at most 1.4 times what its own rounding
-// makes it. As the sum of two, as in the streaming kernel, which waits for memory anyway, P . V would be twice the matrix work here.
+// P enters its product as the sum of two numbers of the storage type, 16 bits or more, as in the streaming kernel, so that a row is as exact
+// in a pass of many rows as in one of few: an output's error is that of its own rounding. One number, half of P . V's matrix work, makes it up to 1.4
+// times as much, 0.0023 of the output's size for 0.0017 (bf16): the chunk with both then takes 392 us where two numbers take 500, the packed
+// documents 57 and 67.
 //
 // LDS: a ring of 4 stages of 32 keys, K and V^T, loaded straight from the pool (global_load_lds): wavefronts 0 and 1 load the
 // two sub-blocks of K, two stages ahead of the scores, 2 and 3 those of V^T, two ahead of P . V. K: the 16-byte chunk c of row r lies at
@@ -71,17 +73,33 @@ __device__ __forceinline__ int wave_most(int x) {
   return __builtin_amdgcn_readlane(x, 63);
 }
 
-// The order of a block of N matrix instructions with operands from LDS two ahead: one, then V vector operations (exponentials among
-// them), and the operand of the one after the next.
-template <int N, int V>
+// The order of a block of matrix instructions, M for each of N operands from LDS two ahead: one, then V vector operations (exponentials
+// among them), and the operand of the one after the next.
+template <int N, int M, int V>
 __device__ __forceinline__ void lay_out() {
   __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
   for (int g = 0; g < N; ++g) {
     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x402, V, 0);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, V, 0);
+    }
   }
+}
+
+// A lane's 16 weights of a stage, two to a dword, as the sum of two numbers of the storage type each.
+struct Weights {
+  u32x4 p[2], rest[2];
+};
+template <int DT>
+__device__ __forceinline__ void put_weights(Weights& w, int sb, int e, float p0, float p1, float& sum) {
+  uint32_t p = pack2<DT>(p0, p1);
+  asm("" : "+v"(p));  // (left alone the compiler converts the lower one once more instead of shifting it out)
+  w.p[sb][e] = p;
+  w.rest[sb][e] = pack2<DT>(p0 - unpack_lo<DT>(p), p1 - unpack_hi<DT>(p));
+  sum = sum2<DT>(w.rest[sb][e], sum2<DT>(p, sum));  // (the weights as the product takes them)
 }
 }  // namespace
 
@@ -185,9 +203,14 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   auto turned = [&](int i) { return kind == 0 ? from ^ uint32_t(swap23(RPL * i) << 4) : from; };
   const uint32_t dst = lds_base + wave * L::kRun;
   // Where this wavefront's next sub-block lies; a stage further is 32 tokens further down. Past the range's end the last sub-block again.
-  int next_raw = n_st > 0 ? key_of(0) + 16 * (wave & 1) : 0, next_key = min(next_raw, last_sub);
-  int next_at = next_key / a.bt, next_t0 = next_key - next_at * a.bt;
-  if (a.ring) next_at %= a.ring;
+  int next_raw, next_key, next_at, next_t0;
+  auto start = [&]() __attribute__((always_inline)) {
+    next_raw = n_st > 0 ? key_of(0) + 16 * (wave & 1) : 0;
+    next_key = min(next_raw, last_sub);
+    next_at = next_key / a.bt;
+    next_t0 = next_key - next_at * a.bt;
+    if (a.ring) next_at %= a.ring;
+  };
   using const_i32 = const int32_t __attribute__((address_space(4)));
   const const_i32* const list = (const const_i32*)a.blocks;
   auto block_id = [&] { return a.ring ? table + next_at : list[table + next_at]; };
@@ -234,12 +257,10 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   const uint32_t v_at = lds_base + 2 * L::kRun + lane * 16;
 
   f32x16 acc[NT];
-  float m_ref = -INFINITY, l_run = 0.0f;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) acc[nt] = f32x16{};
+  float m_ref, l_run;
   // Scores and weights of the stage at work and of the one before, by the stage's parity.
   f32x16 s[2] = {f32x16{}, f32x16{}};
-  u32x4 P[2][2] = {};
+  Weights P[2] = {};
 
   // The bias of index e of this lane's half, linear in the key: right up to the row's own key. A part for the index, which never changes, and
   // one for the stage, which joins the scores where they are taken from the reference.
@@ -272,7 +293,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     }
   };
   // O^T += V^T P^T of stage h.
-  auto weigh = [&](int h, const u32x4 (&p)[2], auto between) __attribute__((always_inline)) {
+  auto weigh = [&](int h, const Weights& w, auto between) __attribute__((always_inline)) {
     u32x4 v[3];
     const uint32_t va = values_of(h);
     auto fetch = [&](int g) { v[g % 3] = value_operand(va, g); };
@@ -281,7 +302,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
 #pragma unroll
     for (int g = 0; g < 2 * NT; ++g) {
       if (g + 2 < 2 * NT) fetch(g + 2);
-      acc[g % NT] = mfma32x16<DT>(v[g % 3], p[g / NT], acc[g % NT]);
+      acc[g % NT] = mfma32x16<DT>(v[g % 3], w.p[g / NT], acc[g % NT]);
+      acc[g % NT] = mfma32x16<DT>(v[g % 3], w.rest[g / NT], acc[g % NT]);
       between(g);
       __builtin_amdgcn_sched_barrier(0x406);
     }
@@ -301,7 +323,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   };
   // With a cap scores are in log2 units, else still in those of the products.
   const float unit = CAP ? 1.0f : a.scale_log2;
-  auto exponentials = [&](const f32x16& x, u32x4 (&p)[2]) __attribute__((always_inline)) {
+  auto exponentials = [&](const f32x16& x, Weights& w) __attribute__((always_inline)) {
     const float off = m_ref == -INFINITY ? 0.0f : m_ref;
     float lx = 0.0f;
 #pragma unroll
@@ -311,8 +333,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
         const int at = 8 * sb + 2 * e;
         const float p0 = fast_exp2(CAP ? x[at] - off : __builtin_fmaf(x[at], unit, -off));
         const float p1 = fast_exp2(CAP ? x[at + 1] - off : __builtin_fmaf(x[at + 1], unit, -off));
-        p[sb][e] = pack2<DT>(p0, p1);
-        (sb ? lx : l_run) = sum2<DT>(p[sb][e], sb ? lx : l_run);  // (the weights as the product takes them)
+        put_weights<DT>(w, sb, e, p0, p1, sb ? lx : l_run);
       }
     l_run += lx;
   };
@@ -379,9 +400,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     }
     if (ln == 0) bad[2 * (uint32_t(h) & (kRing - 1)) + (wave & 1)] = any;
   };
-  bool marked = false;
-  auto marks = [&](int h, const u32x4 (&P)[2]) __attribute__((always_inline)) {
-    const int ln = here(lane);
+  bool marked;
+  auto marks = [&](int h) __attribute__((always_inline)) {
+    const int ln = here(lane), lo = max(rg.from, sight.from), n = max(0, min(rg.end, sight.end) - lo);
 #pragma unroll 1
     for (int w = 0; w < NT; ++w) {
       uint32_t* const word = reinterpret_cast<uint32_t*>(lds + L::kMarks) + (wave * NT + w) * 64 + ln;
@@ -389,18 +410,12 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
 #pragma unroll 1
       for (int t = 0; t < 32; ++t) {
         const int key = key_of(h) + t;
-        if (key < rg.from || key >= rg.end) continue;
-        // The row's weight of the key: element t % 8 of P[t / 16], in the lane half (t / 8) % 2.
-        uint32_t p2 = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p2 = i == 4 * (t >> 4) + ((t >> 1) & 3) ? P[i >> 2][i & 3] : p2;
-        const float p = __shfl((t & 1) ? unpack_hi<DT>(p2) : unpack_lo<DT>(p2), 32 * ((t >> 3) & 1) + (ln & 31));
+        if (key < rg.from || key >= rg.end || uint32_t(key - lo) >= uint32_t(n)) continue;  // (a key that the row sees weighs something)
         const uint16_t* v = a.pool + size_t(a.kv_base) + (size_t(shaped_block(a, table, key / a.bt)) * size_t(a.Hkv) + size_t(kvh)) * head +
                             vt_elem(a.bt, HD, key % a.bt, 32 * w + 4 * (ln >> 5));
 #pragma unroll 1
         for (int e = 0; e < 16; ++e) {
           const uint32_t x = v[(8 * (e >> 2) + (e & 3)) * kVtDim];
-          if (!(p > 0.0f)) continue;
           found |= (not_finite_marks<DT>(x, false) & 0xffffu ? 1u << e : 0u) | (not_finite_marks<DT>(x, true) & 0xffffu ? 0x10000u << e : 0u);
         }
       }
@@ -409,22 +424,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     marked = true;
   };
 
-  // A pair of turns h and h + 1 requests stages h + lead and h + 1 + lead, both in the first turn, so that the barrier behind the second does
-  // not wait for them (2048 rows behind 8000 keys, 16 / 8 heads of 256 dims, capped: 393 to 378 us).
   const int lead = kind == 0 ? 2 : 0;
-  {
-    next_id[0] = block_id();
-    at_t0[0] = next_t0;
-    look_up(1);
-    locate_both();
-    if (kind == 0) {
-      if (n_st > 0) request_all(0, 0);
-      if (n_st > 1) request_all(1, 1);
-      look_up(0);
-      look_up(1);
-      locate_both();
-    }
-  }
   // Q is waited for here, not at its first use in the loop: that wait would be on the counter of the stages on their way.
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
@@ -446,13 +446,13 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     asm volatile("" ::: "memory");
   };
   // A turn of whatever there is to do, one after the other: S and W are the scores and the weights of the last stage.
-  auto mixed_turn = [&](int h, f32x16& S, u32x4 (&W)[2]) __attribute__((always_inline)) {
+  auto mixed_turn = [&](int h, f32x16& S, Weights& W) __attribute__((always_inline)) {
     // On a wavefront's first stage acc is whatever; it is cleared when a row's reference is first set.
     if (within(h - 2, v0, v1)) {
       weigh(h - 2, W, [](int) {});
       if (!within(h - 2, w0, w1)) {
         const int* f = bad + 2 * ((h - 2) & (kRing - 1));
-        if (__builtin_expect(__builtin_amdgcn_readfirstlane(f[0] | f[1]), 0)) marks(h - 2, W);
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(f[0] | f[1]), 0)) marks(h - 2);
       }
     }
     if (within(h - 1, v0, v1)) {
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   // A turn with all three stages to do, the last two seen whole by all rows of the tile: scores of stage h to `to`, those of stage h - 1 in
   // `of`, weights of stage h - 2 in `had`, of stage h - 1 to `W`. No maximum is taken: all weights are positive, so a lane's sum bounds them, and only
   // where one is too large (or the row has no reference yet) does the reference move and the stage's weights are made again.
-  auto whole_turn = [&](auto first, int h, f32x16& to, f32x16& of, const u32x4 (&had)[2], u32x4 (&W)[2]) __attribute__((always_inline)) {
+  auto whole_turn = [&](auto first, int h, f32x16& to, f32x16& of, const Weights& had, Weights& W) __attribute__((always_inline)) {
     const float stage = bias_at(h - 1) * unit;
     float off = m_ref - stage, sum[2] = {0.0f, 0.0f};
     auto weights = [&](int sb) __attribute__((always_inline)) {
@@ -492,14 +492,13 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
         const int at = 8 * sb + 2 * e;
         const float p0 = fast_exp2(CAP ? of[at] - off : __builtin_fmaf(of[at], unit, -off));
         const float p1 = fast_exp2(CAP ? of[at + 1] - off : __builtin_fmaf(of[at + 1], unit, -off));
-        W[sb][e] = pack2<DT>(p0, p1);
-        sum[sb] = sum2<DT>(W[sb][e], sum[sb]);  // (the weights as the product takes them)
+        put_weights<DT>(W, sb, e, p0, p1, sum[sb]);
       }
     };
     auto made_here = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) asm volatile("" : "+v"(of[e]));
-      if constexpr (!CAP) asm volatile("" : "+v"(W[0]), "+v"(sum[0]));
+      if constexpr (!CAP) asm volatile("" : "+v"(W.p[0]), "+v"(W.rest[0]), "+v"(sum[0]));
     };
     // Under the score products: the scores' shape, or without a cap half of the weights.
     auto shaped = [&](auto terms) __attribute__((always_inline)) {
@@ -511,7 +510,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
         if (first && g % 2 == 1 && g < 2 * LOADS) request(h + lead, g / 2, 0);
       });
       if constexpr (!CAP) weights(0);
-      lay_out<KS, (CAP ? (terms == 3 ? 6 : 8) * 16 : 28) / KS>();
+      lay_out<KS, 1, (CAP ? (terms == 3 ? 6 : 8) * 16 : 56) / KS>();
       made_here();
     };
     if constexpr (CAP) {
@@ -528,8 +527,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     });
     if constexpr (CAP) weights(0);
     weights(1);
-    lay_out<2 * NT, (CAP ? 52 : 28) / (2 * NT)>();
-    asm volatile("" : "+v"(W[0]), "+v"(W[1]), "+v"(sum[0]), "+v"(sum[1]));  // (made here, not where the next turn first needs them)
+    lay_out<2 * NT, 2, (CAP ? 104 : 56) / (4 * NT)>();
+    asm volatile("" : "+v"(W.p[0]), "+v"(W.p[1]), "+v"(W.rest[0]), "+v"(W.rest[1]), "+v"(sum[0]), "+v"(sum[1]));  // (made here, not later)
     if (__builtin_expect(__any(!(sum[0] + sum[1] <= kMost)), 0)) {
       float mx = of[0];
 #pragma unroll
@@ -544,79 +543,124 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     l_run += sum[0] + sum[1];
     if constexpr (!first) locate_both();
   };
-  if (n_st > 0) {
-    // Turns [t0, t1) are whole for this wavefront, in pairs.
-    const int t0 = (max(max(f0 + 1, w0 + 2), v0 + 2) + 1) & ~1, t1 = max(t0, min(min(f1, w1) + 1, v1) & ~1);
-    auto mixed_pair = [&](int h) __attribute__((always_inline)) {
-      begin(h, true);
-      if (h + lead < n_st) request_all(h + lead, 0);
-      if (h + 1 + lead < n_st) request_all(h + 1 + lead, 1);
-      look_up(0);
+  // Infinite and NaN values of a stage that all rows see whole go into its products as they are, and there an infinity makes NaN of a weight's
+  // second number, or where a weight has vanished. Rows that have met such a value are walked once more, with all stages looked over as
+  // those with unseen keys are; the tile's other rows are done.
+  int* const met = bad + 2 * kRing;  // [wavefront]
+  bool todo = col0 + l32 < cols_live;
+  for (bool careful = false;; careful = true) {
+    if (careful) f0 = f1 = w0 = w1 = 0;
+    start();
+    m_ref = -INFINITY;
+    l_run = 0.0f;
+    marked = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) acc[nt] = f32x16{};
+    // A pair of turns h and h + 1 requests stages h + lead and h + 1 + lead, both in the first turn, so that the barrier behind the second does
+    // not wait for them (2048 rows behind 8000 keys, 16 / 8 heads of 256 dims, capped: 393 to 378 us).
+    {
+      next_id[0] = block_id();
+      at_t0[0] = next_t0;
       look_up(1);
-#pragma unroll 1
-      for (int x = h; x < h + 2; ++x) mixed_turn(x, s[0], P[0]);
       locate_both();
-    };
-    int h = 0;
-    for (; h < (t1 > t0 ? t0 : n_st + 2); h += 2) mixed_pair(h);
-    for (; h < t1; h += 2) {
-      begin(h, false);
-      whole_turn(std::true_type{}, h, s[1], s[0], P[0], P[1]);
-      whole_turn(std::false_type{}, h + 1, s[0], s[1], P[1], P[0]);
-    }
-    mfma_settle(s[0]);
-    for (; h < n_st + 2; h += 2) mixed_pair(h);
-  }
-
-  // ---- the rows' end
-  const int ln = here(lane), half = ln >> 5;
-  const float l = l_run + __shfl_xor(l_run, 32);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) mfma_settle(acc[nt]);
-  if (__builtin_expect(marked, 0)) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const uint32_t word = reinterpret_cast<const uint32_t*>(lds + L::kMarks)[(wave * NT + nt) * 64 + ln];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        acc[nt][e] += word >> e & 1 ? INFINITY : 0.0f;
-        acc[nt][e] -= word >> (16 + e) & 1 ? INFINITY : 0.0f;
+      if (kind == 0) {
+        if (n_st > 0) request_all(0, 0);
+        if (n_st > 1) request_all(1, 1);
+        look_up(0);
+        look_up(1);
+        locate_both();
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
+    if (n_st > 0) {
+      // Turns [t0, t1) are whole for this wavefront, in pairs.
+      const int t0 = (max(max(f0 + 1, w0 + 2), v0 + 2) + 1) & ~1, t1 = max(t0, min(min(f1, w1) + 1, v1) & ~1);
+      auto mixed_pair = [&](int h) __attribute__((always_inline)) {
+        begin(h, true);
+        if (h + lead < n_st) request_all(h + lead, 0);
+        if (h + 1 + lead < n_st) request_all(h + 1 + lead, 1);
+        look_up(0);
+        look_up(1);
+#pragma unroll 1
+        for (int x = h; x < h + 2; ++x) mixed_turn(x, s[0], P[0]);
+        locate_both();
+      };
+      int h = 0;
+      for (; h < (t1 > t0 ? t0 : n_st + 2); h += 2) mixed_pair(h);
+      for (; h < t1; h += 2) {
+        begin(h, false);
+        whole_turn(std::true_type{}, h, s[1], s[0], P[0], P[1]);
+        whole_turn(std::false_type{}, h + 1, s[0], s[1], P[1], P[0]);
+      }
+      mfma_settle(s[0]);
+      for (; h < n_st + 2; h += 2) mixed_pair(h);
+    }
+
+    // ---- the rows' end
+    const int ln = here(lane), half = ln >> 5;
+    const float l = l_run + __shfl_xor(l_run, 32);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) mfma_settle(acc[nt]);
+    bool again = false;
+    if (!careful) {
+      float nf[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nf[e & 3] = __builtin_fmaf(acc[nt][e], 0.0f, nf[e & 3]);
+      const float odd = (nf[0] + nf[1]) + (nf[2] + nf[3]);  // NaN, or 0
+      again = todo && odd + __shfl_xor(odd, 32) != 0.0f;
+      if (ln == 0) met[wave] = 0;
+      if (again) met[wave] = 1;
+    }
+    if (__builtin_expect(marked, 0)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const uint32_t word = reinterpret_cast<const uint32_t*>(lds + L::kMarks)[(wave * NT + nt) * 64 + ln];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          acc[nt][e] += word >> e & 1 ? INFINITY : 0.0f;
+          acc[nt][e] -= word >> (16 + e) & 1 ? INFINITY : 0.0f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __syncthreads();  // the ring is free
+    const bool repeat = !careful && (met[0] | met[1] | met[2] | met[3]) != 0;
+    const bool done = todo && !again;
+    const bool none = l == 0.0f;  // a row that has seen nothing
+    if (tile.part >= 0) {         // partial records
+      if (done) {
+        const size_t rec = (size_t(tile.part) * a.Hkv + kvh) * a.cols + col0 + (ln & 31);
+        float* const to = a.parts_o + rec * HD + 4 * half;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<f32x4*>(to + 32 * nt + 8 * i) =
+                none ? f32x4{0, 0, 0, 0} : f32x4{acc[nt][4 * i], acc[nt][4 * i + 1], acc[nt][4 * i + 2], acc[nt][4 * i + 3]};
+        if (half == 0) {
+          a.parts_ml[rec * 2] = m_ref;
+          a.parts_ml[rec * 2 + 1] = l;
+        }
+      }
+    } else {
+      const float inv = shaped_inverse(l);
+      char* const ob = lds + wave * (32 * RB);
+      const Place pl = place(ln);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f = none ? 0.0f : inv;
+          auto x = [&](int j) { return none ? 0.0f : acc[nt][4 * i + j] * f; };
+          *reinterpret_cast<u32x2*>(RowsOut<RB>::at(ob, ln & 31, 4 * nt + i) + 8 * half) = u32x2{pack2<DT>(x(0), x(1)), pack2<DT>(x(2), x(3))};
+        }
+      RowsOut<RB>::store(ob, done ? uint64_t(uintptr_t(a.O + size_t(tile.r0 + pl.m) * a.q_ld + size_t(kvh * a.G + pl.hg) * HD)) : 0, ln);
+    }
+    if (__builtin_expect(!repeat, 1)) return;
+    todo = again;
+    __syncthreads();  // the rows have left the ring
   }
-  const bool none = l == 0.0f;  // a row that has seen nothing
-  const int col = col0 + (ln & 31);
-  const bool live = col < cols_live;
-  if (tile.part >= 0) {  // partial records
-    if (!live) return;
-    const size_t rec = (size_t(tile.part) * a.Hkv + kvh) * a.cols + col;
-    float* const to = a.parts_o + rec * HD + 4 * half;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(to + 32 * nt + 8 * i) =
-            none ? f32x4{0, 0, 0, 0} : f32x4{acc[nt][4 * i], acc[nt][4 * i + 1], acc[nt][4 * i + 2], acc[nt][4 * i + 3]};
-    if (half == 0) {
-      a.parts_ml[rec * 2] = m_ref;
-      a.parts_ml[rec * 2 + 1] = l;
-    }
-    return;
-  }
-  __syncthreads();  // the ring is free
-  const float inv = shaped_inverse(l);
-  char* const ob = lds + wave * (32 * RB);
-  const Place pl = place(ln);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float f = none ? 0.0f : inv;
-      auto x = [&](int j) { return none ? 0.0f : acc[nt][4 * i + j] * f; };
-      *reinterpret_cast<u32x2*>(RowsOut<RB>::at(ob, ln & 31, 4 * nt + i) + 8 * half) = u32x2{pack2<DT>(x(0), x(1)), pack2<DT>(x(2), x(3))};
-    }
-  RowsOut<RB>::store(ob, live ? uint64_t(uintptr_t(a.O + size_t(tile.r0 + pl.m) * a.q_ld + size_t(kvh * a.G + pl.hg) * HD)) : 0, ln);
 }
 
 namespace {

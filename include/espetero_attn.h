@@ -418,8 +418,8 @@ int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void
  * front of `prefix` are seen by the rows in front of them too (an image, an instruction). Without spans rows are plain causal. Any numbers may
  * stand in a span; a row that sees nothing gets zeros. Pool, records and append are those of esp_attn_diff: the pass's rows are in the
  * pool, row j of a tree at position P + j of its own block list or ring, and all of them are there before the call, also those that only rows
- * in front of them see. Softmax and sums are held in fp32; the probabilities enter P.V in the storage type (as the sum of two such
- * numbers in passes of few rows), O is rounded once at the end. */
+ * in front of them see. Softmax and sums are held in fp32; the probabilities enter P.V as the sum of two numbers of the storage type, O is
+ * rounded once at the end. An infinite or NaN value shows in the rows that see its key, however little that weighs. */
 typedef struct esp_shape_params {
   const float* slopes;  /* [H] fp32, device memory; NULL: no bias */
   const int32_t* spans; /* int32[2] per row of the pass, device memory; NULL: plain causal rows */

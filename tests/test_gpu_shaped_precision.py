@@ -1,0 +1,116 @@
+"""esp_attn_shaped on the device: the weights' second 16 bits reach the product with V, and infinite values are no less infinite for it."""
+import numpy as np
+import pytest
+
+from shaped_precision import bound
+from shaped_utils import ShapedCase, documents
+from test_gpu_shaped import Run, dev
+from espetero_amd import abi
+from oracle import binding as ob
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = abi.ESP_F16, abi.ESP_BF16
+
+
+def check(c, rows=None, shift=0, **plan):
+    r = Run(c, **plan)
+    want, tol, which = bound(c, shift, rows)
+    got = ob.to_f32(r()[which][:, :c.H * c.hd], c.dtype).astype(np.float64).reshape(want.shape)
+    print(f"  of the bound: {np.max(np.abs(got - want) / tol):.3f}", flush=True)
+    assert np.all(np.abs(got - want) <= tol)
+
+
+SHAPES = [(0.0, False), (20.0, False), (0.0, True), (30.0, True)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("cap,bias", SHAPES)
+@pytest.mark.parametrize("heads,hd,seqs", [((8, 2), 128, [(40, 1), (130, 1)]), ((4, 2), 128, [(200, 16)]), ((8, 2), 256, [(60, 2), (200, 4)])])
+def test_few_rows_hold_their_weights_as_two_numbers(heads, hd, seqs, cap, bias, dtype):
+    c = ShapedCase(*heads, hd, dtype, 16, seqs, cap=cap, bias=bias, sharp=0.25, seed=hd)
+    check(c)
+    check(c, workgroups=4096)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("cap,bias", SHAPES)
+@pytest.mark.parametrize("heads,hd,seqs", [((8, 2), 128, [(0, 150), (333, 70)]), ((4, 4), 128, [(500, 40)]), ((4, 2), 256, [(0, 150), (333, 70)])])
+def test_many_rows_hold_their_weights_as_two_numbers(heads, hd, seqs, cap, bias, dtype):
+    c = ShapedCase(*heads, hd, dtype, 16, seqs, cap=cap, bias=bias, sharp=0.25, seed=hd)
+    check(c, range(0, 150, 7))
+    check(c, range(0, 150, 7), workgroups=2048, cut_batch=True)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+def test_many_rows_of_documents_hold_their_weights_as_two_numbers(hd):
+    """Stages that some rows see in part."""
+    c = ShapedCase(4, 2, hd, BF16, 16, [(45, 150)], spans=[documents(45, 150, [0, 90, 100, 160], 40)], cap=20.0, bias=True, sharp=0.25, seed=hd)
+    check(c, range(0, 150, 5))
+
+
+def with_values(c, values):
+    """The pool with `values` ({(key, KV head, dim): bits}) in the first sequence's V."""
+    pool = c.pool.copy().reshape(c.n_blocks, c.Hkv, 2, c.bt * c.hd)
+    for (j, kvh, dim), bits in values.items():
+        b, t = c.block_list[j // c.bt], j % c.bt
+        pool[b, kvh, 1].reshape(c.bt // 16, c.hd, 16)[t // 16, dim, t % 16] = bits
+    return dev(pool.reshape(-1))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,cap,bias", [(128, 0.0, False), (128, 20.0, True), (256, 0.0, True), (256, 20.0, False)])
+@pytest.mark.parametrize("cut", [False, True])
+def test_infinite_values_that_many_rows_see(cut, hd, cap, bias, dtype):
+    """Far in front of the rows, where stages are seen whole, also where a weight is nothing beside the largest: an infinity of either sign, both (NaN),
+    and one among the rows, which some of them see. Other dims are as exact as ever, other KV heads keep their bits."""
+    P, M = 900, 70
+    c = ShapedCase(4, 2, hd, dtype, 16, [(P, M)], cap=cap, bias=bias, sharp=0.25, seed=3)
+    if bias:
+        c.slopes[:2] = 0.5, 2.0                                        # 2^-900 and less at key 100
+    inf = 0x7C00 if dtype == F16 else 0x7F80
+    r = Run(c, **(dict(workgroups=2048, cut_batch=True) if cut else {}))
+    clean = r().reshape(M, 4, hd)
+    r.pool = with_values(c, {(100, 0, 3): inf, (411, 0, 40): inf | 0x8000, (100, 0, 77): inf, (700, 0, 77): inf | 0x8000, (P + 50, 0, 90): inf})
+    r.O.fill_(0x1234)
+    bits = r().reshape(M, 4, hd)
+    got = ob.to_f32(bits, dtype)
+    assert (got[:, :2, 3] == np.inf).all() and (got[:, :2, 40] == -np.inf).all() and np.isnan(got[:, :2, 77]).all()
+    assert (got[50:, :2, 90] == np.inf).all() and np.isfinite(got[:50, :2, 90]).all()
+    assert (bits[:, 2:] == clean[:, 2:]).all()
+    want, tol, _ = bound(c)
+    tol, want = tol[:, :2], want[:, :2]
+    odd = ~np.isfinite(got[:, :2])
+    assert odd.sum() == 2 * (3 * M + 20)
+    assert np.all(odd | (np.abs(got[:, :2] - want) <= tol))
+
+
+def test_rows_that_meet_no_infinite_value_keep_their_bits():
+    """A NaN key of the first document: the rows of the second, of the same tile, are not walked again."""
+    P, M = 700, 32
+    first = 200
+    spans = [[(0 if m < 5 else first, 0) for m in range(M)]]
+    c = ShapedCase(4, 1, 128, BF16, 16, [(P, M)], spans=spans, cap=30.0, seed=4)
+    r = Run(c)
+    clean = r()
+    pool = c.pool.copy().reshape(c.n_blocks, c.Hkv, 2, c.bt * c.hd)
+    pool[c.block_list[3], 0, 0, 5] = 0x7FC0
+    r.pool = dev(pool.reshape(-1))
+    r.O.fill_(0x1234)
+    bits = r()
+    assert (bits[5:] == clean[5:]).all() and np.isnan(ob.to_f32(bits[:5], BF16)).all()
+
+
+def test_a_value_whose_weight_has_vanished_is_still_infinite():
+    """fp16, a key whose weight is 2^-47 of the largest of its part and 2^-200 of the row's, in a stage that one row does not see whole."""
+    c = ShapedCase(4, 4, 128, F16, 16, [(600, 40)], bias=True, spans=[[(0, 0)] * 39 + [(9, 0)]], seed=6)
+    c.slopes[:] = 0.25
+    for plan in (dict(workgroups=4096, cut_batch=True), {}):
+        r = Run(c, **plan)
+        clean = r().reshape(40, 4, 128)
+        r.pool = with_values(c, {(8, 0, 3): 0x7C00, (8, 0, 60): 0xFC00})
+        r.O.fill_(0x1234)
+        bits = r().reshape(40, 4, 128)
+        got = ob.to_f32(bits, F16)
+        assert (got[:-1, 0, 3] == np.inf).all() and (got[:-1, 0, 60] == -np.inf).all()
+        assert (bits[-1] == clean[-1]).all() and (bits[:, 1:] == clean[:, 1:]).all()
