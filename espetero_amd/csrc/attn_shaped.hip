@@ -22,7 +22,7 @@ struct ShapedUnit {  // 16 keys: K and V^T
 }  // namespace
 
 template <int DT, int HD, int NC, bool CAP>
-__global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped_stream_kernel(const ShapedArgs a) {
+__global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_stream_kernel(const ShapedArgs a) {
   constexpr int MT = HD / 16, KK = HD / 32, LDO = HD + 4, VEC = HD / 64;
   extern __shared__ float smem[];  // [4 wavefronts][NC * 16 columns][LDO] O, then [4][NC * 16][2] m, l
   const int kvh = blockIdx.x;
@@ -79,13 +79,6 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
 
   f32x4 acc[NC][MT];
   float m_run[NC], l_run[NC];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    m_run[c] = -INFINITY;
-    l_run[c] = 0.0f;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) acc[c][mt] = f32x4{0, 0, 0, 0};
-  }
 
   const uint32_t lane_k = uint32_t(c16 * HD + 8 * q4) * 2, lane_v = uint32_t(c16 * kVtDim + 4 * q4) * 2;
   const uint32_t head = uint32_t(2 * a.bt * HD) * 2, to_v = uint32_t(a.bt * HD) * 2;  // bytes of one (block, KV head); from its K to its V^T
@@ -120,9 +113,10 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
   };
   // Online softmax over scores x (log2 units, -inf where masked), then O^T += V^T . P^T. The matrix product takes P in the storage type, as
   // the sum of two such numbers, 16 bits or more: one alone makes the output 1.4 times as inexact as its own rounding does, and the
-  // second product waits for memory anyway. p: the weights before that.
-  auto softmax_pv = [&](const ShapedUnit<HD>& U, const f32x4 (&x)[NC], f32x4 (&p)[NC]) {
+  // second product waits for memory anyway.
+  auto softmax_pv = [&](const ShapedUnit<HD>& U, const f32x4 (&x)[NC]) {
     bool any_change = false;
+    f32x4 p[NC];
     float corr[NC];
     u32x2 pb[NC], pl[NC];
 #pragma unroll
@@ -132,7 +126,7 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       const float m_new = fmaxf(m_run[c], mx);
       const float m_safe = (m_new == -INFINITY) ? 0.0f : m_new;
-      corr[c] = fast_exp2(m_run[c] - m_safe);
+      corr[c] = fmaxf(fast_exp2(m_run[c] - m_safe), 0x1p-126f);  // (what is infinite stays so)
       any_change = any_change || (m_new > m_run[c]);
       m_run[c] = m_new;
 #pragma unroll
@@ -157,12 +151,12 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
       }
   };
   auto interior = [&](int u, const ShapedUnit<HD>& U) {
-    f32x4 s[NC], p[NC];
+    f32x4 s[NC];
     scores(u, U, s);
-    softmax_pv(U, s, p);
+    softmax_pv(U, s);
   };
-  // A unit with keys that some row does not see.
-  auto edge = [&](int u, ShapedUnit<HD>& U) {
+  // A unit with keys that some row does not see, or (careful) with values that may be infinite.
+  auto edge = [&](int u, ShapedUnit<HD>& U, bool careful) {
     // Keys outside the range may be memory never written: their V must not reach the products (0 * NaN).
     const int jv = (u << 4) + 4 * q4;
     uint32_t in[4];
@@ -175,9 +169,9 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
       U.v[mt].y &= in[2] | in[3];
       bad |= not_finite2<DT>(U.v[mt].x) | not_finite2<DT>(U.v[mt].y);
     }
-    // Nor may the infinite V of a key that one row sees reach a row that does not: such elements leave the product, and a product of
-    // marks in their places says which rows see them.
-    const bool rare = rows > 1 && __any(bad != 0);
+    // Nor may the infinite V of a key that one row sees reach a row that does not, or meet a weight's second number, which may be zero or below:
+    // such elements leave the product, and a product of marks in their places says which rows see them.
+    const bool rare = (rows > 1 || careful) && __any(bad != 0);
     if (rare) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -185,7 +179,7 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
         U.v[mt].y &= ~not_finite2<DT>(U.v[mt].y);
       }
     }
-    f32x4 s[NC], p[NC];
+    f32x4 s[NC];
     scores(u, U, s);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -194,8 +188,16 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
         const int from = max(rg.from, sight[c].from), n = max(0, min(rg.end, sight[c].end) - from);
         s[c][e] = uint32_t(jv + e - from) < uint32_t(n) ? s[c][e] : -INFINITY;
       }
-    softmax_pv(U, s, p);
+    softmax_pv(U, s);
     if (__builtin_expect(rare, 0)) {
+      constexpr uint32_t one = DT == ESP_F16 ? 0x3c00u : 0x3f80u;
+      u32x2 sees[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int from = max(rg.from, sight[c].from), n = max(0, min(rg.end, sight[c].end) - from);
+        auto seen = [&](int e) { return uint32_t(jv + e - from) < uint32_t(n) ? one : 0u; };
+        sees[c] = u32x2{seen(0) | seen(1) << 16, seen(2) | seen(3) << 16};
+      }
       const char* const vp = block_of(u) + to_v + lane_v;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -205,8 +207,7 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
         for (int neg = 0; neg < 2; ++neg)
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            const u32x2 pb = {pack2<DT>(p[c][0], p[c][1]), pack2<DT>(p[c][2], p[c][3])};
-            f32x4 seen = mfma16x16<DT>(u32x2{not_finite_marks<DT>(lo, neg != 0), not_finite_marks<DT>(hi, neg != 0)}, pb, f32x4{0, 0, 0, 0});
+            f32x4 seen = mfma16x16<DT>(u32x2{not_finite_marks<DT>(lo, neg != 0), not_finite_marks<DT>(hi, neg != 0)}, sees[c], f32x4{0, 0, 0, 0});
             mfma_settle(seen);
             mfma_settle(acc[c][mt]);
 #pragma unroll
@@ -218,12 +219,21 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
     }
   };
 
-  {
+  // Infinite and NaN values of an interior unit go into its products as they are, where a weight's second number, or one that has vanished, makes
+  // NaN of an infinity: a wavefront that has met one takes its units once more, in the same order, each with such values taken out.
+  for (bool careful = false;; careful = true) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      m_run[c] = -INFINITY;
+      l_run[c] = 0.0f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) acc[c][mt] = f32x4{0, 0, 0, 0};
+    }
     ShapedUnit<HD> U[2];
     const int n_int = ui1 - ui0, n_lo = ui0 - u_lo, n_edge = n_units - n_int;
     const int n_mine = n_int > wave ? (n_int - wave + 3) / 4 : 0;
-    if (n_mine > 0) {
-      const int u0 = ui0 + wave;
+    const int u0 = ui0 + wave;
+    if (!careful && n_mine > 0) {
       load(u0, U[0]);
       int i = 0;
       for (; i + 2 < n_mine; i += 2) {
@@ -240,11 +250,22 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
         interior(u0 + 4 * i, U[0]);
       }
     }
-    for (int i = (wave + 4 - n_int % 4) % 4; i < n_edge; i += 4) {  // go on with the round robin
-      const int u = i < n_lo ? u_lo + i : ui1 + (i - n_lo);
+    const int e0 = (wave + 4 - n_int % 4) % 4;  // go on with the round robin
+    for (int i = e0 - (careful ? 4 * n_mine : 0); i < n_edge; i += 4) {
+      const int u = i < e0 ? u0 + i - e0 + 4 * n_mine : i < n_lo ? u_lo + i : ui1 + (i - n_lo);
       load(u, U[0]);
-      edge(u, U[0]);
+      edge(u, U[0], careful);
     }
+    float nf = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        mfma_settle(acc[c][mt]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) nf = __builtin_fmaf(acc[c][mt][e], 0.0f, nf);
+      }
+    if (careful || __builtin_expect(!__any(nf != 0.0f), 1)) break;  // (NaN, or 0)
   }
 
   // ---- merge the 4 wavefronts in order
@@ -263,7 +284,6 @@ __global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped
     float* dst = o_sh + (wave * NC * 16 + col) * LDO + 4 * q4;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      mfma_settle(acc[c][mt]);
       *reinterpret_cast<f32x4*>(dst + 16 * mt) = acc[c][mt];
     }
   }

@@ -44,6 +44,13 @@ def test_many_rows(heads, hd, P, M, dtype):
     infinite_in_every_part(heads, hd, P, M, dtype, workgroups=2048, cut_batch=True)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,hd,P,M,workgroups", [((8, 4), 128, 700, 3, 64), ((32, 1), 256, 900, 4, 64), ((4, 4), 128, 600, 2, 24), ((32, 8), 128, 1500, 4, 40),
+                                                     ((8, 4), 128, 700, 1, 64)])
+def test_few_rows(heads, hd, P, M, workgroups, dtype):
+    infinite_in_every_part(heads, hd, P, M, dtype, workgroups=workgroups)
+
+
 @pytest.mark.parametrize("M,dtype", [(2, F16), (2, BF16), (40, BF16)])
 def test_a_part_that_weighs_nothing_is_still_infinite(M, dtype):
     """A bias that leaves the part of an early key 2^-200 of the largest weight. (One row does not see the key.)"""

@@ -114,3 +114,30 @@ def test_a_value_whose_weight_has_vanished_is_still_infinite():
         got = ob.to_f32(bits, F16)
         assert (got[:-1, 0, 3] == np.inf).all() and (got[:-1, 0, 60] == -np.inf).all()
         assert (bits[-1] == clean[-1]).all() and (bits[:, 1:] == clean[:, 1:]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,hd,M,cap,bias", [((4, 2), 128, 1, 0.0, False), ((4, 2), 128, 4, 20.0, True), ((8, 2), 128, 8, 0.0, True), ((4, 2), 256, 1, 0.0, True),
+                                                 ((8, 2), 256, 4, 20.0, False)])
+@pytest.mark.parametrize("workgroups", [None, 24])
+def test_infinite_values_that_few_rows_see(workgroups, heads, hd, M, cap, bias, dtype):
+    """Whole tiles and parts: an infinity of either sign, both (NaN), one whose weight is nothing beside the largest, and one among the rows. Whatever meets
+    none of them keeps its bits."""
+    P, G = 900, heads[0] // heads[1]
+    c = ShapedCase(*heads, hd, dtype, 16, [(P, M)], cap=cap, bias=bias, seed=3)
+    if bias:
+        c.slopes[:G] = 2.0                                             # 2^-2300 at key 100
+    inf = 0x7C00 if dtype == F16 else 0x7F80
+    r = Run(c, workgroups=workgroups)
+    clean = r().reshape(M, heads[0], hd)
+    r.pool = with_values(c, {(100, 0, 3): inf, (411, 0, 40): inf | 0x8000, (100, 0, 77): inf, (700, 0, 77): inf | 0x8000, (P + M // 2, 0, 90): inf,
+                             (896, 0, 91): inf | 0x8000})
+    r.O.fill_(0x1234)
+    bits = r().reshape(M, heads[0], hd)
+    got = ob.to_f32(bits, dtype)
+    assert (got[:, :G, 3] == np.inf).all() and (got[:, :G, 40] == -np.inf).all() and np.isnan(got[:, :G, 77]).all()
+    assert (got[M // 2:, :G, 90] == np.inf).all() and (got[:, :G, 91] == -np.inf).all()
+    same = np.ones(bits.shape, bool)
+    same[:, :G, [3, 40, 77, 91]] = False
+    same[M // 2:, :G, 90] = False
+    assert (bits[same] == clean[same]).all()
