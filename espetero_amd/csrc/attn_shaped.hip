@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_stream_ker
   };
   // Online softmax over scores x (log2 units, -inf where masked), then O^T += V^T . P^T. The matrix product takes P in the storage type, as
   // the sum of two such numbers, 16 bits or more: one alone makes the output 1.4 times as inexact as its own rounding does, and the
-  // second product waits for memory anyway.
+  // second product waits for memory anyway. Of fp16 the largest weight is 2^15, so that a number's last step, 2^-24, is 2^-39 of it.
   auto softmax_pv = [&](const ShapedUnit<HD>& U, const f32x4 (&x)[NC]) {
     bool any_change = false;
     f32x4 p[NC];
@@ -130,11 +130,11 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_stream_ker
       any_change = any_change || (m_new > m_run[c]);
       m_run[c] = m_new;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) p[c][e] = fast_exp2(x[c][e] - m_safe);
-      l_run[c] = l_run[c] * corr[c] + (p[c][0] + p[c][1] + p[c][2] + p[c][3]);
+      for (int e = 0; e < 4; ++e) p[c][e] = fast_exp2(DT == ESP_F16 ? (x[c][e] - m_safe) + 15.0f : x[c][e] - m_safe);
       pb[c] = u32x2{pack2<DT>(p[c][0], p[c][1]), pack2<DT>(p[c][2], p[c][3])};
       pl[c] = u32x2{pack2<DT>(p[c][0] - unpack_lo<DT>(pb[c].x), p[c][1] - unpack_hi<DT>(pb[c].x)),
                     pack2<DT>(p[c][2] - unpack_lo<DT>(pb[c].y), p[c][3] - unpack_hi<DT>(pb[c].y))};
+      l_run[c] = l_run[c] * corr[c] + sum2<DT>(pl[c].x, sum2<DT>(pb[c].x, sum2<DT>(pl[c].y, sum2<DT>(pb[c].y, 0.0f))));  // (as the product takes them)
     }
     if (__any(any_change)) {
 #pragma unroll

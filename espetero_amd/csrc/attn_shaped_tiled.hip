@@ -39,7 +39,16 @@ namespace esp {
 namespace {
 constexpr int kRing = 4;
 constexpr float kSlack = 8.0f;  // a row's reference moves when a score exceeds it by more (log2 units): P stays below 2^8
-constexpr float kMost = 256.0f; // and where that is not looked for, when a lane's weights of a stage come to more
+// Of fp16 the reference lies 7 below the score that it is taken from, so that weights go up to 2^15 and a number's last step, 2^-24, is 2^-31 of
+// that score's or less. (Not where fp32 does not hold the difference.)
+template <int DT>
+constexpr float kBelow = DT == ESP_F16 ? 7.0f : 0.0f;
+template <int DT>
+__device__ __forceinline__ float reference_of(float x) {
+  return DT == ESP_F16 && fabsf(x) < 0x1p20f ? x - kBelow<DT> : x;
+}
+template <int DT>
+constexpr float kMost = DT == ESP_F16 ? 0x1p15f : 0x1p8f;  // where slack is not looked for: when a lane's weights of a stage come to more
 
 template <int HD>
 struct TiledLds {
@@ -339,9 +348,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   };
   // A new reference where a score exceeds the old one by more than kSlack. What was weighed by the old one joins the accumulators
   // first; then they go over to the new one.
-  auto move_reference = [&](float mx, bool up) __attribute__((always_inline)) {
-    const float c = m_ref == -INFINITY ? -1.0f : up ? fast_exp2(m_ref - mx) : 1.0f;
-    m_ref = up ? mx : m_ref;
+  auto move_reference = [&](float to, bool up) __attribute__((always_inline)) {
+    const float c = m_ref == -INFINITY ? -1.0f : up ? fast_exp2(m_ref - to) : 1.0f;
+    m_ref = up ? to : m_ref;
     l_run *= c;
     return c;
   };
@@ -425,9 +434,6 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   };
 
   const int lead = kind == 0 ? 2 : 0;
-  // Q is waited for here, not at its first use in the loop: that wait would be on the counter of the stages on their way.
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
   auto within = [](int h, int lo, int hi) { return uint32_t(h - lo) < uint32_t(hi - lo); };  // (lo <= hi)
   const float low_below = CAP ? a.tanh_below : 0.0f, short_below = CAP ? a.tanh_short : 0.0f;
   // Two turns between barriers: 64 keys. Behind the one in front of turns h and h + 1 (h even), K of stages h and h + 1 and V of stages h - 2
@@ -470,9 +476,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
         S[e] = uint32_t(at + k) < uint32_t(n) ? x : -INFINITY;  // the row sees the keys [lo, lo + n)
         mx = fmaxf(mx, S[e]);
       }
-      mx = max_halves(mx) * unit;
-      const bool up = mx > m_ref + kSlack;  // from -inf on: the first key that the row sees
-      if (__any(up)) follow_reference(move_reference(mx, up));
+      const float ref = reference_of<DT>(max_halves(mx) * unit);
+      const bool up = ref - m_ref > kSlack;  // from -inf on: the first key that the row sees
+      if (__any(up)) follow_reference(move_reference(ref, up));
       exponentials(S, W);
     }
     if (within(h, v0, v1)) {
@@ -529,11 +535,11 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     weights(1);
     lay_out<2 * NT, 2, (CAP ? 104 : 56) / (4 * NT)>();
     asm volatile("" : "+v"(W.p[0]), "+v"(W.p[1]), "+v"(W.rest[0]), "+v"(W.rest[1]), "+v"(sum[0]), "+v"(sum[1]));  // (made here, not later)
-    if (__builtin_expect(__any(!(sum[0] + sum[1] <= kMost)), 0)) {
+    if (__builtin_expect(__any(!(sum[0] + sum[1] <= kMost<DT>)), 0)) {
       float mx = of[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, of[e]);
-      mx = max_halves(__builtin_fmaf(mx, unit, stage));
+      mx = reference_of<DT>(max_halves(__builtin_fmaf(mx, unit, stage)));
       follow_reference(move_reference(mx, mx > m_ref));
       off = (m_ref == -INFINITY ? 0.0f : m_ref) - stage;
       sum[0] = sum[1] = 0.0f;
@@ -571,6 +577,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
         locate_both();
       }
     }
+    // Q is waited for here, not at its first use in the loop: that wait would be on the counter of the stages on their way.
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
     if (n_st > 0) {
       // Turns [t0, t1) are whole for this wavefront, in pairs.
       const int t0 = (max(max(f0 + 1, w0 + 2), v0 + 2) + 1) & ~1, t1 = max(t0, min(min(f1, w1) + 1, v1) & ~1);

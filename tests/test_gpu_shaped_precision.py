@@ -5,7 +5,7 @@ import pytest
 from shaped_precision import bound
 from shaped_utils import ShapedCase, documents
 from test_gpu_shaped import Run, dev
-from espetero_amd import abi
+from espetero_amd import abi, synth
 from oracle import binding as ob
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +141,31 @@ def test_infinite_values_that_few_rows_see(workgroups, heads, hd, M, cap, bias, 
     same[:, :G, [3, 40, 77, 91]] = False
     same[M // 2:, :G, 90] = False
     assert (bits[same] == clean[same]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("n", [3000, 30000])
+@pytest.mark.parametrize("M,at", [(1, 7), (1, -9), (3, -9), (40, 7), (40, -50)])
+def test_many_small_weights_beside_a_large_one(M, at, n, hd, dtype):
+    """A flat tail of keys, each of 2^-24.5 of one key's weight (first or last of those that all rows see), whose large values make half of the
+    output: fp16 numbers of the largest weight 1 have no half step there."""
+    c = ShapedCase(1, 1, hd, dtype, 16, [(n, M)], seed=n)
+    at = at if at > 0 else n + at
+    f, to = lambda x: ob.to_f32(x, dtype), lambda x: synth._bits(np.atleast_1d(np.asarray(x, np.float32)), dtype)  # noqa: E731
+    c.Q[:, :] = 0
+    c.Q[:, 0] = to(16.0)[0]
+    c.K[0][:] = 0
+    c.K[0][at, 0, 0] = to(24.5 * np.log(2) / (16.0 * c.scale))[0]
+    rng = np.random.default_rng(n)
+    c.V[0][:] = to(rng.uniform(0.5, 1.0, c.V[0].shape) * 2.0 ** 24.5 / n)
+    c.V[0][at] = to(rng.uniform(0.5, 1.0, c.V[0][at].shape))
+    pool = c.pool.reshape(c.n_blocks, 2, c.bt * hd)
+    for b in range(-(-(n + M) // 16)):
+        k, v = (x[0][16 * b:16 * b + 16, 0] for x in (c.K, c.V))
+        block = pool[c.block_list[b]]
+        block[0].reshape(16, hd)[:len(k)] = k
+        block[1].reshape(hd, 16)[:, :len(v)] = v.T
+    assert f(c.V[0]).max() < 60000
+    check(c, range(0, M, 13), shift=15 if M < 40 else 7)
+    check(c, range(0, M, 13), shift=15 if M < 40 else 7, workgroups=16)
