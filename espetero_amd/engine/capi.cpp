@@ -80,7 +80,8 @@ static int plan_pass(const esp_attn_params* p, Pass kind, const esp_tree* trees,
   if (o->rows_per_tile <= 0 || o->groups_target <= 0 || o->granule <= 0 || o->max_splits <= 0 || o->min_chunk <= 0)
     return put_err(err, errlen, ESP_EINVAL, "plan options must be positive");
   if (o->granule % 16) return put_err(err, errlen, ESP_EINVAL, "granule must be a multiple of 16");
-  if (window > 0 && !pos) return put_err(err, errlen, ESP_EINVAL, "window needs pos");
+  if (kind != Pass::plain) pos = nullptr;  // (their kernels place a row's window by where it lies in the cache)
+  else if (window > 0 && !pos) return put_err(err, errlen, ESP_EINVAL, "window needs pos");
   try {
     AttnPlan A;
     A.trees.assign(trees, trees + n_trees);
@@ -91,7 +92,7 @@ static int plan_pass(const esp_attn_params* p, Pass kind, const esp_tree* trees,
                                               : 1;
     const PlanOptions options = to_cpp(*o);
     if (kind == Pass::shaped && family < 0 && options.balanced)
-      plan_shaped_tiled(A, p->head_dim, p->H, esp::shaped_workgroups_per_cu(p->head_dim, family), groups, window, pos, options);
+      plan_shaped_tiled(A, p->head_dim, p->H, esp::shaped_workgroups_per_cu(p->head_dim, family), groups, window, options);
     else
       plan_tiles(A, groups, window, pos, family < 0 ? options.for_diff_tiled() : options, kind == Pass::diff || family < 0 ? nullptr : p);
     *n_tiles = int32_t(A.tiles.size());

@@ -288,7 +288,7 @@ inline std::vector<int> stream_split(const std::vector<RowTile>& rts, const Plan
 }
 
 // groups: workgroups per tile (KV heads, or KV heads x head splits).
-// window > 0 needs pos (4 ints per row, pos[4 * row] = position).
+// window > 0: pos (4 ints per row, pos[4 * row] = position), or null where a row's position is where it lies in the cache, P + its number.
 // params: the layer the pass is planned for (may be null: a plan that holds for any).
 inline void plan_tiles(AttnPlan& A, int groups, int window, const int32_t* pos, const PlanOptions& o, const esp_attn_params* params = nullptr) {
   const PlanShape shape = plan_shape(params, groups, o.rows_per_tile);
@@ -305,8 +305,8 @@ inline void plan_tiles(AttnPlan& A, int groups, int window, const int32_t* pos, 
       if (window > 0) {
         // The tile's earliest row bounds what any of its rows can still see:
         // cached key j sits at position j, root row j at P + j (gemma.h:88-94).
-        int minpos = INT32_MAX;
-        for (int i = r; i < std::min(t.M, r + R); ++i) minpos = std::min(minpos, pos[4 * (t.base + i)]);
+        int minpos = pos ? INT32_MAX : t.P + r;
+        for (int i = r; pos && i < std::min(t.M, r + R); ++i) minpos = std::min(minpos, pos[4 * (t.base + i)]);
         k0 = std::clamp(minpos - window + 1, 0, t.P);
         b0 = std::max(0, minpos - window + 1 - t.P);
       }
@@ -677,7 +677,7 @@ inline void plan_tiles(AttnPlan& A, int groups, int window, const int32_t* pos, 
 // than the best of them in geometric mean. (24 rows behind 16000 keys, 32 / 8 heads: 400 us whole, 63 in 8 parts, 29 in 32; 1500 fresh rows,
 // 8 / 4 heads of 256: 73 whole, 41 in 60 parts.) A cut has to promise a tenth: spans, which are not known here, may leave a tile fewer keys than it
 // is planned for.
-inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, int groups, int window, const int32_t* pos, const PlanOptions& o) {
+inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, int groups, int window, const PlanOptions& o) {
   constexpr int kStage = 32;
   A.tiles.clear();
   A.combine.clear();
@@ -693,12 +693,7 @@ inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, 
   for (int ti = 0; ti < int(A.trees.size()); ++ti) {
     const esp_tree& t = A.trees[size_t(ti)];
     for (int r = 0; r < t.M; r += R) {
-      int lo = 0;
-      if (window > 0) {
-        int first = INT32_MAX;
-        for (int i = r; i < std::min(t.M, r + R); ++i) first = std::min(first, pos[4 * (t.base + i)]);
-        lo = std::clamp(first - window + 1, 0, t.P + r) / 16 * 16;
-      }
+      const int lo = window > 0 ? std::max(0, t.P + r - window + 1) / 16 * 16 : 0;
       const int hi = t.P + std::min(t.M, r + R), stages = (hi - lo + kStage - 1) / kStage;
       tiles.push_back({ti, r, lo, hi, stages});
       whole += stages;

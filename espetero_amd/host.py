@@ -104,7 +104,7 @@ def options_mi355x(rows, workgroups):
 
 def plan_tiles(trees, groups, window, pos, options):
     """trees: TREE_DT array. groups: plan_hint's, which plans for that layer (attn_diff_hint's: for differential attention on it, attn_shaped_hint's:
-    for attention with shaped scores), or a number, which plans for any. Returns (tiles TILE_DT, jobs COMBINE_DT, n_parts)."""
+    for attention with shaped scores; either reads no pos), or a number, which plans for any. Returns (tiles TILE_DT, jobs COMBINE_DT, n_parts)."""
     lib = engine_lib()
     trees = np.ascontiguousarray(trees, dtype=abi.TREE_DT)
     pos_a = None if pos is None else np.ascontiguousarray(pos, dtype=np.int32)

@@ -435,7 +435,7 @@ int esp_attn_shaped_hint(const esp_attn_params* p, int device, int32_t* workgrou
 /* Bytes of workspace for a plan of n_parts partial records. Host-only arithmetic. */
 size_t esp_attn_shaped_workspace_bytes(const esp_attn_params* p, int32_t n_parts);
 /* Of p: head_dim 128 or 256, H / Hkv at most 128, scale from 2^-64 to 2^64, no gate, no bidi; kv_ld is not read. Q and O [n_rows][q_ld];
- * rows outside the tiles are left as they are. Tiles, trees and jobs as planned by esp_plan_tiles_shaped (include/espetero_engine.h; a plan of esp_plan_tiles runs too, slower);
+ * rows outside the tiles are left as they are. Tiles, trees and jobs as planned by esp_plan_tiles_shaped (include/espetero_engine.h; a plan of esp_plan_tiles runs too, slower, with a window made from positions P + row number);
  * what the records have to promise is what esp_attn_validate_for(ESP_PASS_SHAPED) checks. Tiles with k1 = INT32_MAX end at the tree's
  * cached length as it is when the kernel runs (decode chains). */
 int esp_attn_shaped(const esp_attn_params* p, const esp_shape_params* shape, const void* Q, const void* kv_pool, const int32_t* blocks, void* O,

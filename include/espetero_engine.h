@@ -70,7 +70,8 @@ int esp_plan_tiles_for(const esp_attn_params* p, const esp_tree* trees, int32_t 
  * esp_plan_options_mi355x: where the tiled kernel serves p, those of a streaming pass (its tiles may have few rows, by which that
  * function tells the two apart) become its own, the pass's own rows are cut like cached keys (cut_batch), and its tiles come longest
  * last, which is the order the kernel starts them in, reversed. Fields that do not hold what that function gives a streaming pass stay as
- * they are, those of options for more than 32 rows among them (min_chunk 512, min_span 1024). */
+ * they are, those of options for more than 32 rows among them (min_chunk 512, min_span 1024). The kernel places a row's window by where the
+ * row lies in the cache, P + its number, whatever its position in rotary angles, and so does the plan: pos is not read and may be NULL. */
 int esp_plan_tiles_diff(const esp_attn_params* p, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
                         const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                         int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen);
@@ -78,7 +79,7 @@ int esp_plan_tiles_diff(const esp_attn_params* p, const esp_tree* trees, int32_t
 /* And for a pass of esp_attn_shaped (p: its parameters; groups: what esp_attn_shaped_hint reports): passes of the streaming kernel as
  * esp_plan_tiles_for plans them; on the tiled one every tile in parts of one length, cached keys and the pass's own rows alike, the length by
  * what the hand-out of their workgroups to the chip comes to (o: rows_per_tile, groups_target, max_splits, and a min_chunk that is not
- * esp_plan_options_mi355x's). The planner does not see the rows' spans. */
+ * esp_plan_options_mi355x's). The planner does not see the rows' spans; pos as above. */
 int esp_plan_tiles_shaped(const esp_attn_params* p, const esp_tree* trees, int32_t n_trees, int32_t groups, int32_t window, const int32_t* pos,
                           const esp_plan_options* o, esp_tile* tiles, int32_t tiles_cap, int32_t* n_tiles, esp_combine* jobs,
                           int32_t jobs_cap, int32_t* n_jobs, int32_t* n_parts, char* err, size_t errlen);
