@@ -832,6 +832,8 @@ int esp_attn_shaped(const esp_attn_params* p, const esp_shape_params* shape, con
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(err, errlen, ESP_EINVAL, "workspace must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(shape->spans) % 8 || reinterpret_cast<uintptr_t>(shape->slopes) % 4)
     return fail(err, errlen, ESP_EINVAL, "spans must be 8-byte, slopes 4-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(kv_pool)) % 16 || reinterpret_cast<uintptr_t>(O) % 8)
+    return fail(err, errlen, ESP_EINVAL, "Q and kv_pool must be 16-byte, O 8-byte aligned");
   DeviceState* dev = nullptr;
   if (int rc = device_state(&dev, err, errlen)) return rc;
   esp::ShapedArgs a{};
@@ -1150,6 +1152,7 @@ int esp_linear_attn(const esp_linear_params* p, const void* Q, const void* K, co
   if ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V) | reinterpret_cast<uintptr_t>(O) |
        reinterpret_cast<uintptr_t>(states) | reinterpret_cast<uintptr_t>(workspace)) % 16)
     return fail(err, errlen, ESP_EINVAL, "Q, K, V, O, states and workspace must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(decay) % 4) return fail(err, errlen, ESP_EINVAL, "decay must be 4-byte aligned");
   if (n_few > 65535 || n_tiles - n_few > 65535) return fail(err, errlen, ESP_EUNSUPPORTED, "%d and %d tiles in one pass: at most 65535 of each kind", n_few, n_tiles - n_few);
   const esp::LinearCarve c = esp::carve_linear(p->H, p->dk, p->dv, n_parts);
   if (n_parts > 0 && (!workspace || workspace_bytes < c.total))

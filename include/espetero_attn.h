@@ -403,9 +403,9 @@ int esp_attn_diff_hint(const esp_attn_params* p, int device, int32_t* workgroups
 size_t esp_attn_diff_workspace_bytes(const esp_attn_params* p, int32_t n_parts);
 /* Of p: head_dim 128, H and Hkv even, no gate, no bidi; kv_ld is not read. Q and O [n_rows][q_ld], O's pair i at column
  * 2 * head_dim * i; rows outside the tiles are left as they are. Tiles, trees and jobs as planned by esp_plan_tiles_diff
- * (include/espetero_engine.h; a plan of esp_plan_tiles runs too, slower); what the records have to promise is what
- * esp_attn_validate_for(ESP_PASS_DIFF) checks. Tiles with k1 = INT32_MAX end at the tree's cached length as it is when the
- * kernel runs (decode chains). */
+ * (include/espetero_engine.h; a plan of esp_plan_tiles runs too, slower, of a window the one for positions P + row number);
+ * what the records have to promise is what esp_attn_validate_for(ESP_PASS_DIFF) checks. Tiles with k1 = INT32_MAX end at the
+ * tree's cached length as it is when the kernel runs (decode chains). */
 int esp_attn_diff(const esp_attn_params* p, const esp_diff_params* d, const void* Q, const void* kv_pool, const int32_t* blocks, void* O,
                   const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees, int32_t n_trees, const esp_combine* jobs, int32_t n_jobs,
                   int32_t n_parts, int32_t n_rows, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t errlen);
@@ -434,9 +434,10 @@ int32_t esp_attn_shaped_rows(const esp_attn_params* p, int32_t rows);
 int esp_attn_shaped_hint(const esp_attn_params* p, int device, int32_t* workgroups, int32_t* groups_per_tile, char* err, size_t errlen);
 /* Bytes of workspace for a plan of n_parts partial records. Host-only arithmetic. */
 size_t esp_attn_shaped_workspace_bytes(const esp_attn_params* p, int32_t n_parts);
-/* Of p: head_dim 128 or 256, H / Hkv at most 128, scale from 2^-64 to 2^64, no gate, no bidi; kv_ld is not read. Q and O [n_rows][q_ld];
- * rows outside the tiles are left as they are. Tiles, trees and jobs as planned by esp_plan_tiles_shaped (include/espetero_engine.h; a plan of esp_plan_tiles runs too, slower, with a window made from positions P + row number);
- * what the records have to promise is what esp_attn_validate_for(ESP_PASS_SHAPED) checks. Tiles with k1 = INT32_MAX end at the tree's
+/* Of p: head_dim 128 or 256, H / Hkv at most 128, scale from 2^-64 to 2^64, no gate, no bidi; kv_ld is not read. Q and O [n_rows][q_ld], Q
+ * and the pool 16-byte, O 8-byte, spans 8-byte aligned; rows outside the tiles are left as they are. Tiles, trees and jobs as planned by
+ * esp_plan_tiles_shaped (include/espetero_engine.h; a plan of esp_plan_tiles runs too, slower, of a window the one for positions P + row
+ * number); what the records have to promise is what esp_attn_validate_for(ESP_PASS_SHAPED) checks. Tiles with k1 = INT32_MAX end at the tree's
  * cached length as it is when the kernel runs (decode chains). */
 int esp_attn_shaped(const esp_attn_params* p, const esp_shape_params* shape, const void* Q, const void* kv_pool, const int32_t* blocks, void* O,
                     const esp_tile* tiles, int32_t n_tiles, const esp_tree* trees, int32_t n_trees, const esp_combine* jobs, int32_t n_jobs,
@@ -581,7 +582,7 @@ typedef struct esp_linear_tile {
 int esp_linear_hint(const esp_linear_params* p, int device, int32_t* workgroups, char* err, size_t errlen);
 /* Never less for more parts. Host-only arithmetic. */
 size_t esp_linear_workspace_bytes(const esp_linear_params* p, int32_t n_parts);
-/* Q [n_rows][q_ld], K [n_rows][k_ld], V [n_rows][v_ld], O [n_rows][o_ld], 16-byte aligned like the workspace and the states; head h of V
+/* Q [n_rows][q_ld], K [n_rows][k_ld], V [n_rows][v_ld], O [n_rows][o_ld], 16-byte aligned like the workspace and the states (decay: 4); head h of V
  * and O at column h * dv, head i of Q and K at i * dk. tiles: device copies of esp_plan_linear's, n_few of them in front for the kernel that
  * takes sequences of few rows. Rows in no tile and slots that are no tile's dst are left as they are. O must not overlap Q, K or V. */
 int esp_linear_attn(const esp_linear_params* p, const void* Q, const void* K, const void* V, const float* decay, float* states, void* O,
