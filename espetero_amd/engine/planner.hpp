@@ -670,13 +670,13 @@ inline void plan_tiles(AttnPlan& A, int groups, int window, const int32_t* pos, 
 
 // Attention with shaped scores on its tiled kernel: every tile of rows in parts of at most so many stages of 32 keys, whichever of them the cache
 // and whichever the pass itself holds. What comes of a cut is worked out by handing its workgroups to the chip's slots, longest first (as the
-// records are ordered; the kernel takes them from the end); figures in microseconds, of 128 and 256 dims: 7.5 and 8.6 for a workgroup's
-// set-up and end, 1.05 and 1.76 for each of its first six stages (masked ones, turns not yet full), 0.75 and 1.05 for the others, 1.21 times as
-// much beside another workgroup on the compute unit, 4.9 and 5.0 for the merge, and the partial records at 3 MB a microsecond. Fitted to 109
-// passes of 13 to 1976 rows over 0 to 16000 keys, each timed whole and in up to 24 cuts: right within 12 %; what it picks takes 1.5 % longer
-// than the best of them in geometric mean. (24 rows behind 16000 keys, 32 / 8 heads: 400 us whole, 63 in 8 parts, 29 in 32; 1500 fresh rows,
-// 8 / 4 heads of 256: 73 whole, 41 in 60 parts.) A cut has to promise a tenth: spans, which are not known here, may leave a tile fewer keys than it
-// is planned for.
+// records are ordered; the kernel takes them from the end); figures in microseconds, of 128 and 256 dims: 9.3 and 8.8 for a workgroup's
+// set-up and end, 1.12 and 2.34 for each of its first six stages (masked ones, turns not yet full), 0.82 and 1.34 for the others, 1.2 times as
+// much beside another workgroup on the compute unit, 6.5 and 4.3 for the merge, and the partial records at 3.6 and 2.8 MB a microsecond. Fitted to
+// 109 passes of 13 to 1976 rows over 0 to 16000 keys, each timed whole and in up to 24 cuts: right within 14 % and 11 %; what it picks takes
+// 3.7 % longer than the fastest of those runs in geometric mean, 5.3 % over 109 others. (24 rows behind 16000 keys, 32 / 8 heads: 500 us whole, 76 in
+// 8 parts, 34 in 63; 1500 fresh rows, 8 / 4 heads of 256: 80 whole, 47 in 60 parts.) A cut has to promise a tenth: spans, which are not known
+// here, may leave a tile fewer keys than it is planned for.
 inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, int groups, int window, const PlanOptions& o) {
   constexpr int kStage = 32;
   A.tiles.clear();
@@ -702,7 +702,7 @@ inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, 
   }
   const int slots = std::max(per_cu, o.groups_target), units = std::max(1, slots / per_cu);
   const bool wide = head_dim == 256;
-  const double end = wide ? 8.6 : 7.5, first = wide ? 1.76 : 1.05, further = wide ? 1.05 : 0.75, merge = wide ? 5.0 : 4.9;
+  const double end = wide ? 8.8 : 9.3, first = wide ? 2.34 : 1.12, further = wide ? 1.34 : 0.82, merge = wide ? 4.3 : 6.5, rate = wide ? 2.8 : 3.6;
   struct Cut {
     int parts, each;
   };
@@ -731,7 +731,7 @@ inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, 
     free_at.push({0.0, few ? units : slots});
     double last = 0;
     for (const int stages : lengths) {
-      const double cost = end + (std::min(stages, 6) * first + std::max(stages - 6, 0) * further) * (few || per_cu == 1 ? 1.0 : 1.21);
+      const double cost = end + (std::min(stages, 6) * first + std::max(stages - 6, 0) * further) * (few || per_cu == 1 ? 1.0 : 1.2);
       for (long long left = groups; left > 0;) {
         const Free f = free_at.top();
         const long long take = std::min(left, f.second);
@@ -742,7 +742,7 @@ inline void plan_shaped_tiled(AttnPlan& A, int head_dim, int heads, int per_cu, 
         left -= take;
       }
     }
-    return last + (records > 0 ? merge + records * heads * head_dim * 4e-6 / 3.0 : 0.0);
+    return last + (records > 0 ? merge + records * heads * head_dim * 4e-6 / rate : 0.0);
   };
   int most = longest;
   if ((long long)tiles.size() * groups < 4LL * slots && whole > 0) {
