@@ -22,7 +22,7 @@ struct ShapedUnit {  // 16 keys: K and V^T
 }  // namespace
 
 template <int DT, int HD, int NC, bool CAP>
-__global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_stream_kernel(const ShapedArgs a) {
+__global__ __launch_bounds__(256, HD == 128 && NC == 1 ? 2 : 1) void attn_shaped_stream_kernel(const ShapedArgs a) {
   constexpr int MT = HD / 16, KK = HD / 32, LDO = HD + 4, VEC = HD / 64;
   extern __shared__ float smem[];  // [4 wavefronts][NC * 16 columns][LDO] O, then [4][NC * 16][2] m, l
   const int kvh = blockIdx.x;
@@ -219,9 +219,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_stream_ker
     }
   };
 
-  // Infinite and NaN values of an interior unit go into its products as they are, where a weight's second number, or one that has vanished, makes
-  // NaN of an infinity: a wavefront that has met one takes its units once more, in the same order, each with such values taken out.
-  for (bool careful = false;; careful = true) {
+  auto clear = [&] {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       m_run[c] = -INFINITY;
@@ -229,33 +227,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_stream_ker
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) acc[c][mt] = f32x4{0, 0, 0, 0};
     }
-    ShapedUnit<HD> U[2];
-    const int n_int = ui1 - ui0, n_lo = ui0 - u_lo, n_edge = n_units - n_int;
-    const int n_mine = n_int > wave ? (n_int - wave + 3) / 4 : 0;
-    const int u0 = ui0 + wave;
-    if (!careful && n_mine > 0) {
-      load(u0, U[0]);
-      int i = 0;
-      for (; i + 2 < n_mine; i += 2) {
-        load(u0 + 4 * (i + 1), U[1]);
-        interior(u0 + 4 * i, U[0]);
-        load(u0 + 4 * (i + 2), U[0]);
-        interior(u0 + 4 * (i + 1), U[1]);
-      }
-      if (i + 2 == n_mine) {
-        load(u0 + 4 * (i + 1), U[1]);
-        interior(u0 + 4 * i, U[0]);
-        interior(u0 + 4 * (i + 1), U[1]);
-      } else {
-        interior(u0 + 4 * i, U[0]);
-      }
-    }
-    const int e0 = (wave + 4 - n_int % 4) % 4;  // go on with the round robin
-    for (int i = e0 - (careful ? 4 * n_mine : 0); i < n_edge; i += 4) {
-      const int u = i < e0 ? u0 + i - e0 + 4 * n_mine : i < n_lo ? u_lo + i : ui1 + (i - n_lo);
-      load(u, U[0]);
-      edge(u, U[0], careful);
-    }
+  };
+  auto odd = [&] {  // is some sum infinite or NaN?
     float nf = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -265,7 +238,49 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_stream_ker
 #pragma unroll
         for (int e = 0; e < 4; ++e) nf = __builtin_fmaf(acc[c][mt][e], 0.0f, nf);
       }
-    if (careful || __builtin_expect(!__any(nf != 0.0f), 1)) break;  // (NaN, or 0)
+    return __any(nf != 0.0f) != 0;  // (NaN, or 0)
+  };
+  const int n_int = ui1 - ui0, n_lo = ui0 - u_lo, n_edge = n_units - n_int;
+  const int n_mine = n_int > wave ? (n_int - wave + 3) / 4 : 0;
+  const int u0 = ui0 + wave, e0 = (wave + 4 - n_int % 4) % 4;  // edges go on with the round robin
+  auto edge_unit = [&](int i) { return i < n_lo ? u_lo + i : ui1 + (i - n_lo); };
+  ShapedUnit<HD> U[2];
+  clear();
+  if (n_mine > 0) {
+    load(u0, U[0]);
+    int i = 0;
+    for (; i + 2 < n_mine; i += 2) {
+      load(u0 + 4 * (i + 1), U[1]);
+      interior(u0 + 4 * i, U[0]);
+      load(u0 + 4 * (i + 2), U[0]);
+      interior(u0 + 4 * (i + 1), U[1]);
+    }
+    if (i + 2 == n_mine) {
+      load(u0 + 4 * (i + 1), U[1]);
+      interior(u0 + 4 * i, U[0]);
+      interior(u0 + 4 * (i + 1), U[1]);
+    } else {
+      interior(u0 + 4 * i, U[0]);
+    }
+  }
+  for (int i = e0; i < n_edge; i += 4) {
+    load(edge_unit(i), U[0]);
+    edge(edge_unit(i), U[0], false);
+  }
+  // Infinite and NaN values of an interior unit go into its products as they are, where a weight's second number, or one that has vanished, makes
+  // NaN of an infinity: a wavefront that has met one takes its units once more, in the same order, each with such values taken out.
+  if (__builtin_expect(odd(), 0)) {
+    clear();
+#pragma unroll 1
+    for (int i = e0 - 4 * n_mine; i < n_edge; i += 4) {
+      const int u = i < e0 ? u0 + i - e0 + 4 * n_mine : edge_unit(i);
+      load(u, U[0]);
+      edge(u, U[0], true);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) mfma_settle(acc[c][mt]);
   }
 
   // ---- merge the 4 wavefronts in order
