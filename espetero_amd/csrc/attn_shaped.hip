@@ -5,8 +5,8 @@
 // Streaming kernel: decode and short trees. Bound by HBM: every visible key's K and V are read once for all G query heads of a KV head and
 // all rows of the tile. One workgroup is one tile and one KV head; up to 16 packed rows (row in tile * G + head of the group) are the columns
 // of a matrix tile, NC such tiles. A wavefront takes 16-key units round robin straight from HBM with the next unit's loads in
-// flight; the four wavefronts' sums meet in LDS at the end. 24 sequences of 300 to 9000 keys, 32 / 8 heads of 128 dims: 89 us for 540 MB, 6.0 TB/s
-// of the 6.6 that a plain read of such pages reaches, and 5 us for the merge; two or three units ahead in place of one: 88.
+// flight; the four wavefronts' sums meet in LDS at the end. 24 sequences of 300 to 9000 keys, 32 / 8 heads of 128 dims: 90 us for 540 MB, 6.0 TB/s
+// of the 6.6 that a plain read of such pages reaches, and 5 us for the merge; two or three units ahead in place of one: 1 us less.
 #include "shaped_math.hpp"
 
 namespace esp {
@@ -456,8 +456,8 @@ hipError_t launch_stream_t(const ShapedArgs& a, int n_tiles, hipStream_t st) {
   return a.cap_log2 > 0.0f ? launch_stream_c<DT, HD, NC, true>(a, n_tiles, st) : launch_stream_c<DT, HD, NC, false>(a, n_tiles, st);
 }
 
-// Pass and merge with one wavefront an output and with four, us: 16 parts of one tile 9.0 and 8.0, 63 of one 23.6 and 17.6 (of 24 rows 32.5 and 28), 64 of
-// eight 30.3 and 29.2, 57 of eighteen 83.8 and 84.9. (2048 workgroups of four wavefronts are what the chip holds.)
+// Pass and merge with one wavefront an output and with four, us: 16 parts of one tile 9.8 and 8.3, 63 of one 24.4 and 18.5 (of 24 rows 37 and 31), 64 of
+// eight 27.0 and 26.6, 54 of eighteen 89.7 and 90.1. (2048 workgroups of four wavefronts are what the chip holds.)
 template <int DT, int HD>
 void launch_merge_t(const ShapedArgs& a, const esp_combine* jobs, int n_jobs, int n_parts, hipStream_t st) {
   const unsigned outs = unsigned(a.R * a.H), jobs_n = unsigned(n_jobs);

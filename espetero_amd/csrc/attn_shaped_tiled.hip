@@ -13,15 +13,14 @@
 // Scores: the bias is what the score product's accumulator starts from (without a cap; behind a cap it is the last step's addend), but for
 // what it has of the stage, which is taken from the reference. A cap is tanh as an odd polynomial where all of a wavefront's scores of the
 // stage are below 0.2 caps (four operations a score) or 0.7 (six), else by an exponential and a reciprocal (eleven). 2048 rows behind 8000 keys,
-// 32 / 8 heads of 128 dims, bf16, 303 billion operations, by the card's clock: plain 310 to 350 us, with slopes 295 to 335, with a cap 370 (scores
-// below 0.2 caps; else 395), with both 395 (425), 0.72 to 0.77 PFLOP/s, where the vector units issue in two thirds of the clocks. Short ranges are
-// bound by their ends: three prompts of 500 to 2000 rows in six documents each take 52 to 57 us, of which a tile's seven stages are a third, its first
-// loads from memory another.
+// 32 / 8 heads of 128 dims, bf16, 303 billion operations, us: plain 424, with slopes 416, with a cap, with slopes or without, 472 (scores below 0.2
+// caps), 494 (0.7) and 505 (above), 0.60 to 0.73 PFLOP/s and half as much again with the weights' second numbers, matrix units busy 47 % and vector
+// units 60 % of the clocks; 16 / 8 heads of 256 dims: plain 421, with a cap 462, 473 and 476. Short ranges are bound by their ends: three prompts of
+// 500 to 2000 rows in six documents each take 60 to 66 us, of which a tile's seven stages are a third, its first loads from memory another.
 //
 // P enters its product as the sum of two numbers of the storage type, 16 bits or more, as in the streaming kernel, so that a row is as exact
 // in a pass of many rows as in one of few: an output's error is that of its own rounding. One number, half of P . V's matrix work, makes it up to 1.4
-// times as much, 0.0023 of the output's size for 0.0017 (bf16): the chunk with both then takes 392 us where two numbers take 500, the packed
-// documents 57 and 67.
+// times as much, 0.0023 of the output's size for 0.0017 (bf16): the chunk with both then takes 392 us, the packed documents 52 to 57.
 //
 // LDS: a ring of 4 stages of 32 keys, K and V^T, loaded straight from the pool (global_load_lds): wavefronts 0 and 1 load the
 // two sub-blocks of K, two stages ahead of the scores, 2 and 3 those of V^T, two ahead of P . V. K: the 16-byte chunk c of row r lies at
@@ -172,8 +171,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   const Sight rg = shaped_range(tile, tree, whole.some_from, whole.some_end);
 
   // ---- stages of 32 keys, the last ones first: a bias makes near keys' scores the largest, and taken from the far ones on every stage's would
-  // move the reference (2048 rows behind 8000 keys, 32 / 8 heads, 8 of them of slopes above 0.17: 500 us). Stage h holds the keys from
-  // key_of(h) on, the last stage's from the sub-block of the first key on. Which stages this wavefront's rows see, and which whole:
+  // move the reference (2048 rows behind 8000 keys, 32 / 8 heads, 8 of them of slopes above 0.17, with single weights: 500 us for 354). Stage h
+  // holds the keys from key_of(h) on, the last stage's from the sub-block of the first key on. Which stages this wavefront's rows see, and which
+  // whole:
   const int s0 = rg.from & ~15;
   const int n_st = rg.end > rg.from ? (rg.end - s0 + 31) >> 5 : 0;
   auto key_of = [&](int h) { return s0 + 32 * (n_st - 1 - h); };
@@ -563,7 +563,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) acc[nt] = f32x16{};
     // A pair of turns h and h + 1 requests stages h + lead and h + 1 + lead, both in the first turn, so that the barrier behind the second does
-    // not wait for them (2048 rows behind 8000 keys, 16 / 8 heads of 256 dims, capped: 393 to 378 us).
+    // not wait for them (2048 rows behind 8000 keys, 16 / 8 heads of 256 dims, capped, with single weights: 393 to 378 us).
     {
       next_id[0] = block_id();
       at_t0[0] = next_t0;

@@ -76,9 +76,9 @@ constexpr DiffCarve carve_diff(int H, int rows_per_tile, int64_t n_parts) {
 }
 
 // Attention with shaped scores: 1 or 2, the streaming kernel with that many column tiles; -1, the tiled one, up to 128 packed rows; 0, no
-// kernel. Streaming and tiled, bf16, us: 24 sequences of 300 to 6000 keys, 4 packed rows of 128 dims 64 and 72, 16 65 and 74, 32 75 and 79 (with 4
-// KV heads 40 and 36), 16 of 256 dims 132 and 145; one of 1000 keys, 4 packed rows 8.2 and 9.9, 32 11.4 and 11.5. From 17 to 32 the
-// streaming kernel's two numbers for a weight are the reason; of 256 dims a second column tile does not fit its registers.
+// kernel. Streaming and tiled, bf16, us: 24 sequences of 300 to 6000 keys, 4 packed rows of 128 dims 67 and 79, 16 68 and 81, 32 78 and 84 (with 4
+// KV heads 41 and 46), 16 of 256 dims 134 and 161; one of 1000 keys, 4 packed rows 8.0 and 10.7, 32 11.5 and 11.5. Of 256 dims a second column
+// tile does not fit the streaming kernel's registers.
 constexpr int shaped_family(int head_dim, int rows_per_tile, int G) {
   if (rows_per_tile <= 0 || G <= 0 || rows_per_tile > 128 / G) return 0;
   const int nc = (rows_per_tile * G + 15) / 16;

@@ -104,8 +104,10 @@ __global__ __launch_bounds__(256) void linear_few_kernel(const LinearArgs a) {
 // one a wavefront, P by one a row, V' by one a column: they lose what lies 2^-39 below the largest.
 //
 // Bound by the matrix units and what feeds them: with the numbers counted a chunk of 64 rows, 128 x 128, is 13.6 million operations, 2 us of
-// a compute unit's matrix units; two workgroups beside each other take 6.9 us for one each. 40 heads of 4 x 2048 rows, 128 x 128, bf16: 139 us;
-// 32 heads of 16000 rows, 64 x 128: 152 us, in 16 segments.
+// a compute unit's matrix units; two workgroups beside each other take 6.9 us for one each. 40 heads of 4 x 2048 rows, 128 x 128, bf16: 133 to 137 us;
+// 32 heads of 16000 rows, 64 x 128, on 8 heads of Q and K: 146 to 152 us, in 16 segments. 539 and 655 MB move in
+// that, at 4.0 and 4.4 TB/s, but they are the lesser part of what bounds it: the same passes with one head of Q and K for all heads, which is half of
+// the first one's bytes, take 17 % and 5 % less.
 //
 // A sequence may be cut into segments: a first launch makes each segment's own state from zero (STATE; the first one's from
 // the sequence's), and the segments then start from the sum of those in front of them, each decayed over the segments between.

@@ -15,8 +15,9 @@ constexpr int kLinearChunk = 64;  // rows that the chunked kernel takes at a tim
 // 6.3 and 9.1, of 12 8.0 and 9.2.
 constexpr int kLinearFew = 8;
 
-// Columns of V that a workgroup of the chunked kernel takes: P is made once more for every other 64. 128 and 64 columns, bf16, us: four prompts of
-// 2048 rows, 40 heads of 128 x 128, 138 and 193; 24 of 300, 32 heads, 85 and 121; one of 2000, 32 heads, 45 and 54, 8 heads 38 and 34.
+// Columns of V that a workgroup of the chunked kernel takes: P is made once more for every other 64. 128 and 64 columns, bf16, us, passes without
+// a pause between them: four prompts of 2048 rows, 40 heads of 128 x 128, 157 and 194; 24 of 300, 32 heads, 91 and 120; one of 2000, 32 heads,
+// 44 and 49, 8 heads 30 and 29.5.
 constexpr int linear_cols(int dv) { return dv % 128 == 0 ? 128 : 64; }
 constexpr bool linear_dims(int dk, int dv) { return (dk == 64 || dk == 128) && dv >= 64 && dv <= 512 && dv % 64 == 0; }
 
