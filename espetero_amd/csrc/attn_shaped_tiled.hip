@@ -410,23 +410,36 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     if (ln == 0) bad[2 * (uint32_t(h) & (kRing - 1)) + (wave & 1)] = any;
   };
   bool marked;
+  // A product of marks in such values' places with the keys that the rows see, which weigh something however little, says which outputs they reach.
+  // (2048 rows behind 8000 keys, 32 / 8 heads: 520 us, 1330 with one infinite value, which is the second walk, 5300 with some in every stage.)
   auto marks = [&](int h) __attribute__((always_inline)) {
     const int ln = here(lane), lo = max(rg.from, sight.from), n = max(0, min(rg.end, sight.end) - lo);
+    constexpr uint32_t one = DT == ESP_F16 ? 0x3c00u : 0x3f80u;
 #pragma unroll 1
     for (int w = 0; w < NT; ++w) {
       uint32_t* const word = reinterpret_cast<uint32_t*>(lds + L::kMarks) + (wave * NT + w) * 64 + ln;
       uint32_t found = marked ? *word : 0u;
 #pragma unroll 1
-      for (int t = 0; t < 32; ++t) {
-        const int key = key_of(h) + t;
-        if (key < rg.from || key >= rg.end || uint32_t(key - lo) >= uint32_t(n)) continue;  // (a key that the row sees weighs something)
-        const uint16_t* v = a.pool + size_t(a.kv_base) + (size_t(shaped_block(a, table, key / a.bt)) * size_t(a.Hkv) + size_t(kvh)) * head +
-                            vt_elem(a.bt, HD, key % a.bt, 32 * w + 4 * (ln >> 5));
+      for (int neg = 0; neg < 2; ++neg) {
+        f32x16 seen = f32x16{};
 #pragma unroll 1
-        for (int e = 0; e < 16; ++e) {
-          const uint32_t x = v[(8 * (e >> 2) + (e & 3)) * kVtDim];
-          found |= (not_finite_marks<DT>(x, false) & 0xffffu ? 1u << e : 0u) | (not_finite_marks<DT>(x, true) & 0xffffu ? 0x10000u << e : 0u);
+        for (int key = key_of(h); key <= min(key_of(h) + 16, last_sub); key += 16) {
+          const uint16_t* v = a.pool + size_t(a.kv_base) + (size_t(shaped_block(a, table, key / a.bt)) * size_t(a.Hkv) + size_t(kvh)) * head +
+                              vt_elem(a.bt, HD, key % a.bt, 32 * w + (ln & 31)) + 8 * (ln >> 5);
+          u32x4 x = *reinterpret_cast<const u32x4*>(v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = not_finite_marks<DT>(x[e], neg != 0);
+          u32x4 sees;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = key + 8 * (ln >> 5) + 2 * e - lo;
+            sees[e] = (uint32_t(at) < uint32_t(n) ? one : 0u) | (uint32_t(at + 1) < uint32_t(n) ? one << 16 : 0u);
+          }
+          seen = mfma32x16<DT>(x, sees, seen);
+          mfma_settle(seen);
         }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) found |= seen[e] > 0.0f ? (neg ? 0x10000u : 1u) << e : 0u;
       }
       *word = found;
     }

@@ -169,3 +169,22 @@ def test_many_small_weights_beside_a_large_one(M, at, n, hd, dtype):
     assert f(c.V[0]).max() < 60000
     check(c, range(0, M, 13), shift=15 if M < 40 else 7)
     check(c, range(0, M, 13), shift=15 if M < 40 else 7, workgroups=16)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,hd,M", [((4, 2), 128, 70), ((4, 2), 256, 40), ((4, 2), 128, 3)])
+def test_infinite_values_of_every_key(heads, hd, M, dtype):
+    """A dim of KV head 0 that is infinite for every key, the other KV head NaN throughout; two documents and a prefix."""
+    P, inf = 300, 0x7C00 if dtype == F16 else 0x7F80
+    c = ShapedCase(*heads, hd, dtype, 32, [(P, M)], spans=[documents(P, M, [0, 60, P + M // 2], 50)], bias=True, sharp=0.25, seed=11)
+    r = Run(c)
+    pool = c.pool.copy().reshape(c.n_blocks, c.Hkv, 2, c.bt // 16, hd * 16)
+    V = pool[:, :, 1].reshape(c.n_blocks, c.Hkv, c.bt // 16, hd, 16)
+    V[:, 0, :, 17], V[:, 1] = inf | 0x8000, 0x7E00 if dtype == F16 else 0x7FC0
+    pool[:, :, 1] = V.reshape(c.n_blocks, c.Hkv, c.bt // 16, hd * 16)
+    r.pool = dev(pool.reshape(-1))
+    got = ob.to_f32(r(), dtype).reshape(M, 4, hd)
+    want, tol, _ = bound(c)
+    assert np.isnan(got[:, 2:]).all() and (got[:, :2, 17] == -np.inf).all()
+    keep = np.arange(hd) != 17
+    assert np.all(np.abs(got[:, :2, keep] - want[:, :2, keep]) <= tol[:, :2, keep])
