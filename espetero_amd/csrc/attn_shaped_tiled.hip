@@ -332,19 +332,24 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   };
   // With a cap scores are in log2 units, else still in those of the products.
   const float unit = CAP ? 1.0f : a.scale_log2;
-  auto exponentials = [&](const f32x16& x, Weights& w) __attribute__((always_inline)) {
-    const float off = m_ref == -INFINITY ? 0.0f : m_ref;
+  // `far`: each score rounded as the reference it was taken for, and then their difference, where fp32 tells scores of millions and more apart by
+  // whole units only: as one operation the largest's own would be as far off 0.
+  auto weights_of = [&](auto far, const f32x16& x, float off, Weights& w) __attribute__((always_inline)) {
     float lx = 0.0f;
 #pragma unroll
     for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int at = 8 * sb + 2 * e;
-        const float p0 = fast_exp2(CAP ? x[at] - off : __builtin_fmaf(x[at], unit, -off));
-        const float p1 = fast_exp2(CAP ? x[at + 1] - off : __builtin_fmaf(x[at + 1], unit, -off));
-        put_weights<DT>(w, sb, e, p0, p1, sb ? lx : l_run);
+        auto less = [&](float y) { return CAP ? y - off : far ? __builtin_fmaf(y, unit, 0.0f) - off : __builtin_fmaf(y, unit, -off); };
+        put_weights<DT>(w, sb, e, fast_exp2(less(x[at])), fast_exp2(less(x[at + 1])), sb ? lx : l_run);
       }
     l_run += lx;
+  };
+  auto exponentials = [&](const f32x16& x, Weights& w) __attribute__((always_inline)) {
+    const float off = m_ref == -INFINITY ? 0.0f : m_ref;
+    if (!CAP && __builtin_expect(__any(fabsf(off) >= 0x1p20f), 0)) weights_of(std::true_type{}, x, off, w);
+    else weights_of(std::false_type{}, x, off, w);
   };
   // A new reference where a score exceeds the old one by more than kSlack. What was weighed by the old one joins the accumulators
   // first; then they go over to the new one.
@@ -505,13 +510,12 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   auto whole_turn = [&](auto first, int h, f32x16& to, f32x16& of, const Weights& had, Weights& W) __attribute__((always_inline)) {
     const float stage = bias_at(h - 1) * unit;
     float off = m_ref - stage, sum[2] = {0.0f, 0.0f};
-    auto weights = [&](int sb) __attribute__((always_inline)) {
+    auto weights = [&](int sb, bool again) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int at = 8 * sb + 2 * e;
-        const float p0 = fast_exp2(CAP ? of[at] - off : __builtin_fmaf(of[at], unit, -off));
-        const float p1 = fast_exp2(CAP ? of[at + 1] - off : __builtin_fmaf(of[at + 1], unit, -off));
-        put_weights<DT>(W, sb, e, p0, p1, sum[sb]);
+        auto less = [&](float x) { return again ? __builtin_fmaf(x, unit, stage) - off : CAP ? x - off : __builtin_fmaf(x, unit, -off); };
+        put_weights<DT>(W, sb, e, fast_exp2(less(of[at])), fast_exp2(less(of[at + 1])), sum[sb]);
       }
     };
     auto made_here = [&]() __attribute__((always_inline)) {
@@ -528,7 +532,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
         // Requests one by one: together at the turn's beginning they stand in line behind those of the other wavefronts.
         if (first && g % 2 == 1 && g < 2 * LOADS) request(h + lead, g / 2, 0);
       });
-      if constexpr (!CAP) weights(0);
+      if constexpr (!CAP) weights(0, false);
       lay_out<KS, 1, (CAP ? (terms == 3 ? 6 : 8) * 16 : 56) / KS>();
       made_here();
     };
@@ -544,8 +548,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
     weigh(h - 2, had, [&](int g) __attribute__((always_inline)) {
       if (first && g % 2 == 1 && g < 2 * LOADS) request(h + 1 + lead, g / 2, 1);
     });
-    if constexpr (CAP) weights(0);
-    weights(1);
+    if constexpr (CAP) weights(0, false);
+    weights(1, false);
     lay_out<2 * NT, 2, (CAP ? 104 : 56) / (4 * NT)>();
     asm volatile("" : "+v"(W.p[0]), "+v"(W.p[1]), "+v"(W.rest[0]), "+v"(W.rest[1]), "+v"(sum[0]), "+v"(sum[1]));  // (made here, not later)
     if (__builtin_expect(__any(!(sum[0] + sum[1] <= kMost<DT>)), 0)) {
@@ -554,10 +558,10 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, of[e]);
       mx = reference_of<DT>(max_halves(__builtin_fmaf(mx, unit, stage)));
       follow_reference(move_reference(mx, mx > m_ref));
-      off = (m_ref == -INFINITY ? 0.0f : m_ref) - stage;
+      off = m_ref == -INFINITY ? 0.0f : m_ref;
       sum[0] = sum[1] = 0.0f;
-      weights(0);
-      weights(1);
+      weights(0, true);  // (of scores rounded as the reference is)
+      weights(1, true);
     }
     l_run += sum[0] + sum[1];
     if constexpr (!first) locate_both();

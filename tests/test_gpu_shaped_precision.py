@@ -188,3 +188,30 @@ def test_infinite_values_of_every_key(heads, hd, M, dtype):
     assert np.isnan(got[:, 2:]).all() and (got[:, :2, 17] == -np.inf).all()
     keep = np.arange(hd) != 17
     assert np.all(np.abs(got[:, :2, keep] - want[:, :2, keep]) <= tol[:, :2, keep])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (0.0, True), (1.0, False), (1.0, True)])
+@pytest.mark.parametrize("hd,M", [(128, 1), (128, 80), (256, 3), (256, 80)])
+@pytest.mark.parametrize("scale", [20, 27, 30, 40, 60, 64])
+def test_scores_beyond_what_fp32_tells_apart(scale, hd, M, cap, bias, dtype):
+    """Scores of 2^20 to 2^69, with caps a hundredth of that or none: rows stay finite and between the values they see, and a row whose largest score is far
+    ahead of the others has that key's value."""
+    c = ShapedCase(4, 2, hd, dtype, 16, [(700, M)], cap=0.0, bias=bias, seed=21)
+    c.scale = 2.0 ** scale
+    c.cap = 0.1 * c.scale * cap
+    if bias:
+        c.slopes *= np.float32(2.0 ** (scale - 8))
+    for plan in ({}, dict(workgroups=2048, cut_batch=True)):
+        got = ob.to_f32(Run(c, **plan)(), dtype).astype(np.float64).reshape(M, 4, hd)
+        assert np.isfinite(got).all()
+        for m in (0, M - 1):
+            for h in range(4):
+                K, V = (ob.to_f32(x[0], dtype).astype(np.float64)[:700 + m + 1, h // 2] for x in (c.K, c.V))
+                assert (np.abs(got[m, h]) <= np.abs(V).max(0) * (1 + 2.0 ** -7)).all()
+                x = K @ ob.to_f32(c.Q, dtype).astype(np.float64)[m, h * hd:(h + 1) * hd] * c.scale
+                x = c.cap * np.tanh(x / c.cap) if c.cap else x
+                x = x - (float(c.slopes[h]) * (700 + m - np.arange(700 + m + 1)) if bias else 0)
+                top = np.argsort(x)[-2:]
+                if x[top[1]] - x[top[0]] > 2.0 ** -10 * np.abs(x).max() + 200:
+                    assert (np.abs(got[m, h] - V[top[1]]) <= 2.0 ** -7 * np.abs(V).max(0)).all()
