@@ -26,6 +26,10 @@ def bound(c, shift=0, rows=None):
             n, ago = end - lo, np.abs(P + m - np.arange(lo, end))
             which.append(base + m)
             for h in range(c.H):
+                if n == 0:                                             # a row that sees nothing
+                    O.append(np.zeros(hd))
+                    tol.append(np.zeros(hd))
+                    continue
                 k, v, q = K[lo:end, h // G], V[lo:end, h // G], Q[base + m, h]
                 x = k @ q * c.scale
                 e = (hd + 4) * c.scale * (np.abs(k) @ np.abs(q)).max()
@@ -36,7 +40,7 @@ def bound(c, shift=0, rows=None):
                     b = float(c.slopes[h]) * ago
                     x = x - b
                     near = x > x.max() - 100                           # what weighs anything
-                    e += 2 * b[near].max() + 6 * np.abs(x[near]).max()
+                    e += 2 * np.abs(b[near]).max() + 6 * np.abs(x[near]).max()
                 else:
                     e += 6 * np.abs(x).max()
                 w = np.exp(x - x.max())
