@@ -332,16 +332,17 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   };
   // With a cap scores are in log2 units, else still in those of the products.
   const float unit = CAP ? 1.0f : a.scale_log2;
-  // `far`: each score rounded as the reference it was taken for, and then their difference, where fp32 tells scores of millions and more apart by
-  // whole units only: as one operation the largest's own would be as far off 0.
+  // `far`: for rows whose reference is in the millions or more, where fp32 tells scores apart by whole units only, each score rounded as the
+  // reference it was taken for, and then their difference: as one operation the largest's own would be as far off 0.
   auto weights_of = [&](auto far, const f32x16& x, float off, Weights& w) __attribute__((always_inline)) {
+    const bool apart = far && fabsf(off) >= 0x1p20f;  // (by row: the others keep their bits)
     float lx = 0.0f;
 #pragma unroll
     for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int at = 8 * sb + 2 * e;
-        auto less = [&](float y) { return CAP ? y - off : far ? __builtin_fmaf(y, unit, 0.0f) - off : __builtin_fmaf(y, unit, -off); };
+        auto less = [&](float y) { return CAP ? y - off : apart ? __builtin_fmaf(y, unit, 0.0f) - off : __builtin_fmaf(y, unit, -off); };
         put_weights<DT>(w, sb, e, fast_exp2(less(x[at])), fast_exp2(less(x[at + 1])), sb ? lx : l_run);
       }
     l_run += lx;
@@ -510,11 +511,11 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
   auto whole_turn = [&](auto first, int h, f32x16& to, f32x16& of, const Weights& had, Weights& W) __attribute__((always_inline)) {
     const float stage = bias_at(h - 1) * unit;
     float off = m_ref - stage, sum[2] = {0.0f, 0.0f};
-    auto weights = [&](int sb, bool again) __attribute__((always_inline)) {
+    auto weights = [&](int sb, bool apart) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int at = 8 * sb + 2 * e;
-        auto less = [&](float x) { return again ? __builtin_fmaf(x, unit, stage) - off : CAP ? x - off : __builtin_fmaf(x, unit, -off); };
+        auto less = [&](float x) { return apart ? __builtin_fmaf(x, unit, stage) - m_ref : CAP ? x - off : __builtin_fmaf(x, unit, -off); };
         put_weights<DT>(W, sb, e, fast_exp2(less(of[at])), fast_exp2(less(of[at + 1])), sum[sb]);
       }
     };
@@ -558,10 +559,11 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_shaped_tiled_kern
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, of[e]);
       mx = reference_of<DT>(max_halves(__builtin_fmaf(mx, unit, stage)));
       follow_reference(move_reference(mx, mx > m_ref));
-      off = m_ref == -INFINITY ? 0.0f : m_ref;
+      off = (m_ref == -INFINITY ? 0.0f : m_ref) - stage;
+      const bool apart = fabsf(m_ref) >= 0x1p20f && m_ref != -INFINITY;
       sum[0] = sum[1] = 0.0f;
-      weights(0, true);  // (of scores rounded as the reference is)
-      weights(1, true);
+      weights(0, apart);
+      weights(1, apart);
     }
     l_run += sum[0] + sum[1];
     if constexpr (!first) locate_both();

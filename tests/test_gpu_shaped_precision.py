@@ -215,3 +215,28 @@ def test_scores_beyond_what_fp32_tells_apart(scale, hd, M, cap, bias, dtype):
                 top = np.argsort(x)[-2:]
                 if x[top[1]] - x[top[0]] > 2.0 ** -10 * np.abs(x).max() + 200:
                     assert (np.abs(got[m, h] - V[top[1]]) <= 2.0 ** -7 * np.abs(V).max(0)).all()
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("P", [40, 600])
+def test_rows_beside_others_of_any_scores(P, hd, bias):
+    """Rows of a tile whose scores are beyond 2^20, infinite or NaN, or whose largest come late: the others are as exact as ever, and where no stage is
+    seen whole by all of them they keep their bits."""
+    M = 24
+    c = ShapedCase(8, 2, hd, BF16, 16, [(P, M)], bias=bias, seed=31)
+    r = Run(c, workgroups=1)
+    clean = r()
+    odd = [1, 2, 9, 16, 23]
+    Q = c.Q.copy()
+    for m, by in zip(odd, [2.0 ** 24, 2.0 ** 40, 30.0, 8.0, 1.0]):
+        Q[m] = synth._bits(ob.to_f32(Q[m], BF16) * np.float32(by), BF16)
+    Q[odd[0], 5], Q[odd[4], 7] = 0x7F80, 0x7FC0                          # an infinity, NaN
+    r.Q = dev(Q)
+    r.O.fill_(0x1234)
+    bits = r()
+    keep = np.setdiff1d(np.arange(M), odd)
+    if P == 40:
+        assert (bits[keep] == clean[keep]).all()
+    want, tol, _ = bound(c, 0, keep)
+    assert np.all(np.abs(ob.to_f32(bits[keep], BF16).reshape(want.shape) - want) <= tol)
